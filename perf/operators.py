@@ -254,9 +254,10 @@ class _Kv:
 
 
 class _Rows:
-    """Rows of a cache tensor in device memory, for torch.as_tensor."""
+    """Rows of a cache tensor in device memory, for torch.as_tensor; the cache lives as long as they do."""
 
-    def __init__(self, ptr, shape, kind):
+    def __init__(self, kv, ptr, shape, kind):
+        self.kv = kv
         self.__cuda_array_interface__ = dict(data=(ptr, False), shape=shape, typestr=kind, version=3)
 
 
@@ -271,8 +272,8 @@ def _own_rope(case, s):
         s["rows"] = [torch.empty((t, hk, d), device="cuda", dtype=torch.float16) for _ in range(2)]
     else:
         elt, kind = (4, "<f4") if case["cache"] == "f32" else (2, "<f2")
-        s["rows"] = [torch.as_tensor(_Rows(lib.kv_view(s["kv"].h, 0, w)[0] + past * hk * d * elt, (t, hk, d), kind),
-                                     device="cuda") for w in range(2)]
+        s["rows"] = [torch.as_tensor(_Rows(s["kv"], lib.kv_view(s["kv"].h, 0, w)[0] + past * hk * d * elt, (t, hk, d),
+                                           kind), device="cuda") for w in range(2)]
 
 
 def _own_cache(case, s):
