@@ -202,13 +202,26 @@ int mi_hip_set_decode_mode(int32_t mode);
 
 typedef struct mi_hip_kv mi_hip_kv;
 
+/* Cache elements of 8 bits (a cache type only: no tensor of the engine has it).
+ * A group of values shares a scale d, the smallest f16 number with
+ * 127 d >= max |x|; each value is kept as the int8 nearest to x / d (ties to
+ * even) and stands for that many times d, so it is at most d / 2 off. A K row
+ * has a group for each 32 dims, a V row is one group. 1.06 and 1.02 to 1.03
+ * bytes per value. A group with an infinity or a NaN, or with max |x| above
+ * 8319008, reads back as NaN. Everything that takes a cache handle takes one of
+ * this type, except mi_hip_attn_fwd_reference_order and
+ * mi_hip_attn_decode_batch_noalloc (MI_HIP_E_UNSUPPORTED). mi_hip_kv_view gives
+ * the int8 values, mi_hip_kv_scales the scales. No counterpart in the
+ * reference. */
+#define MI_HIP_TYPE_Q8 100
+
 typedef struct mi_hip_kv_desc {
   int32_t n_layer;
   int32_t n_ctx;
   int32_t n_head_kv;
   int32_t head_dim;  /* 64 or 128 */
   int32_t n_head;    /* Q heads (multiple of n_head_kv); sizes staging */
-  int32_t type;      /* MI_TYPE_F32 or MI_TYPE_F16 cache elements */
+  int32_t type;      /* MI_TYPE_F32, MI_TYPE_F16 or MI_HIP_TYPE_Q8 cache elements */
 } mi_hip_kv_desc;
 
 /* One device allocation holding every layer's K and V as
@@ -230,13 +243,35 @@ int mi_hip_kv_view(mi_hip_kv* kv, int layer, int which, void** data, int64_t ne[
 
 /* Writes n_tokens F32 rows src[head_dim, n_head_kv, n_tokens] (byte strides
  * src_nb[0..2]) into positions [pos0, pos0 + n_tokens) of layer `layer`'s
- * K (which = 0) or V (which = 1); F16 caches round to nearest even.
+ * K (which = 0) or V (which = 1); F16 caches round to nearest even, 8-bit
+ * caches quantise each row.
  * src_on_device = 0 for a host source, 1 for a device source.
  * This is the CPY-into-kv_write_view node (src/model_qwen2.cpp:99-103,
  * 156-159; src/ops_cpu.cpp:446-460). Host sources are synchronous. */
 int mi_hip_kv_write(mi_hip_kv* kv, int layer, int which, int pos0, int n_tokens,
                     const float* src, const size_t src_nb[3], int src_on_device,
                     void* stream);
+
+/* Device view of the scales of one layer of an 8-bit cache: f16
+ * [head_dim / 32, n_head_kv, n_ctx] of K (which = 0), [1, n_head_kv, n_ctx] of
+ * V (which = 1). */
+int mi_hip_kv_scales(mi_hip_kv* kv, int layer, int which, void** data, int64_t ne[4],
+                     size_t nb[4]);
+
+/* Reads positions [pos0, pos0 + n_tokens) of layer `layer`'s K (which = 0) or
+ * V (which = 1) into device rows dst[head_dim, n_head_kv, n_tokens] (byte
+ * strides dst_nb[0..2]) of type MI_TYPE_F32 or MI_TYPE_F16 (rounded to nearest
+ * even). The values are what the attention reads: exact for an F32 dst. No
+ * counterpart in the reference. */
+int mi_hip_kv_read(mi_hip_kv* kv, int layer, int which, int pos0, int n_tokens, void* dst,
+                   int dst_type, const size_t dst_nb[3], void* stream);
+
+/* Keeps the accepted rows of a tree of drafted tokens: row n_past + idx[i]
+ * becomes row n_past + i, i < n_idx, of K and V of every layer. idx (host) is
+ * strictly increasing, at most 256 rows and at most 32767 behind n_past; rows
+ * from n_past + n_idx on keep what they hold. No counterpart in the
+ * reference. */
+int mi_hip_kv_keep(mi_hip_kv* kv, int n_past, const int32_t* idx, int n_idx, void* stream);
 
 /* Associates the engine's host KV tensor (the persistent leaf whose
  * view_src-flattened views the CPY nodes write through, and which the
@@ -321,6 +356,37 @@ int mi_hip_attn_decode_batch(const mi_hip_attn_args* items, int n_items, void* s
  * not be issued; calls ordered on one stream are safe. */
 int mi_hip_attn_decode_batch_noalloc(const mi_hip_attn_args* items, int n_items, void* stream);
 
+/* ---- attention of a tree of drafted tokens ------------------------------ */
+
+/* Which of its own keys each query of an item sees: bit i % 64 of word i / 64
+ * of row j is set if query j sees key n_past + i, i < n_tokens (bits past that
+ * are not read). Device memory, rows nb bytes apart, 8-byte aligned. bits NULL:
+ * query j sees keys n_past + 0 .. n_past + j (a chain). Every query sees the
+ * n_past keys before. */
+typedef struct mi_hip_tree_mask {
+  const uint64_t* bits;
+  size_t nb;
+} mi_hip_tree_mask;
+
+/* Attention of n_tokens queries per item whose own K/V rows are the cache rows
+ * n_past .. n_past + n_tokens - 1 (a tree of drafted tokens appended in one
+ * step, a chunk of a prompt, or one token): out_j = softmax over the keys that
+ * query j sees of scale q_j.k_t, times v_t. F32, F16 and 8-bit caches; items
+ * share the head shape, element type and scale, n_past and n_tokens may differ.
+ * masks: one per item, or NULL (every item a chain). A query that sees no key
+ * gives zeros, and so does one whose every score is -inf. What lies in rows that
+ * a query does not see never shows in its output, infinities and NaN included;
+ * an infinite or NaN value in a V row that it sees may give NaN for infinity.
+ * Scratch for joining the parts of long caches: ws of the first item, else its
+ * cache's workspace, else the library default; calls that share one must be
+ * ordered. Nothing is kept in it between calls, so unlike the other decode entry
+ * points this one may be captured into a graph (pointers, n_past and n_tokens
+ * as at the capture; the masks are read at each replay). The same bits on every
+ * run. mi_hip_attn_fwd and mi_hip_attn_decode_batch on an 8-bit cache run this.
+ * No counterpart in the reference. */
+int mi_hip_attn_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* masks, int n_items,
+                     void* stream);
+
 /* ---- node-level operators on device tensors ----------------------------- */
 /*
  * Same signature idea as the engine's kernels (src/ops_cpu.h:3-12): the node
@@ -393,6 +459,75 @@ typedef struct mi_hip_rope_args {
 } mi_hip_rope_args;
 
 int mi_hip_rope_append(const mi_hip_rope_args* args);
+
+/* mi_hip_rope_append for models that norm queries and keys per head, and for
+ * tokens at positions of their own. Per row x of Q and K (one head of one
+ * token): y = x / sqrt(mean(x^2) + eps) * w where the norm's weights are given,
+ * then the rotation of MI_OP_ROPE at the token's position (the angle is one
+ * float product, position * frequency); Q into q_out (which may equal q), K and
+ * V into the cache rows n_past + token. Without weights, pos and freq the
+ * results of mi_hip_rope_append. Any cache type. No counterpart in the
+ * reference. */
+typedef struct mi_hip_norm_rope_args {
+  mi_hip_kv* kv;
+  int32_t layer;
+  int32_t n_past;       /* first cache row written */
+  int32_t n_tokens;
+  int32_t n_dims;       /* rotated dims (even, <= head_dim) */
+  float freq_base;      /* frequencies freq_base^(-2p / n_dims), unless freq is given */
+  const float* freq;    /* host, n_dims / 2 frequencies, or NULL */
+  const int32_t* pos;   /* device, n_tokens positions, or NULL: n_past + token */
+  float eps;
+  const float* q_norm;  /* device, head_dim weights, or NULL: no norm */
+  const float* k_norm;
+  int32_t n_head;       /* Q heads */
+  const float* q;       /* may be NULL (no Q) */
+  size_t q_nb[3];
+  float* q_out;
+  size_t q_out_nb[3];
+  const float* k;
+  size_t k_nb[3];
+  const float* v;
+  size_t v_nb[3];
+  void* stream;
+} mi_hip_norm_rope_args;
+
+int mi_hip_norm_rope_append(const mi_hip_norm_rope_args* args);
+
+/* ---- from logits to greedy ids ------------------------------------------- */
+
+/* Penalties, biases and a grammar's mask on rows of logits (one per sequence,
+ * or per drafted token), and the greedy id of each row. For token t that stands
+ * c times in the row's history, each step rounded to float:
+ *   c > 0:  y = x > 0 ? x / repeat : x * repeat;  y -= c * frequency + presence
+ *   y += the sum of t's biases, in the list's order
+ *   y = -inf where the mask's bit t is clear
+ * ids: the lowest t with the largest y (mi_qwen2_sample_greedy's rule,
+ * src/model_qwen2.cpp:690-700), -1 if every y is -inf or NaN. All pointers are
+ * device memory; offsets have n_rows + 1 entries, row r's list is
+ * [off[r], off[r + 1]). Ids outside [0, n_vocab) in the lists are passed over.
+ * May be captured into a graph. No counterpart in the reference. */
+typedef struct mi_hip_logits_args {
+  const float* logits;
+  size_t nb;                /* bytes between rows */
+  float* out;               /* may be logits */
+  size_t out_nb;
+  int32_t n_vocab;
+  int32_t n_rows;
+  const float* penalties;   /* repeat, frequency, presence of each row, or NULL (with no history) */
+  const int32_t* hist;      /* token ids, or NULL */
+  const int32_t* hist_off;
+  const int32_t* bias_id;   /* token ids, or NULL */
+  const float* bias;
+  const int32_t* bias_off;
+  const uint32_t* mask;     /* bit t % 32 of word t / 32: token t is allowed; or NULL */
+  size_t mask_nb;           /* bytes between rows; 0: one row for all */
+  int32_t* ids;             /* greedy ids, or NULL */
+  mi_hip_workspace* ws;     /* scratch for ids, or NULL: the library default */
+  void* stream;
+} mi_hip_logits_args;
+
+int mi_hip_logits_adjust(const mi_hip_logits_args* args);
 
 /* ---- executor hook for host-resident graphs ------------------------------ */
 

@@ -101,6 +101,38 @@ struct PrefillParams {
 };
 
 // ---------------------------------------------------------------------------
+// Tree attention (tree.hip): several query tokens per item, a visibility mask
+// over the keys that are theirs.
+// ---------------------------------------------------------------------------
+constexpr int kTreeMaxItems = 32;  // items per launch (they ride in kernarg)
+
+struct TreeItem {
+  const char* k;        // layer's K and V (8-bit caches: the int8 values)
+  const char* v;
+  const char* k_scale;  // 8-bit caches: f16 [head_dim / 32, n_head_kv, n_ctx] and [n_head_kv, n_ctx]
+  const char* v_scale;
+  const float* q;
+  float* out;
+  const char* mask;     // row j: bit i of its 64-bit words, does query j see key n_past + i; null: i <= j
+  int64_t mask_nb;      // bytes between mask rows
+  int32_t n_past, n_tokens;
+  int32_t n_rt;             // row tiles per KV head
+  int32_t n_split;          // key splits (1: no records, the kernel writes the output)
+  int32_t tiles_per_split;  // 32-key tiles
+  int32_t rec0;             // the item's first record
+};
+
+struct TreeParams {
+  int64_t k_s1, k_s2, v_s1, v_s2;  // bytes, the same for every item
+  int64_t q_s1, q_s2, o_s1, o_s2;
+  int32_t n_rep, n_head_kv;
+  float scale_log2e;
+  float* rec;  // records of the items with more than one split
+  TreeItem item[kTreeMaxItems];  // grid row y serves item y
+};
+static_assert(sizeof(TreeParams) <= 4096 - 64, "kernel arguments");
+
+// ---------------------------------------------------------------------------
 // Device helpers.
 // ---------------------------------------------------------------------------
 typedef __amdgpu_buffer_rsrc_t rsrc_t;

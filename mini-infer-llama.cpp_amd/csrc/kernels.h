@@ -86,6 +86,82 @@ struct RopeAppend {
 hipError_t launch_rope_node(const RopeNode& p, hipStream_t stream);
 hipError_t launch_rope_append(const RopeAppend& p, bool f16, hipStream_t stream);
 
+// tree.hip. Query rows per row tile for `rows` rows per KV head, and the
+// floats of one record (a row tile's part from one split).
+int tree_tile_rows(int rows);
+size_t tree_record_floats(int head_dim, int tile_rows);
+// elt: bytes of a cache element (4 F32, 2 F16, 1 8-bit). Every item's n_rt is
+// in tiles of tile_rows.
+hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, hipStream_t stream);
+
+// kv8.hip -- rows on their way into and out of a cache.
+// A layer's K and V of a cache: element type by elt (4 F32, 2 F16, 1 8-bit
+// with its scales), byte strides of heads and positions; the scales' strides
+// follow from n_head_kv (see CacheRows in kv8.hip).
+struct CacheView {
+  char* t[2];      // K, V
+  char* scale[2];  // 8-bit: f16 [head_dim / 32, n_head_kv, n_ctx], [n_head_kv, n_ctx]
+  int64_t s1, s2;
+  int32_t head_dim, n_head_kv, elt;
+};
+// src F32 [head_dim, n_head_kv, n_tokens] -> rows pos0.. of K (which = 0) or V
+// of an 8-bit cache.
+hipError_t launch_kv_quantize(const CacheView& c, int which, const char* src, const int64_t src_nb[3], int pos0,
+                              int n_tokens, hipStream_t stream);
+// rows pos0.. of K or V -> dst [head_dim, n_head_kv, n_tokens], F32 or F16
+hipError_t launch_kv_read(const CacheView& c, int which, int pos0, int n_tokens, char* dst, bool dst_f16,
+                          const int64_t dst_nb[3], hipStream_t stream);
+// row n_past + idx[i] -> row n_past + i of K, V and scales of every layer
+// (idx strictly increasing). `bytes`: one position's bytes of each of the
+// planes, `layer` the bytes from a layer's plane to the next layer's.
+constexpr int kKeepMax = 256;
+struct KvKeep {
+  char* plane[4];
+  int64_t layer[4];
+  int32_t bytes[4];
+  int32_t n_planes, n_layer, n_past, n;
+  int16_t idx[kKeepMax];
+};
+hipError_t launch_kv_keep(const KvKeep& p, hipStream_t stream);
+
+// Norms of Q and K per head (optional), their rotation, and the append.
+struct NormRope {
+  const char* q;  // may be null
+  char* q_out;
+  const char* k;
+  const char* v;
+  const int32_t* pos;   // device; null: n_past + token
+  const float* q_norm;  // device, head_dim weights; null: no norm
+  const float* k_norm;
+  CacheView cache;
+  int64_t q_nb[3], qo_nb[3], k_nb[3], v_nb[3];
+  int32_t n_tokens, n_head, n_past, n_dims;
+  float eps;
+  float freq[kRopeMaxPairs];
+};
+hipError_t launch_norm_rope(const NormRope& p, hipStream_t stream);
+
+// logits.hip. One row per sequence or tree node; the lists' offsets have
+// n_rows + 1 entries.
+struct LogitsAdjust {
+  const char* in;
+  char* out;
+  int64_t in_nb, out_nb;   // bytes between rows
+  const float* penalties;  // repeat, frequency, presence of each row; null: none
+  const int32_t* hist;     // token histories; null: none
+  const int32_t* hist_off;
+  const int32_t* bias_id;  // biased tokens; null: none
+  const float* bias;
+  const int32_t* bias_off;
+  const char* mask;        // bit t of a row's 32-bit words: token t is allowed; null: all
+  int64_t mask_nb;
+  int32_t* ids;            // greedy ids; null: not asked for
+  uint64_t* part;          // n_rows * logits_chunks(n_vocab) words of scratch when ids are
+  int32_t n_vocab, n_rows;
+};
+int logits_chunks(int n_vocab);
+hipError_t launch_logits_adjust(const LogitsAdjust& p, hipStream_t stream);
+
 // mul_mat.hip. Activation rows (F32, ne0 a multiple of 32, contiguous within
 // a row) -> Q8_0_ACT blocks; Q8_0 weight rows . activation columns -> F32.
 struct Q8Quantize {

@@ -328,10 +328,12 @@ bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) %
 }  // namespace
 
 // ---------------------------------------------------------------------------
-// Decode workspace: [status words][two counter sets][records], each part
+// Decode workspace: [status words][two counter sets][records][parts], each
 // 256-byte aligned. Zeroed once at creation; afterwards the kernels keep the
 // counter sets zero between launches (see decode.hip) and the epoch stamps
-// make stale records recognisable.
+// make stale records recognisable. The parts belong to the launches that keep
+// nothing between calls (tree attention's split records, the logits' chunk
+// maxima): each writes what it then reads.
 // ---------------------------------------------------------------------------
 struct mi_hip_workspace {
   int groups = 0;           // groups one launch may have (counter-set capacity)
@@ -341,6 +343,8 @@ struct mi_hip_workspace {
   unsigned* status = nullptr;
   unsigned* cnt = nullptr;
   float* rec = nullptr;
+  size_t part_bytes = 0;    // capacity of the parts (0: none)
+  char* part = nullptr;
   std::mutex mu;
   uint32_t epoch = 0;       // stamp of the last launch
   int dirty[2] = {0, 0};    // counter set s: groups [0, dirty[s]) the last launch on it used
@@ -363,20 +367,32 @@ size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 size_t ws_counter_bytes(int groups) { return 2 * (size_t)groups * mi::kCtrInts * sizeof(unsigned); }
 
-// Bytes of a workspace covering `groups` groups and `rec_bytes` of records.
-size_t ws_total_bytes(int groups, size_t rec_bytes) {
-  return kWsAlign + round_up(ws_counter_bytes(groups), kWsAlign) + round_up(rec_bytes, kWsAlign);
+// Bytes of a workspace covering `groups` groups, `rec_bytes` of records and
+// `part_bytes` of parts.
+size_t ws_total_bytes(int groups, size_t rec_bytes, size_t part_bytes) {
+  return kWsAlign + round_up(ws_counter_bytes(groups), kWsAlign) + round_up(rec_bytes, kWsAlign) +
+         round_up(part_bytes, kWsAlign);
+}
+
+// Bytes of parts that let a tree-attention launch split its keys over
+// kTreeWgPerCu workgroups per CU (see plan_tree), each with a record of 64 rows.
+constexpr int kTreeWgPerCu = 2;
+size_t ws_part_bytes(int head_dim) {
+  return (size_t)kTreeWgPerCu * g.n_cu * mi::tree_record_floats(head_dim, 64) * sizeof(float);
 }
 
 // Lays a workspace over [base, base + bytes).
-void ws_layout(mi_hip_workspace* ws, char* base, int groups, size_t rec_bytes) {
+void ws_layout(mi_hip_workspace* ws, char* base, int groups, size_t rec_bytes, size_t part_bytes) {
   ws->base = base;
   ws->groups = groups;
   ws->rec_bytes = rec_bytes;
-  ws->bytes = ws_total_bytes(groups, rec_bytes);
+  ws->part_bytes = part_bytes;
+  ws->bytes = ws_total_bytes(groups, rec_bytes, part_bytes);
   ws->status = reinterpret_cast<unsigned*>(base);
   ws->cnt = reinterpret_cast<unsigned*>(base + kWsAlign);
-  ws->rec = reinterpret_cast<float*>(base + kWsAlign + round_up(ws_counter_bytes(groups), kWsAlign));
+  char* const rec = base + kWsAlign + round_up(ws_counter_bytes(groups), kWsAlign);
+  ws->rec = reinterpret_cast<float*>(rec);
+  ws->part = part_bytes ? rec + round_up(rec_bytes, kWsAlign) : nullptr;
 }
 
 // Groups and record bytes that cover every decode launch of a head shape: up
@@ -391,12 +407,12 @@ void ws_capacity(int n_head_kv, int n_rep, int head_dim, int* groups, size_t* re
   *rec_bytes = (size_t)wgs * mi::decode_record_floats(head_dim, group) * sizeof(float);
 }
 
-int ws_create(int groups, size_t rec_bytes, mi_hip_workspace** out) {
+int ws_create(int groups, size_t rec_bytes, size_t part_bytes, mi_hip_workspace** out) {
   *out = nullptr;
   mi_hip_workspace* ws = new (std::nothrow) mi_hip_workspace();
   if (!ws) return fail(MI_HIP_E_NOMEM, "host allocation failed");
   void* p = nullptr;
-  const size_t bytes = ws_total_bytes(groups, rec_bytes);
+  const size_t bytes = ws_total_bytes(groups, rec_bytes, part_bytes);
   int rc = dev_alloc(&p, bytes, "decode workspace");
   if (rc) {
     delete ws;
@@ -409,7 +425,7 @@ int ws_create(int groups, size_t rec_bytes, mi_hip_workspace** out) {
     delete ws;
     return hip_fail(e, "workspace init");
   }
-  ws_layout(ws, static_cast<char*>(p), groups, rec_bytes);
+  ws_layout(ws, static_cast<char*>(p), groups, rec_bytes, part_bytes);
   *out = ws;
   return MI_HIP_OK;
 }
@@ -419,8 +435,8 @@ int ws_over_scratch(void* ptr, mi_hip_workspace** out) {
   *out = nullptr;
   mi_hip_workspace* ws = new (std::nothrow) mi_hip_workspace();
   if (!ws) return fail(MI_HIP_E_NOMEM, "host allocation failed");
-  const size_t rec = kScratchBytes - (ws_total_bytes(kScratchGroups, 0) - 0);
-  ws_layout(ws, static_cast<char*>(ptr), kScratchGroups, rec & ~(kWsAlign - 1));
+  const size_t rec = kScratchBytes - ws_total_bytes(kScratchGroups, 0, 0);
+  ws_layout(ws, static_cast<char*>(ptr), kScratchGroups, rec & ~(kWsAlign - 1), 0);
   ws->borrowed = true;
   *out = ws;
   return MI_HIP_OK;
@@ -470,9 +486,31 @@ struct mi_hip_kv {
   size_t stage_bytes = 0;
   size_t q_floats = 0, row_floats = 0;
   hipStream_t stream = nullptr;
+  // 8-bit caches: the scales of every layer behind the values, one layer's K
+  // scales (one per 32 dims) and V scales (one per row) scale_bytes apart.
+  size_t scale_at[2] = {0, 0};  // of layer 0, from base
+  size_t scale_bytes = 0;       // of one layer
 
   char* tensor(int layer, int which) const {
     return base + (size_t)(2 * layer + which) * tensor_bytes;
+  }
+  bool q8() const { return d.type == MI_HIP_TYPE_Q8; }
+  int scales_per_row(int which) const { return which == 0 ? d.head_dim / 32 : 1; }
+  char* scale(int layer, int which) const {
+    return q8() ? base + scale_at[which] + (size_t)layer * scale_bytes : nullptr;
+  }
+  mi::CacheView view(int layer) const {
+    mi::CacheView c{};
+    for (int w = 0; w < 2; ++w) {
+      c.t[w] = tensor(layer, w);
+      c.scale[w] = scale(layer, w);
+    }
+    c.s1 = s1;
+    c.s2 = s2;
+    c.head_dim = d.head_dim;
+    c.n_head_kv = d.n_head_kv;
+    c.elt = elt;
+    return c;
   }
 };
 
@@ -483,6 +521,9 @@ struct Resolved {
   const char* v;
   int64_t k_s1, k_s2, v_s1, v_s2;
   bool f16;
+  bool q8;
+  const char* k_scale;  // 8-bit caches
+  const char* v_scale;
   int head_dim, n_head_kv;
   int n_ctx;  // -1 when unknown (explicit tensors)
 };
@@ -497,6 +538,9 @@ int resolve_kv(const mi_hip_attn_args* a, Resolved* r) {
     r->k_s1 = r->v_s1 = kv->s1;
     r->k_s2 = r->v_s2 = kv->s2;
     r->f16 = kv->d.type == MI_TYPE_F16;
+    r->q8 = kv->q8();
+    r->k_scale = kv->scale(a->layer, 0);
+    r->v_scale = kv->scale(a->layer, 1);
     r->head_dim = kv->d.head_dim;
     r->n_head_kv = kv->d.n_head_kv;
     r->n_ctx = kv->d.n_ctx;
@@ -504,7 +548,8 @@ int resolve_kv(const mi_hip_attn_args* a, Resolved* r) {
   }
   if (!a->k || !a->v) return fail(MI_HIP_E_INVALID, "no KV source: kv and k/v are NULL");
   if (a->kv_type != MI_TYPE_F32 && a->kv_type != MI_TYPE_F16)
-    return fail(MI_HIP_E_UNSUPPORTED, "K/V type %d: only F32 (0) and F16 (1)", a->kv_type);
+    return fail(MI_HIP_E_UNSUPPORTED, "K/V type %d: only F32 (0) and F16 (1); an 8-bit cache is named by its handle",
+                a->kv_type);
   const int elt = a->kv_type == MI_TYPE_F16 ? 2 : 4;
   if (a->k_nb[0] != (size_t)elt || a->v_nb[0] != (size_t)elt)
     return fail(MI_HIP_E_UNSUPPORTED, "K/V nb[0] must be the element size (%d)", elt);
@@ -521,6 +566,8 @@ int resolve_kv(const mi_hip_attn_args* a, Resolved* r) {
   r->v_s1 = (int64_t)a->v_nb[1];
   r->v_s2 = (int64_t)a->v_nb[2];
   r->f16 = a->kv_type == MI_TYPE_F16;
+  r->q8 = false;
+  r->k_scale = r->v_scale = nullptr;
   r->head_dim = a->head_dim;
   r->n_head_kv = a->n_head_kv;
   r->n_ctx = -1;
@@ -718,6 +765,123 @@ int run_prefill(const mi_hip_attn_args* a, const Resolved& r, hipStream_t stream
   return MI_HIP_OK;
 }
 
+// Tree attention. The launch is cut so that it has about kTreeWgPerCu
+// workgroups per CU: row tiles first (they cost no second read from HBM worth
+// naming, since a unit's row tiles share an L2), then the keys, each split at
+// least one 32-key tile per wave. Every item's splits have the same number of
+// tiles, so a launch of ragged items is even.
+void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int tile_rows, size_t part_bytes) {
+  constexpr int kMinTiles = 4;  // one per wave
+  const int64_t want = (int64_t)kTreeWgPerCu * g.n_cu;
+  const int64_t cap = (int64_t)(part_bytes / (mi::tree_record_floats(head_dim, tile_rows) * sizeof(float)));
+  int64_t units = 0, tiles = 0, longest = 0;
+  auto tiles_of = [&](const mi::TreeItem& it) { return ((int64_t)it.n_past + it.n_tokens + 31) / 32; };
+  for (int i = 0; i < n_items; ++i) {
+    mi::TreeItem& it = p.item[i];
+    it.n_rt = (int32_t)(((int64_t)it.n_tokens * p.n_rep + tile_rows - 1) / tile_rows);
+    units += (int64_t)p.n_head_kv * it.n_rt;
+    tiles += (int64_t)p.n_head_kv * it.n_rt * tiles_of(it);
+    longest = std::max(longest, tiles_of(it));
+  }
+  int64_t per = longest;
+  if (units < want) {
+    per = std::max<int64_t>(kMinTiles, (tiles + want - 1) / want);
+    // rounding up per item can pass what is wanted, and what the parts hold
+    auto records = [&](int64_t n) {
+      int64_t r = 0;
+      for (int i = 0; i < n_items; ++i)
+        r += (int64_t)p.n_head_kv * p.item[i].n_rt * ((tiles_of(p.item[i]) + n - 1) / n);
+      return r;
+    };
+    while (per < longest && records(per) > std::min(want, cap)) per += std::max<int64_t>(1, per / 16);
+    if (records(per) > cap) per = longest;
+  }
+  int64_t rec = 0;
+  for (int i = 0; i < n_items; ++i) {
+    mi::TreeItem& it = p.item[i];
+    it.tiles_per_split = (int32_t)std::min<int64_t>(per, tiles_of(it));
+    it.n_split = (int32_t)((tiles_of(it) + it.tiles_per_split - 1) / it.tiles_per_split);
+    it.rec0 = (int32_t)rec;
+    if (it.n_split > 1) rec += (int64_t)p.n_head_kv * it.n_rt * it.n_split;
+  }
+}
+
+int run_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* masks, int n, hipStream_t stream,
+             mi_hip_workspace* ws) {
+  if (!ws) return fail(MI_HIP_E_STATE, "no workspace (the library default is gone)");
+  Resolved r0;
+  int rc = resolve_kv(&items[0], &r0);
+  if (rc) return rc;
+  const int elt = r0.q8 ? 1 : r0.f16 ? 2 : 4;
+  for (int i = 0; i < n; ++i) {
+    const mi_hip_attn_args* a = &items[i];
+    Resolved r;
+    if ((rc = resolve_kv(a, &r))) return rc;
+    if ((rc = check_problem(a, r))) return rc;
+    if (r.head_dim != r0.head_dim || r.f16 != r0.f16 || r.q8 != r0.q8 || r.n_head_kv != r0.n_head_kv ||
+        a->n_rep != items[0].n_rep || a->scale != items[0].scale)
+      return fail(MI_HIP_E_INVALID, "item %d: shape, type or scale differs from item 0", i);
+    const int64_t row_bytes = (int64_t)r.head_dim * elt;
+    if (r.k_s2 < row_bytes || r.v_s2 < row_bytes)
+      return fail(MI_HIP_E_UNSUPPORTED, "item %d: position stride below one row", i);
+    if (32 * r.k_s2 > INT32_MAX || 32 * r.v_s2 > INT32_MAX)
+      return fail(MI_HIP_E_UNSUPPORTED, "item %d: position stride above 2^26 bytes", i);
+    if ((int64_t)a->n_past + a->n_tokens > INT32_MAX - 64 || (int64_t)a->n_tokens * a->n_head > (1 << 26))
+      return fail(MI_HIP_E_UNSUPPORTED, "item %d: more than 2^26 query rows or 2^31 keys", i);
+    if (masks && masks[i].bits) {
+      if (masks[i].nb % 8 || !aligned(masks[i].bits, 8))
+        return fail(MI_HIP_E_UNSUPPORTED, "item %d: mask rows must be 8-byte aligned", i);
+      if (a->n_tokens > 1 && masks[i].nb < (size_t)(a->n_tokens + 63) / 64 * 8)
+        return fail(MI_HIP_E_INVALID, "item %d: mask row stride below %d words", i, (a->n_tokens + 63) / 64);
+    }
+  }
+  if ((rc = bind_device())) return rc;
+  mi::TreeParams p{};
+  p.n_rep = items[0].n_rep;
+  p.n_head_kv = r0.n_head_kv;
+  p.scale_log2e = items[0].scale * kLog2e;
+  p.rec = reinterpret_cast<float*>(ws->part);
+  // Launches of up to kTreeMaxItems consecutive items that share all strides.
+  for (int base = 0; base < n;) {
+    int cnt = 0, most = 0;
+    for (; cnt < mi::kTreeMaxItems && base + cnt < n; ++cnt) {
+      const mi_hip_attn_args* a = &items[base + cnt];
+      Resolved r;
+      if ((rc = resolve_kv(a, &r))) return rc;
+      const int64_t s[8] = {r.k_s1, r.k_s2, r.v_s1, r.v_s2, (int64_t)a->q_nb[1], (int64_t)a->q_nb[2],
+                            (int64_t)a->out_nb[1], (int64_t)a->out_nb[2]};
+      int64_t* const d[8] = {&p.k_s1, &p.k_s2, &p.v_s1, &p.v_s2, &p.q_s1, &p.q_s2, &p.o_s1, &p.o_s2};
+      bool same = true;
+      for (int i = 0; i < 8; ++i) {
+        if (cnt == 0) *d[i] = s[i];
+        same = same && *d[i] == s[i];
+      }
+      if (!same) break;
+      mi::TreeItem& it = p.item[cnt];
+      it = mi::TreeItem{};
+      it.k = r.k;
+      it.v = r.v;
+      it.k_scale = r.k_scale;
+      it.v_scale = r.v_scale;
+      it.q = a->q;
+      it.out = a->out;
+      it.n_past = a->n_past;
+      it.n_tokens = a->n_tokens;
+      if (masks && masks[base + cnt].bits) {
+        it.mask = reinterpret_cast<const char*>(masks[base + cnt].bits);
+        it.mask_nb = (int64_t)masks[base + cnt].nb;
+      }
+      most = std::max(most, a->n_tokens * a->n_rep);
+    }
+    const int tile_rows = mi::tree_tile_rows(most);
+    plan_tree(p, cnt, r0.head_dim, tile_rows, ws->part_bytes);
+    hipError_t e = mi::launch_tree(p, cnt, r0.head_dim, elt, tile_rows, stream);
+    if (e != hipSuccess) return hip_fail(e, "tree attention launch");
+    base += cnt;
+  }
+  return MI_HIP_OK;
+}
+
 // ---------------------------------------------------------------------------
 // Executor hook tables (no allocation per step)
 // ---------------------------------------------------------------------------
@@ -908,10 +1072,11 @@ int mi_hip_init(int device) {
   g.knobs.stream_min = env_int("MI_HIP_DECODE_STREAM_MIN", 0);
   g.ready = true;
   // The default workspace: head_dim up to 128, groups of up to 8 heads, up to
-  // 1024 groups per launch (e.g. 32 items x 32 KV heads), ~11 MB.
+  // 1024 groups per launch (e.g. 32 items x 32 KV heads), ~11 MB, and 17 MB of
+  // parts.
   const int groups = 1024;
   const size_t rec = (size_t)(g.n_cu + groups) * mi::decode_record_floats(128, 8) * sizeof(float);
-  int rc = ws_create(groups, rec, &g.default_ws);
+  int rc = ws_create(groups, rec, ws_part_bytes(128), &g.default_ws);
   if (rc) {
     g.ready = false;
     return rc;
@@ -1015,19 +1180,29 @@ int mi_hip_kv_create(const mi_hip_kv_desc* d, mi_hip_kv** out) {
                 d->n_head_kv);
   if (d->head_dim != 64 && d->head_dim != 128)
     return fail(MI_HIP_E_UNSUPPORTED, "head_dim %d: the kernels cover 64 and 128", d->head_dim);
-  if (d->type != MI_TYPE_F32 && d->type != MI_TYPE_F16)
-    return fail(MI_HIP_E_UNSUPPORTED, "cache type %d: F32 (0) or F16 (1)", d->type);
+  if (d->type != MI_TYPE_F32 && d->type != MI_TYPE_F16 && d->type != MI_HIP_TYPE_Q8)
+    return fail(MI_HIP_E_UNSUPPORTED, "cache type %d: F32 (0), F16 (1) or MI_HIP_TYPE_Q8 (%d)", d->type,
+                MI_HIP_TYPE_Q8);
   int rc = bind_device();
   if (rc) return rc;
 
   mi_hip_kv* kv = new (std::nothrow) mi_hip_kv();
   if (!kv) return fail(MI_HIP_E_NOMEM, "host allocation failed");
   kv->d = *d;
-  kv->elt = d->type == MI_TYPE_F16 ? 2 : 4;
+  kv->elt = d->type == MI_HIP_TYPE_Q8 ? 1 : d->type == MI_TYPE_F16 ? 2 : 4;
   kv->s1 = (int64_t)d->head_dim * kv->elt;
   kv->s2 = kv->s1 * d->n_head_kv;
   kv->tensor_bytes = (size_t)kv->s2 * d->n_ctx;
   kv->bytes = kv->tensor_bytes * 2 * d->n_layer;
+  if (kv->q8()) {
+    size_t plane[2];
+    for (int w = 0; w < 2; ++w)
+      plane[w] = round_up((size_t)d->n_ctx * d->n_head_kv * kv->scales_per_row(w) * 2, kWsAlign);
+    kv->scale_at[0] = round_up(kv->bytes, kWsAlign);
+    kv->scale_at[1] = kv->scale_at[0] + plane[0];
+    kv->scale_bytes = plane[0] + plane[1];
+    kv->bytes = kv->scale_at[0] + kv->scale_bytes * d->n_layer;
+  }
   kv->q_floats = (size_t)d->n_ctx * d->n_head * d->head_dim;
   kv->row_floats = (size_t)d->n_ctx * d->n_head_kv * d->head_dim;
   kv->stage_bytes = (2 * kv->q_floats + kv->row_floats) * sizeof(float);
@@ -1055,7 +1230,7 @@ int mi_hip_kv_create(const mi_hip_kv_desc* d, mi_hip_kv** out) {
   int groups;
   size_t rec_bytes;
   ws_capacity(d->n_head_kv, d->n_head / d->n_head_kv, d->head_dim, &groups, &rec_bytes);
-  if ((rc = ws_create(groups, rec_bytes, &kv->ws))) {
+  if ((rc = ws_create(groups, rec_bytes, ws_part_bytes(d->head_dim), &kv->ws))) {
     (void)hipStreamDestroy(kv->stream);
     dev_free(kv->stage, kv->stage_bytes);
     dev_free(kv->base, kv->bytes);
@@ -1104,7 +1279,7 @@ int mi_hip_workspace_create(const mi_hip_workspace_desc* d, mi_hip_workspace** o
   int groups;
   size_t rec_bytes;
   ws_capacity(d->n_head_kv, d->n_head / d->n_head_kv, d->head_dim, &groups, &rec_bytes);
-  return ws_create(groups, rec_bytes, out);
+  return ws_create(groups, rec_bytes, ws_part_bytes(d->head_dim), out);
 }
 
 int mi_hip_workspace_destroy(mi_hip_workspace* ws) {
@@ -1241,11 +1416,92 @@ int mi_hip_kv_write(mi_hip_kv* kv, int layer, int which, int pos0, int n_tokens,
     nb[1] = 4LL * D;
     nb[2] = 4LL * D * H;
   }
-  hipError_t e = mi::launch_kv_append(dst, kv->s1, kv->s2, kv->elt == 2, dev_src, nb, D, H, pos0,
-                                      n_tokens, st);
+  hipError_t e = kv->q8() ? mi::launch_kv_quantize(kv->view(layer), which, dev_src, nb, pos0, n_tokens, st)
+                          : mi::launch_kv_append(dst, kv->s1, kv->s2, kv->elt == 2, dev_src, nb, D, H, pos0,
+                                                 n_tokens, st);
   if (e != hipSuccess) return hip_fail(e, "kv append launch");
   if (!src_on_device) MI_TRY_HIP(hipStreamSynchronize(st), "hipStreamSynchronize");
   return MI_HIP_OK;
+}
+
+int mi_hip_kv_scales(mi_hip_kv* kv, int layer, int which, void** data, int64_t ne[4], size_t nb[4]) {
+  if (!kv || !data) return fail(MI_HIP_E_INVALID, "kv and data must be non-NULL");
+  if (layer < 0 || layer >= kv->d.n_layer || (which != 0 && which != 1))
+    return fail(MI_HIP_E_INVALID, "layer %d / which %d out of range", layer, which);
+  if (!kv->q8()) return fail(MI_HIP_E_UNSUPPORTED, "only an 8-bit cache has scales");
+  *data = kv->scale(layer, which);
+  const int n = kv->scales_per_row(which);
+  if (ne) {
+    ne[0] = n;
+    ne[1] = kv->d.n_head_kv;
+    ne[2] = kv->d.n_ctx;
+    ne[3] = 1;
+  }
+  if (nb) {
+    nb[0] = 2;
+    nb[1] = 2 * (size_t)n;
+    nb[2] = nb[1] * kv->d.n_head_kv;
+    nb[3] = nb[2] * kv->d.n_ctx;
+  }
+  return MI_HIP_OK;
+}
+
+int mi_hip_kv_read(mi_hip_kv* kv, int layer, int which, int pos0, int n_tokens, void* dst, int dst_type,
+                   const size_t dst_nb[3], void* stream) {
+  if (!kv || !dst || !dst_nb) return fail(MI_HIP_E_INVALID, "kv, dst and dst_nb must be non-NULL");
+  if (layer < 0 || layer >= kv->d.n_layer || (which != 0 && which != 1))
+    return fail(MI_HIP_E_INVALID, "layer %d / which %d out of range", layer, which);
+  if (pos0 < 0 || n_tokens < 0 || (int64_t)pos0 + n_tokens > kv->d.n_ctx)
+    return fail(MI_HIP_E_INVALID, "positions [%d, %lld) outside [0, %d)", pos0, (long long)pos0 + n_tokens,
+                kv->d.n_ctx);
+  if (dst_type != MI_TYPE_F32 && dst_type != MI_TYPE_F16)
+    return fail(MI_HIP_E_UNSUPPORTED, "dst type %d: F32 (0) or F16 (1)", dst_type);
+  const size_t elt = dst_type == MI_TYPE_F16 ? 2 : 4;
+  if (dst_nb[0] % elt || dst_nb[1] % elt || dst_nb[2] % elt || !aligned(dst, elt))
+    return fail(MI_HIP_E_INVALID, "dst and its strides must be multiples of %zu bytes", elt);
+  if (n_tokens == 0) return MI_HIP_OK;
+  int rc = bind_device();
+  if (rc) return rc;
+  const int64_t nb[3] = {(int64_t)dst_nb[0], (int64_t)dst_nb[1], (int64_t)dst_nb[2]};
+  hipError_t e = mi::launch_kv_read(kv->view(layer), which, pos0, n_tokens, static_cast<char*>(dst), elt == 2, nb,
+                                    static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "kv read launch");
+}
+
+int mi_hip_kv_keep(mi_hip_kv* kv, int n_past, const int32_t* idx, int n_idx, void* stream) {
+  if (!kv || (n_idx > 0 && !idx)) return fail(MI_HIP_E_INVALID, "kv and idx must be non-NULL");
+  if (n_idx < 0 || n_idx > mi::kKeepMax)
+    return fail(MI_HIP_E_UNSUPPORTED, "n_idx %d: at most %d rows are kept", n_idx, mi::kKeepMax);
+  if (n_past < 0 || n_past > kv->d.n_ctx)
+    return fail(MI_HIP_E_INVALID, "n_past %d outside [0, %d]", n_past, kv->d.n_ctx);
+  mi::KvKeep p{};
+  bool moves = false;
+  for (int i = 0; i < n_idx; ++i) {
+    if (idx[i] < 0 || (i > 0 && idx[i] <= idx[i - 1]))
+      return fail(MI_HIP_E_INVALID, "idx[%d] = %d: rows must be >= 0 and strictly increasing", i, idx[i]);
+    if ((int64_t)n_past + idx[i] >= kv->d.n_ctx || idx[i] > INT16_MAX)
+      return fail(MI_HIP_E_INVALID, "idx[%d] = %d: row outside the cache, or more than %d behind n_past", i, idx[i],
+                  INT16_MAX);
+    p.idx[i] = (int16_t)idx[i];
+    moves = moves || idx[i] != i;
+  }
+  if (!moves) return MI_HIP_OK;
+  int rc = bind_device();
+  if (rc) return rc;
+  for (int w = 0; w < 2; ++w) {
+    p.plane[w] = kv->tensor(0, w);
+    p.layer[w] = 2 * (int64_t)kv->tensor_bytes;
+    p.bytes[w] = (int32_t)kv->s2;
+    p.plane[2 + w] = kv->scale(0, w);
+    p.layer[2 + w] = (int64_t)kv->scale_bytes;
+    p.bytes[2 + w] = kv->d.n_head_kv * kv->scales_per_row(w) * 2;
+  }
+  p.n_planes = kv->q8() ? 4 : 2;
+  p.n_layer = kv->d.n_layer;
+  p.n_past = n_past;
+  p.n = n_idx;
+  hipError_t e = mi::launch_kv_keep(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "kv keep launch");
 }
 
 int mi_hip_kv_bind(mi_hip_kv* kv, int layer, int which, const mi_tensor* host_kv) {
@@ -1268,6 +1524,7 @@ int mi_hip_attn_fwd(const mi_hip_attn_args* a) {
   if ((rc = check_problem(a, r))) return rc;
   if ((rc = bind_device())) return rc;
   hipStream_t st = static_cast<hipStream_t>(a->stream);
+  if (r.q8) return run_tree(a, nullptr, 1, st, workspace_of(a));
   return a->n_tokens == 1 ? run_decode(a, 1, st, workspace_of(a)) : run_prefill(a, r, st);
 }
 
@@ -1277,7 +1534,7 @@ int mi_hip_attn_fwd_reference_order(const mi_hip_attn_args* a) {
   int rc = resolve_kv(a, &r);
   if (rc) return rc;
   if ((rc = check_problem(a, r))) return rc;
-  if (r.f16) return fail(MI_HIP_E_UNSUPPORTED, "reference-order attention reads an F32 cache (the reference's)");
+  if (r.f16 || r.q8) return fail(MI_HIP_E_UNSUPPORTED, "reference-order attention reads an F32 cache (the reference's)");
   const int64_t n_kv = (int64_t)a->n_past + a->n_tokens;
   if (n_kv > mi::kExactMaxKeys)
     return fail(MI_HIP_E_UNSUPPORTED, "reference-order attention covers up to %d keys", mi::kExactMaxKeys);
@@ -1318,12 +1575,18 @@ int mi_hip_attn_decode_batch(const mi_hip_attn_args* items, int n_items, void* s
     if ((rc = resolve_kv(&items[i], &r))) return rc;
     if ((rc = check_problem(&items[i], r))) return rc;
     if (items[i].n_tokens != 1) return fail(MI_HIP_E_INVALID, "item %d: n_tokens must be 1", i);
-    if (r.head_dim != r0.head_dim || r.f16 != r0.f16 || r.n_head_kv != r0.n_head_kv ||
+    if (r.head_dim != r0.head_dim || r.f16 != r0.f16 || r.q8 != r0.q8 || r.n_head_kv != r0.n_head_kv ||
         items[i].n_rep != items[0].n_rep || items[i].scale != items[0].scale)
       return fail(MI_HIP_E_INVALID, "item %d: shape, type or scale differs from item 0", i);
   }
   if ((rc = bind_device())) return rc;
+  if (r0.q8) return run_tree(items, nullptr, n_items, static_cast<hipStream_t>(stream), workspace_of(&items[0]));
   return run_decode(items, n_items, static_cast<hipStream_t>(stream), workspace_of(&items[0]));
+}
+
+int mi_hip_attn_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* masks, int n_items, void* stream) {
+  if (!items || n_items <= 0) return fail(MI_HIP_E_INVALID, "need at least one item");
+  return run_tree(items, masks, n_items, static_cast<hipStream_t>(stream), workspace_of(&items[0]));
 }
 
 int mi_hip_attn_decode_batch_noalloc(const mi_hip_attn_args* items, int n_items, void* stream) {
@@ -1336,10 +1599,13 @@ int mi_hip_attn_decode_batch_noalloc(const mi_hip_attn_args* items, int n_items,
     if ((rc = resolve_kv(&items[i], &r))) return rc;
     if ((rc = check_problem(&items[i], r))) return rc;
     if (items[i].n_tokens != 1) return fail(MI_HIP_E_INVALID, "item %d: n_tokens must be 1", i);
-    if (r.head_dim != r0.head_dim || r.f16 != r0.f16 || r.n_head_kv != r0.n_head_kv ||
+    if (r.head_dim != r0.head_dim || r.f16 != r0.f16 || r.q8 != r0.q8 || r.n_head_kv != r0.n_head_kv ||
         items[i].n_rep != items[0].n_rep || items[i].scale != items[0].scale)
       return fail(MI_HIP_E_INVALID, "item %d: shape, type or scale differs from item 0", i);
   }
+  if (r0.q8)
+    return fail(MI_HIP_E_UNSUPPORTED, "an 8-bit cache's records do not fit the static scratch: use "
+                                      "mi_hip_attn_decode_batch, which does not allocate either");
   if ((rc = bind_device())) return rc;
   // run_decode refuses launches beyond the scratch's groups or record bytes.
   return run_decode(items, n_items, static_cast<hipStream_t>(stream), g.scratch_ws);
@@ -1454,6 +1720,28 @@ int mi_hip_rope_append(const mi_hip_rope_args* a) {
   if (!strides4(a->k_nb) || !strides4(a->v_nb))
     return fail(MI_HIP_E_INVALID, "K/V strides must be multiples of 4 bytes");
   if (a->n_tokens == 0) return MI_HIP_OK;
+  if (kv->q8()) {
+    mi_hip_norm_rope_args n{};
+    n.kv = a->kv;
+    n.layer = a->layer;
+    n.n_past = a->n_past;
+    n.n_tokens = a->n_tokens;
+    n.n_dims = a->n_dims;
+    n.freq_base = a->freq_base;
+    n.n_head = a->n_head;
+    n.q = a->q;
+    n.q_out = a->q_out;
+    n.k = a->k;
+    n.v = a->v;
+    for (int i = 0; i < 3; ++i) {
+      n.q_nb[i] = a->q_nb[i];
+      n.q_out_nb[i] = a->q_out_nb[i];
+      n.k_nb[i] = a->k_nb[i];
+      n.v_nb[i] = a->v_nb[i];
+    }
+    n.stream = a->stream;
+    return mi_hip_norm_rope_append(&n);
+  }
   mi::RopeAppend p{};
   p.q = reinterpret_cast<const char*>(a->q);
   p.q_out = reinterpret_cast<char*>(a->q_out);
@@ -1479,6 +1767,114 @@ int mi_hip_rope_append(const mi_hip_rope_args* a) {
   if ((rc = bind_device())) return rc;
   hipError_t e = mi::launch_rope_append(p, kv->elt == 2, static_cast<hipStream_t>(a->stream));
   return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "rope append launch");
+}
+
+int mi_hip_norm_rope_append(const mi_hip_norm_rope_args* a) {
+  if (!a || !a->kv || !a->k || !a->v) return fail(MI_HIP_E_INVALID, "args, kv, k and v must be non-NULL");
+  const mi_hip_kv* kv = a->kv;
+  if (a->layer < 0 || a->layer >= kv->d.n_layer)
+    return fail(MI_HIP_E_INVALID, "layer %d out of range [0, %d)", a->layer, kv->d.n_layer);
+  if (a->n_past < 0 || a->n_tokens < 0 || (int64_t)a->n_past + a->n_tokens > kv->d.n_ctx)
+    return fail(MI_HIP_E_INVALID, "rows [%d, %lld) outside [0, %d)", a->n_past, (long long)a->n_past + a->n_tokens,
+                kv->d.n_ctx);
+  int rc;
+  if ((rc = check_rope_dims(a->n_dims, kv->d.head_dim))) return rc;
+  if ((a->q_norm || a->k_norm) && !(a->eps >= 0.f && std::isfinite(a->eps)))
+    return fail(MI_HIP_E_INVALID, "eps must be finite and >= 0");
+  if (a->q) {
+    if (!a->q_out) return fail(MI_HIP_E_INVALID, "q_out is NULL");
+    if (a->n_head <= 0 || a->n_head % kv->d.n_head_kv)
+      return fail(MI_HIP_E_INVALID, "n_head %d must be a positive multiple of n_head_kv %d", a->n_head,
+                  kv->d.n_head_kv);
+    if (!strides4(a->q_nb) || !strides4(a->q_out_nb))
+      return fail(MI_HIP_E_INVALID, "Q strides must be multiples of 4 bytes");
+  }
+  if (!strides4(a->k_nb) || !strides4(a->v_nb))
+    return fail(MI_HIP_E_INVALID, "K/V strides must be multiples of 4 bytes");
+  for (const void* x : {(const void*)a->q, (const void*)a->q_out, (const void*)a->k, (const void*)a->v,
+                        (const void*)a->pos, (const void*)a->q_norm, (const void*)a->k_norm})
+    if (!aligned(x, 4)) return fail(MI_HIP_E_INVALID, "device pointers must be 4-byte aligned");
+  if (a->n_tokens == 0) return MI_HIP_OK;
+  mi::NormRope p{};
+  p.q = reinterpret_cast<const char*>(a->q);
+  p.q_out = reinterpret_cast<char*>(a->q_out);
+  p.k = reinterpret_cast<const char*>(a->k);
+  p.v = reinterpret_cast<const char*>(a->v);
+  p.pos = a->pos;
+  p.q_norm = a->q_norm;
+  p.k_norm = a->k_norm;
+  p.cache = kv->view(a->layer);
+  for (int i = 0; i < 3; ++i) {
+    p.q_nb[i] = (int64_t)a->q_nb[i];
+    p.qo_nb[i] = (int64_t)a->q_out_nb[i];
+    p.k_nb[i] = (int64_t)a->k_nb[i];
+    p.v_nb[i] = (int64_t)a->v_nb[i];
+  }
+  p.n_tokens = a->n_tokens;
+  p.n_head = a->q ? a->n_head : 0;
+  p.n_past = a->n_past;
+  p.n_dims = a->n_dims;
+  p.eps = a->eps;
+  if (a->freq) std::copy(a->freq, a->freq + a->n_dims / 2, p.freq);
+  else rope_freqs(p.freq, a->n_dims, a->freq_base);
+  if ((rc = bind_device())) return rc;
+  hipError_t e = mi::launch_norm_rope(p, static_cast<hipStream_t>(a->stream));
+  return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "norm rope append launch");
+}
+
+int mi_hip_logits_adjust(const mi_hip_logits_args* a) {
+  if (!a || !a->logits || !a->out) return fail(MI_HIP_E_INVALID, "args, logits and out must be non-NULL");
+  if (a->n_vocab <= 0 || a->n_rows < 0) return fail(MI_HIP_E_INVALID, "n_vocab must be positive and n_rows >= 0");
+  if (a->n_vocab > INT32_MAX - (1 << 16)) return fail(MI_HIP_E_UNSUPPORTED, "n_vocab %d", a->n_vocab);
+  if (a->nb % 4 || a->out_nb % 4 || !aligned(a->logits, 4) || !aligned(a->out, 4))
+    return fail(MI_HIP_E_INVALID, "logits, out and their row strides must be multiples of 4 bytes");
+  const size_t row = 4 * (size_t)a->n_vocab;
+  if (a->n_rows > 1 && (a->nb < row || a->out_nb < row))
+    return fail(MI_HIP_E_INVALID, "row strides must be at least %zu bytes", row);
+  if (a->logits == a->out && a->nb != a->out_nb && a->n_rows > 1)
+    return fail(MI_HIP_E_INVALID, "in place, both row strides must be the same");
+  if ((a->hist == nullptr) != (a->hist_off == nullptr) || (a->hist && !a->penalties))
+    return fail(MI_HIP_E_INVALID, "a history needs its offsets and the rows' penalties");
+  if ((a->bias_id == nullptr) != (a->bias == nullptr) || (a->bias_id == nullptr) != (a->bias_off == nullptr))
+    return fail(MI_HIP_E_INVALID, "biases need ids, values and offsets");
+  if (a->mask && (a->mask_nb % 4 || !aligned(a->mask, 4) ||
+                  (a->mask_nb != 0 && a->mask_nb < ((size_t)a->n_vocab + 31) / 32 * 4)))
+    return fail(MI_HIP_E_INVALID, "mask rows must be 4-byte aligned and %d words apart or one for all (0)",
+                (a->n_vocab + 31) / 32);
+  for (const void* x : {(const void*)a->penalties, (const void*)a->hist, (const void*)a->hist_off,
+                        (const void*)a->bias_id, (const void*)a->bias, (const void*)a->bias_off, (const void*)a->ids})
+    if (!aligned(x, 4)) return fail(MI_HIP_E_INVALID, "device pointers must be 4-byte aligned");
+  if (a->n_rows == 0) return MI_HIP_OK;
+  int rc = bind_device();
+  if (rc) return rc;
+  mi_hip_workspace* const ws = a->ws ? a->ws : g.default_ws;
+  if (!ws) return fail(MI_HIP_E_STATE, "no workspace (the library default is gone)");
+  // as many rows a launch as their chunks' maxima have room for (and the grid)
+  const int64_t row_part = (int64_t)mi::logits_chunks(a->n_vocab) * 8;
+  const int64_t most = std::min<int64_t>(65535, a->ids ? (int64_t)ws->part_bytes / row_part : 65535);
+  if (most < 1) return fail(MI_HIP_E_UNSUPPORTED, "n_vocab %d: the workspace does not hold one row's parts", a->n_vocab);
+  mi::LogitsAdjust p{};
+  p.in_nb = (int64_t)a->nb;
+  p.out_nb = (int64_t)a->out_nb;
+  p.hist = a->hist;
+  p.bias_id = a->bias_id;
+  p.bias = a->bias;
+  p.mask_nb = (int64_t)a->mask_nb;
+  p.part = reinterpret_cast<uint64_t*>(ws->part);
+  p.n_vocab = a->n_vocab;
+  for (int64_t r = 0; r < a->n_rows; r += most) {
+    p.n_rows = (int32_t)std::min(most, a->n_rows - r);
+    p.in = reinterpret_cast<const char*>(a->logits) + r * p.in_nb;
+    p.out = reinterpret_cast<char*>(a->out) + r * p.out_nb;
+    p.penalties = a->penalties ? a->penalties + 3 * r : nullptr;
+    p.hist_off = a->hist_off ? a->hist_off + r : nullptr;
+    p.bias_off = a->bias_off ? a->bias_off + r : nullptr;
+    p.mask = a->mask ? reinterpret_cast<const char*>(a->mask) + r * p.mask_nb : nullptr;
+    p.ids = a->ids ? a->ids + r : nullptr;
+    hipError_t e = mi::launch_logits_adjust(p, static_cast<hipStream_t>(a->stream));
+    if (e != hipSuccess) return hip_fail(e, "logits launch");
+  }
+  return MI_HIP_OK;
 }
 
 int mi_hip_op_quantize_q8_0(mi_tensor* dst, void* stream) {

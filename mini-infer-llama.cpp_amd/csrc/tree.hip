@@ -1,0 +1,729 @@
+// tree.hip -- attention of several query tokens per sequence over a KV cache
+// whose last n_tokens rows are those tokens' own (a tree of drafted tokens
+// with a visibility mask, a causal chunk, or one token), F32, F16 or 8-bit
+// cache, several sequences in one launch.
+//
+// Mathematics. Query j of a sequence sees key t when t < n_past, or when bit
+// t - n_past of its mask row is set (no mask: t - n_past <= j). Its output is
+// sum_t p_t v_t / sum_t p_t with p_t = 2^(s_t - m), s_t = scale log2(e) q.k_t
+// and m the running maximum over the keys seen so far, so the keys pass once;
+// when m moves, what has been summed is rescaled by 2^(m_old - m_new). A row
+// that sees no key has m = -inf and an output of zeros.
+//
+// Decomposition. The n_tokens * n_rep query rows that read one KV head are
+// cut into row tiles of 32 RT rows (row r is token r / n_rep, head r % n_rep
+// of the group); the keys into splits of whole 32-key tiles. A workgroup owns
+// (item, KV head, row tile, split); its waves take the split's key tiles in
+// turn, every wave all of the tile's rows, so K and V come from memory once
+// per row tile and straight to registers. The waves meet in LDS; with one
+// split the result is the output, otherwise it is a record in the workspace
+// that tree_combine_kernel joins (a second launch, so that neither needs a
+// counter and both may be captured into a graph).
+//
+// Per key tile (lane = (c = lane % 32, kh = lane / 32)), 32x32 MFMAs:
+//   S^T = K . Q^T: A is K (key c), B the queries (row c); a lane ends up with
+//   the 16 keys 8 (i / 4) + 4 kh + i % 4 of row c, so the softmax runs within
+//   lanes but for one exchange between lane and lane ^ 32, and P is already
+//   the B operand of O^T += V^T . P^T. V's A operand is loaded as rows: lane
+//   (c, kh) takes the NDB = D / 32 consecutive dims NDB c .. of its 16 keys,
+//   so row c of output block db is dim NDB c + db.
+//
+// Products. F32 cache: v_mfma_f32_32x32x2f32. F16 and 8-bit caches: the cache
+// operand is exact in f16, the queries and the probabilities are f16 pairs
+// hi = RNE(x), lo = RNE(x - hi), two v_mfma_f32_32x32x16_f16 a step. So that
+// lo stays normal, each query row is scaled by the power of two that puts its
+// largest element in [2^13, 2^14) (undone in the exponent's multiply-add), and
+// the probabilities are 2^14 p (undone by the division by their sum): 2^-22
+// relative to the row's largest element.
+//   8-bit K: a row's scales (one per 32 dims) multiply the S^T of their own
+//   32 dims. 8-bit V: the row's one scale multiplies the probability, taken
+//   relative to vref, the power of two above the largest V scale so far
+//   (raised like the running maximum), so that the pair stays normal there too.
+#include <algorithm>
+
+#include "attn_common.h"
+#include "kernels.h"
+
+namespace mi {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+namespace {
+
+constexpr int kTreeWaves = 4;
+constexpr int kTreeKeys = 32;  // keys per tile
+
+// lane ^ 32's x and x itself, in some order. As asm: the compiler's builtin
+// drops one of the two results when they are used as floats. s_nop: the two
+// wait states that a VALU write of an operand needs before the swap reads it.
+__device__ inline void swap32(float x, float& a, float& b) {
+  float y = x;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  a = x;
+  b = y;
+}
+__device__ inline float max32(float x) {
+  float a, b;
+  swap32(x, a, b);
+  return fmaxf(a, b);
+}
+__device__ inline float sum32(float x) {
+  float a, b;
+  swap32(x, a, b);
+  return a + b;
+}
+
+__device__ inline u32x4 buf_b128(rsrc_t r, unsigned vo) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, vo, 0, 0));
+}
+__device__ inline u32x2 buf_b64(rsrc_t r, unsigned vo) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, vo, 0, 0));
+}
+__device__ inline unsigned buf_b32(rsrc_t r, unsigned vo) {
+  return __builtin_amdgcn_raw_buffer_load_b32(r, vo, 0, 0);
+}
+__device__ inline unsigned buf_b16(rsrc_t r, unsigned vo) {
+  return __builtin_amdgcn_raw_buffer_load_b16(r, vo, 0, 0);
+}
+__device__ inline floatx16 mfma_f16(f16x8 a, f16x8 b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx16 mfma_f32(float a, float b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+
+// Bytes i and j of (hi : lo) -- 0..3 in lo, 4..7 in hi -- as two f16 numbers
+// (b - 128) 2^-10, for bytes that hold an int8 value plus 128: as f16 bits the
+// zero-extended byte is b 2^-24, and one packed multiply-add is exact.
+template <int I, int J>
+__device__ inline f16x2 bytes_f16(unsigned hi, unsigned lo) {
+  const unsigned x = __builtin_amdgcn_perm(hi, lo, 0x0c000c00u | (unsigned)J << 16 | (unsigned)I);
+  const _Float16 up = (_Float16)16384.f, off = (_Float16)-0.125f;
+  return __builtin_bit_cast(f16x2, x) * f16x2{up, up} + f16x2{off, off};
+}
+constexpr float kByteUnscale = 1024.f;  // what the 2^-10 above takes away
+
+__device__ inline void split(float x, _Float16& hi, _Float16& lo) {
+  hi = (_Float16)x;
+  lo = (_Float16)(x - (float)hi);
+}
+
+__device__ inline bool not_finite(float x) { return (__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u; }
+// of two f16: bit 0 for the low one, bit 1 for the high one
+__device__ inline unsigned not_finite2(unsigned x) {
+  return ((x & 0x7c00u) == 0x7c00u ? 1u : 0u) | ((x & 0x7c000000u) == 0x7c000000u ? 2u : 0u);
+}
+
+}  // namespace
+
+// KT: float, _Float16 or int8_t.
+template <int D, typename KT, int RT>
+struct TreeCfg {
+  static constexpr int ELT = (int)sizeof(KT);
+  static constexpr bool Q8 = ELT == 1, F32 = ELT == 4;
+  static constexpr int NDB = D / 32;             // output blocks of 32 dims; scales per 8-bit K row
+  static constexpr int ROWS = 32 * RT;
+  static constexpr int KW = D * ELT / 8;         // 32-bit words of K per lane and tile
+  static constexpr int VW = NDB * ELT >= 4 ? NDB * ELT / 4 : 1;  // words of V per lane and key
+  static constexpr int XS = 36;                  // exchange row stride (floats)
+  static constexpr int L_X = 0;                  // waves' outputs of one 32-dim block
+  static constexpr int L_ML = kTreeWaves * ROWS * XS * 4;  // m, l per wave and row
+  static constexpr int L_VR = L_ML + kTreeWaves * ROWS * 2 * 4;  // vref per wave
+  static constexpr int LDS = L_VR + kTreeWaves * 4;
+  // While the keys stream, a wave keeps the tile's scales in its own part of
+  // the exchange area: NDB blocks of 32 K scales, then 32 V scales.
+  static constexpr int SC = (NDB + 1) * 32 * 4;
+  static_assert(SC <= ROWS * XS * 4, "scales fit a wave's exchange area");
+};
+
+template <int D, typename KT, int RT>
+__global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kernel(const TreeParams p) {
+  typedef TreeCfg<D, KT, RT> C;
+  constexpr int NDB = C::NDB, ROWS = C::ROWS, ELT = C::ELT, KW = C::KW, VW = C::VW;
+  constexpr bool Q8 = C::Q8, F32 = C::F32;
+  __shared__ __attribute__((aligned(16))) char lds_raw[C::LDS];
+  lds_t* const lds = (lds_t*)lds_raw;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int c = lane & 31, kh = lane >> 5;
+
+  // Workgroup -> (KV head, split) unit and row tile. The row tiles of a unit
+  // read the same keys, so they are numbered 8 apart: workgroups go to the 8
+  // XCDs in turn, and theirs then share an L2. Later row tiles of a causal
+  // chunk see more keys, so they come first.
+  const TreeItem& it = p.item[blockIdx.y];
+  const int n_rt = it.n_rt, n_split = it.n_split;
+  const int y = blockIdx.x / 8;
+  const int rt = n_rt - 1 - y % n_rt;
+  const int unit = (y / n_rt) * 8 + (int)(blockIdx.x % 8);
+  if (unit >= p.n_head_kv * n_split) return;
+  const int g = unit / n_split, sp = unit % n_split;
+  const int n_kv = it.n_past + it.n_tokens;
+  const int rows = it.n_tokens * p.n_rep;
+  const int row0 = rt * ROWS;
+  // keys that some row of the tile may see
+  const int last_token = min(row0 + ROWS - 1, rows - 1) / p.n_rep;
+  const int lim = it.mask ? n_kv : min(n_kv, it.n_past + last_token + 1);
+  const int tile0 = sp * it.tiles_per_split;
+  const int tile1 = min(tile0 + it.tiles_per_split, (lim + kTreeKeys - 1) / kTreeKeys);
+
+  const char* const kbase = it.k + (int64_t)g * p.k_s1;
+  const char* const vbase = it.v + (int64_t)g * p.v_s1;
+  const int ks2 = (int)p.k_s2, vs2 = (int)p.v_s2;
+
+  // ---- queries ------------------------------------------------------------
+  // Dims of B's step s, lane half kh, element j (A's are loaded the same way):
+  // F32 8 (s / 4) + 4 kh + s % 4; F16 16 s + 8 kh + j; 8-bit
+  // 32 (s / 2) + 16 kh + 8 (s % 2) + j. Each is 16 consecutive bytes of K.
+  float qf[F32 ? RT : 1][F32 ? D / 2 : 1];
+  f16x8 qh[F32 ? 1 : RT][F32 ? 1 : D / 16], ql[F32 ? 1 : RT][F32 ? 1 : D / 16];
+  float unscale[RT];
+  int token[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int r = row0 + 32 * i + c;
+    const bool valid = r < rows;
+    token[i] = valid ? r / p.n_rep : 0;
+    const int h = g * p.n_rep + (valid ? r - token[i] * p.n_rep : 0);
+    const char* const qp = reinterpret_cast<const char*>(it.q) + (int64_t)token[i] * p.q_s2 + (int64_t)h * p.q_s1;
+    const float sc = valid ? p.scale_log2e : 0.f;
+    unscale[i] = 1.f;
+    if constexpr (F32) {
+#pragma unroll
+      for (int s = 0; s < D / 2; s += 4) {
+        const f32x4 x = gload<f32x4>(qp + 4 * (2 * s + 4 * kh));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qf[i][s + j] = valid ? x[j] * sc : 0.f;
+      }
+    } else {
+      float x[D / 2];
+      float amax = 0.f;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        const int dim = Q8 ? 32 * (s / 2) + 16 * kh + 8 * (s % 2) : 16 * s + 8 * kh;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const f32x4 v = gload<f32x4>(qp + 4 * (dim + 4 * e));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[8 * s + 4 * e + j] = valid ? v[j] * sc : 0.f;
+            amax = fmaxf(amax, fabsf(x[8 * s + 4 * e + j]));
+          }
+        }
+      }
+      amax = max32(amax);
+      float f = 1.f;
+      if (amax > 0.f && amax < INFINITY) {
+        const int e = min(13 - ilogbf(amax), 100);
+        f = ldexpf(1.f, e);
+        unscale[i] = ldexpf(1.f, -e);
+      }
+      if constexpr (Q8) unscale[i] *= kByteUnscale;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          _Float16 hi, lo;
+          split(x[8 * s + j] * f, hi, lo);
+          qh[i][s][j] = hi;
+          ql[i][s][j] = lo;
+        }
+    }
+  }
+
+  // ---- state --------------------------------------------------------------
+  floatx16 o[RT][NDB];
+  float m[RT], l[RT];
+  float vref = 0x1p-24f;  // the smallest scale there is
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[i][db] = (floatx16)(0.f);
+  }
+
+  // ---- loads of a key tile --------------------------------------------------
+  // The descriptors start at the tile's first row (64-bit), so a cache of any
+  // length is addressed, and end after its last valid row: rows past n_kv
+  // read zeros.
+  unsigned kw[KW], vw[16 * VW];
+  unsigned ksc[1], ksc2[1], vsc = 0;
+  ksc[0] = ksc2[0] = 0;
+  const unsigned ko = (unsigned)(c * ks2 + 16 * kh);
+  const unsigned vo = (unsigned)(4 * kh * vs2 + c * NDB * ELT);
+  lds_t* const sc_lds = lds + wave * ROWS * C::XS * 4;
+  auto load_k = [&](int tile) __attribute__((always_inline)) {
+    const int key0 = tile * kTreeKeys;
+    const int n = min(n_kv - key0, kTreeKeys);
+    const rsrc_t r = make_rsrc(kbase + (int64_t)key0 * ks2, (unsigned)((n - 1) * ks2 + D * ELT));
+#pragma unroll
+    for (int s = 0; s < KW / 4; ++s) {
+      const u32x4 x = buf_b128(r, ko + 32 * s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) kw[4 * s + j] = x[j];
+    }
+    if constexpr (Q8) {
+      // the scales of key c: lane half kh takes half of the K row's
+      const int64_t at = (int64_t)key0 * p.n_head_kv + g;
+      const rsrc_t rk = make_rsrc(it.k_scale + at * (2 * NDB), (unsigned)((n - 1) * p.n_head_kv * 2 * NDB + 2 * NDB));
+      if constexpr (NDB == 4)
+        ksc[0] = buf_b32(rk, (unsigned)(c * p.n_head_kv * 8 + 4 * kh));
+      else
+        ksc[0] = buf_b16(rk, (unsigned)(c * p.n_head_kv * 4 + 2 * kh));
+      const rsrc_t rv = make_rsrc(it.v_scale + at * 2, (unsigned)((n - 1) * p.n_head_kv * 2 + 2));
+      vsc = buf_b16(rv, (unsigned)(c * p.n_head_kv * 2));
+    }
+  };
+  auto load_v = [&](int tile) __attribute__((always_inline)) {
+    const int key0 = tile * kTreeKeys;
+    const int n = min(n_kv - key0, kTreeKeys);
+    const rsrc_t r = make_rsrc(vbase + (int64_t)key0 * vs2, (unsigned)((n - 1) * vs2 + D * ELT));
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      const unsigned at = vo + (unsigned)((8 * (t >> 2) + (t & 3)) * vs2);
+      if constexpr (NDB * ELT == 16) {
+        const u32x4 x = buf_b128(r, at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vw[4 * t + j] = x[j];
+      } else if constexpr (NDB * ELT == 8) {
+        const u32x2 x = buf_b64(r, at);
+        vw[2 * t] = x[0];
+        vw[2 * t + 1] = x[1];
+      } else if constexpr (NDB * ELT == 4) {
+        vw[t] = buf_b32(r, at);
+      } else {
+        vw[t] = buf_b16(r, at);
+      }
+    }
+  };
+
+  int tile = tile0 + wave;
+  if (tile < tile1) {
+    load_k(tile);
+    load_v(tile);
+  }
+  for (; tile < tile1; tile += kTreeWaves) {
+    const int key0 = tile * kTreeKeys;
+    const int next = tile + kTreeWaves;
+    // ---- S^T = K . Q^T ------------------------------------------------------
+    floatx16 s[RT];
+    f32x4 pv_scale[4];  // V scales of the lane's keys times 2^14 / vref
+    float alpha_v = 1.f;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) s[i] = (floatx16)(0.f);
+    if constexpr (F32) {
+#pragma unroll
+      for (int st = 0; st < D / 2; ++st)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) s[i] = mfma_f32(__builtin_bit_cast(float, kw[st]), qf[i][st], s[i]);
+    } else if constexpr (!Q8) {
+#pragma unroll
+      for (int st = 0; st < D / 16; ++st) {
+        const f16x8 k8 = __builtin_bit_cast(f16x8, u32x4{kw[4 * st], kw[4 * st + 1], kw[4 * st + 2], kw[4 * st + 3]});
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          s[i] = mfma_f16(k8, ql[i][st], s[i]);
+          s[i] = mfma_f16(k8, qh[i][st], s[i]);
+        }
+      }
+    } else {
+      // the scales, to where each lane can read those of its own 16 keys
+      auto h2f = [](unsigned x) { return (float)__builtin_bit_cast(_Float16, (unsigned short)x); };
+      if constexpr (NDB == 4) {
+        lds_store<float>(sc_lds + (64 * kh + c) * 4, h2f(ksc[0] & 0xffffu));
+        lds_store<float>(sc_lds + (64 * kh + 32 + c) * 4, h2f(ksc[0] >> 16));
+      } else {
+        lds_store<float>(sc_lds + (32 * kh + c) * 4, h2f(ksc[0]));
+      }
+      if (kh == 0) lds_store<float>(sc_lds + (32 * NDB + c) * 4, h2f(vsc));
+      wave_lds_fence();
+#pragma unroll
+      for (int b = 0; b < NDB; ++b) {
+        floatx16 part[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) part[i] = (floatx16)(0.f);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const unsigned w0 = kw[4 * b + 2 * e] ^ 0x80808080u, w1 = kw[4 * b + 2 * e + 1] ^ 0x80808080u;
+          const f16x2 x0 = bytes_f16<0, 1>(w0, w0), x1 = bytes_f16<2, 3>(w0, w0);
+          const f16x2 x2 = bytes_f16<0, 1>(w1, w1), x3 = bytes_f16<2, 3>(w1, w1);
+          const f16x8 k8 = {x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            part[i] = mfma_f16(k8, ql[i][2 * b + e], part[i]);
+            part[i] = mfma_f16(k8, qh[i][2 * b + e], part[i]);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 sc = lds_load<f32x4>(sc_lds + (32 * b + 8 * q + 4 * kh) * 4);
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[i][4 * q + j] = fmaf(part[i][4 * q + j], sc[j], s[i][4 * q + j]);
+        }
+      }
+      float mx = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        pv_scale[q] = lds_load<f32x4>(sc_lds + (32 * NDB + 8 * q + 4 * kh) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, pv_scale[q][j] < INFINITY ? pv_scale[q][j] : 0.f);
+      }
+      mx = max32(mx);  // the same in every lane
+      if (mx > vref) {
+        const float up = ldexpf(1.f, ilogbf(mx) + 1);
+        alpha_v = vref / up;
+        vref = up;
+      }
+      const float inv = 16384.f / vref;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) pv_scale[q] *= inv;
+      wave_lds_fence();  // the scales are read before the next tile's are written
+    }
+    if (next < tile1) load_k(next);
+
+    // ---- mask -----------------------------------------------------------------
+    unsigned vis[RT];
+    const bool masked = key0 + kTreeKeys > it.n_past;  // a tile of drafted keys
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int b0 = key0 - it.n_past;  // the tile's first key as a bit of the mask row
+        unsigned v;
+        if (it.mask) {
+          const char* const mrow = it.mask + (int64_t)token[i] * it.mask_nb;
+          const int n_words = (it.n_tokens + 63) / 64;
+          if (b0 >= 0) {
+            const int w = b0 >> 6, sh = b0 & 63;
+            uint64_t x = gload<uint64_t>(mrow + 8 * (int64_t)w) >> sh;
+            if (sh > 32 && w + 1 < n_words) x |= gload<uint64_t>(mrow + 8 * (int64_t)(w + 1)) << (64 - sh);
+            v = (unsigned)x;
+          } else {
+            v = (unsigned)gload<uint64_t>(mrow) << -b0 | ((1u << -b0) - 1u);
+          }
+          const int n = n_kv - key0;
+          if (n < 32) v &= (1u << n) - 1u;
+        } else {
+          const int n = b0 < 0 ? token[i] + 1 - b0 : token[i] - b0 + 1;  // keys of the tile that the row sees
+          v = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+        }
+        vis[i] = v;
+        const unsigned mine = v >> (4 * kh);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[i][e] = mine >> (8 * (e >> 2) + (e & 3)) & 1u ? s[i][e] : -INFINITY;
+      }
+    }
+
+    // ---- softmax ------------------------------------------------------------
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      float mx = fmaxf(s[i][0], s[i][1]);
+#pragma unroll
+      for (int e = 2; e < 16; ++e) mx = fmaxf(mx, s[i][e]);
+      mx = max32(mx) * unscale[i];
+      const float mn = fmaxf(m[i], mx);
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float alpha = fast_exp2(m[i] - mu);
+      const float boost = F32 || Q8 ? mu : mu - 14.f;
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[i][e] = fast_exp2(fmaf(s[i][e], unscale[i], -boost));
+        sum += s[i][e];
+      }
+      l[i] = l[i] * alpha + sum;
+      m[i] = mn;
+      const float ao = alpha * alpha_v;
+      if (__builtin_amdgcn_ballot_w64(ao != 1.f) != 0ull) {
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) o[i][db] *= ao;
+      }
+      if constexpr (Q8) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[i][e] *= pv_scale[e >> 2][e & 3];
+        if (masked) {  // (a scale may not be finite: 0 times it is not 0)
+          const unsigned mine = vis[i] >> (4 * kh);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[i][e] = mine >> (8 * (e >> 2) + (e & 3)) & 1u ? s[i][e] : 0.f;
+        }
+      }
+    }
+
+    // ---- values that are not finite, in a tile that some rows do not see --------
+    // Their products with a masked key's probability of 0 would not be 0: they
+    // are taken as zeros, and the rows that do see them get NaN there.
+    unsigned nf[NDB];  // bit t: the lane's key t, dim NDB c + db
+    bool any_nf = false;
+    if constexpr (!Q8) {
+      if (masked) {
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) nf[db] = 0u;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            if constexpr (F32) {
+              if (not_finite(__builtin_bit_cast(float, vw[VW * t + w]))) {
+                nf[w] |= 1u << t;
+                vw[VW * t + w] = 0u;
+              }
+            } else {
+              const unsigned b = not_finite2(vw[VW * t + w]);
+              nf[2 * w] |= (b & 1u) << t;
+              nf[2 * w + 1] |= (b >> 1) << t;
+              vw[VW * t + w] &= (b & 1u ? 0u : 0xffffu) | (b & 2u ? 0u : 0xffff0000u);
+            }
+          }
+        }
+        unsigned all = 0u;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) all |= nf[db];
+        any_nf = __builtin_amdgcn_ballot_w64(all != 0u) != 0ull;
+      }
+    }
+
+    // ---- O^T += V^T . P^T -----------------------------------------------------
+    if constexpr (F32) {
+#pragma unroll
+      for (int t = 0; t < 16; ++t)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+            o[i][db] = mfma_f32(__builtin_bit_cast(float, vw[VW * t + db]), s[i][t], o[i][db]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f16x8 ph[RT], pl[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            _Float16 hi, lo;
+            split(s[i][8 * u + j], hi, lo);
+            ph[i][j] = hi;
+            pl[i][j] = lo;
+          }
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          f16x8 v8;
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const int t = 8 * u + j;
+            f16x2 x;
+            if constexpr (Q8) {
+              const unsigned w0 = vw[t] ^ 0x80808080u, w1 = vw[t + 1] ^ 0x80808080u;
+              x = db == 0 ? bytes_f16<0, 4>(w1, w0) : db == 1 ? bytes_f16<1, 5>(w1, w0)
+                : db == 2 ? bytes_f16<2, 6>(w1, w0) : bytes_f16<3, 7>(w1, w0);
+            } else {
+              const unsigned w0 = vw[VW * t + db / 2], w1 = vw[VW * (t + 1) + db / 2];
+              x = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(w1, w0, db & 1 ? 0x07060302u : 0x05040100u));
+            }
+            v8[j] = x[0];
+            v8[j + 1] = x[1];
+          }
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            o[i][db] = mfma_f16(v8, pl[i], o[i][db]);
+            o[i][db] = mfma_f16(v8, ph[i], o[i][db]);
+          }
+        }
+      }
+    }
+    if constexpr (!Q8) {
+      if (masked && any_nf) {
+        for (int src = 0; src < kWave; ++src) {  // the lane that holds the values
+          const int sc = src & 31, sh = src >> 5;
+          unsigned bits[NDB], some = 0u;
+#pragma unroll
+          for (int db = 0; db < NDB; ++db) {
+            bits[db] = (unsigned)__builtin_amdgcn_readlane((int)nf[db], src);
+            some |= bits[db];
+          }
+          if (some == 0u) continue;
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            const unsigned x = vis[i] >> (4 * sh);  // the row's sight of that lane's keys, bit t
+            const unsigned seen = (x & 0xfu) | (x >> 4 & 0xf0u) | (x >> 8 & 0xf00u) | (x >> 12 & 0xf000u);
+#pragma unroll
+            for (int db = 0; db < NDB; ++db)
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if ((bits[db] & seen) != 0u && 8 * (e >> 2) + 4 * kh + (e & 3) == sc) o[i][db][e] = NAN;
+          }
+        }
+      }
+    }
+    if (next < tile1) load_v(next);
+  }
+
+  // ---- the waves' parts ---------------------------------------------------------
+  wave_lds_fence();
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const float lt = sum32(l[i]);
+    if (kh == 0) {
+      lds_store<float>(lds + C::L_ML + ((wave * ROWS + 32 * i + c) * 2) * 4, m[i]);
+      lds_store<float>(lds + C::L_ML + ((wave * ROWS + 32 * i + c) * 2 + 1) * 4, lt);
+    }
+  }
+  __syncthreads();
+  // 8-bit: O holds 2^14 / vref of the sum (and 2^-10 of the bytes' values)
+  const float unit_o = Q8 ? vref * (kByteUnscale / 16384.f) : 1.f;
+  float mt[RT], lt[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    mt[i] = -INFINITY;
+    lt[i] = 0.f;
+    f32x2 ml[kTreeWaves];
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; ++w) {
+      ml[w] = lds_load<f32x2>(lds + C::L_ML + ((w * ROWS + 32 * i + c) * 2) * 4);
+      mt[i] = fmaxf(mt[i], ml[w][0]);
+    }
+    const float mu = mt[i] == -INFINITY ? 0.f : mt[i];
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; ++w) lt[i] += ml[w][1] * fast_exp2(ml[w][0] - mu);
+    const float wt = fast_exp2(m[i] - mu) * unit_o;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[i][db] *= wt;
+  }
+  // One 32-dim block at a time through LDS; thread (row pr, column cc) sums the
+  // waves' parts of its columns.
+  constexpr int PER = ROWS * 32 / (kTreeWaves * kWave);  // (row, column) pairs per thread
+  float acc[PER][NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) {
+    if (db > 0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        lds_store<f32x4>(lds + ((wave * ROWS + 32 * i + c) * C::XS + 8 * q + 4 * kh) * 4,
+                         f32x4{o[i][db][4 * q], o[i][db][4 * q + 1], o[i][db][4 * q + 2], o[i][db][4 * q + 3]});
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const int idx = e * kTreeWaves * kWave + threadIdx.x;
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < kTreeWaves; ++w)
+        x += lds_load<float>(lds + ((w * ROWS + idx / 32) * C::XS + idx % 32) * 4);
+      acc[e][db] = x;
+    }
+  }
+  if (n_split > 1) {
+    // record: ROWS rows of D, then m, then l
+    float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * n_rt + rt) * n_split + sp) * (ROWS * (D + 2));
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const int idx = e * kTreeWaves * kWave + threadIdx.x;
+      float* const w = rec + (int64_t)(idx / 32) * D + NDB * (idx % 32);
+      if constexpr (NDB == 4) gstore(w, f32x4{acc[e][0], acc[e][1], acc[e][2], acc[e][3]});
+      else gstore(w, f32x2{acc[e][0], acc[e][1]});
+    }
+    if (wave == 0 && kh == 0) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        rec[ROWS * D + 32 * i + c] = mt[i];
+        rec[ROWS * D + ROWS + 32 * i + c] = lt[i];
+      }
+    }
+    return;
+  }
+  // the rows' sums to where the storing threads read them
+  if (wave == 0 && kh == 0) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i) lds_store<float>(lds + C::L_ML + (32 * i + c) * 4, mt[i] == -INFINITY ? 0.f : 1.f / lt[i]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int idx = e * kTreeWaves * kWave + threadIdx.x;
+    const int r = row0 + idx / 32;
+    if (r >= rows) continue;
+    const float inv = lds_load<float>(lds + C::L_ML + (idx / 32) * 4);
+    const int t = r / p.n_rep, h = g * p.n_rep + r % p.n_rep;
+    char* const w = reinterpret_cast<char*>(it.out) + (int64_t)t * p.o_s2 + (int64_t)h * p.o_s1 + 4 * NDB * (idx % 32);
+    if constexpr (NDB == 4) gstore(w, f32x4{acc[e][0] * inv, acc[e][1] * inv, acc[e][2] * inv, acc[e][3] * inv});
+    else gstore(w, f32x2{acc[e][0] * inv, acc[e][1] * inv});
+  }
+}
+
+// Joins the splits' records of a row: out = sum_s 2^(m_s - M) O_s / sum_s
+// 2^(m_s - M) l_s. D / 4 threads a row, four dims each; the records were just
+// written and are read once, from the caches.
+template <int D>
+__global__ __launch_bounds__(256) void tree_combine_kernel(const TreeParams p, int tile_rows) {
+  const TreeItem& it = p.item[blockIdx.y];
+  const int rows = it.n_tokens * p.n_rep, n_split = it.n_split;
+  const int idx = blockIdx.x * 256 + threadIdx.x;
+  const int row = idx / (D / 4), d4 = idx % (D / 4);  // row over the KV heads
+  if (n_split <= 1 || row >= rows * p.n_head_kv) return;
+  const int g = row / rows, r = row % rows;
+  const int64_t rec_floats = (int64_t)tile_rows * (D + 2);
+  const float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * it.n_rt + r / tile_rows) * n_split) * rec_floats;
+  const int rr = r % tile_rows;
+  float mx = -INFINITY;
+  for (int s = 0; s < n_split; ++s) mx = fmaxf(mx, gload<float>(rec + s * rec_floats + tile_rows * D + rr));
+  const float mu = mx == -INFINITY ? 0.f : mx;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  for (int s = 0; s < n_split; ++s) {
+    const float* const q = rec + s * rec_floats;
+    const float w = fast_exp2(gload<float>(q + tile_rows * D + rr) - mu);
+    l += w * gload<float>(q + tile_rows * (D + 1) + rr);
+    acc += w * gload<f32x4>(q + rr * D + 4 * d4);
+  }
+  const float inv = mx == -INFINITY ? 0.f : 1.f / l;
+  const int t = r / p.n_rep, h = g * p.n_rep + r % p.n_rep;
+  gstore(reinterpret_cast<char*>(it.out) + (int64_t)t * p.o_s2 + (int64_t)h * p.o_s1 + 16 * d4, acc * inv);
+}
+
+int tree_tile_rows(int rows) { return rows > 32 ? 64 : 32; }
+
+size_t tree_record_floats(int head_dim, int tile_rows) { return (size_t)tile_rows * (head_dim + 2); }
+
+template <int D, typename KT, int RT>
+static hipError_t launch_tree_t(const TreeParams& p, int n_items, hipStream_t stream) {
+  unsigned gx = 0, cx = 0;
+  for (int i = 0; i < n_items; ++i) {
+    const TreeItem& it = p.item[i];
+    const unsigned units = (unsigned)p.n_head_kv * it.n_split;
+    gx = std::max(gx, (units + 7) / 8 * 8 * (unsigned)it.n_rt);
+    if (it.n_split > 1)
+      cx = std::max(cx, ((unsigned)it.n_tokens * p.n_rep * p.n_head_kv * (D / 4) + 255) / 256);
+  }
+  hipLaunchKernelGGL((tree_kernel<D, KT, RT>), dim3(gx, n_items), dim3(kTreeWaves * kWave), 0, stream, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || cx == 0) return e;
+  hipLaunchKernelGGL((tree_combine_kernel<D>), dim3(cx, n_items), dim3(256), 0, stream, p, 32 * RT);
+  return hipGetLastError();
+}
+
+template <int D, typename KT>
+static hipError_t launch_tree_d(const TreeParams& p, int n_items, int tile_rows, hipStream_t stream) {
+  return tile_rows == 64 ? launch_tree_t<D, KT, 2>(p, n_items, stream) : launch_tree_t<D, KT, 1>(p, n_items, stream);
+}
+
+hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, hipStream_t stream) {
+  if (head_dim == 64)
+    return elt == 1   ? launch_tree_d<64, int8_t>(p, n_items, tile_rows, stream)
+           : elt == 2 ? launch_tree_d<64, _Float16>(p, n_items, tile_rows, stream)
+                      : launch_tree_d<64, float>(p, n_items, tile_rows, stream);
+  if (head_dim == 128)
+    return elt == 1   ? launch_tree_d<128, int8_t>(p, n_items, tile_rows, stream)
+           : elt == 2 ? launch_tree_d<128, _Float16>(p, n_items, tile_rows, stream)
+                      : launch_tree_d<128, float>(p, n_items, tile_rows, stream);
+  return hipErrorInvalidValue;
+}
+
+}  // namespace mi

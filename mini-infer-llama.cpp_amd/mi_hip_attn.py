@@ -15,6 +15,7 @@ MI_TYPE_F32 = 0
 MI_TYPE_F16 = 1
 MI_TYPE_Q8_0 = 2
 MI_TYPE_Q8_0_ACT = 4
+MI_HIP_TYPE_Q8 = 100  # cache elements only
 
 MI_OP_NONE = 0
 MI_OP_MUL_MAT = 5
@@ -143,6 +144,58 @@ class RopeArgs(ctypes.Structure):
     ]
 
 
+class NormRopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("kv", ctypes.c_void_p),
+        ("layer", ctypes.c_int32),
+        ("n_past", ctypes.c_int32),
+        ("n_tokens", ctypes.c_int32),
+        ("n_dims", ctypes.c_int32),
+        ("freq_base", ctypes.c_float),
+        ("freq", ctypes.POINTER(ctypes.c_float)),
+        ("pos", ctypes.c_void_p),
+        ("eps", ctypes.c_float),
+        ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p),
+        ("n_head", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("q_nb", ctypes.c_size_t * 3),
+        ("q_out", ctypes.c_void_p),
+        ("q_out_nb", ctypes.c_size_t * 3),
+        ("k", ctypes.c_void_p),
+        ("k_nb", ctypes.c_size_t * 3),
+        ("v", ctypes.c_void_p),
+        ("v_nb", ctypes.c_size_t * 3),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class TreeMask(ctypes.Structure):
+    _fields_ = [("bits", ctypes.c_void_p), ("nb", ctypes.c_size_t)]
+
+
+class LogitsArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("nb", ctypes.c_size_t),
+        ("out", ctypes.c_void_p),
+        ("out_nb", ctypes.c_size_t),
+        ("n_vocab", ctypes.c_int32),
+        ("n_rows", ctypes.c_int32),
+        ("penalties", ctypes.c_void_p),
+        ("hist", ctypes.c_void_p),
+        ("hist_off", ctypes.c_void_p),
+        ("bias_id", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("bias_off", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("mask_nb", ctypes.c_size_t),
+        ("ids", ctypes.c_void_p),
+        ("ws", ctypes.c_void_p),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
 class Qwen2Hparams(ctypes.Structure):
     """ABI mirror of mi_hip_qwen2_hparams (include/mi_hip_qwen2.h)."""
     _fields_ = [("n_vocab", ctypes.c_int32), ("n_embd", ctypes.c_int32),
@@ -183,11 +236,16 @@ SIGNATURES = {
     "mi_hip_kv_view": ([_P, _I, _I, ctypes.POINTER(ctypes.c_void_p),
                         ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_size_t)], _I),
     "mi_hip_kv_write": ([_P, _I, _I, _I, _I, _P, ctypes.POINTER(ctypes.c_size_t), _I, _P], _I),
+    "mi_hip_kv_scales": ([_P, _I, _I, ctypes.POINTER(ctypes.c_void_p),
+                          ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_size_t)], _I),
+    "mi_hip_kv_read": ([_P, _I, _I, _I, _I, _P, _I, ctypes.POINTER(ctypes.c_size_t), _P], _I),
+    "mi_hip_kv_keep": ([_P, _I, _P, _I, _P], _I),
     "mi_hip_kv_bind": ([_P, _I, _I, ctypes.POINTER(MiTensor)], _I),
     "mi_hip_attn_fwd": ([ctypes.POINTER(AttnArgs)], _I),
     "mi_hip_attn_fwd_reference_order": ([ctypes.POINTER(AttnArgs)], _I),
     "mi_hip_attn_decode_batch": ([ctypes.POINTER(AttnArgs), _I, _P], _I),
     "mi_hip_attn_decode_batch_noalloc": ([ctypes.POINTER(AttnArgs), _I, _P], _I),
+    "mi_hip_attn_tree": ([ctypes.POINTER(AttnArgs), ctypes.POINTER(TreeMask), _I, _P], _I),
     "mi_hip_op_attn_qk": ([ctypes.POINTER(MiTensor), _P], _I),
     "mi_hip_op_softmax": ([ctypes.POINTER(MiTensor), _P], _I),
     "mi_hip_op_attn_kqv": ([ctypes.POINTER(MiTensor), _P], _I),
@@ -196,6 +254,8 @@ SIGNATURES = {
     "mi_hip_op_quantize_q8_0": ([ctypes.POINTER(MiTensor), _P], _I),
     "mi_hip_op_mul_mat": ([ctypes.POINTER(MiTensor), _P], _I),
     "mi_hip_rope_append": ([ctypes.POINTER(RopeArgs)], _I),
+    "mi_hip_norm_rope_append": ([ctypes.POINTER(NormRopeArgs)], _I),
+    "mi_hip_logits_adjust": ([ctypes.POINTER(LogitsArgs)], _I),
     "mi_hip_memread": ([_P, ctypes.c_size_t, _P, ctypes.c_int32, _P], _I),
     "mi_hip_graph_prepare": ([ctypes.POINTER(MiCgraph)], _I),
     "mi_hip_compute_forward": ([ctypes.POINTER(MiTensor), _I, _I], _I),
@@ -282,6 +342,28 @@ class Lib:
         self.check(self.so.mi_hip_kv_view(kv, layer, which, ctypes.byref(data), ne, nb))
         return data.value, list(ne), list(nb)
 
+    def kv_scales(self, kv, layer, which):
+        data = ctypes.c_void_p()
+        ne = (ctypes.c_int64 * 4)()
+        nb = (ctypes.c_size_t * 4)()
+        self.check(self.so.mi_hip_kv_scales(kv, layer, which, ctypes.byref(data), ne, nb))
+        return data.value, list(ne), list(nb)
+
+    def kv_write(self, kv, layer, which, pos0, src, stream):
+        """Rows of an F32 device tensor (n_tokens, n_head_kv, head_dim) into K (which 0) or V (1)."""
+        self.check(self.so.mi_hip_kv_write(kv, layer, which, pos0, src.shape[0], src.data_ptr(),
+                                           (ctypes.c_size_t * 3)(*nb3_of(src)), 1, stream))
+
+    def kv_read(self, kv, layer, which, pos0, dst, stream):
+        """Cache rows into a device tensor (n_tokens, n_head_kv, head_dim), F32 or F16."""
+        kind = MI_TYPE_F16 if dst.element_size() == 2 else MI_TYPE_F32
+        self.check(self.so.mi_hip_kv_read(kv, layer, which, pos0, dst.shape[0], dst.data_ptr(), kind,
+                                          (ctypes.c_size_t * 3)(*nb3_of(dst)), stream))
+
+    def kv_keep(self, kv, n_past, idx, stream):
+        """Rows n_past + idx[i] become rows n_past + i (idx: whole numbers on the host, increasing)."""
+        self.check(self.so.mi_hip_kv_keep(kv, n_past, (ctypes.c_int32 * len(idx))(*idx), len(idx), stream))
+
 
 _lib = None
 
@@ -346,6 +428,61 @@ def rope_args(kv, layer, n_past, n_dims, freq_base, stream, k, v, q=None, q_out=
         a.q_out_nb[:] = nb3_of(q_out)
         a.n_head = q.shape[1]
     a.stream = stream
+    return a
+
+
+def norm_rope_args(kv, layer, n_past, n_dims, freq_base, stream, k, v, q=None, q_out=None, pos=None, freq=None,
+                   q_norm=None, k_norm=None, eps=0.0):
+    """Builds NormRopeArgs from torch tensors as rope_args does; pos (n_tokens, int32) and the
+    norms' weights (head_dim) are device tensors, freq n_dims / 2 floats on the host."""
+    a = NormRopeArgs()
+    a.kv, a.layer, a.n_past, a.n_dims = kv, layer, n_past, n_dims
+    a.freq_base, a.eps = freq_base, eps
+    a.n_tokens = k.shape[0]
+    a.k, a.v = k.data_ptr(), v.data_ptr()
+    a.k_nb[:] = nb3_of(k)
+    a.v_nb[:] = nb3_of(v)
+    if freq is not None:
+        a.freq = (ctypes.c_float * len(freq))(*freq)
+    for name, t in (("pos", pos), ("q_norm", q_norm), ("k_norm", k_norm)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    if q is not None:
+        q_out = q if q_out is None else q_out
+        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+        a.q_nb[:] = nb3_of(q)
+        a.q_out_nb[:] = nb3_of(q_out)
+        a.n_head = q.shape[1]
+    a.stream = stream
+    return a
+
+
+def tree_masks(bits):
+    """An array of TreeMask from one device tensor of 64-bit words (n_tokens, words) per item, or
+    None for an item whose tokens are a chain."""
+    return (TreeMask * len(bits))(*[TreeMask() if b is None else TreeMask(b.data_ptr(), b.stride(0) * 8)
+                                    for b in bits])
+
+
+def logits_args(logits, out, stream, penalties=None, hist=None, hist_off=None, bias_id=None, bias=None,
+                bias_off=None, mask=None, ids=None, ws=None):
+    """Builds LogitsArgs from device tensors: logits and out (n_rows, n_vocab), penalties
+    (n_rows, 3), int32 lists and offsets, mask (n_rows, words) of 32 bits or one row for all."""
+    a = LogitsArgs()
+    a.n_rows, a.n_vocab = logits.shape
+    a.logits, a.nb = logits.data_ptr(), logits.stride(0) * 4
+    a.out, a.out_nb = out.data_ptr(), out.stride(0) * 4
+    for name, t in (("penalties", penalties), ("hist", hist), ("hist_off", hist_off), ("bias_id", bias_id),
+                    ("bias", bias), ("bias_off", bias_off), ("mask", mask), ("ids", ids)):
+        if t is not None and (t.numel() > 0 or name.endswith("_off")):
+            setattr(a, name, t.data_ptr())
+    if mask is not None:
+        a.mask_nb = mask.stride(0) * 4 if mask.shape[0] > 1 else 0
+    if not a.hist:
+        a.hist_off = None
+    if not a.bias_id:
+        a.bias_off = a.bias = None
+    a.ws, a.stream = ws, stream
     return a
 
 
