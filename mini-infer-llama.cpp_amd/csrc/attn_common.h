@@ -105,6 +105,7 @@ struct PrefillParams {
 // over the keys that are theirs.
 // ---------------------------------------------------------------------------
 constexpr int kTreeMaxItems = 32;  // items per launch (they ride in kernarg)
+constexpr int kTreeTile = 32;      // keys per tile
 
 struct TreeItem {
   const char* k;        // layer's K and V (8-bit caches: the int8 values)
@@ -118,7 +119,7 @@ struct TreeItem {
   int32_t n_past, n_tokens;
   int32_t n_rt;             // row tiles per KV head
   int32_t n_split;          // key splits (1: no records, the kernel writes the output)
-  int32_t tiles_per_split;  // 32-key tiles
+  int32_t tiles_per_split;  // key tiles (an even number where there is more than one split)
   int32_t rec0;             // the item's first record
 };
 

@@ -88,11 +88,14 @@ hipError_t launch_rope_append(const RopeAppend& p, bool f16, hipStream_t stream)
 
 // tree.hip. Query rows per row tile for `rows` rows per KV head, and the
 // floats of one record (a row tile's part from one split).
-int tree_tile_rows(int rows);
+int tree_tile_rows(int rows, int elt);
 size_t tree_record_floats(int head_dim, int tile_rows);
 // elt: bytes of a cache element (4 F32, 2 F16, 1 8-bit). Every item's n_rt is
 // in tiles of tile_rows.
 hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, hipStream_t stream);
+
+// tree_wide.hip: the kernel for tiles of 128 rows (F16 and 8-bit caches).
+hipError_t launch_tree_wide(const TreeParams& p, dim3 grid, int head_dim, int elt, hipStream_t stream);
 
 // kv8.hip -- rows on their way into and out of a cache.
 // A layer's K and V of a cache: element type by elt (4 F32, 2 F16, 1 8-bit

@@ -375,10 +375,10 @@ size_t ws_total_bytes(int groups, size_t rec_bytes, size_t part_bytes) {
 }
 
 // Bytes of parts that let a tree-attention launch split its keys over
-// kTreeWgPerCu workgroups per CU (see plan_tree), each with a record of 64 rows.
+// kTreeWgPerCu workgroups per CU (see plan_tree), each with a record of up to 128 rows.
 constexpr int kTreeWgPerCu = 2;
 size_t ws_part_bytes(int head_dim) {
-  return (size_t)kTreeWgPerCu * g.n_cu * mi::tree_record_floats(head_dim, 64) * sizeof(float);
+  return (size_t)kTreeWgPerCu * g.n_cu * mi::tree_record_floats(head_dim, 128) * sizeof(float);
 }
 
 // Lays a workspace over [base, base + bytes).
@@ -793,7 +793,8 @@ void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int tile_rows, size
         r += (int64_t)p.n_head_kv * p.item[i].n_rt * ((tiles_of(p.item[i]) + n - 1) / n);
       return r;
     };
-    while (per < longest && records(per) > std::min(want, cap)) per += std::max<int64_t>(1, per / 16);
+    per += per & 1;  // whole 64-key tiles
+    while (per < longest && records(per) > std::min(want, cap)) per += std::max<int64_t>(1, per / 32) * 2;
     if (records(per) > cap) per = longest;
   }
   int64_t rec = 0;
@@ -873,7 +874,7 @@ int run_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* masks, int n
       }
       most = std::max(most, a->n_tokens * a->n_rep);
     }
-    const int tile_rows = mi::tree_tile_rows(most);
+    const int tile_rows = mi::tree_tile_rows(most, elt);
     plan_tree(p, cnt, r0.head_dim, tile_rows, ws->part_bytes);
     hipError_t e = mi::launch_tree(p, cnt, r0.head_dim, elt, tile_rows, stream);
     if (e != hipSuccess) return hip_fail(e, "tree attention launch");
@@ -1072,7 +1073,7 @@ int mi_hip_init(int device) {
   g.knobs.stream_min = env_int("MI_HIP_DECODE_STREAM_MIN", 0);
   g.ready = true;
   // The default workspace: head_dim up to 128, groups of up to 8 heads, up to
-  // 1024 groups per launch (e.g. 32 items x 32 KV heads), ~11 MB, and 17 MB of
+  // 1024 groups per launch (e.g. 32 items x 32 KV heads), ~11 MB, and 34 MB of
   // parts.
   const int groups = 1024;
   const size_t rec = (size_t)(g.n_cu + groups) * mi::decode_record_floats(128, 8) * sizeof(float);

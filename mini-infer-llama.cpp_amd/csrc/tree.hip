@@ -43,84 +43,9 @@
 
 #include "attn_common.h"
 #include "kernels.h"
+#include "tree_common.h"
 
 namespace mi {
-
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-
-namespace {
-
-constexpr int kTreeWaves = 4;
-constexpr int kTreeKeys = 32;  // keys per tile
-
-// lane ^ 32's x and x itself, in some order. As asm: the compiler's builtin
-// drops one of the two results when they are used as floats. s_nop: the two
-// wait states that a VALU write of an operand needs before the swap reads it.
-__device__ inline void swap32(float x, float& a, float& b) {
-  float y = x;
-  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
-  a = x;
-  b = y;
-}
-__device__ inline float max32(float x) {
-  float a, b;
-  swap32(x, a, b);
-  return fmaxf(a, b);
-}
-__device__ inline float sum32(float x) {
-  float a, b;
-  swap32(x, a, b);
-  return a + b;
-}
-
-__device__ inline u32x4 buf_b128(rsrc_t r, unsigned vo) {
-  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, vo, 0, 0));
-}
-__device__ inline u32x2 buf_b64(rsrc_t r, unsigned vo) {
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, vo, 0, 0));
-}
-__device__ inline unsigned buf_b32(rsrc_t r, unsigned vo) {
-  return __builtin_amdgcn_raw_buffer_load_b32(r, vo, 0, 0);
-}
-__device__ inline unsigned buf_b16(rsrc_t r, unsigned vo) {
-  return __builtin_amdgcn_raw_buffer_load_b16(r, vo, 0, 0);
-}
-__device__ inline floatx16 mfma_f16(f16x8 a, f16x8 b, floatx16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-__device__ inline floatx16 mfma_f32(float a, float b, floatx16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
-}
-
-// Bytes i and j of (hi : lo) -- 0..3 in lo, 4..7 in hi -- as two f16 numbers
-// (b - 128) 2^-10, for bytes that hold an int8 value plus 128: as f16 bits the
-// zero-extended byte is b 2^-24, and one packed multiply-add is exact.
-template <int I, int J>
-__device__ inline f16x2 bytes_f16(unsigned hi, unsigned lo) {
-  const unsigned x = __builtin_amdgcn_perm(hi, lo, 0x0c000c00u | (unsigned)J << 16 | (unsigned)I);
-  const _Float16 up = (_Float16)16384.f, off = (_Float16)-0.125f;
-  return __builtin_bit_cast(f16x2, x) * f16x2{up, up} + f16x2{off, off};
-}
-constexpr float kByteUnscale = 1024.f;  // what the 2^-10 above takes away
-
-__device__ inline void split(float x, _Float16& hi, _Float16& lo) {
-  hi = (_Float16)x;
-  lo = (_Float16)(x - (float)hi);
-}
-
-__device__ inline bool not_finite(float x) { return (__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u; }
-// of two f16: bit 0 for the low one, bit 1 for the high one
-__device__ inline unsigned not_finite2(unsigned x) {
-  return ((x & 0x7c00u) == 0x7c00u ? 1u : 0u) | ((x & 0x7c000000u) == 0x7c000000u ? 2u : 0u);
-}
-
-}  // namespace
 
 // KT: float, _Float16 or int8_t.
 template <int D, typename KT, int RT>
@@ -171,7 +96,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
   const int last_token = min(row0 + ROWS - 1, rows - 1) / p.n_rep;
   const int lim = it.mask ? n_kv : min(n_kv, it.n_past + last_token + 1);
   const int tile0 = sp * it.tiles_per_split;
-  const int tile1 = min(tile0 + it.tiles_per_split, (lim + kTreeKeys - 1) / kTreeKeys);
+  const int tile1 = min(tile0 + it.tiles_per_split, (lim + kTreeTile - 1) / kTreeTile);
 
   const char* const kbase = it.k + (int64_t)g * p.k_s1;
   const char* const vbase = it.v + (int64_t)g * p.v_s1;
@@ -228,11 +153,13 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
 #pragma unroll
       for (int s = 0; s < D / 16; ++s)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          _Float16 hi, lo;
-          split(x[8 * s + j] * f, hi, lo);
-          qh[i][s][j] = hi;
-          ql[i][s][j] = lo;
+        for (int j = 0; j < 8; j += 2) {
+          f16x2 hi, lo;
+          split2(x[8 * s + j] * f, x[8 * s + j + 1] * f, hi, lo);
+          qh[i][s][j] = hi[0];
+          qh[i][s][j + 1] = hi[1];
+          ql[i][s][j] = lo[0];
+          ql[i][s][j + 1] = lo[1];
         }
     }
   }
@@ -260,8 +187,8 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
   const unsigned vo = (unsigned)(4 * kh * vs2 + c * NDB * ELT);
   lds_t* const sc_lds = lds + wave * ROWS * C::XS * 4;
   auto load_k = [&](int tile) __attribute__((always_inline)) {
-    const int key0 = tile * kTreeKeys;
-    const int n = min(n_kv - key0, kTreeKeys);
+    const int key0 = tile * kTreeTile;
+    const int n = min(n_kv - key0, kTreeTile);
     const rsrc_t r = make_rsrc(kbase + (int64_t)key0 * ks2, (unsigned)((n - 1) * ks2 + D * ELT));
 #pragma unroll
     for (int s = 0; s < KW / 4; ++s) {
@@ -282,8 +209,8 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
     }
   };
   auto load_v = [&](int tile) __attribute__((always_inline)) {
-    const int key0 = tile * kTreeKeys;
-    const int n = min(n_kv - key0, kTreeKeys);
+    const int key0 = tile * kTreeTile;
+    const int n = min(n_kv - key0, kTreeTile);
     const rsrc_t r = make_rsrc(vbase + (int64_t)key0 * vs2, (unsigned)((n - 1) * vs2 + D * ELT));
 #pragma unroll
     for (int t = 0; t < 16; ++t) {
@@ -310,7 +237,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
     load_v(tile);
   }
   for (; tile < tile1; tile += kTreeWaves) {
-    const int key0 = tile * kTreeKeys;
+    const int key0 = tile * kTreeTile;
     const int next = tile + kTreeWaves;
     // ---- S^T = K . Q^T ------------------------------------------------------
     floatx16 s[RT];
@@ -392,29 +319,11 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
 
     // ---- mask -----------------------------------------------------------------
     unsigned vis[RT];
-    const bool masked = key0 + kTreeKeys > it.n_past;  // a tile of drafted keys
+    const bool masked = key0 + kTreeTile > it.n_past;  // a tile of drafted keys
     if (masked) {
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
-        const int b0 = key0 - it.n_past;  // the tile's first key as a bit of the mask row
-        unsigned v;
-        if (it.mask) {
-          const char* const mrow = it.mask + (int64_t)token[i] * it.mask_nb;
-          const int n_words = (it.n_tokens + 63) / 64;
-          if (b0 >= 0) {
-            const int w = b0 >> 6, sh = b0 & 63;
-            uint64_t x = gload<uint64_t>(mrow + 8 * (int64_t)w) >> sh;
-            if (sh > 32 && w + 1 < n_words) x |= gload<uint64_t>(mrow + 8 * (int64_t)(w + 1)) << (64 - sh);
-            v = (unsigned)x;
-          } else {
-            v = (unsigned)gload<uint64_t>(mrow) << -b0 | ((1u << -b0) - 1u);
-          }
-          const int n = n_kv - key0;
-          if (n < 32) v &= (1u << n) - 1u;
-        } else {
-          const int n = b0 < 0 ? token[i] + 1 - b0 : token[i] - b0 + 1;  // keys of the tile that the row sees
-          v = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
-        }
+        const unsigned v = visible_bits(it, token[i], key0);
         vis[i] = v;
         const unsigned mine = v >> (4 * kh);
 #pragma unroll
@@ -506,11 +415,13 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            _Float16 hi, lo;
-            split(s[i][8 * u + j], hi, lo);
-            ph[i][j] = hi;
-            pl[i][j] = lo;
+          for (int j = 0; j < 8; j += 2) {
+            f16x2 hi, lo;
+            split2(s[i][8 * u + j], s[i][8 * u + j + 1], hi, lo);
+            ph[i][j] = hi[0];
+            ph[i][j + 1] = hi[1];
+            pl[i][j] = lo[0];
+            pl[i][j + 1] = lo[1];
           }
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
@@ -688,42 +599,48 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const TreeParams p, i
   gstore(reinterpret_cast<char*>(it.out) + (int64_t)t * p.o_s2 + (int64_t)h * p.o_s1 + 16 * d4, acc * inv);
 }
 
-int tree_tile_rows(int rows) { return rows > 32 ? 64 : 32; }
+// F32: 32 or 64 rows. F16 and 8-bit caches: the wide kernel's 128 once 64 do
+// not hold them.
+int tree_tile_rows(int rows, int elt) { return rows <= 32 ? 32 : rows <= 64 || elt == 4 ? 64 : 128; }
 
 size_t tree_record_floats(int head_dim, int tile_rows) { return (size_t)tile_rows * (head_dim + 2); }
 
 template <int D, typename KT, int RT>
-static hipError_t launch_tree_t(const TreeParams& p, int n_items, hipStream_t stream) {
+static hipError_t launch_tree_t(const TreeParams& p, dim3 grid, hipStream_t stream) {
+  hipLaunchKernelGGL((tree_kernel<D, KT, RT>), grid, dim3(kTreeWaves * kWave), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <int D, typename KT>
+static hipError_t launch_tree_d(const TreeParams& p, dim3 grid, int tile_rows, hipStream_t stream) {
+  return tile_rows == 64 ? launch_tree_t<D, KT, 2>(p, grid, stream) : launch_tree_t<D, KT, 1>(p, grid, stream);
+}
+
+hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, hipStream_t stream) {
   unsigned gx = 0, cx = 0;
   for (int i = 0; i < n_items; ++i) {
     const TreeItem& it = p.item[i];
     const unsigned units = (unsigned)p.n_head_kv * it.n_split;
     gx = std::max(gx, (units + 7) / 8 * 8 * (unsigned)it.n_rt);
     if (it.n_split > 1)
-      cx = std::max(cx, ((unsigned)it.n_tokens * p.n_rep * p.n_head_kv * (D / 4) + 255) / 256);
+      cx = std::max(cx, ((unsigned)it.n_tokens * p.n_rep * p.n_head_kv * (head_dim / 4) + 255) / 256);
   }
-  hipLaunchKernelGGL((tree_kernel<D, KT, RT>), dim3(gx, n_items), dim3(kTreeWaves * kWave), 0, stream, p);
-  hipError_t e = hipGetLastError();
+  const dim3 grid(gx, n_items);
+  hipError_t e = hipErrorInvalidValue;
+  if (tile_rows == 128)
+    e = launch_tree_wide(p, grid, head_dim, elt, stream);
+  else if (head_dim == 64)
+    e = elt == 1   ? launch_tree_d<64, int8_t>(p, grid, tile_rows, stream)
+        : elt == 2 ? launch_tree_d<64, _Float16>(p, grid, tile_rows, stream)
+                   : launch_tree_d<64, float>(p, grid, tile_rows, stream);
+  else
+    e = elt == 1   ? launch_tree_d<128, int8_t>(p, grid, tile_rows, stream)
+        : elt == 2 ? launch_tree_d<128, _Float16>(p, grid, tile_rows, stream)
+                   : launch_tree_d<128, float>(p, grid, tile_rows, stream);
   if (e != hipSuccess || cx == 0) return e;
-  hipLaunchKernelGGL((tree_combine_kernel<D>), dim3(cx, n_items), dim3(256), 0, stream, p, 32 * RT);
+  if (head_dim == 64) hipLaunchKernelGGL(tree_combine_kernel<64>, dim3(cx, n_items), dim3(256), 0, stream, p, tile_rows);
+  else hipLaunchKernelGGL(tree_combine_kernel<128>, dim3(cx, n_items), dim3(256), 0, stream, p, tile_rows);
   return hipGetLastError();
-}
-
-template <int D, typename KT>
-static hipError_t launch_tree_d(const TreeParams& p, int n_items, int tile_rows, hipStream_t stream) {
-  return tile_rows == 64 ? launch_tree_t<D, KT, 2>(p, n_items, stream) : launch_tree_t<D, KT, 1>(p, n_items, stream);
-}
-
-hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, hipStream_t stream) {
-  if (head_dim == 64)
-    return elt == 1   ? launch_tree_d<64, int8_t>(p, n_items, tile_rows, stream)
-           : elt == 2 ? launch_tree_d<64, _Float16>(p, n_items, tile_rows, stream)
-                      : launch_tree_d<64, float>(p, n_items, tile_rows, stream);
-  if (head_dim == 128)
-    return elt == 1   ? launch_tree_d<128, int8_t>(p, n_items, tile_rows, stream)
-           : elt == 2 ? launch_tree_d<128, _Float16>(p, n_items, tile_rows, stream)
-                      : launch_tree_d<128, float>(p, n_items, tile_rows, stream);
-  return hipErrorInvalidValue;
 }
 
 }  // namespace mi
