@@ -570,30 +570,72 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
 }
 
 // Joins the splits' records of a row: out = sum_s 2^(m_s - M) O_s / sum_s
-// 2^(m_s - M) l_s. D / 4 threads a row, four dims each; the records were just
-// written and are read once, from the caches.
+// 2^(m_s - M) l_s. D / 4 threads (four dims each) times `slices` threads a row:
+// a slice takes every slices-th record with a running maximum, kInFlight of
+// them on their way at once, and the slices meet in LDS in order. The records
+// were just written and come from the caches, so the time is their latency:
+// few records in turn per thread is what counts.
 template <int D>
-__global__ __launch_bounds__(256) void tree_combine_kernel(const TreeParams p, int tile_rows) {
+__global__ __launch_bounds__(256) void tree_combine_kernel(const TreeParams p, int tile_rows, int slices) {
+  constexpr int LANES = D / 4;          // threads per (row, slice)
+  constexpr int GROUPS = 256 / LANES;   // (row, slice) pairs per workgroup
+  constexpr int kInFlight = 4;
+  __shared__ f32x4 part[256];
+  __shared__ f32x2 ml[GROUPS];
   const TreeItem& it = p.item[blockIdx.y];
   const int rows = it.n_tokens * p.n_rep, n_split = it.n_split;
-  const int idx = blockIdx.x * 256 + threadIdx.x;
-  const int row = idx / (D / 4), d4 = idx % (D / 4);  // row over the KV heads
-  if (n_split <= 1 || row >= rows * p.n_head_kv) return;
-  const int g = row / rows, r = row % rows;
+  if (n_split <= 1) return;
+  const int grp = threadIdx.x / LANES, d4 = threadIdx.x % LANES;
+  const int slice = grp % slices;
+  const int row = blockIdx.x * (GROUPS / slices) + grp / slices;  // over the KV heads
+  const bool valid = row < rows * p.n_head_kv;
+  const int g = valid ? row / rows : 0, r = valid ? row % rows : 0;
   const int64_t rec_floats = (int64_t)tile_rows * (D + 2);
   const float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * it.n_rt + r / tile_rows) * n_split) * rec_floats;
   const int rr = r % tile_rows;
-  float mx = -INFINITY;
-  for (int s = 0; s < n_split; ++s) mx = fmaxf(mx, gload<float>(rec + s * rec_floats + tile_rows * D + rr));
-  const float mu = mx == -INFINITY ? 0.f : mx;
+  float mx = -INFINITY, l = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  for (int s = 0; s < n_split; ++s) {
-    const float* const q = rec + s * rec_floats;
-    const float w = fast_exp2(gload<float>(q + tile_rows * D + rr) - mu);
-    l += w * gload<float>(q + tile_rows * (D + 1) + rr);
-    acc += w * gload<f32x4>(q + rr * D + 4 * d4);
+  for (int s0 = slice; s0 < n_split; s0 += kInFlight * slices) {
+    float ms[kInFlight], ls[kInFlight];
+    f32x4 os[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int s = s0 + u * slices;
+      const float* const q = rec + (s < n_split ? s : s0) * rec_floats;
+      ms[u] = gload<float>(q + tile_rows * D + rr);
+      ls[u] = gload<float>(q + tile_rows * (D + 1) + rr);
+      os[u] = gload<f32x4>(q + rr * D + 4 * d4);
+    }
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      if (s0 + u * slices >= n_split) continue;
+      const float mn = fmaxf(mx, ms[u]);
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float a = fast_exp2(mx - mu), b = fast_exp2(ms[u] - mu);
+      acc = acc * a + os[u] * b;
+      l = l * a + ls[u] * b;
+      mx = mn;
+    }
   }
+  if (slices > 1) {
+    part[threadIdx.x] = acc;
+    if (d4 == 0) ml[grp] = f32x2{mx, l};
+    __syncthreads();
+    if (slice != 0) return;
+    float top = mx;
+    for (int s = 1; s < slices; ++s) top = fmaxf(top, ml[grp + s][0]);
+    const float mu = top == -INFINITY ? 0.f : top;
+    const float a = fast_exp2(mx - mu);
+    acc *= a;
+    l *= a;
+    for (int s = 1; s < slices; ++s) {
+      const float b = fast_exp2(ml[grp + s][0] - mu);
+      acc += part[threadIdx.x + s * LANES] * b;
+      l += ml[grp + s][1] * b;
+    }
+    mx = top;
+  }
+  if (!valid) return;
   const float inv = mx == -INFINITY ? 0.f : 1.f / l;
   const int t = r / p.n_rep, h = g * p.n_rep + r % p.n_rep;
   gstore(reinterpret_cast<char*>(it.out) + (int64_t)t * p.o_s2 + (int64_t)h * p.o_s1 + 16 * d4, acc * inv);
@@ -617,13 +659,15 @@ static hipError_t launch_tree_d(const TreeParams& p, dim3 grid, int tile_rows, h
 }
 
 hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, hipStream_t stream) {
-  unsigned gx = 0, cx = 0;
+  unsigned gx = 0;
+  int64_t rows = 0;  // of the longest split item, over its KV heads
+  int splits = 1;
   for (int i = 0; i < n_items; ++i) {
     const TreeItem& it = p.item[i];
     const unsigned units = (unsigned)p.n_head_kv * it.n_split;
     gx = std::max(gx, (units + 7) / 8 * 8 * (unsigned)it.n_rt);
-    if (it.n_split > 1)
-      cx = std::max(cx, ((unsigned)it.n_tokens * p.n_rep * p.n_head_kv * (head_dim / 4) + 255) / 256);
+    if (it.n_split > 1) rows = std::max(rows, (int64_t)it.n_tokens * p.n_rep * p.n_head_kv);
+    splits = std::max(splits, it.n_split);
   }
   const dim3 grid(gx, n_items);
   hipError_t e = hipErrorInvalidValue;
@@ -637,9 +681,14 @@ hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, 
     e = elt == 1   ? launch_tree_d<128, int8_t>(p, grid, tile_rows, stream)
         : elt == 2 ? launch_tree_d<128, _Float16>(p, grid, tile_rows, stream)
                    : launch_tree_d<128, float>(p, grid, tile_rows, stream);
-  if (e != hipSuccess || cx == 0) return e;
-  if (head_dim == 64) hipLaunchKernelGGL(tree_combine_kernel<64>, dim3(cx, n_items), dim3(256), 0, stream, p, tile_rows);
-  else hipLaunchKernelGGL(tree_combine_kernel<128>, dim3(cx, n_items), dim3(256), 0, stream, p, tile_rows);
+  if (e != hipSuccess || rows == 0) return e;
+  // slices: about four records each, as many as a workgroup has groups
+  const int groups = 256 / (head_dim / 4);
+  int slices = 1;
+  while (slices < groups && slices * 4 < splits) slices *= 2;
+  const dim3 cgrid((unsigned)((rows * slices + groups - 1) / groups), n_items);
+  if (head_dim == 64) hipLaunchKernelGGL(tree_combine_kernel<64>, cgrid, dim3(256), 0, stream, p, tile_rows, slices);
+  else hipLaunchKernelGGL(tree_combine_kernel<128>, cgrid, dim3(256), 0, stream, p, tile_rows, slices);
   return hipGetLastError();
 }
 
