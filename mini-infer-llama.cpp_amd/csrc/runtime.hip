@@ -765,45 +765,62 @@ int run_prefill(const mi_hip_attn_args* a, const Resolved& r, hipStream_t stream
   return MI_HIP_OK;
 }
 
-// Tree attention. The launch is cut so that it has about kTreeWgPerCu
-// workgroups per CU: row tiles first (they cost no second read from HBM worth
-// naming, since a unit's row tiles share an L2), then the keys, each split at
-// least one 32-key tile per wave. Every item's splits have the same number of
-// tiles, so a launch of ragged items is even.
+// Tree attention: how many key tiles one workgroup takes. A unit (item, KV
+// head, split) brings n_rt workgroups, one per row tile, to one XCD; units go
+// to the XCDs in turn through all items. The launch runs in rounds of
+// kTreeWgPerCu workgroups per CU of an XCD, so what a number of tiles per split
+// costs is rounds x (tiles + what a workgroup spends before and after them),
+// with a second launch to join the parts when there are any. Every item's
+// splits have the same number of tiles.
 void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int tile_rows, size_t part_bytes) {
-  constexpr int kMinTiles = 4;  // one per wave
-  const int64_t want = (int64_t)kTreeWgPerCu * g.n_cu;
+  constexpr int64_t kMinTiles = 4, kXcds = 8;
+  constexpr int64_t kFixed = 6, kJoin = 4;  // in tiles
   const int64_t cap = (int64_t)(part_bytes / (mi::tree_record_floats(head_dim, tile_rows) * sizeof(float)));
-  int64_t units = 0, tiles = 0, longest = 0;
-  auto tiles_of = [&](const mi::TreeItem& it) { return ((int64_t)it.n_past + it.n_tokens + 31) / 32; };
+  const int64_t slots = std::max<int64_t>(1, kTreeWgPerCu * g.n_cu / kXcds);
+  auto tiles_of = [&](const mi::TreeItem& it) {
+    return ((int64_t)it.n_past + it.n_tokens + mi::kTreeTile - 1) / mi::kTreeTile;
+  };
+  int64_t longest = 0;
   for (int i = 0; i < n_items; ++i) {
     mi::TreeItem& it = p.item[i];
     it.n_rt = (int32_t)(((int64_t)it.n_tokens * p.n_rep + tile_rows - 1) / tile_rows);
-    units += (int64_t)p.n_head_kv * it.n_rt;
-    tiles += (int64_t)p.n_head_kv * it.n_rt * tiles_of(it);
     longest = std::max(longest, tiles_of(it));
   }
-  int64_t per = longest;
-  if (units < want) {
-    per = std::max<int64_t>(kMinTiles, (tiles + want - 1) / want);
-    // rounding up per item can pass what is wanted, and what the parts hold
-    auto records = [&](int64_t n) {
-      int64_t r = 0;
-      for (int i = 0; i < n_items; ++i)
-        r += (int64_t)p.n_head_kv * p.item[i].n_rt * ((tiles_of(p.item[i]) + n - 1) / n);
-      return r;
-    };
-    per += per & 1;  // whole 64-key tiles
-    while (per < longest && records(per) > std::min(want, cap)) per += std::max<int64_t>(1, per / 32) * 2;
-    if (records(per) > cap) per = longest;
+  // (records, rounds) with `per` tiles per split
+  auto load = [&](int64_t per, int64_t* records) {
+    int64_t at = 0, wgs[kXcds] = {};
+    *records = 0;
+    for (int i = 0; i < n_items; ++i) {
+      const mi::TreeItem& it = p.item[i];
+      const int64_t split = (tiles_of(it) + per - 1) / per, units = split * p.n_head_kv;
+      if (split > 1) *records += units * it.n_rt;
+      for (int64_t x = 0; x < kXcds; ++x) wgs[(at + x) % kXcds] += (units + kXcds - 1 - x) / kXcds * it.n_rt;
+      at += units;
+    }
+    return (*std::max_element(wgs, wgs + kXcds) + slots - 1) / slots;
+  };
+  int64_t best = 0, best_per = longest;
+  for (int64_t split = 1; split <= std::max<int64_t>(1, longest / kMinTiles); split += 1 + split / 8) {
+    int64_t per = (longest + split - 1) / split;
+    if (split > 1) per += per & 1;  // whole 64-key tiles
+    int64_t records;
+    const int64_t rounds = load(per, &records);
+    if (records > cap) continue;
+    const int64_t cost = rounds * (per + kFixed) + (records ? kJoin : 0);
+    if (split == 1 || cost < best) {
+      best = cost;
+      best_per = per;
+    }
   }
-  int64_t rec = 0;
+  int64_t rec = 0, at = 0;
   for (int i = 0; i < n_items; ++i) {
     mi::TreeItem& it = p.item[i];
-    it.tiles_per_split = (int32_t)std::min<int64_t>(per, tiles_of(it));
+    it.tiles_per_split = (int32_t)std::min<int64_t>(best_per, tiles_of(it));
     it.n_split = (int32_t)((tiles_of(it) + it.tiles_per_split - 1) / it.tiles_per_split);
     it.rec0 = (int32_t)rec;
+    it.xcd0 = (uint32_t)(at % kXcds);
     if (it.n_split > 1) rec += (int64_t)p.n_head_kv * it.n_rt * it.n_split;
+    at += (int64_t)p.n_head_kv * it.n_split;
   }
 }
 

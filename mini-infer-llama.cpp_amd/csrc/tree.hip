@@ -33,12 +33,13 @@
 // hi = RNE(x), lo = RNE(x - hi), two v_mfma_f32_32x32x16_f16 a step. So that
 // lo stays normal, each query row is scaled by the power of two that puts its
 // largest element in [2^13, 2^14) (undone in the exponent's multiply-add), and
-// the probabilities are 2^14 p (undone by the division by their sum): 2^-22
-// relative to the row's largest element.
+// the probabilities are taken relative to ref = m - 14 instead of m (2^14 p;
+// the division by their sum undoes it): 2^-22 relative to the row's largest
+// element.
 //   8-bit K: a row's scales (one per 32 dims) multiply the S^T of their own
-//   32 dims. 8-bit V: the row's one scale multiplies the probability, taken
-//   relative to vref, the power of two above the largest V scale so far
-//   (raised like the running maximum), so that the pair stays normal there too.
+//   32 dims. 8-bit V: the row's one scale multiplies the probability, which is
+//   at most 2^14 again when ref = m - 14 + e, 2^e above the largest V scale so
+//   far (e rises like the maximum, and what has been summed goes by ref).
 #include <algorithm>
 
 #include "attn_common.h"
@@ -59,8 +60,7 @@ struct TreeCfg {
   static constexpr int XS = 36;                  // exchange row stride (floats)
   static constexpr int L_X = 0;                  // waves' outputs of one 32-dim block
   static constexpr int L_ML = kTreeWaves * ROWS * XS * 4;  // m, l per wave and row
-  static constexpr int L_VR = L_ML + kTreeWaves * ROWS * 2 * 4;  // vref per wave
-  static constexpr int LDS = L_VR + kTreeWaves * 4;
+  static constexpr int LDS = L_ML + kTreeWaves * ROWS * 2 * 4;
   // While the keys stream, a wave keeps the tile's scales in its own part of
   // the exchange area: NDB blocks of 32 K scales, then 32 V scales.
   static constexpr int SC = (NDB + 1) * 32 * 4;
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
   const int n_rt = it.n_rt, n_split = it.n_split;
   const int y = blockIdx.x / 8;
   const int rt = n_rt - 1 - y % n_rt;
-  const int unit = (y / n_rt) * 8 + (int)(blockIdx.x % 8);
+  const int unit = (y / n_rt) * 8 + (int)((blockIdx.x - it.xcd0) % 8);
   if (unit >= p.n_head_kv * n_split) return;
   const int g = unit / n_split, sp = unit % n_split;
   const int n_kv = it.n_past + it.n_tokens;
@@ -166,11 +166,11 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
 
   // ---- state --------------------------------------------------------------
   floatx16 o[RT][NDB];
-  float m[RT], l[RT];
-  float vref = 0x1p-24f;  // the smallest scale there is
+  float m[RT], ref[RT], l[RT];
+  int vexp = -24;  // the smallest V scale there is
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
-    m[i] = -INFINITY;
+    m[i] = ref[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
     for (int db = 0; db < NDB; ++db) o[i][db] = (floatx16)(0.f);
@@ -241,8 +241,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
     const int next = tile + kTreeWaves;
     // ---- S^T = K . Q^T ------------------------------------------------------
     floatx16 s[RT];
-    f32x4 pv_scale[4];  // V scales of the lane's keys times 2^14 / vref
-    float alpha_v = 1.f;
+    f32x4 pv_scale[4];  // V scales of the lane's keys
 #pragma unroll
     for (int i = 0; i < RT; ++i) s[i] = (floatx16)(0.f);
     if constexpr (F32) {
@@ -297,22 +296,12 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
             for (int j = 0; j < 4; ++j) s[i][4 * q + j] = fmaf(part[i][4 * q + j], sc[j], s[i][4 * q + j]);
         }
       }
-      float mx = 0.f;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        pv_scale[q] = lds_load<f32x4>(sc_lds + (32 * NDB + 8 * q + 4 * kh) * 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, pv_scale[q][j] < INFINITY ? pv_scale[q][j] : 0.f);
-      }
-      mx = max32(mx);  // the same in every lane
-      if (mx > vref) {
-        const float up = ldexpf(1.f, ilogbf(mx) + 1);
-        alpha_v = vref / up;
-        vref = up;
-      }
-      const float inv = 16384.f / vref;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) pv_scale[q] *= inv;
+      for (int q = 0; q < 4; ++q) pv_scale[q] = lds_load<f32x4>(sc_lds + (32 * NDB + 8 * q + 4 * kh) * 4);
+      const float v = h2f(vsc);
+      float top = row_max16(v < INFINITY ? v : 0.f);
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));  // the same in every lane
+      vexp = max(vexp, scale_exponent(top));
       wave_lds_fence();  // the scales are read before the next tile's are written
     }
     if (next < tile1) load_k(next);
@@ -337,23 +326,22 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
       float mx = fmaxf(s[i][0], s[i][1]);
 #pragma unroll
       for (int e = 2; e < 16; ++e) mx = fmaxf(mx, s[i][e]);
-      mx = max32(mx) * unscale[i];
-      const float mn = fmaxf(m[i], mx);
-      const float mu = mn == -INFINITY ? 0.f : mn;
-      const float alpha = fast_exp2(m[i] - mu);
-      const float boost = F32 || Q8 ? mu : mu - 14.f;
-      float sum = 0.f;
+      m[i] = fmaxf(m[i], max32(mx) * unscale[i]);
+      const float boost = F32 ? 0.f : (float)((Q8 ? vexp : 0) - 14);
+      const float now = m[i] == -INFINITY ? -INFINITY : m[i] + boost;
+      const float at = m[i] == -INFINITY ? 0.f : now;
+      const float alpha = fast_exp2(ref[i] - at);
+      ref[i] = now;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[i][e] = fast_exp2(fmaf(s[i][e], unscale[i], -boost));
-        sum += s[i][e];
+        s[i][e] = fast_exp2(fmaf(s[i][e], unscale[i], -at));
+        sum[e & 3] += s[i][e];
       }
-      l[i] = l[i] * alpha + sum;
-      m[i] = mn;
-      const float ao = alpha * alpha_v;
-      if (__builtin_amdgcn_ballot_w64(ao != 1.f) != 0ull) {
+      l[i] = l[i] * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0ull) {
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) o[i][db] *= ao;
+        for (int db = 0; db < NDB; ++db) o[i][db] *= alpha;
       }
       if constexpr (Q8) {
 #pragma unroll
@@ -482,13 +470,12 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
   for (int i = 0; i < RT; ++i) {
     const float lt = sum32(l[i]);
     if (kh == 0) {
-      lds_store<float>(lds + C::L_ML + ((wave * ROWS + 32 * i + c) * 2) * 4, m[i]);
+      lds_store<float>(lds + C::L_ML + ((wave * ROWS + 32 * i + c) * 2) * 4, ref[i]);
       lds_store<float>(lds + C::L_ML + ((wave * ROWS + 32 * i + c) * 2 + 1) * 4, lt);
     }
   }
   __syncthreads();
-  // 8-bit: O holds 2^14 / vref of the sum (and 2^-10 of the bytes' values)
-  const float unit_o = Q8 ? vref * (kByteUnscale / 16384.f) : 1.f;
+  constexpr float unit_o = Q8 ? kByteUnscale : 1.f;  // of the values' 2^-10
   float mt[RT], lt[RT];
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
@@ -503,7 +490,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
     const float mu = mt[i] == -INFINITY ? 0.f : mt[i];
 #pragma unroll
     for (int w = 0; w < kTreeWaves; ++w) lt[i] += ml[w][1] * fast_exp2(ml[w][0] - mu);
-    const float wt = fast_exp2(m[i] - mu) * unit_o;
+    const float wt = fast_exp2(ref[i] - mu) * unit_o;
 #pragma unroll
     for (int db = 0; db < NDB; ++db) o[i][db] *= wt;
   }
@@ -532,7 +519,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
     }
   }
   if (n_split > 1) {
-    // record: ROWS rows of D, then m, then l
+    // record: ROWS rows of D, then ref, then l
     float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * n_rt + rt) * n_split + sp) * (ROWS * (D + 2));
 #pragma unroll
     for (int e = 0; e < PER; ++e) {

@@ -74,6 +74,10 @@ __device__ inline void split2(float x0, float x1, f16x2& hi, f16x2& lo) {
   lo = __builtin_convertvector((f32x2{fmaf((float)hi[0], -1.f, x0), fmaf((float)hi[1], -1.f, x1)}), f16x2);
 }
 
+// The e for which scales up to `top` are below 2^e (at least that of the
+// smallest scale there is).
+__device__ inline int scale_exponent(float top) { return top > 0.f ? ilogbf(top) + 1 : -24; }
+
 // Which keys key0 .. key0 + 31 the query `token` sees, as bits: those of the
 // item's first n_past all, the rest by the mask or (none) up to its own.
 __device__ inline unsigned visible_bits(const TreeItem& it, int token, int key0) {

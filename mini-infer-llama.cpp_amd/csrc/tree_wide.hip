@@ -50,8 +50,8 @@ struct WideCfg {
   static constexpr int PER = 4096 / 8 / (kTreeWaves * kWave);  // slots a thread fetches of K, and of V
   static constexpr int TILE = 8192;              // bytes of a K or V tile
   static constexpr int L_K = 0, L_V = 2 * TILE;  // two buffers each
-  static constexpr int L_SC = 4 * TILE;          // per buffer: K scales [NDB][TK], V scales [TK], f16
-  static constexpr int SC = (NDB + 1) * TK * 2;
+  static constexpr int L_SC = 4 * TILE;          // per buffer: K scales [NDB][TK], V scales [TK], f16, the V scales' exponent
+  static constexpr int SC = (NDB + 1) * TK * 2 + 16;
   static constexpr int L_NF = L_SC + (Q8 ? 2 * SC : 0);  // per buffer: the last tile with values that are not finite
   static constexpr int LDS = L_NF + 16;
 };
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
   const int n_rt = it.n_rt, n_split = it.n_split;
   const int y = blockIdx.x / 8;
   const int rt = n_rt - 1 - y % n_rt;
-  const int unit = (y / n_rt) * 8 + (int)(blockIdx.x % 8);
+  const int unit = (y / n_rt) * 8 + (int)((blockIdx.x - it.xcd0) % 8);
   if (unit >= p.n_head_kv * n_split) return;
   const int g = unit / n_split, sp = unit % n_split;
   const int n_kv = it.n_past + it.n_tokens;
@@ -100,6 +100,13 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
     ko[i] = (unsigned)(r * ks2 + 8 * ELT * s);
     vo[i] = (unsigned)(r * vs2 + 8 * ELT * s);
   }
+  // 8-bit: thread t's scale of a tile: the K scales (key t / NDB, group t % NDB),
+  // then the V scales. Every thread loads one (those behind the last scale that
+  // of key 0, not stored) from a row that is there.
+  const bool sc_k = tid < TK * NDB, sc_v = !sc_k && tid < TK * (NDB + 1);
+  const int sc_key = sc_k ? tid / NDB : sc_v ? tid - TK * NDB : 0;
+  const int sc_stride = p.n_head_kv * 2 * (sc_k ? NDB : 1);
+  const char* const sc_src = Q8 ? (sc_k ? it.k_scale + 2 * (g * NDB + tid % NDB) : it.v_scale + 2 * g) : nullptr;
   auto fetch = [&](int key0) __attribute__((always_inline)) {
     const int n = min(n_kv - key0, TK);
     const rsrc_t rk = make_rsrc(kbase + (int64_t)key0 * ks2, (unsigned)((n - 1) * ks2 + D * ELT));
@@ -123,16 +130,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
       }
     }
     if constexpr (Q8) {
-      // threads 0 .. TK NDB - 1: K scales (key tid / NDB, group tid % NDB), the
-      // next TK: V scales
-      const int64_t at = (int64_t)key0 * p.n_head_kv + g;
-      if (tid < TK * NDB) {
-        const rsrc_t r = make_rsrc(it.k_scale + at * (2 * NDB), (unsigned)((n - 1) * p.n_head_kv * 2 * NDB + 2 * NDB));
-        scw = buf_b16(r, (unsigned)((tid / NDB) * p.n_head_kv * 2 * NDB + 2 * (tid % NDB)));
-      } else if (tid < TK * (NDB + 1)) {
-        const rsrc_t r = make_rsrc(it.v_scale + at * 2, (unsigned)((n - 1) * p.n_head_kv * 2 + 2));
-        scw = buf_b16(r, (unsigned)((tid - TK * NDB) * p.n_head_kv * 2));
-      }
+      scw = gload<unsigned short>(sc_src + (int64_t)(key0 + min(sc_key, n - 1)) * sc_stride);
     }
   };
   // Eight values as f16: an 8-bit value v as v 2^-10 (see bytes_f16).
@@ -173,8 +171,15 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
     }
     if constexpr (Q8) {
       lds_t* const sc = lds + C::L_SC + buf * C::SC;
-      if (tid < TK * NDB) lds_store<unsigned short>(sc + ((tid % NDB) * TK + tid / NDB) * 2, (unsigned short)scw);
-      else if (tid < TK * (NDB + 1)) lds_store<unsigned short>(sc + tid * 2, (unsigned short)scw);
+      if (sc_k) lds_store<unsigned short>(sc + ((tid % NDB) * TK + sc_key) * 2, (unsigned short)scw);
+      if (sc_v) {  // TK threads of one wave
+        lds_store<unsigned short>(sc + tid * 2, (unsigned short)scw);
+        const float v = (float)__builtin_bit_cast(_Float16, (unsigned short)scw);
+        float top = row_max16(v < INFINITY ? v : 0.f);
+#pragma unroll
+        for (int off = 16; off < TK; off *= 2) top = fmaxf(top, __shfl_xor(top, off, kWave));
+        if (tid == TK * NDB) lds_store<int>(sc + (NDB + 1) * TK * 2, scale_exponent(top));
+      }
     }
   };
   if (tid < 2) lds_store<int>(lds + C::L_NF + 4 * tid, -1);
@@ -224,7 +229,8 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
   floatx16 o[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) o[db] = (floatx16)(0.f);
-  float m = -INFINITY, l = 0.f, vref = 0x1p-24f;
+  float m = -INFINITY, ref = -INFINITY, l = 0.f;
+  int vexp = -24;  // the smallest V scale there is
 
   // lane parts of the LDS addresses
   const lds_t* const krow = lds + C::L_K + c * (2 * D);
@@ -242,7 +248,8 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
 
     // ---- S^T = K . Q^T ----------------------------------------------------------
     floatx16 s[SUB];
-    const lds_t* const sc = lds + C::L_SC + buf * C::SC + 8 * kh;  // the lane's keys 8 q + 4 kh ..
+    const lds_t* const sc_base = lds + C::L_SC + buf * C::SC;
+    const lds_t* const sc = sc_base + 8 * kh;  // the lane's keys 8 q + 4 kh ..
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       s[u] = (floatx16)(0.f);
@@ -282,52 +289,36 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
       }
     }
 
-    // ---- softmax ----------------------------------------------------------------
-    float alpha;
-    {
-      float mx = s[0][0];
+    // ---- softmax, relative to ref ---------------------------------------------------
+    if constexpr (Q8) vexp = max(vexp, lds_load<int>(sc_base + (NDB + 1) * TK * 2));
+    float mx = s[0][0];
 #pragma unroll
-      for (int u = 0; u < SUB; ++u)
+    for (int u = 0; u < SUB; ++u)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
-      mx = max32(mx) * unscale;
-      const float mn = fmaxf(m, mx);
-      const float mu = mn == -INFINITY ? 0.f : mn;
-      alpha = fast_exp2(m - mu);
-      const float shift = Q8 ? mu : mu - 14.f;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
+    m = fmaxf(m, max32(mx) * unscale);
+    const float now = m == -INFINITY ? -INFINITY : m + (float)(Q8 ? vexp - 14 : -14);
+    const float at = m == -INFINITY ? 0.f : now;
+    const float alpha = fast_exp2(ref - at);
+    ref = now;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < SUB; ++u)
+    for (int u = 0; u < SUB; ++u)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[u][e] = fast_exp2(fmaf(s[u][e], unscale, -shift));
-          sum[e & 3] += s[u][e];
-        }
-      l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-      m = mn;
-    }
+      for (int e = 0; e < 16; ++e) {
+        s[u][e] = fast_exp2(fmaf(s[u][e], unscale, -at));
+        sum[e & 3] += s[u][e];
+      }
+    l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
     if constexpr (Q8) {
-      f16x4 vsc[SUB][4];
-      float mx = 0.f;
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          vsc[u][q] = lds_load<f16x4>(sc + (NDB * TK + 32 * u + 8 * q) * 2);
+          const f16x4 x = lds_load<f16x4>(sc + (NDB * TK + 32 * u + 8 * q) * 2);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mx = fmaxf(mx, (float)vsc[u][q][j] < INFINITY ? (float)vsc[u][q][j] : 0.f);
+          for (int j = 0; j < 4; ++j) s[u][4 * q + j] *= (float)x[j];
         }
-      mx = max32(mx);  // the same in every lane
-      if (mx > vref) {
-        const float up = ldexpf(1.f, ilogbf(mx) + 1);
-        alpha *= vref / up;
-        vref = up;
-      }
-      const float inv = 16384.f / vref;
-#pragma unroll
-      for (int u = 0; u < SUB; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[u][e] *= (float)vsc[u][e >> 2][e & 3] * inv;
       if (masked) {  // (a scale may not be finite: 0 times it is not 0)
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
@@ -392,8 +383,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
 
   // ---- the wave's rows ------------------------------------------------------------
   const float lt = sum32(l);
-  // 8-bit: O holds 2^14 / vref of the sum, of values 2^-10 times theirs
-  const float unit_o = Q8 ? vref * (kByteUnscale / 16384.f) : 1.f;
+  constexpr float unit_o = Q8 ? kByteUnscale : 1.f;  // of the values' 2^-10
   if (n_split > 1) {
     float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * n_rt + rt) * n_split + sp) * (ROWS * (D + 2));
     const int rr = 32 * wave + c;
@@ -404,7 +394,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
         gstore(rec + rr * D + 32 * db + 8 * q + 4 * kh,
                f32x4{o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]} * unit_o);
     if (kh == 0) {
-      rec[ROWS * D + rr] = m;
+      rec[ROWS * D + rr] = ref;
       rec[ROWS * D + ROWS + rr] = lt;
     }
     return;
