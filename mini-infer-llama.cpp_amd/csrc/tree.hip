@@ -6,7 +6,7 @@
 // Mathematics. Query j of a sequence sees key t when t < n_past, or when bit
 // t - n_past of its mask row is set (no mask: t - n_past <= j). Its output is
 // sum_t p_t v_t / sum_t p_t with p_t = 2^(s_t - m), s_t = scale log2(e) q.k_t
-// and m the running maximum over the keys seen so far, so the keys pass once;
+// and m near the maximum over the keys seen so far, so the keys pass once;
 // when m moves, what has been summed is rescaled by 2^(m_old - m_new). A row
 // that sees no key has m = -inf and an output of zeros.
 //
@@ -33,13 +33,12 @@
 // hi = RNE(x), lo = RNE(x - hi), two v_mfma_f32_32x32x16_f16 a step. So that
 // lo stays normal, each query row is scaled by the power of two that puts its
 // largest element in [2^13, 2^14) (undone in the exponent's multiply-add), and
-// the probabilities are taken relative to ref = m - 14 instead of m (2^14 p;
-// the division by their sum undoes it): 2^-22 relative to the row's largest
-// element.
+// the probabilities are 2^(s - ref) for a reference that keeps the largest
+// between 2^6 and 2^14 (move_ref; the division by their sum undoes it): 2^-22
+// relative to the row's largest element.
 //   8-bit K: a row's scales (one per 32 dims) multiply the S^T of their own
-//   32 dims. 8-bit V: the row's one scale multiplies the probability, which is
-//   at most 2^14 again when ref = m - 14 + e, 2^e above the largest V scale so
-//   far (e rises like the maximum, and what has been summed goes by ref).
+//   32 dims. 8-bit V: the row's one scale multiplies the probability; ref keeps
+//   the largest probability times the tile's largest scale in that range.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -166,11 +165,10 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
 
   // ---- state --------------------------------------------------------------
   floatx16 o[RT][NDB];
-  float m[RT], ref[RT], l[RT];
-  int vexp = -24;  // the smallest V scale there is
+  float ref[RT], l[RT];
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
-    m[i] = ref[i] = -INFINITY;
+    ref[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
     for (int db = 0; db < NDB; ++db) o[i][db] = (floatx16)(0.f);
@@ -242,6 +240,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
     // ---- S^T = K . Q^T ------------------------------------------------------
     floatx16 s[RT];
     f32x4 pv_scale[4];  // V scales of the lane's keys
+    float vexp = 0.f;   // and the exponent above the tile's largest
 #pragma unroll
     for (int i = 0; i < RT; ++i) s[i] = (floatx16)(0.f);
     if constexpr (F32) {
@@ -299,9 +298,8 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
 #pragma unroll
       for (int q = 0; q < 4; ++q) pv_scale[q] = lds_load<f32x4>(sc_lds + (32 * NDB + 8 * q + 4 * kh) * 4);
       const float v = h2f(vsc);
-      float top = row_max16(v < INFINITY ? v : 0.f);
-      top = fmaxf(top, __shfl_xor(top, 16, kWave));  // the same in every lane
-      vexp = max(vexp, scale_exponent(top));
+      const float most = row_max16(v < INFINITY ? v : 0.f);
+      vexp = (float)scale_exponent(fmaxf(most, __shfl_xor(most, 16, kWave)));  // the same in every lane
       wave_lds_fence();  // the scales are read before the next tile's are written
     }
     if (next < tile1) load_k(next);
@@ -323,15 +321,8 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
     // ---- softmax ------------------------------------------------------------
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      float mx = fmaxf(s[i][0], s[i][1]);
-#pragma unroll
-      for (int e = 2; e < 16; ++e) mx = fmaxf(mx, s[i][e]);
-      m[i] = fmaxf(m[i], max32(mx) * unscale[i]);
-      const float boost = F32 ? 0.f : (float)((Q8 ? vexp : 0) - 14);
-      const float now = m[i] == -INFINITY ? -INFINITY : m[i] + boost;
-      const float at = m[i] == -INFINITY ? 0.f : now;
-      const float alpha = fast_exp2(ref[i] - at);
-      ref[i] = now;
+      const float alpha = move_ref(ref[i], max32(max16(s[i], -INFINITY)) * unscale[i] + vexp);
+      const float at = ref[i] == -INFINITY ? 0.f : ref[i];
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < 16; ++e) {

@@ -68,10 +68,39 @@ __device__ inline f16x2 bytes_f16(unsigned hi, unsigned lo) {
 }
 constexpr float kByteUnscale = 1024.f;  // what the 2^-10 above takes away
 
-// hi = RNE(x), lo = RNE(x - hi) of two values (x - hi is exact in float).
+// hi = RNE(x), lo = RNE(x - hi) of two values (x - hi is exact in float). The
+// differences as asm: mixed-precision multiply-adds, which read hi as f16; the
+// compiler widens it first, an instruction more for each.
 __device__ inline void split2(float x0, float x1, f16x2& hi, f16x2& lo) {
   hi = __builtin_convertvector((f32x2{x0, x1}), f16x2);
-  lo = __builtin_convertvector((f32x2{fmaf((float)hi[0], -1.f, x0), fmaf((float)hi[1], -1.f, x1)}), f16x2);
+  const unsigned h = __builtin_bit_cast(unsigned, hi);
+  float d0, d1;
+  asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d0) : "v"(h), "v"(x0));
+  asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d1) : "v"(h), "v"(x1));
+  lo = __builtin_convertvector((f32x2{d0, d1}), f16x2);
+}
+
+// The largest of 16 and `x`; NaN if one is (the row's output is then NaN, what
+// it is compared with does not matter). The maximum that passes NaN on has a
+// three-operand instruction; fmaxf would take one more for each operand.
+__device__ inline float max16(const floatx16& s, float x) {
+#pragma unroll
+  for (int e = 0; e < 16; e += 2) x = __builtin_elementwise_maximum(__builtin_elementwise_maximum(x, s[e]), s[e + 1]);
+  return x;
+}
+
+// A softmax row's running reference: probabilities are 2^(s - ref). It moves
+// only when one would pass 2^14 (f16's range holds it, and the products with
+// what it scales), and then to 2^6 for the largest seen: rows move after their
+// first tile hardly ever, so that what has been summed is hardly ever rescaled.
+// `top`: the tile's largest score (plus the V scales' exponent). Returns the
+// factor of what has been summed.
+constexpr float kRefMost = 14.f, kRefNew = 6.f;
+__device__ inline float move_ref(float& ref, float top) {
+  if (!(top - ref > kRefMost)) return 1.f;
+  const float now = top - kRefNew, alpha = fast_exp2(ref - now);
+  ref = now;
+  return alpha;
 }
 
 // The e for which scales up to `top` are below 2^e (at least that of the

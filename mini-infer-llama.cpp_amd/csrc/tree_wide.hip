@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
         float top = row_max16(v < INFINITY ? v : 0.f);
 #pragma unroll
         for (int off = 16; off < TK; off *= 2) top = fmaxf(top, __shfl_xor(top, off, kWave));
-        if (tid == TK * NDB) lds_store<int>(sc + (NDB + 1) * TK * 2, scale_exponent(top));
+        if (tid == TK * NDB) lds_store<float>(sc + (NDB + 1) * TK * 2, (float)scale_exponent(top));
       }
     }
   };
@@ -229,8 +229,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
   floatx16 o[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) o[db] = (floatx16)(0.f);
-  float m = -INFINITY, ref = -INFINITY, l = 0.f;
-  int vexp = -24;  // the smallest V scale there is
+  float ref = -INFINITY, l = 0.f;
 
   // lane parts of the LDS addresses
   const lds_t* const krow = lds + C::L_K + c * (2 * D);
@@ -290,17 +289,13 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
     }
 
     // ---- softmax, relative to ref ---------------------------------------------------
-    if constexpr (Q8) vexp = max(vexp, lds_load<int>(sc_base + (NDB + 1) * TK * 2));
-    float mx = s[0][0];
+    float top = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
-    m = fmaxf(m, max32(mx) * unscale);
-    const float now = m == -INFINITY ? -INFINITY : m + (float)(Q8 ? vexp - 14 : -14);
-    const float at = m == -INFINITY ? 0.f : now;
-    const float alpha = fast_exp2(ref - at);
-    ref = now;
+    for (int u = 0; u < SUB; ++u) top = max16(s[u], top);
+    top = max32(top) * unscale;
+    if constexpr (Q8) top += lds_load<float>(sc_base + (NDB + 1) * TK * 2);
+    const float alpha = move_ref(ref, top);
+    const float at = ref == -INFINITY ? 0.f : ref;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
@@ -317,7 +312,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
         for (int q = 0; q < 4; ++q) {
           const f16x4 x = lds_load<f16x4>(sc + (NDB * TK + 32 * u + 8 * q) * 2);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[u][4 * q + j] *= (float)x[j];
+          for (int j = 0; j < 4; ++j) s[u][4 * q + j] = fmaf(s[u][4 * q + j], (float)x[j], 0.f);
         }
       if (masked) {  // (a scale may not be finite: 0 times it is not 0)
 #pragma unroll
@@ -400,7 +395,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
     return;
   }
   if (!valid) return;
-  const float inv = m == -INFINITY ? 0.f : unit_o / lt;
+  const float inv = ref == -INFINITY ? 0.f : unit_o / lt;
   char* const out = reinterpret_cast<char*>(it.out) + (int64_t)token * p.o_s2 + (int64_t)h * p.o_s1;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
