@@ -88,7 +88,7 @@ hipError_t launch_rope_append(const RopeAppend& p, bool f16, hipStream_t stream)
 
 // tree.hip. Query rows per row tile for `rows` rows per KV head, and the
 // floats of one record (a row tile's part from one split).
-int tree_tile_rows(int rows, int elt);
+int tree_tile_rows(int rows);
 size_t tree_record_floats(int head_dim, int tile_rows);
 // elt: bytes of a cache element (4 F32, 2 F16, 1 8-bit). Every item's n_rt is
 // in tiles of tile_rows.

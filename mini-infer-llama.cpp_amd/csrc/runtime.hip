@@ -891,7 +891,7 @@ int run_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* masks, int n
       }
       most = std::max(most, a->n_tokens * a->n_rep);
     }
-    const int tile_rows = mi::tree_tile_rows(most, elt);
+    const int tile_rows = mi::tree_tile_rows(most);
     plan_tree(p, cnt, r0.head_dim, tile_rows, ws->part_bytes);
     hipError_t e = mi::launch_tree(p, cnt, r0.head_dim, elt, tile_rows, stream);
     if (e != hipSuccess) return hip_fail(e, "tree attention launch");

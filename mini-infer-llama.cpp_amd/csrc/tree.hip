@@ -619,9 +619,9 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const TreeParams p, i
   gstore(reinterpret_cast<char*>(it.out) + (int64_t)t * p.o_s2 + (int64_t)h * p.o_s1 + 16 * d4, acc * inv);
 }
 
-// F32: 32 or 64 rows. F16 and 8-bit caches: the wide kernel's 128 once 64 do
-// not hold them.
-int tree_tile_rows(int rows, int elt) { return rows <= 32 ? 32 : rows <= 64 || elt == 4 ? 64 : 128; }
+// The kernel that streams keys to registers for up to 32 rows, else the wide
+// kernel (tree_wide.hip), whose waves without rows only fetch.
+int tree_tile_rows(int rows) { return rows <= 32 ? 32 : 128; }
 
 size_t tree_record_floats(int head_dim, int tile_rows) { return (size_t)tile_rows * (head_dim + 2); }
 
