@@ -510,14 +510,13 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
     }
   }
   if (n_split > 1) {
-    // record: ROWS rows of D, then ref, then l
     float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * n_rt + rt) * n_split + sp) * (ROWS * (D + 2));
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
       const int idx = e * kTreeWaves * kWave + threadIdx.x;
-      float* const w = rec + (int64_t)(idx / 32) * D + NDB * (idx % 32);
+      float* const w = rec + tree_record_at(D, idx / 32, (NDB * (idx % 32)) & ~3);
       if constexpr (NDB == 4) gstore(w, f32x4{acc[e][0], acc[e][1], acc[e][2], acc[e][3]});
-      else gstore(w, f32x2{acc[e][0], acc[e][1]});
+      else gstore(w + 2 * (idx % 2), f32x2{acc[e][0], acc[e][1]});
     }
     if (wave == 0 && kh == 0) {
 #pragma unroll
@@ -547,30 +546,31 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
   }
 }
 
-// Joins the splits' records of a row: out = sum_s 2^(m_s - M) O_s / sum_s
-// 2^(m_s - M) l_s. D / 4 threads (four dims each) times `slices` threads a row:
-// a slice takes every slices-th record with a running maximum, kInFlight of
-// them on their way at once, and the slices meet in LDS in order. The records
-// were just written and come from the caches, so the time is their latency:
-// few records in turn per thread is what counts.
+// Joins the splits' records: out = sum_s 2^(ref_s - M) O_s / sum_s 2^(ref_s - M)
+// l_s. A wave takes 1 KB of the records, eight dims of 32 rows (lane: row lane %
+// 32, dims 4 (lane / 32) ..), `slices` waves every slices-th record each with a
+// running maximum, kInFlight of them on their way at once; the slices meet in
+// LDS in order. The records were just written and come from the caches, so the
+// time is their latency: few records in turn per wave is what counts.
 template <int D>
 __global__ __launch_bounds__(256) void tree_combine_kernel(const TreeParams p, int tile_rows, int slices) {
-  constexpr int LANES = D / 4;          // threads per (row, slice)
-  constexpr int GROUPS = 256 / LANES;   // (row, slice) pairs per workgroup
   constexpr int kInFlight = 4;
-  __shared__ f32x4 part[256];
-  __shared__ f32x2 ml[GROUPS];
+  __shared__ f32x4 part[4][kWave];
+  __shared__ f32x2 ml[4][kWave];
   const TreeItem& it = p.item[blockIdx.y];
   const int rows = it.n_tokens * p.n_rep, n_split = it.n_split;
   if (n_split <= 1) return;
-  const int grp = threadIdx.x / LANES, d4 = threadIdx.x % LANES;
-  const int slice = grp % slices;
-  const int row = blockIdx.x * (GROUPS / slices) + grp / slices;  // over the KV heads
-  const bool valid = row < rows * p.n_head_kv;
-  const int g = valid ? row / rows : 0, r = valid ? row % rows : 0;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int slice = wave % slices;
+  const int groups = (rows + 31) / 32;  // of 32 rows, per KV head
+  const int unit = blockIdx.x * (4 / slices) + wave / slices;
+  const int chunk = unit % (D / 8), grp = unit / (D / 8) % groups, g = unit / (D / 8) / groups;
+  const bool valid = g < p.n_head_kv;
   const int64_t rec_floats = (int64_t)tile_rows * (D + 2);
-  const float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * it.n_rt + r / tile_rows) * n_split) * rec_floats;
-  const int rr = r % tile_rows;
+  const int rt = grp * 32 / tile_rows, rr = grp * 32 % tile_rows;
+  const float* const rec =
+      p.rec + ((int64_t)it.rec0 + (int64_t)((valid ? g : 0) * it.n_rt + rt) * n_split) * rec_floats;
+  const int o_at = rr * D + chunk * 256 + lane * 4, m_at = tile_rows * D + rr + lane % 32, l_at = m_at + tile_rows;
   float mx = -INFINITY, l = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = slice; s0 < n_split; s0 += kInFlight * slices) {
@@ -580,9 +580,9 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const TreeParams p, i
     for (int u = 0; u < kInFlight; ++u) {
       const int s = s0 + u * slices;
       const float* const q = rec + (s < n_split ? s : s0) * rec_floats;
-      ms[u] = gload<float>(q + tile_rows * D + rr);
-      ls[u] = gload<float>(q + tile_rows * (D + 1) + rr);
-      os[u] = gload<f32x4>(q + rr * D + 4 * d4);
+      ms[u] = gload<float>(q + m_at);
+      ls[u] = gload<float>(q + l_at);
+      os[u] = gload<f32x4>(q + o_at);
     }
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
@@ -596,27 +596,29 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const TreeParams p, i
     }
   }
   if (slices > 1) {
-    part[threadIdx.x] = acc;
-    if (d4 == 0) ml[grp] = f32x2{mx, l};
+    part[wave][lane] = acc;
+    ml[wave][lane] = f32x2{mx, l};
     __syncthreads();
     if (slice != 0) return;
     float top = mx;
-    for (int s = 1; s < slices; ++s) top = fmaxf(top, ml[grp + s][0]);
+    for (int s = 1; s < slices; ++s) top = fmaxf(top, ml[wave + s][lane][0]);
     const float mu = top == -INFINITY ? 0.f : top;
     const float a = fast_exp2(mx - mu);
     acc *= a;
     l *= a;
     for (int s = 1; s < slices; ++s) {
-      const float b = fast_exp2(ml[grp + s][0] - mu);
-      acc += part[threadIdx.x + s * LANES] * b;
-      l += ml[grp + s][1] * b;
+      const float b = fast_exp2(ml[wave + s][lane][0] - mu);
+      acc += part[wave + s][lane] * b;
+      l += ml[wave + s][lane][1] * b;
     }
     mx = top;
   }
-  if (!valid) return;
+  const int r = grp * 32 + lane % 32;
+  if (!valid || r >= rows) return;
   const float inv = mx == -INFINITY ? 0.f : 1.f / l;
   const int t = r / p.n_rep, h = g * p.n_rep + r % p.n_rep;
-  gstore(reinterpret_cast<char*>(it.out) + (int64_t)t * p.o_s2 + (int64_t)h * p.o_s1 + 16 * d4, acc * inv);
+  gstore(reinterpret_cast<char*>(it.out) + (int64_t)t * p.o_s2 + (int64_t)h * p.o_s1 + 32 * chunk + 16 * (lane / 32),
+         acc * inv);
 }
 
 // The kernel that streams keys to registers for up to 32 rows, else the wide
@@ -638,13 +640,13 @@ static hipError_t launch_tree_d(const TreeParams& p, dim3 grid, int tile_rows, h
 
 hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, hipStream_t stream) {
   unsigned gx = 0;
-  int64_t rows = 0;  // of the longest split item, over its KV heads
+  int64_t units = 0;  // waves' worth of records to join, of the largest item
   int splits = 1;
   for (int i = 0; i < n_items; ++i) {
     const TreeItem& it = p.item[i];
-    const unsigned units = (unsigned)p.n_head_kv * it.n_split;
-    gx = std::max(gx, (units + 7) / 8 * 8 * (unsigned)it.n_rt);
-    if (it.n_split > 1) rows = std::max(rows, (int64_t)it.n_tokens * p.n_rep * p.n_head_kv);
+    gx = std::max(gx, ((unsigned)p.n_head_kv * it.n_split + 7) / 8 * 8 * (unsigned)it.n_rt);
+    if (it.n_split > 1)
+      units = std::max(units, ((int64_t)it.n_tokens * p.n_rep + 31) / 32 * p.n_head_kv * (head_dim / 8));
     splits = std::max(splits, it.n_split);
   }
   const dim3 grid(gx, n_items);
@@ -659,12 +661,10 @@ hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, 
     e = elt == 1   ? launch_tree_d<128, int8_t>(p, grid, tile_rows, stream)
         : elt == 2 ? launch_tree_d<128, _Float16>(p, grid, tile_rows, stream)
                    : launch_tree_d<128, float>(p, grid, tile_rows, stream);
-  if (e != hipSuccess || rows == 0) return e;
-  // slices: about four records each, as many as a workgroup has groups
-  const int groups = 256 / (head_dim / 4);
-  int slices = 1;
-  while (slices < groups && slices * 4 < splits) slices *= 2;
-  const dim3 cgrid((unsigned)((rows * slices + groups - 1) / groups), n_items);
+  if (e != hipSuccess || units == 0) return e;
+  // slices: about four records each
+  const int slices = splits > 8 ? 4 : splits > 4 ? 2 : 1;
+  const dim3 cgrid((unsigned)((units * slices + 3) / 4), n_items);
   if (head_dim == 64) hipLaunchKernelGGL(tree_combine_kernel<64>, cgrid, dim3(256), 0, stream, p, tile_rows, slices);
   else hipLaunchKernelGGL(tree_combine_kernel<128>, cgrid, dim3(256), 0, stream, p, tile_rows, slices);
   return hipGetLastError();

@@ -103,6 +103,14 @@ __device__ inline float move_ref(float& ref, float top) {
   return alpha;
 }
 
+// A record (a row tile's part from one split): its sums, then every row's
+// reference, then every row's sum of probabilities. The four dims d, d + 1, ..
+// (d a multiple of 4) of row r: 32 rows' pieces of 16 bytes lie together, those
+// of d and d + 4 in 1 KB, as the lanes of a wave hold them.
+__device__ inline int tree_record_at(int head_dim, int r, int d) {
+  return (r / 32) * 32 * head_dim + (d / 8) * 256 + ((d / 4) % 2) * 128 + (r % 32) * 4;
+}
+
 // The e for which scales up to `top` are below 2^e (at least that of the
 // smallest scale there is).
 __device__ inline int scale_exponent(float top) { return top > 0.f ? ilogbf(top) + 1 : -24; }

@@ -500,16 +500,15 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
   constexpr float unit_o = Q8 ? kByteUnscale : 1.f;  // of the values' 2^-10
   if (n_split > 1) {
     float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * n_rt + rt) * n_split + sp) * (ROWS * (D + 2));
-    const int rr = 32 * wave + c;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        gstore(rec + rr * D + 32 * db + 8 * q + 4 * kh,
+        gstore(rec + tree_record_at(D, 32 * wave + c, 32 * db + 8 * q + 4 * kh),
                f32x4{o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]} * unit_o);
     if (kh == 0) {
-      rec[ROWS * D + rr] = ref;
-      rec[ROWS * D + ROWS + rr] = lt;
+      rec[ROWS * D + 32 * wave + c] = ref;
+      rec[ROWS * D + ROWS + 32 * wave + c] = lt;
     }
     return;
   }
