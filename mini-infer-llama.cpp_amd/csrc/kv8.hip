@@ -17,6 +17,7 @@
 // Every kernel here reads each input once and writes each output once; the
 // arithmetic is far below what the memory takes.
 #include <cmath>
+#include <type_traits>
 
 #include "attn_common.h"
 #include "kernels.h"
@@ -24,6 +25,11 @@
 namespace mi {
 
 namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kGroup = 32;  // dims per K scale
 
@@ -68,6 +74,27 @@ __device__ inline float group_sum(float x) {
 #pragma unroll
   for (int off = N / 2; off >= 1; off >>= 1) x += __shfl_xor(x, off, kWave);
   return x;
+}
+
+// Over aligned groups of N = 4, 8 or 16 lanes (DPP moves within rows of 16).
+template <int N, typename T, typename F>
+__device__ inline T fold_lanes(T x, F f) {
+  auto move = [](T v, auto ctrl) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  x = f(x, move(x, std::integral_constant<int, 0xB1>{}));  // quad_perm [1,0,3,2]
+  x = f(x, move(x, std::integral_constant<int, 0x4E>{}));  // quad_perm [2,3,0,1]
+  if constexpr (N >= 8) x = f(x, move(x, std::integral_constant<int, 0x141>{}));   // row_half_mirror
+  if constexpr (N >= 16) x = f(x, move(x, std::integral_constant<int, 0x140>{}));  // row_mirror
+  return x;
+}
+template <int N>
+__device__ inline unsigned max_of_lanes(unsigned x) {
+  return fold_lanes<N>(x, [](unsigned a, unsigned b) { return max(a, b); });
+}
+template <int N>
+__device__ inline float sum_of_lanes(float x) {
+  return fold_lanes<N>(x, [](float a, float b) { return a + b; });
 }
 
 __device__ inline float ldf(const char* p, int64_t off) { return gload<float>(p + off); }
@@ -144,10 +171,57 @@ __global__ __launch_bounds__(256) void kv_quantize_kernel(const QuantizeArgs p) 
   store_row<E>(p.c, p.which, p.pos0 + t, h, lane, x);
 }
 
+// Rows of contiguous, 16-byte aligned values: a lane takes eight dims (a K
+// group is four lanes, a row D / 8), reads 32 bytes and writes 8.
+template <int D, int WHICH>
+__global__ __launch_bounds__(256) void kv_quantize_rows_kernel(const QuantizeArgs p) {
+  constexpr int LANES = D / 8;
+  const unsigned r = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int d = 8 * (threadIdx.x % LANES);
+  if (r >= (unsigned)p.rows) return;
+  const unsigned t = r / (unsigned)p.c.n_head_kv, h = r - t * (unsigned)p.c.n_head_kv;
+  const char* const src = p.src + t * p.nb[2] + h * p.nb[1] + 4 * d;
+  const f32x4 a = gload<f32x4>(src), b = gload<f32x4>(src + 16);
+  float x[8];
+  unsigned most = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = i < 4 ? a[i] : b[i - 4];
+    most = max(most, abs_bits(x[i]));
+  }
+  most = max_of_lanes<WHICH == 0 ? 4 : LANES>(most);
+  const unsigned sb = scale_bits(__builtin_bit_cast(float, most));
+  const float sc = f16_bits(sb), inv = inverse(sc);
+  u32x2 q = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q[i / 4] |= ((unsigned)quantize(x[i], sc, inv) & 0xffu) << (8 * (i % 4));
+  const int64_t pos = (int64_t)p.pos0 + t;
+  gstore(row_of(p.c, WHICH, pos, h) + d, q);
+  if (d % (WHICH == 0 ? kGroup : D) == 0)
+    gstore<unsigned short>(scale_of(p.c, WHICH, pos, h) + 2 * (d / kGroup), (unsigned short)sb);
+}
+
+// Whether rows (byte strides nb) can be read or written 16 bytes at a time,
+// `elt` bytes an element.
+static bool rows_aligned(const char* p, const int64_t nb[3], int elt) {
+  return nb[0] == elt && nb[1] % 16 == 0 && nb[2] % 16 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+}
+
 hipError_t launch_kv_quantize(const CacheView& c, int which, const char* src, const int64_t src_nb[3], int pos0,
                               int n_tokens, hipStream_t stream) {
   QuantizeArgs p{c, src, {src_nb[0], src_nb[1], src_nb[2]}, (int64_t)n_tokens * c.n_head_kv, which, pos0};
   if (p.rows == 0) return hipSuccess;
+  if (rows_aligned(src, src_nb, 4) && p.rows < INT32_MAX) {
+    const dim3 grid((unsigned)((p.rows * (c.head_dim / 8) + 255) / 256));
+    if (c.head_dim == 64) {
+      if (which == 0) hipLaunchKernelGGL((kv_quantize_rows_kernel<64, 0>), grid, dim3(256), 0, stream, p);
+      else hipLaunchKernelGGL((kv_quantize_rows_kernel<64, 1>), grid, dim3(256), 0, stream, p);
+    } else {
+      if (which == 0) hipLaunchKernelGGL((kv_quantize_rows_kernel<128, 0>), grid, dim3(256), 0, stream, p);
+      else hipLaunchKernelGGL((kv_quantize_rows_kernel<128, 1>), grid, dim3(256), 0, stream, p);
+    }
+    return hipGetLastError();
+  }
   const dim3 grid((unsigned)((p.rows + 3) / 4));
   if (c.head_dim == 64) hipLaunchKernelGGL(kv_quantize_kernel<1>, grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL(kv_quantize_kernel<2>, grid, dim3(256), 0, stream, p);
@@ -181,10 +255,65 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const ReadArgs p) {
   gstore<DT>(p.dst + t * p.nb[2] + h * p.nb[1] + d * p.nb[0], (DT)x);
 }
 
+// Into contiguous, 16-byte aligned rows: a lane takes eight dims.
+template <int D, int ELT, typename DT>
+__global__ __launch_bounds__(256) void kv_read_rows_kernel(const ReadArgs p) {
+  constexpr int LANES = D / 8;
+  const unsigned r = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int d = 8 * (threadIdx.x % LANES);
+  if (r >= (unsigned)p.rows) return;
+  const unsigned t = r / (unsigned)p.c.n_head_kv, h = r - t * (unsigned)p.c.n_head_kv;
+  const int64_t pos = (int64_t)p.pos0 + t;
+  const char* const row = row_of(p.c, p.which, pos, h) + d * ELT;
+  float x[8];
+  if constexpr (ELT == 1) {
+    const float sc = (float)gload<_Float16>(scale_of(p.c, p.which, pos, h) + (p.which == 0 ? 2 * (d / kGroup) : 0));
+    const u32x2 q = gload<u32x2>(row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)(int8_t)(q[i / 4] >> (8 * (i % 4)) & 0xffu) * sc;
+  } else if constexpr (ELT == 2) {
+    const f16x8 q = gload<f16x8>(row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)q[i];
+  } else {
+    const f32x4 a = gload<f32x4>(row), b = gload<f32x4>(row + 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < 4 ? a[i] : b[i - 4];
+  }
+  char* const dst = p.dst + t * p.nb[2] + h * p.nb[1] + d * (int)sizeof(DT);
+  if constexpr (sizeof(DT) == 2) {
+    f16x8 y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = (_Float16)x[i];
+    gstore(dst, y);
+  } else {
+    gstore(dst, f32x4{x[0], x[1], x[2], x[3]});
+    gstore(dst + 16, f32x4{x[4], x[5], x[6], x[7]});
+  }
+}
+
+template <int D, typename DT>
+static void launch_kv_read_rows(const ReadArgs& p, hipStream_t stream) {
+  const dim3 grid((unsigned)((p.rows * (D / 8) + 255) / 256));
+  if (p.c.elt == 1) hipLaunchKernelGGL((kv_read_rows_kernel<D, 1, DT>), grid, dim3(256), 0, stream, p);
+  else if (p.c.elt == 2) hipLaunchKernelGGL((kv_read_rows_kernel<D, 2, DT>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((kv_read_rows_kernel<D, 4, DT>), grid, dim3(256), 0, stream, p);
+}
+
 hipError_t launch_kv_read(const CacheView& c, int which, int pos0, int n_tokens, char* dst, bool dst_f16,
                           const int64_t dst_nb[3], hipStream_t stream) {
   ReadArgs p{c, dst, {dst_nb[0], dst_nb[1], dst_nb[2]}, (int64_t)n_tokens * c.n_head_kv, which, pos0};
   if (p.rows == 0) return hipSuccess;
+  if (rows_aligned(dst, dst_nb, dst_f16 ? 2 : 4) && p.rows < INT32_MAX) {
+    if (c.head_dim == 64) {
+      if (dst_f16) launch_kv_read_rows<64, _Float16>(p, stream);
+      else launch_kv_read_rows<64, float>(p, stream);
+    } else {
+      if (dst_f16) launch_kv_read_rows<128, _Float16>(p, stream);
+      else launch_kv_read_rows<128, float>(p, stream);
+    }
+    return hipGetLastError();
+  }
   const dim3 grid((unsigned)((p.rows * c.head_dim + 255) / 256));
   if (dst_f16) hipLaunchKernelGGL(kv_read_kernel<_Float16>, grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL(kv_read_kernel<float>, grid, dim3(256), 0, stream, p);
@@ -193,15 +322,25 @@ hipError_t launch_kv_read(const CacheView& c, int which, int pos0, int n_tokens,
 
 // Two bytes of one position's plane per thread, the kept rows in order: row
 // n_past + i is written after it has been read (as some idx[j] <= i, j <= i),
-// by the same thread, so the move may overlap itself.
+// by the same thread, so the move may overlap itself. kInFlight rows are read
+// before they are written: the rows of a batch lie at or behind where it writes
+// (idx[j] >= j), and so do those of the batches after it.
 __global__ __launch_bounds__(256) void kv_keep_kernel(const KvKeep p) {
+  constexpr int kInFlight = 8;
   const int plane = blockIdx.y % p.n_planes, layer = blockIdx.y / p.n_planes;
   const int at = 2 * (blockIdx.x * 256 + threadIdx.x);
   const int64_t row = p.bytes[plane];
   if (at >= row) return;
   char* const base = p.plane[plane] + layer * p.layer[plane] + (int64_t)p.n_past * row + at;
-  for (int i = 0; i < p.n; ++i)
-    if (p.idx[i] != i) gstore<unsigned short>(base + i * row, gload<unsigned short>(base + p.idx[i] * row));
+  for (int i = 0; i < p.n; i += kInFlight) {
+    unsigned short x[kInFlight];
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j)
+      if (i + j < p.n) x[j] = gload<unsigned short>(base + p.idx[i + j] * row);
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j)
+      if (i + j < p.n) gstore<unsigned short>(base + (i + j) * row, x[j]);
+  }
 }
 
 hipError_t launch_kv_keep(const KvKeep& p, hipStream_t stream) {
@@ -276,7 +415,154 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
   }
 }
 
+// All dims rotated, rows contiguous and 16-byte aligned: D / 8 lanes a row, each
+// with dims 4 j .. 4 j + 3 and their partners D / 2 further on. A workgroup
+// takes `tokens` tokens (gridDim.y pieces of their rows): the angles' cosines
+// and sines once per token in LDS (double precision, about as much work as the
+// rest of a token's rows together), then the rows from registers to the cache.
+// K on its way to an 8-bit cache stays in double precision until it is
+// quantised, since a value next to a border between two steps should not cross
+// it by a rounding.
+constexpr int kRopeTokens = 4;
+
+template <int D>
+__global__ __launch_bounds__(256) void norm_rope_kernel(const NormRope p, int tokens) {
+  constexpr int LANES = D / 8, HALF = D / 2;
+  __shared__ float2 cs[kRopeTokens][HALF];
+  __shared__ double cs_d[kRopeTokens][HALF][2];  // 8-bit caches
+  const int hkv = p.cache.n_head_kv, per_tok = p.n_head + 2 * hkv;
+  const int t0 = blockIdx.x * tokens, nt = min(tokens, p.n_tokens - t0);
+  const bool q8 = p.cache.elt == 1;
+  for (int i = threadIdx.x; i < nt * HALF; i += 256) {
+    const int t = i / HALF, j = i % HALF;
+    const int pos = p.pos ? gload<int>(p.pos + t0 + t) : p.n_past + t0 + t;
+    double sn, c;
+    sincos((double)((float)pos * p.freq[j]), &sn, &c);
+    cs[t][j] = float2{(float)c, (float)sn};
+    if (q8) {
+      cs_d[t][j][0] = c;
+      cs_d[t][j][1] = sn;
+    }
+  }
+  __syncthreads();
+  const int j4 = 4 * (threadIdx.x % LANES);
+  const int step = 256 / LANES * gridDim.y;
+  for (int row = blockIdx.y * (256 / LANES) + threadIdx.x / LANES; row < nt * per_tok; row += step) {
+    const int t = row / per_tok;
+    int h = row - t * per_tok;
+    const int kind = h < p.n_head ? 0 : h < p.n_head + hkv ? 1 : 2;  // Q, K, V
+    h -= kind == 0 ? 0 : kind == 1 ? p.n_head : p.n_head + hkv;
+    const char* const src = (kind == 0 ? p.q : kind == 1 ? p.k : p.v) +
+                            (t0 + t) * (kind == 0 ? p.q_nb[2] : kind == 1 ? p.k_nb[2] : p.v_nb[2]) +
+                            h * (kind == 0 ? p.q_nb[1] : kind == 1 ? p.k_nb[1] : p.v_nb[1]) + 4 * j4;
+    f32x4 a = gload<f32x4>(src), b = gload<f32x4>(src + 4 * HALF);
+    if (kind < 2) {
+      const float* const w = kind == 0 ? p.q_norm : p.k_norm;
+      f32x4 wa = {1.f, 1.f, 1.f, 1.f}, wb = wa;
+      if (w) {
+        wa = gload<f32x4>(w + j4);
+        wb = gload<f32x4>(w + HALF + j4);
+      }
+      if (q8 && kind == 1) {
+        double inv = 1.0;
+        if (w) {
+          double ss = 0.0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ss += (double)a[i] * a[i] + (double)b[i] * b[i];
+#pragma unroll
+          for (int off = LANES / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, kWave);
+          inv = 1.0 / sqrt(ss / D + (double)p.eps);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const double x = a[i] * inv * wa[i], y = b[i] * inv * wb[i];
+          const double c = cs_d[t][j4 + i][0], sn = cs_d[t][j4 + i][1];
+          a[i] = (float)(x * c - y * sn);
+          b[i] = (float)(x * sn + y * c);
+        }
+      } else {
+#pragma clang fp contract(off)
+        if (w) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ss += a[i] * a[i] + b[i] * b[i];
+          const float inv = 1.f / sqrtf(sum_of_lanes<LANES>(ss) / D + p.eps);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            a[i] = a[i] * inv * wa[i];
+            b[i] = b[i] * inv * wb[i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 r = cs[t][j4 + i];
+          const float x = a[i], y = b[i];
+          a[i] = x * r.x - y * r.y;
+          b[i] = x * r.y + y * r.x;
+        }
+      }
+    }
+    if (kind == 0) {
+      char* const o = p.q_out + (t0 + t) * p.qo_nb[2] + h * p.qo_nb[1] + 4 * j4;
+      gstore(o, a);
+      gstore(o + 4 * HALF, b);
+      continue;
+    }
+    const int64_t pos = (int64_t)p.n_past + t0 + t;
+    char* const o = row_of(p.cache, kind - 1, pos, h);
+    if (q8) {
+      unsigned ma = 0, mb = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ma = max(ma, abs_bits(a[i]));
+        mb = max(mb, abs_bits(b[i]));
+      }
+      if (kind == 1) {
+        ma = max_of_lanes<8>(ma);
+        mb = max_of_lanes<8>(mb);
+      } else {
+        ma = mb = max_of_lanes<LANES>(max(ma, mb));
+      }
+      const unsigned ba = scale_bits(__builtin_bit_cast(float, ma)), bb = scale_bits(__builtin_bit_cast(float, mb));
+      const float da = f16_bits(ba), db = f16_bits(bb), ia = inverse(da), ib = inverse(db);
+      unsigned qa = 0, qb = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        qa |= ((unsigned)quantize(a[i], da, ia) & 0xffu) << (8 * i);
+        qb |= ((unsigned)quantize(b[i], db, ib) & 0xffu) << (8 * i);
+      }
+      gstore(o + j4, qa);
+      gstore(o + HALF + j4, qb);
+      char* const sc = scale_of(p.cache, kind - 1, pos, h);
+      if (kind == 1 && j4 % kGroup == 0) {
+        gstore<unsigned short>(sc + 2 * (j4 / kGroup), (unsigned short)ba);
+        gstore<unsigned short>(sc + 2 * ((HALF + j4) / kGroup), (unsigned short)bb);
+      }
+      if (kind == 2 && j4 == 0) gstore<unsigned short>(sc, (unsigned short)ba);
+    } else if (p.cache.elt == 2) {
+      gstore(o + 2 * j4, f16x4{(_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3]});
+      gstore(o + 2 * (HALF + j4), f16x4{(_Float16)b[0], (_Float16)b[1], (_Float16)b[2], (_Float16)b[3]});
+    } else {
+      gstore(o + 4 * j4, a);
+      gstore(o + 4 * (HALF + j4), b);
+    }
+  }
+}
+
 hipError_t launch_norm_rope(const NormRope& p, hipStream_t stream) {
+  const auto at16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
+  if (p.n_dims == p.cache.head_dim && (!p.q || (rows_aligned(p.q, p.q_nb, 4) && rows_aligned(p.q_out, p.qo_nb, 4))) &&
+      rows_aligned(p.k, p.k_nb, 4) && rows_aligned(p.v, p.v_nb, 4) && at16(p.q_norm) && at16(p.k_norm)) {
+    if (p.n_tokens == 0) return hipSuccess;
+    // few tokens: a workgroup per 256 lanes' worth of a token's rows
+    const int per_tok = p.n_head + 2 * p.cache.n_head_kv, rows = 256 / (p.cache.head_dim / 8);
+    const bool few = p.n_tokens < 512;
+    const dim3 grid((unsigned)(few ? p.n_tokens : (p.n_tokens + kRopeTokens - 1) / kRopeTokens),
+                    (unsigned)(few ? (per_tok + rows - 1) / rows : 1));
+    if (p.cache.head_dim == 64) hipLaunchKernelGGL(norm_rope_kernel<64>, grid, dim3(256), 0, stream, p, few ? 1 : kRopeTokens);
+    else hipLaunchKernelGGL(norm_rope_kernel<128>, grid, dim3(256), 0, stream, p, few ? 1 : kRopeTokens);
+    return hipGetLastError();
+  }
   const int64_t rows = (int64_t)p.n_tokens * (p.n_head + 2 * p.cache.n_head_kv);
   if (rows == 0) return hipSuccess;
   const dim3 grid((unsigned)((rows + 3) / 4));

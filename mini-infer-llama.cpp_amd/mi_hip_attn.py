@@ -210,6 +210,9 @@ class AllocStats(ctypes.Structure):
                 ("bytes_live", ctypes.c_uint64), ("bytes_peak", ctypes.c_uint64)]
 
 
+_Strides = ctypes.c_size_t * 3
+
+
 # Every symbol include/mi_hip_attn.h and include/mi_hip_qwen2.h declare, with
 # its ctypes signature.
 _P = ctypes.c_void_p
@@ -352,13 +355,13 @@ class Lib:
     def kv_write(self, kv, layer, which, pos0, src, stream):
         """Rows of an F32 device tensor (n_tokens, n_head_kv, head_dim) into K (which 0) or V (1)."""
         self.check(self.so.mi_hip_kv_write(kv, layer, which, pos0, src.shape[0], src.data_ptr(),
-                                           (ctypes.c_size_t * 3)(*nb3_of(src)), 1, stream))
+                                           _Strides(*nb3_of(src)), 1, stream))
 
     def kv_read(self, kv, layer, which, pos0, dst, stream):
         """Cache rows into a device tensor (n_tokens, n_head_kv, head_dim), F32 or F16."""
         kind = MI_TYPE_F16 if dst.element_size() == 2 else MI_TYPE_F32
         self.check(self.so.mi_hip_kv_read(kv, layer, which, pos0, dst.shape[0], dst.data_ptr(), kind,
-                                          (ctypes.c_size_t * 3)(*nb3_of(dst)), stream))
+                                          _Strides(*nb3_of(dst)), stream))
 
     def kv_keep(self, kv, n_past, idx, stream):
         """Rows n_past + idx[i] become rows n_past + i (idx: whole numbers on the host, increasing)."""
