@@ -159,11 +159,11 @@ struct LogitsAdjust {
   const char* mask;        // bit t of a row's 32-bit words: token t is allowed; null: all
   int64_t mask_nb;
   int32_t* ids;            // greedy ids; null: not asked for
-  uint64_t* part;          // n_rows * logits_chunks(n_vocab) words of scratch when ids are
+  uint64_t* part;          // scratch for ids: logits_chunks(n_vocab) words a row
   int32_t n_vocab, n_rows;
 };
 int logits_chunks(int n_vocab);
-hipError_t launch_logits_adjust(const LogitsAdjust& p, hipStream_t stream);
+hipError_t launch_logits_adjust(const LogitsAdjust& p, int n_cu, hipStream_t stream);
 
 // mul_mat.hip. Activation rows (F32, ne0 a multiple of 32, contiguous within
 // a row) -> Q8_0_ACT blocks; Q8_0 weight rows . activation columns -> F32.

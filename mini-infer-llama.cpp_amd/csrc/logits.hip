@@ -8,12 +8,15 @@
 // every product, sum and quotient rounded on its own, and id = the lowest t of
 // the largest y that is neither -inf nor NaN, -1 if there is none.
 //
-// A workgroup owns a chunk of one row. It counts the history's tokens that lie
-// in its chunk in LDS (whole numbers, so the atomics' order does not show),
-// adds up the biases, passes over its logits once and leaves the chunk's best
-// as one 64-bit key (value order, then lower token); a second kernel takes
-// the row's best. Each logit is read and written once; a row's history is
-// read by every chunk of the row, from the caches.
+// A workgroup owns a chunk of one row. Its logits are on their way while it
+// counts the history's tokens that lie in the chunk in LDS (whole numbers, so the
+// atomics' order does not show) and one wave adds up the biases; then each logit
+// is finished, stored, and the chunk's best kept as one 64-bit key (value order,
+// then lower token). A second kernel takes the row's best. Each logit is read
+// and written once; a row's history is read by every chunk of the row, from the
+// caches. Bound: memory for many rows, the chain of dependent loads (offsets,
+// history, LDS) for few; there the chunks are smaller, so that more workgroups
+// share a row.
 #include "attn_common.h"
 #include "kernels.h"
 
@@ -23,8 +26,14 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kChunk = 4096;
+// Chunks of 2048: 16 KB of LDS, so that eight workgroups fit a CU and their
+// chains of loads overlap (64 rows of 151936 with histories and a mask: 29.7 us;
+// 4096 a chunk 35.0, 1024, where the histories are read twice as often, 34.7).
+// Chunks of 1024 while a launch has at most four of them per CU (one row of
+// 151936: 149 workgroups instead of 75).
 constexpr int kThreads = 256;
+constexpr int kSmallChunk = 4 * kThreads, kChunk = 8 * kThreads;
+constexpr int64_t kFewPerCu = 4;
 
 // Larger for the larger value, and for the lower token among equal values; 0
 // for what is never chosen.
@@ -47,85 +56,116 @@ __device__ inline uint64_t wave_max_u64(uint64_t x) {
 
 }  // namespace
 
+template <int CHUNK>
 __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) {
-  __shared__ unsigned count[kChunk];
-  __shared__ float bias[kChunk];
+  constexpr int PER = CHUNK / (4 * kThreads);  // groups of four logits per thread
+  constexpr int kInFlight = 8;                 // history ids per thread
+  __shared__ __attribute__((aligned(16))) unsigned count[CHUNK];
+  __shared__ __attribute__((aligned(16))) float bias[CHUNK];
   __shared__ uint64_t best[kThreads / kWave];
-  const int row = blockIdx.y, base = blockIdx.x * kChunk;
-  const int n = min(kChunk, p.n_vocab - base);
+  const int row = blockIdx.y, base = blockIdx.x * CHUNK;
+  const int n = min(CHUNK, p.n_vocab - base);
   const int tid = threadIdx.x, lane = tid % kWave;
-  const int h0 = p.hist && p.penalties ? p.hist_off[row] : 0, h1 = p.hist && p.penalties ? p.hist_off[row + 1] : 0;
+  const int h0 = p.hist ? p.hist_off[row] : 0, h1 = p.hist ? p.hist_off[row + 1] : 0;
   const int b0 = p.bias_id ? p.bias_off[row] : 0, b1 = p.bias_id ? p.bias_off[row + 1] : 0;
   const bool counts = h1 > h0, biases = b1 > b0;
-  if (counts || biases) {
-    for (int i = tid; i < kChunk; i += kThreads) {
-      count[i] = 0u;
-      bias[i] = 0.f;
-    }
-    __syncthreads();
-    for (int i = h0 + tid; i < h1; i += kThreads) {
-      const unsigned at = (unsigned)p.hist[i] - (unsigned)base;
-      if (at < (unsigned)n) atomicAdd(&count[at], 1u);
-    }
-    // One wave adds the biases, lane by lane, so that a token that is listed
-    // twice gets the same sum every time.
-    if (tid < kWave) {
-      for (int i = b0; i < b1; i += kWave) {
-        const unsigned at = i + lane < b1 ? (unsigned)p.bias_id[i + lane] - (unsigned)base : ~0u;
-        const float v = i + lane < b1 ? p.bias[i + lane] : 0.f;
-        uint64_t todo = __builtin_amdgcn_ballot_w64(at < (unsigned)n);
-        while (todo) {
-          const int who = __builtin_ctzll(todo);
-          todo &= todo - 1;
-          if (lane == who) bias[at] += v;
-          wave_lds_fence();
-        }
-      }
-    }
-    __syncthreads();
-  }
-  const float repeat = p.penalties ? p.penalties[3 * row] : 1.f;
-  const float frequency = p.penalties ? p.penalties[3 * row + 1] : 0.f;
-  const float presence = p.penalties ? p.penalties[3 * row + 2] : 0.f;
   const char* const in = p.in + row * p.in_nb + 4 * (int64_t)base;
   char* const out = p.out + row * p.out_nb + 4 * (int64_t)base;
   const char* const mask = p.mask ? p.mask + row * p.mask_nb + base / 8 : nullptr;
   const bool vec = ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  uint64_t top = 0ull;
-  for (int i = 4 * tid; i < n; i += 4 * kThreads) {
-#pragma clang fp contract(off)
-    float x[4];
-    const int m = min(4, n - i);
-    if (vec && m == 4) {
+
+  // Group k of thread tid: logits 4 (tid + 256 k) .. of the chunk.
+  float x[PER][4];
+  unsigned allow[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = 4 * (tid + kThreads * k);
+    allow[k] = ~0u;
+    if (vec && i + 4 <= n) {
       const f32x4 v = gload<f32x4>(in + 4 * i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = v[j];
+      for (int j = 0; j < 4; ++j) x[k][j] = v[j];
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = j < m ? gload<float>(in + 4 * (i + j)) : -INFINITY;
+      for (int j = 0; j < 4; ++j) x[k][j] = i + j < n ? gload<float>(in + 4 * (i + j)) : -INFINITY;
     }
-    const unsigned allow = mask ? gload<unsigned>(mask + (i / 32) * 4) >> (i % 32) : ~0u;
+    if (mask && i < n) allow[k] = gload<unsigned>(mask + (i / 32) * 4) >> (i % 32);
+  }
+  if (counts || biases) {
+    // (the lists' first loads are on their way while LDS is cleared)
+    unsigned at[kInFlight];
+    auto read_hist = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+        at[u] = i + u * kThreads < h1 ? (unsigned)p.hist[i + u * kThreads] - (unsigned)base : ~0u;
+    };
+    unsigned bat = ~0u;
+    float bval = 0.f;
+    auto read_bias = [&](int i) __attribute__((always_inline)) {
+      bat = i < b1 ? (unsigned)p.bias_id[i] - (unsigned)base : ~0u;
+      bval = i < b1 ? p.bias[i] : 0.f;
+    };
+    read_hist(h0 + tid);
+    if (tid < kWave) read_bias(b0 + lane);
+    for (int i = 4 * tid; i < CHUNK; i += 4 * kThreads) {
+      *reinterpret_cast<f32x4*>(count + i) = f32x4{0.f, 0.f, 0.f, 0.f};
+      *reinterpret_cast<f32x4*>(bias + i) = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __syncthreads();
+    for (int i = h0 + tid; i < h1;) {
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+        if (at[u] < (unsigned)n) atomicAdd(&count[at[u]], 1u);
+      i += kInFlight * kThreads;
+      if (i < h1) read_hist(i);
+    }
+    // One wave adds the biases, lane by lane, so that a token that is listed
+    // twice gets the same sum every time.
+    if (tid < kWave) {
+      for (int i = b0; i < b1;) {
+        uint64_t todo = __builtin_amdgcn_ballot_w64(bat < (unsigned)n);
+        while (todo) {
+          const int who = __builtin_ctzll(todo);
+          todo &= todo - 1;
+          if (lane == who) bias[bat] += bval;
+          wave_lds_fence();
+        }
+        i += kWave;
+        if (i < b1) read_bias(i + lane);
+      }
+    }
+    __syncthreads();
+  }
+  const float repeat = counts ? p.penalties[3 * row] : 1.f;
+  const float frequency = counts ? p.penalties[3 * row + 1] : 0.f;
+  const float presence = counts ? p.penalties[3 * row + 2] : 0.f;
+  uint64_t top = 0ull;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+#pragma clang fp contract(off)
+    const int i = 4 * (tid + kThreads * k);
+    if (i >= n) break;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (j >= m) continue;
+      float y = x[k][j];
       if (counts) {
         const unsigned c = count[i + j];
-        if (c > 0u) {
-          const float y = x[j] > 0.f ? x[j] / repeat : x[j] * repeat;
-          x[j] = y - ((float)c * frequency + presence);
-        }
+        if (c > 0u) y = (y > 0.f ? y / repeat : y * repeat) - ((float)c * frequency + presence);
       }
-      if (biases) x[j] += bias[i + j];
-      if (!(allow >> j & 1u)) x[j] = -INFINITY;
-      const uint64_t k = key_of(x[j], base + i + j);
-      top = k > top ? k : top;
+      if (biases) y += bias[i + j];
+      if (!(allow[k] >> j & 1u)) y = -INFINITY;
+      x[k][j] = y;
+      if (i + j < n) {
+        const uint64_t key = key_of(y, base + i + j);
+        top = key > top ? key : top;
+      }
     }
-    if (vec && m == 4) {
-      gstore(out + 4 * i, f32x4{x[0], x[1], x[2], x[3]});
+    if (vec && i + 4 <= n) {
+      gstore(out + 4 * i, f32x4{x[k][0], x[k][1], x[k][2], x[k][3]});
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (j < m) gstore<float>(out + 4 * (i + j), x[j]);
+        if (i + j < n) gstore<float>(out + 4 * (i + j), x[k][j]);
     }
   }
   if (!p.ids) return;
@@ -150,11 +190,14 @@ __global__ __launch_bounds__(kWave) void logits_best_kernel(const uint64_t* part
   if (threadIdx.x == 0) ids[blockIdx.x] = top ? (int32_t)~(unsigned)top : -1;
 }
 
-int logits_chunks(int n_vocab) { return (n_vocab + kChunk - 1) / kChunk; }
+int logits_chunks(int n_vocab) { return (n_vocab + kSmallChunk - 1) / kSmallChunk; }
 
-hipError_t launch_logits_adjust(const LogitsAdjust& p, hipStream_t stream) {
-  const int chunks = logits_chunks(p.n_vocab);
-  hipLaunchKernelGGL(logits_kernel, dim3(chunks, p.n_rows), dim3(kThreads), 0, stream, p);
+hipError_t launch_logits_adjust(const LogitsAdjust& p, int n_cu, hipStream_t stream) {
+  // small chunks while they leave at most a few workgroups per CU
+  const bool small = (int64_t)logits_chunks(p.n_vocab) * p.n_rows <= kFewPerCu * n_cu;
+  const int chunk = small ? kSmallChunk : kChunk, chunks = (p.n_vocab + chunk - 1) / chunk;
+  if (small) hipLaunchKernelGGL(logits_kernel<kSmallChunk>, dim3(chunks, p.n_rows), dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL(logits_kernel<kChunk>, dim3(chunks, p.n_rows), dim3(kThreads), 0, stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.ids) return e;
   hipLaunchKernelGGL(logits_best_kernel, dim3(p.n_rows), dim3(kWave), 0, stream, p.part, chunks, p.ids);

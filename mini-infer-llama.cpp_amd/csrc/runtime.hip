@@ -1889,7 +1889,7 @@ int mi_hip_logits_adjust(const mi_hip_logits_args* a) {
     p.bias_off = a->bias_off ? a->bias_off + r : nullptr;
     p.mask = a->mask ? reinterpret_cast<const char*>(a->mask) + r * p.mask_nb : nullptr;
     p.ids = a->ids ? a->ids + r : nullptr;
-    hipError_t e = mi::launch_logits_adjust(p, static_cast<hipStream_t>(a->stream));
+    hipError_t e = mi::launch_logits_adjust(p, g.n_cu, static_cast<hipStream_t>(a->stream));
     if (e != hipSuccess) return hip_fail(e, "logits launch");
   }
   return MI_HIP_OK;
