@@ -47,7 +47,9 @@ __device__ inline u32x2 lds_transposed(const lds_t* p) {
 // The exponents of F32 rows: 2^-e times the row's largest lies in [2^14, 2^15).
 // Not below -90: the probabilities of a row are relative to what includes e
 // (move_ref), and their sum has to stay in float's range.
-__device__ inline int row_exponent(float most) { return most > 0.f ? max(ilogbf(most) - 14, -90) : -90; }
+__device__ inline int row_exponent(float most) {
+  return max((int)(__builtin_bit_cast(unsigned, most) >> 23) - 127 - 14, -90);
+}
 
 // Maximum over aligned groups of N = 8 or 16 lanes.
 template <int N>
@@ -82,10 +84,13 @@ struct WideCfg {
   static constexpr int SC_K = 0, SC_V = Q8 ? NDB * TK * 2 : TK * 4, SC_E = SC_V + TK * 4, SC = SC_E + TK * 2;
   static constexpr int L_NF = L_SC + (ELT == 2 ? 0 : 2 * SC);  // per buffer: the last tile with values that are not finite
   static constexpr int LDS = L_NF + 16;
+  // F32 tiles at head_dim 128 take more registers than two workgroups per CU
+  // leave each other.
+  static constexpr int WAVES_PER_SIMD = D == 128 && F32 ? 1 : 2;
 };
 
 template <int D, typename KT>
-__global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const TreeParams p) {
+__global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)) void tree_wide_kernel(const TreeParams p) {
   typedef WideCfg<D, KT> C;
   constexpr int NDB = C::NDB, ROWS = C::ROWS, ELT = C::ELT, TK = C::TK, SUB = C::SUB, NSLOT = C::NSLOT, PER = C::PER;
   constexpr int PL = C::PL, PLANE = C::PLANE;
@@ -181,9 +186,16 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
   auto row_most = [](const unsigned (&w)[WORDS]) __attribute__((always_inline)) {
     float most = 0.f;
 #pragma unroll
-    for (int j = 0; j < WORDS; ++j) {
-      const float x = fabsf(__builtin_bit_cast(float, w[j]));
-      most = fmaxf(most, x < INFINITY ? x : 0.f);
+    for (int j = 0; j < WORDS; j += 2)
+      most = __builtin_elementwise_maximum(__builtin_elementwise_maximum(most, fabsf(__builtin_bit_cast(float, w[j]))),
+                                           fabsf(__builtin_bit_cast(float, w[j + 1])));
+    if (__builtin_amdgcn_ballot_w64(!(most < INFINITY)) != 0ull) {
+      most = 0.f;
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j) {
+        const float x = fabsf(__builtin_bit_cast(float, w[j]));
+        most = fmaxf(most, x < INFINITY ? x : 0.f);
+      }
     }
     return max_lanes<NSLOT>(most);
   };
@@ -201,7 +213,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
       int e = 0;
       if constexpr (F32) {
         e = row_exponent(row_most(kw[i]));
-        if (s == 0) lds_store<int>(sc + C::SC_K + 4 * r, e);
+        lds_store<int>(sc + C::SC_K + 4 * r, e);  // (by all of the row's threads)
       }
       widen(kw[i], e, x);
 #pragma unroll
@@ -209,10 +221,8 @@ __global__ __launch_bounds__(kTreeWaves* kWave, 2) void tree_wide_kernel(const T
         lds_store<u32x4>(lds + C::L_K + buf * C::TILE + pl * PLANE + r * (2 * D) + 16 * (s ^ swz<NSLOT>(r)), x[pl]);
       if constexpr (F32) {
         e = row_exponent(row_most(vw[i]));
-        if (s == 0) {
-          lds_store<float>(sc + C::SC_V + 4 * r, ldexpf(1.f, e));
-          lds_store<_Float16>(sc + C::SC_E + 2 * r, (_Float16)e);
-        }
+        lds_store<float>(sc + C::SC_V + 4 * r, ldexpf(1.f, e));
+        lds_store<_Float16>(sc + C::SC_E + 2 * r, (_Float16)e);
       }
       if constexpr (!Q8) {
         if (masked) {
