@@ -11,14 +11,15 @@
 // that sees no key has m = -inf and an output of zeros.
 //
 // Decomposition. The n_tokens * n_rep query rows that read one KV head are
-// cut into row tiles of 32 RT rows (row r is token r / n_rep, head r % n_rep
-// of the group); the keys into splits of whole 32-key tiles. A workgroup owns
-// (item, KV head, row tile, split); its waves take the split's key tiles in
-// turn, every wave all of the tile's rows, so K and V come from memory once
-// per row tile and straight to registers. The waves meet in LDS; with one
-// split the result is the output, otherwise it is a record in the workspace
-// that tree_combine_kernel joins (a second launch, so that neither needs a
-// counter and both may be captured into a graph).
+// cut into row tiles (row r is token r / n_rep, head r % n_rep of the group),
+// the keys into splits of whole 32-key tiles. A workgroup owns (item, KV head,
+// row tile, split). With one split its result is the output, otherwise it is a
+// record in the workspace that tree_combine_kernel joins (a second launch, so
+// that neither needs a counter and both may be captured into a graph).
+//
+// This kernel: row tiles of 32, for calls that need no more. Its waves take the
+// split's key tiles in turn, K and V straight to registers, and meet in LDS at
+// the end. (More rows: tree_wide.hip.)
 //
 // Per key tile (lane = (c = lane % 32, kh = lane / 32)), 32x32 MFMAs:
 //   S^T = K . Q^T: A is K (key c), B the queries (row c); a lane ends up with
@@ -38,7 +39,7 @@
 // relative to the row's largest element.
 //   8-bit K: a row's scales (one per 32 dims) multiply the S^T of their own
 //   32 dims. 8-bit V: the row's one scale multiplies the probability; ref keeps
-//   the largest probability times the tile's largest scale in that range.
+//   the largest such product in that range.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -48,27 +49,29 @@
 namespace mi {
 
 // KT: float, _Float16 or int8_t.
-template <int D, typename KT, int RT>
+template <int D, typename KT>
 struct TreeCfg {
   static constexpr int ELT = (int)sizeof(KT);
   static constexpr bool Q8 = ELT == 1, F32 = ELT == 4;
   static constexpr int NDB = D / 32;             // output blocks of 32 dims; scales per 8-bit K row
-  static constexpr int ROWS = 32 * RT;
+  static constexpr int ROWS = 32;
   static constexpr int KW = D * ELT / 8;         // 32-bit words of K per lane and tile
   static constexpr int VW = NDB * ELT >= 4 ? NDB * ELT / 4 : 1;  // words of V per lane and key
   static constexpr int XS = 36;                  // exchange row stride (floats)
   static constexpr int L_X = 0;                  // waves' outputs of one 32-dim block
-  static constexpr int L_ML = kTreeWaves * ROWS * XS * 4;  // m, l per wave and row
+  static constexpr int L_ML = kTreeWaves * ROWS * XS * 4;  // reference, sum per wave and row
   static constexpr int LDS = L_ML + kTreeWaves * ROWS * 2 * 4;
   // While the keys stream, a wave keeps the tile's scales in its own part of
-  // the exchange area: NDB blocks of 32 K scales, then 32 V scales.
-  static constexpr int SC = (NDB + 1) * 32 * 4;
+  // the exchange area: NDB blocks of 32 K scales, 32 V scales, 32 exponents.
+  static constexpr int SC = (NDB + 2) * 32 * 4;
   static_assert(SC <= ROWS * XS * 4, "scales fit a wave's exchange area");
+  // head_dim 128 takes more registers than two workgroups per CU leave.
+  static constexpr int WAVES_PER_SIMD = D == 64 ? 2 : 1;
 };
 
-template <int D, typename KT, int RT>
-__global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kernel(const TreeParams p) {
-  typedef TreeCfg<D, KT, RT> C;
+template <int D, typename KT>
+__global__ __launch_bounds__(kTreeWaves* kWave, (TreeCfg<D, KT>::WAVES_PER_SIMD)) void tree_kernel(const TreeParams p) {
+  typedef TreeCfg<D, KT> C;
   constexpr int NDB = C::NDB, ROWS = C::ROWS, ELT = C::ELT, KW = C::KW, VW = C::VW;
   constexpr bool Q8 = C::Q8, F32 = C::F32;
   __shared__ __attribute__((aligned(16))) char lds_raw[C::LDS];
@@ -88,99 +91,23 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
   const int unit = (y / n_rt) * 8 + (int)((blockIdx.x - it.xcd0) % 8);
   if (unit >= p.n_head_kv * n_split) return;
   const int g = unit / n_split, sp = unit % n_split;
-  const int n_kv = it.n_past + it.n_tokens;
+  const int n_past = it.n_past, n_kv = n_past + it.n_tokens;
   const int rows = it.n_tokens * p.n_rep;
   const int row0 = rt * ROWS;
   // keys that some row of the tile may see
   const int last_token = min(row0 + ROWS - 1, rows - 1) / p.n_rep;
-  const int lim = it.mask ? n_kv : min(n_kv, it.n_past + last_token + 1);
+  const int lim = it.mask ? n_kv : min(n_kv, n_past + last_token + 1);
   const int tile0 = sp * it.tiles_per_split;
   const int tile1 = min(tile0 + it.tiles_per_split, (lim + kTreeTile - 1) / kTreeTile);
-
-  const char* const kbase = it.k + (int64_t)g * p.k_s1;
-  const char* const vbase = it.v + (int64_t)g * p.v_s1;
-  const int ks2 = (int)p.k_s2, vs2 = (int)p.v_s2;
-
-  // ---- queries ------------------------------------------------------------
-  // Dims of B's step s, lane half kh, element j (A's are loaded the same way):
-  // F32 8 (s / 4) + 4 kh + s % 4; F16 16 s + 8 kh + j; 8-bit
-  // 32 (s / 2) + 16 kh + 8 (s % 2) + j. Each is 16 consecutive bytes of K.
-  float qf[F32 ? RT : 1][F32 ? D / 2 : 1];
-  f16x8 qh[F32 ? 1 : RT][F32 ? 1 : D / 16], ql[F32 ? 1 : RT][F32 ? 1 : D / 16];
-  float unscale[RT];
-  int token[RT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int r = row0 + 32 * i + c;
-    const bool valid = r < rows;
-    token[i] = valid ? r / p.n_rep : 0;
-    const int h = g * p.n_rep + (valid ? r - token[i] * p.n_rep : 0);
-    const char* const qp = reinterpret_cast<const char*>(it.q) + (int64_t)token[i] * p.q_s2 + (int64_t)h * p.q_s1;
-    const float sc = valid ? p.scale_log2e : 0.f;
-    unscale[i] = 1.f;
-    if constexpr (F32) {
-#pragma unroll
-      for (int s = 0; s < D / 2; s += 4) {
-        const f32x4 x = gload<f32x4>(qp + 4 * (2 * s + 4 * kh));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) qf[i][s + j] = valid ? x[j] * sc : 0.f;
-      }
-    } else {
-      float x[D / 2];
-      float amax = 0.f;
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        const int dim = Q8 ? 32 * (s / 2) + 16 * kh + 8 * (s % 2) : 16 * s + 8 * kh;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const f32x4 v = gload<f32x4>(qp + 4 * (dim + 4 * e));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[8 * s + 4 * e + j] = valid ? v[j] * sc : 0.f;
-            amax = fmaxf(amax, fabsf(x[8 * s + 4 * e + j]));
-          }
-        }
-      }
-      amax = max32(amax);
-      float f = 1.f;
-      if (amax > 0.f && amax < INFINITY) {
-        const int e = min(13 - ilogbf(amax), 100);
-        f = ldexpf(1.f, e);
-        unscale[i] = ldexpf(1.f, -e);
-      }
-      if constexpr (Q8) unscale[i] *= kByteUnscale;
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          f16x2 hi, lo;
-          split2(x[8 * s + j] * f, x[8 * s + j + 1] * f, hi, lo);
-          qh[i][s][j] = hi[0];
-          qh[i][s][j + 1] = hi[1];
-          ql[i][s][j] = lo[0];
-          ql[i][s][j + 1] = lo[1];
-        }
-    }
-  }
-
-  // ---- state --------------------------------------------------------------
-  floatx16 o[RT][NDB];
-  float ref[RT], l[RT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    ref[i] = -INFINITY;
-    l[i] = 0.f;
-#pragma unroll
-    for (int db = 0; db < NDB; ++db) o[i][db] = (floatx16)(0.f);
-  }
 
   // ---- loads of a key tile --------------------------------------------------
   // The descriptors start at the tile's first row (64-bit), so a cache of any
   // length is addressed, and end after its last valid row: rows past n_kv
   // read zeros.
-  unsigned kw[KW], vw[16 * VW];
-  unsigned ksc[1], ksc2[1], vsc = 0;
-  ksc[0] = ksc2[0] = 0;
+  const char* const kbase = it.k + (int64_t)g * p.k_s1;
+  const char* const vbase = it.v + (int64_t)g * p.v_s1;
+  const int ks2 = (int)p.k_s2, vs2 = (int)p.v_s2;
+  unsigned kw[KW], vw[16 * VW], ksc = 0, vsc = 0;
   const unsigned ko = (unsigned)(c * ks2 + 16 * kh);
   const unsigned vo = (unsigned)(4 * kh * vs2 + c * NDB * ELT);
   lds_t* const sc_lds = lds + wave * ROWS * C::XS * 4;
@@ -198,10 +125,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
       // the scales of key c: lane half kh takes half of the K row's
       const int64_t at = (int64_t)key0 * p.n_head_kv + g;
       const rsrc_t rk = make_rsrc(it.k_scale + at * (2 * NDB), (unsigned)((n - 1) * p.n_head_kv * 2 * NDB + 2 * NDB));
-      if constexpr (NDB == 4)
-        ksc[0] = buf_b32(rk, (unsigned)(c * p.n_head_kv * 8 + 4 * kh));
-      else
-        ksc[0] = buf_b16(rk, (unsigned)(c * p.n_head_kv * 4 + 2 * kh));
+      ksc = NDB == 4 ? buf_b32(rk, (unsigned)(c * p.n_head_kv * 8 + 4 * kh)) : buf_b16(rk, (unsigned)(c * p.n_head_kv * 4 + 2 * kh));
       const rsrc_t rv = make_rsrc(it.v_scale + at * 2, (unsigned)((n - 1) * p.n_head_kv * 2 + 2));
       vsc = buf_b16(rv, (unsigned)(c * p.n_head_kv * 2));
     }
@@ -228,120 +152,171 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
       }
     }
   };
-
   int tile = tile0 + wave;
   if (tile < tile1) {
     load_k(tile);
     load_v(tile);
   }
+
+  // ---- queries ------------------------------------------------------------
+  // Dims of B's step s, lane half kh, element j (A's are loaded the same way):
+  // F32 8 (s / 4) + 4 kh + s % 4; F16 16 s + 8 kh + j; 8-bit
+  // 32 (s / 2) + 16 kh + 8 (s % 2) + j. Each is 16 consecutive bytes of K.
+  float qf[F32 ? D / 2 : 1];
+  f16x8 qh[F32 ? 1 : D / 16], ql[F32 ? 1 : D / 16];
+  float unscale = 1.f;
+  const bool valid = row0 + c < rows;
+  const int token = valid ? (row0 + c) / p.n_rep : 0;
+  {
+    const int h = g * p.n_rep + (valid ? row0 + c - token * p.n_rep : 0);
+    const char* const qp = reinterpret_cast<const char*>(it.q) + (int64_t)token * p.q_s2 + (int64_t)h * p.q_s1;
+    if constexpr (F32) {
+#pragma unroll
+      for (int s = 0; s < D / 2; s += 4) {
+        const f32x4 x = gload<f32x4>(qp + 4 * (2 * s + 4 * kh));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qf[s + j] = valid ? x[j] * p.scale_log2e : 0.f;
+      }
+    } else {
+      float x[D / 2];
+      float amax = 0.f;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        const int dim = Q8 ? 32 * (s / 2) + 16 * kh + 8 * (s % 2) : 16 * s + 8 * kh;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const f32x4 v = gload<f32x4>(qp + 4 * (dim + 4 * e));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[8 * s + 4 * e + j] = valid ? v[j] * p.scale_log2e : 0.f;
+            amax = fmaxf(amax, fabsf(x[8 * s + 4 * e + j]));
+          }
+        }
+      }
+      amax = max32(amax);
+      int qexp = 0;
+      if (amax > 0.f && amax < INFINITY) qexp = max(ilogbf(amax) - 13, -100);
+      unscale = ldexpf(Q8 ? kByteUnscale : 1.f, qexp);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          f16x2 hi, lo;
+          split2(ldexpf(x[8 * s + j], -qexp), ldexpf(x[8 * s + j + 1], -qexp), hi, lo);
+          qh[s][j] = hi[0];
+          qh[s][j + 1] = hi[1];
+          ql[s][j] = lo[0];
+          ql[s][j + 1] = lo[1];
+        }
+    }
+  }
+
+  // ---- state --------------------------------------------------------------
+  floatx16 o[NDB];
+  float ref = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) o[db] = (floatx16)(0.f);
+
   for (; tile < tile1; tile += kTreeWaves) {
     const int key0 = tile * kTreeTile;
     const int next = tile + kTreeWaves;
     // ---- S^T = K . Q^T ------------------------------------------------------
-    floatx16 s[RT];
-    f32x4 pv_scale[4];  // V scales of the lane's keys
-    float vexp = 0.f;   // and the exponent above the tile's largest
-#pragma unroll
-    for (int i = 0; i < RT; ++i) s[i] = (floatx16)(0.f);
+    floatx16 s = (floatx16)(0.f);
+    f32x4 vfac[4], vexp[4];  // 8-bit: V scales of the lane's keys and their exponents
     if constexpr (F32) {
 #pragma unroll
-      for (int st = 0; st < D / 2; ++st)
-#pragma unroll
-        for (int i = 0; i < RT; ++i) s[i] = mfma_f32(__builtin_bit_cast(float, kw[st]), qf[i][st], s[i]);
+      for (int st = 0; st < D / 2; ++st) s = mfma_f32(__builtin_bit_cast(float, kw[st]), qf[st], s);
     } else if constexpr (!Q8) {
 #pragma unroll
       for (int st = 0; st < D / 16; ++st) {
         const f16x8 k8 = __builtin_bit_cast(f16x8, u32x4{kw[4 * st], kw[4 * st + 1], kw[4 * st + 2], kw[4 * st + 3]});
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          s[i] = mfma_f16(k8, ql[i][st], s[i]);
-          s[i] = mfma_f16(k8, qh[i][st], s[i]);
-        }
+        s = mfma_f16(k8, ql[st], s);
+        s = mfma_f16(k8, qh[st], s);
       }
     } else {
       // the scales, to where each lane can read those of its own 16 keys
       auto h2f = [](unsigned x) { return (float)__builtin_bit_cast(_Float16, (unsigned short)x); };
       if constexpr (NDB == 4) {
-        lds_store<float>(sc_lds + (64 * kh + c) * 4, h2f(ksc[0] & 0xffffu));
-        lds_store<float>(sc_lds + (64 * kh + 32 + c) * 4, h2f(ksc[0] >> 16));
+        lds_store<float>(sc_lds + (64 * kh + c) * 4, h2f(ksc & 0xffffu));
+        lds_store<float>(sc_lds + (64 * kh + 32 + c) * 4, h2f(ksc >> 16));
       } else {
-        lds_store<float>(sc_lds + (32 * kh + c) * 4, h2f(ksc[0]));
+        lds_store<float>(sc_lds + (32 * kh + c) * 4, h2f(ksc));
       }
-      if (kh == 0) lds_store<float>(sc_lds + (32 * NDB + c) * 4, h2f(vsc));
+      const float v = h2f(vsc);
+      if (kh == 0) {
+        lds_store<float>(sc_lds + (32 * NDB + c) * 4, v);
+        lds_store<float>(sc_lds + (32 * NDB + 32 + c) * 4, (float)scale_exponent(v < INFINITY ? v : 0.f));
+      }
       wave_lds_fence();
 #pragma unroll
       for (int b = 0; b < NDB; ++b) {
-        floatx16 part[RT];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) part[i] = (floatx16)(0.f);
+        floatx16 part = (floatx16)(0.f);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const unsigned w0 = kw[4 * b + 2 * e] ^ 0x80808080u, w1 = kw[4 * b + 2 * e + 1] ^ 0x80808080u;
           const f16x2 x0 = bytes_f16<0, 1>(w0, w0), x1 = bytes_f16<2, 3>(w0, w0);
           const f16x2 x2 = bytes_f16<0, 1>(w1, w1), x3 = bytes_f16<2, 3>(w1, w1);
           const f16x8 k8 = {x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
-#pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            part[i] = mfma_f16(k8, ql[i][2 * b + e], part[i]);
-            part[i] = mfma_f16(k8, qh[i][2 * b + e], part[i]);
-          }
+          part = mfma_f16(k8, ql[2 * b + e], part);
+          part = mfma_f16(k8, qh[2 * b + e], part);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f32x4 sc = lds_load<f32x4>(sc_lds + (32 * b + 8 * q + 4 * kh) * 4);
 #pragma unroll
-          for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[i][4 * q + j] = fmaf(part[i][4 * q + j], sc[j], s[i][4 * q + j]);
+          for (int j = 0; j < 4; ++j) s[4 * q + j] = fmaf(part[4 * q + j], sc[j], s[4 * q + j]);
         }
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) pv_scale[q] = lds_load<f32x4>(sc_lds + (32 * NDB + 8 * q + 4 * kh) * 4);
-      const float v = h2f(vsc);
-      const float most = row_max16(v < INFINITY ? v : 0.f);
-      vexp = (float)scale_exponent(fmaxf(most, __shfl_xor(most, 16, kWave)));  // the same in every lane
+      for (int q = 0; q < 4; ++q) {
+        vfac[q] = lds_load<f32x4>(sc_lds + (32 * NDB + 8 * q + 4 * kh) * 4);
+        vexp[q] = lds_load<f32x4>(sc_lds + (32 * NDB + 32 + 8 * q + 4 * kh) * 4);
+      }
       wave_lds_fence();  // the scales are read before the next tile's are written
     }
     if (next < tile1) load_k(next);
 
     // ---- mask -----------------------------------------------------------------
-    unsigned vis[RT];
-    const bool masked = key0 + kTreeTile > it.n_past;  // a tile of drafted keys
+    unsigned vis = ~0u;
+    const bool masked = key0 + kTreeTile > n_past;  // a tile of drafted keys
     if (masked) {
+      vis = visible_bits(it, token, key0);
+      const unsigned mine = vis >> (4 * kh);
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        const unsigned v = visible_bits(it, token[i], key0);
-        vis[i] = v;
-        const unsigned mine = v >> (4 * kh);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[i][e] = mine >> (8 * (e >> 2) + (e & 3)) & 1u ? s[i][e] : -INFINITY;
-      }
+      for (int e = 0; e < 16; ++e) s[e] = mine >> (8 * (e >> 2) + (e & 3)) & 1u ? s[e] : -INFINITY;
     }
 
-    // ---- softmax ------------------------------------------------------------
+    // ---- softmax, relative to ref -----------------------------------------------
+    float top;
+    if constexpr (Q8) {  // of the probability times the V row's scale
+      floatx16 x;
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const float alpha = move_ref(ref[i], max32(max16(s[i], -INFINITY)) * unscale[i] + vexp);
-      const float at = ref[i] == -INFINITY ? 0.f : ref[i];
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int e = 0; e < 16; ++e) x[e] = fmaf(s[e], unscale, vexp[e >> 2][e & 3]);
+      top = max32(max16(x, -INFINITY));
+    } else {
+      top = max32(max16(s, -INFINITY)) * unscale;
+    }
+    const float alpha = move_ref(ref, top);
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0ull) {
+      l *= alpha;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[i][e] = fast_exp2(fmaf(s[i][e], unscale[i], -at));
-        sum[e & 3] += s[i][e];
-      }
-      l[i] = l[i] * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0ull) {
+      for (int db = 0; db < NDB; ++db) o[db] *= alpha;
+    }
+    const float at = ref == -INFINITY ? 0.f : ref;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) o[i][db] *= alpha;
-      }
-      if constexpr (Q8) {
+    for (int e = 0; e < 16; ++e) {
+      s[e] = fast_exp2(fmaf(s[e], unscale, -at));
+      sum[e & 3] += s[e];
+    }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    if constexpr (Q8) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[i][e] *= pv_scale[e >> 2][e & 3];
-        if (masked) {  // (a scale may not be finite: 0 times it is not 0)
-          const unsigned mine = vis[i] >> (4 * kh);
+      for (int e = 0; e < 16; ++e) s[e] *= vfac[e >> 2][e & 3];
+      if (masked) {  // (a scale may not be finite: 0 times it is not 0)
+        const unsigned mine = vis >> (4 * kh);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[i][e] = mine >> (8 * (e >> 2) + (e & 3)) & 1u ? s[i][e] : 0.f;
-        }
+        for (int e = 0; e < 16; ++e) s[e] = mine >> (8 * (e >> 2) + (e & 3)) & 1u ? s[e] : 0.f;
       }
     }
 
@@ -383,25 +358,20 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
 #pragma unroll
       for (int t = 0; t < 16; ++t)
 #pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-          for (int i = 0; i < RT; ++i)
-            o[i][db] = mfma_f32(__builtin_bit_cast(float, vw[VW * t + db]), s[i][t], o[i][db]);
+        for (int db = 0; db < NDB; ++db) o[db] = mfma_f32(__builtin_bit_cast(float, vw[VW * t + db]), s[t], o[db]);
     } else {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        f16x8 ph[RT], pl[RT];
+        f16x8 ph, pl;
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            f16x2 hi, lo;
-            split2(s[i][8 * u + j], s[i][8 * u + j + 1], hi, lo);
-            ph[i][j] = hi[0];
-            ph[i][j + 1] = hi[1];
-            pl[i][j] = lo[0];
-            pl[i][j + 1] = lo[1];
-          }
+        for (int j = 0; j < 8; j += 2) {
+          f16x2 hi, lo;
+          split2(s[8 * u + j], s[8 * u + j + 1], hi, lo);
+          ph[j] = hi[0];
+          ph[j + 1] = hi[1];
+          pl[j] = lo[0];
+          pl[j + 1] = lo[1];
+        }
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
           f16x8 v8;
@@ -420,11 +390,8 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
             v8[j] = x[0];
             v8[j + 1] = x[1];
           }
-#pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            o[i][db] = mfma_f16(v8, pl[i], o[i][db]);
-            o[i][db] = mfma_f16(v8, ph[i], o[i][db]);
-          }
+          o[db] = mfma_f16(v8, pl, o[db]);
+          o[db] = mfma_f16(v8, ph, o[db]);
         }
       }
     }
@@ -439,16 +406,13 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
             some |= bits[db];
           }
           if (some == 0u) continue;
+          const unsigned x = vis >> (4 * sh);  // the row's sight of that lane's keys, bit t
+          const unsigned seen = (x & 0xfu) | (x >> 4 & 0xf0u) | (x >> 8 & 0xf00u) | (x >> 12 & 0xf000u);
 #pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            const unsigned x = vis[i] >> (4 * sh);  // the row's sight of that lane's keys, bit t
-            const unsigned seen = (x & 0xfu) | (x >> 4 & 0xf0u) | (x >> 8 & 0xf00u) | (x >> 12 & 0xf000u);
+          for (int db = 0; db < NDB; ++db)
 #pragma unroll
-            for (int db = 0; db < NDB; ++db)
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if ((bits[db] & seen) != 0u && 8 * (e >> 2) + 4 * kh + (e & 3) == sc) o[i][db][e] = NAN;
-          }
+            for (int e = 0; e < 16; ++e)
+              if ((bits[db] & seen) != 0u && 8 * (e >> 2) + 4 * kh + (e & 3) == sc) o[db][e] = NAN;
         }
       }
     }
@@ -457,55 +421,46 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
 
   // ---- the waves' parts ---------------------------------------------------------
   wave_lds_fence();
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const float lt = sum32(l[i]);
-    if (kh == 0) {
-      lds_store<float>(lds + C::L_ML + ((wave * ROWS + 32 * i + c) * 2) * 4, ref[i]);
-      lds_store<float>(lds + C::L_ML + ((wave * ROWS + 32 * i + c) * 2 + 1) * 4, lt);
-    }
+  const float ls = sum32(l);
+  if (kh == 0) {
+    lds_store<float>(lds + C::L_ML + ((wave * ROWS + c) * 2) * 4, ref);
+    lds_store<float>(lds + C::L_ML + ((wave * ROWS + c) * 2 + 1) * 4, ls);
   }
   __syncthreads();
-  constexpr float unit_o = Q8 ? kByteUnscale : 1.f;  // of the values' 2^-10
-  float mt[RT], lt[RT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    mt[i] = -INFINITY;
-    lt[i] = 0.f;
+  float mt = -INFINITY, lt = 0.f;
+  {
+    constexpr float unit_o = Q8 ? kByteUnscale : 1.f;  // of the values' 2^-10
     f32x2 ml[kTreeWaves];
 #pragma unroll
     for (int w = 0; w < kTreeWaves; ++w) {
-      ml[w] = lds_load<f32x2>(lds + C::L_ML + ((w * ROWS + 32 * i + c) * 2) * 4);
-      mt[i] = fmaxf(mt[i], ml[w][0]);
+      ml[w] = lds_load<f32x2>(lds + C::L_ML + ((w * ROWS + c) * 2) * 4);
+      mt = fmaxf(mt, ml[w][0]);
     }
-    const float mu = mt[i] == -INFINITY ? 0.f : mt[i];
+    const float mu = mt == -INFINITY ? 0.f : mt;
 #pragma unroll
-    for (int w = 0; w < kTreeWaves; ++w) lt[i] += ml[w][1] * fast_exp2(ml[w][0] - mu);
-    const float wt = fast_exp2(ref[i] - mu) * unit_o;
+    for (int w = 0; w < kTreeWaves; ++w) lt += ml[w][1] * fast_exp2(ml[w][0] - mu);
+    const float wt = fast_exp2(ref - mu) * unit_o;
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) o[i][db] *= wt;
+    for (int db = 0; db < NDB; ++db) o[db] *= wt;
   }
-  // One 32-dim block at a time through LDS; thread (row pr, column cc) sums the
-  // waves' parts of its columns.
-  constexpr int PER = ROWS * 32 / (kTreeWaves * kWave);  // (row, column) pairs per thread
+  // One 32-dim block at a time through LDS; a thread sums the waves' parts of
+  // its (row, column) pairs.
+  constexpr int PER = ROWS * 32 / (kTreeWaves * kWave);
   float acc[PER][NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) {
     if (db > 0) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        lds_store<f32x4>(lds + ((wave * ROWS + 32 * i + c) * C::XS + 8 * q + 4 * kh) * 4,
-                         f32x4{o[i][db][4 * q], o[i][db][4 * q + 1], o[i][db][4 * q + 2], o[i][db][4 * q + 3]});
+    for (int q = 0; q < 4; ++q)
+      lds_store<f32x4>(lds + ((wave * ROWS + c) * C::XS + 8 * q + 4 * kh) * 4,
+                       f32x4{o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]});
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
       const int idx = e * kTreeWaves * kWave + threadIdx.x;
       float x = 0.f;
 #pragma unroll
-      for (int w = 0; w < kTreeWaves; ++w)
-        x += lds_load<float>(lds + ((w * ROWS + idx / 32) * C::XS + idx % 32) * 4);
+      for (int w = 0; w < kTreeWaves; ++w) x += lds_load<float>(lds + ((w * ROWS + idx / 32) * C::XS + idx % 32) * 4);
       acc[e][db] = x;
     }
   }
@@ -514,24 +469,19 @@ __global__ __launch_bounds__(kTreeWaves* kWave, RT == 1 ? 2 : 1) void tree_kerne
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
       const int idx = e * kTreeWaves * kWave + threadIdx.x;
+      if (row0 + idx / 32 >= rows) continue;
       float* const w = rec + tree_record_at(D, idx / 32, (NDB * (idx % 32)) & ~3);
       if constexpr (NDB == 4) gstore(w, f32x4{acc[e][0], acc[e][1], acc[e][2], acc[e][3]});
       else gstore(w + 2 * (idx % 2), f32x2{acc[e][0], acc[e][1]});
     }
     if (wave == 0 && kh == 0) {
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        rec[ROWS * D + 32 * i + c] = mt[i];
-        rec[ROWS * D + ROWS + 32 * i + c] = lt[i];
-      }
+      rec[ROWS * D + c] = mt;
+      rec[ROWS * D + ROWS + c] = lt;
     }
     return;
   }
   // the rows' sums to where the storing threads read them
-  if (wave == 0 && kh == 0) {
-#pragma unroll
-    for (int i = 0; i < RT; ++i) lds_store<float>(lds + C::L_ML + (32 * i + c) * 4, mt[i] == -INFINITY ? 0.f : 1.f / lt[i]);
-  }
+  if (wave == 0 && kh == 0) lds_store<float>(lds + C::L_ML + c * 4, mt == -INFINITY ? 0.f : 1.f / lt);
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
@@ -627,15 +577,12 @@ int tree_tile_rows(int rows) { return rows <= 32 ? 32 : 128; }
 
 size_t tree_record_floats(int head_dim, int tile_rows) { return (size_t)tile_rows * (head_dim + 2); }
 
-template <int D, typename KT, int RT>
-static hipError_t launch_tree_t(const TreeParams& p, dim3 grid, hipStream_t stream) {
-  hipLaunchKernelGGL((tree_kernel<D, KT, RT>), grid, dim3(kTreeWaves * kWave), 0, stream, p);
+template <int D>
+static hipError_t launch_narrow(const TreeParams& p, dim3 grid, int elt, hipStream_t stream) {
+  if (elt == 1) hipLaunchKernelGGL((tree_kernel<D, int8_t>), grid, dim3(kTreeWaves * kWave), 0, stream, p);
+  else if (elt == 2) hipLaunchKernelGGL((tree_kernel<D, _Float16>), grid, dim3(kTreeWaves * kWave), 0, stream, p);
+  else hipLaunchKernelGGL((tree_kernel<D, float>), grid, dim3(kTreeWaves * kWave), 0, stream, p);
   return hipGetLastError();
-}
-
-template <int D, typename KT>
-static hipError_t launch_tree_d(const TreeParams& p, dim3 grid, int tile_rows, hipStream_t stream) {
-  return tile_rows == 64 ? launch_tree_t<D, KT, 2>(p, grid, stream) : launch_tree_t<D, KT, 1>(p, grid, stream);
 }
 
 hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, hipStream_t stream) {
@@ -650,17 +597,9 @@ hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, 
     splits = std::max(splits, it.n_split);
   }
   const dim3 grid(gx, n_items);
-  hipError_t e = hipErrorInvalidValue;
-  if (tile_rows == 128)
-    e = launch_tree_wide(p, grid, head_dim, elt, stream);
-  else if (head_dim == 64)
-    e = elt == 1   ? launch_tree_d<64, int8_t>(p, grid, tile_rows, stream)
-        : elt == 2 ? launch_tree_d<64, _Float16>(p, grid, tile_rows, stream)
-                   : launch_tree_d<64, float>(p, grid, tile_rows, stream);
-  else
-    e = elt == 1   ? launch_tree_d<128, int8_t>(p, grid, tile_rows, stream)
-        : elt == 2 ? launch_tree_d<128, _Float16>(p, grid, tile_rows, stream)
-                   : launch_tree_d<128, float>(p, grid, tile_rows, stream);
+  const hipError_t e = tile_rows == 128  ? launch_tree_wide(p, grid, head_dim, elt, stream)
+                       : head_dim == 64 ? launch_narrow<64>(p, grid, elt, stream)
+                                        : launch_narrow<128>(p, grid, elt, stream);
   if (e != hipSuccess || units == 0) return e;
   // slices: about four records each
   const int slices = splits > 8 ? 4 : splits > 4 ? 2 : 1;

@@ -111,6 +111,11 @@ __device__ inline int tree_record_at(int head_dim, int r, int d) {
   return (r / 32) * 32 * head_dim + (d / 8) * 256 + ((d / 4) % 2) * 128 + (r % 32) * 4;
 }
 
+// A record's values are for other XCDs, after the kernel: nontemporal, so that
+// less is left in the L2 to be written back at its end (a 25-token tree over
+// 4107 F16 keys, 8 MB of records: 16.2 -> 15.0 us, the join 0.6 us more).
+__device__ inline void put_record(float* at, f32x4 x) { __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(at)); }
+
 // The e for which scales up to `top` are below 2^e (at least that of the
 // smallest scale there is).
 __device__ inline int scale_exponent(float top) { return top > 0.f ? ilogbf(top) + 1 : -24; }

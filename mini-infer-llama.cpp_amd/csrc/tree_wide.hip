@@ -285,6 +285,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
           amax = fmaxf(amax, fabsf(x[8 * s + 4 * e + j]));
         }
       }
+    if (key_begin < key_end) put(0, key_begin);  // (under the queries' loads)
     amax = max32(amax);
     if (amax > 0.f && amax < INFINITY) qexp = max(ilogbf(amax) - 13, -100);
 #pragma unroll
@@ -493,7 +494,6 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
     }
   };
 
-  if (key_begin < key_end) put(0, key_begin);
   __syncthreads();
   int buf = 0;
   for (int key0 = key_begin; key0 < key_end; key0 += TK, buf ^= 1) {
@@ -514,8 +514,8 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        gstore(rec + tree_record_at(D, 32 * wave + c, 32 * db + 8 * q + 4 * kh),
-               f32x4{o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]} * unit_o);
+        put_record(rec + tree_record_at(D, 32 * wave + c, 32 * db + 8 * q + 4 * kh),
+                   f32x4{o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]} * unit_o);
     if (kh == 0) {
       rec[ROWS * D + 32 * wave + c] = ref;
       rec[ROWS * D + ROWS + 32 * wave + c] = lt;
