@@ -119,7 +119,7 @@ struct TreeItem {
   int32_t n_past, n_tokens;
   int32_t n_rt;             // row tiles per KV head
   int32_t n_split;          // key splits (1: no records, the kernel writes the output)
-  int32_t tiles_per_split;  // key tiles (an even number where there is more than one split)
+  int32_t tiles_per_split;  // key tiles (where there is more than one split: whole tiles of the kernel)
   int32_t rec0;             // the item's first record
   uint32_t xcd0;            // XCD of the item's first unit (their units go to the 8 XCDs in turn)
 };

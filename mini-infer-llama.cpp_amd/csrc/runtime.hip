@@ -375,7 +375,8 @@ size_t ws_total_bytes(int groups, size_t rec_bytes, size_t part_bytes) {
 }
 
 // Bytes of parts that let a tree-attention launch split its keys over
-// kTreeWgPerCu workgroups per CU (see plan_tree), each with a record of up to 128 rows.
+// kTreeWgPerCu workgroups per CU (see plan_tree), each with a record of up to 128
+// rows.
 constexpr int kTreeWgPerCu = 2;
 size_t ws_part_bytes(int head_dim) {
   return (size_t)kTreeWgPerCu * g.n_cu * mi::tree_record_floats(head_dim, 128) * sizeof(float);
@@ -766,48 +767,64 @@ int run_prefill(const mi_hip_attn_args* a, const Resolved& r, hipStream_t stream
 }
 
 // Tree attention: how many key tiles one workgroup takes. A unit (item, KV
-// head, split) brings n_rt workgroups, one per row tile, to one XCD; units go
-// to the XCDs in turn through all items. The launch runs in rounds of
-// kTreeWgPerCu workgroups per CU of an XCD, so what a number of tiles per split
-// costs is rounds x (tiles + what a workgroup spends before and after them),
-// with a second launch to join the parts when there are any. Every item's
-// splits have the same number of tiles.
-void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int tile_rows, size_t part_bytes) {
-  constexpr int64_t kMinTiles = 4, kXcds = 8;
-  constexpr int64_t kFixed = 6, kJoin = 4;  // in tiles
+// head, split) brings n_rt workgroups, one per row tile, to one XCD; units go to
+// the XCDs in turn through all items. What a number of tiles per split costs
+// follows what the kernels were measured to take (us; one workgroup alone on
+// its CU): kTileUs per key tile, kStartUs besides, 1.7 times the tiles when two
+// share a CU; records that are to be joined kJoinUs for the second launch and
+// kRecordUs per MB. Measured against this, best of all splits: a 25-token tree
+// over 4107 F16 keys (28/4 heads of 128) 20.0 us at 6 tiles (4: 22.3, 12: 23.4,
+// all in one: 136), one token over 32000 (14/2 heads of 64) 12.7 at 8 (4: 15.8,
+// 32: 14.4), over 500 7.8 unsplit (4: 11.0), a 64-token tree over 16000 F32 keys
+// (28/4 of 128) 91 at 32 (16: 101, 64: 166).
+constexpr float kTileUs[2][3][2] = {
+    // head_dim 64, 128 of 8-bit, F16, F32 caches
+    {{0.26f, 0.48f}, {0.16f, 0.37f}, {0.45f, 1.06f}},  // up to 32 rows
+    {{0.84f, 1.42f}, {0.55f, 1.00f}, {1.20f, 2.40f}},  // tiles of 128 rows
+};
+constexpr float kStartUs = 6.f, kJoinUs = 4.f, kRecordUs = 0.25f, kSharedCu = 1.7f;
+
+void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, size_t part_bytes) {
+  constexpr int kXcds = 8;
+  const bool wide = tile_rows > 32;
+  const int per_cu = head_dim == 128 && (!wide || elt == 4) ? 1 : 2;  // workgroups (registers)
+  const float tile_us = kTileUs[wide][elt == 1 ? 0 : elt == 2 ? 1 : 2][head_dim == 128];
+  const float record_mb = mi::tree_record_floats(head_dim, tile_rows) * sizeof(float) * 1e-6f;
   const int64_t cap = (int64_t)(part_bytes / (mi::tree_record_floats(head_dim, tile_rows) * sizeof(float)));
-  const int64_t slots = std::max<int64_t>(1, kTreeWgPerCu * g.n_cu / kXcds);
-  auto tiles_of = [&](const mi::TreeItem& it) {
-    return ((int64_t)it.n_past + it.n_tokens + mi::kTreeTile - 1) / mi::kTreeTile;
-  };
-  int64_t longest = 0;
+  // a workgroup's least: a tile for each wave, or (wide) one tile of its own
+  const int least = !wide ? 4 : head_dim == 64 ? 2 : 1;
+  int tiles[mi::kTreeMaxItems], longest = 0;
+  float whole = 0.f, seen = 0.f;  // key tiles of all row tiles, and those that some row sees
   for (int i = 0; i < n_items; ++i) {
     mi::TreeItem& it = p.item[i];
-    it.n_rt = (int32_t)(((int64_t)it.n_tokens * p.n_rep + tile_rows - 1) / tile_rows);
-    longest = std::max(longest, tiles_of(it));
+    it.n_rt = (it.n_tokens * p.n_rep + tile_rows - 1) / tile_rows;
+    tiles[i] = (int)(((int64_t)it.n_past + it.n_tokens + mi::kTreeTile - 1) / mi::kTreeTile);
+    longest = std::max(longest, tiles[i]);
+    const float all = (float)it.n_rt * tiles[i];
+    whole += all;
+    seen += it.mask ? all : (float)it.n_rt * (tiles[i] - 0.5f * it.n_tokens / mi::kTreeTile);
   }
-  // (records, rounds) with `per` tiles per split
-  auto load = [&](int64_t per, int64_t* records) {
-    int64_t at = 0, wgs[kXcds] = {};
-    *records = 0;
+  float best = 0.f;
+  int best_per = longest;
+  // all in one, then 1, 2, .. 7, 8, 10, 12, 14, 16, 20, .. times the least
+  for (int k = 0; k * least < longest; k += k < 8 ? 1 : 1 << (29 - __builtin_clz((unsigned)k))) {
+    const int per = k == 0 ? longest : k * least;
+    int64_t records = 0, units = 0;
+    int rt = 1;
     for (int i = 0; i < n_items; ++i) {
-      const mi::TreeItem& it = p.item[i];
-      const int64_t split = (tiles_of(it) + per - 1) / per, units = split * p.n_head_kv;
-      if (split > 1) *records += units * it.n_rt;
-      for (int64_t x = 0; x < kXcds; ++x) wgs[(at + x) % kXcds] += (units + kXcds - 1 - x) / kXcds * it.n_rt;
-      at += units;
+      const int n = (tiles[i] + per - 1) / per * p.n_head_kv;
+      units += n;
+      if (n > p.n_head_kv) records += (int64_t)n * p.item[i].n_rt;
+      rt = std::max(rt, p.item[i].n_rt);
     }
-    return (*std::max_element(wgs, wgs + kXcds) + slots - 1) / slots;
-  };
-  int64_t best = 0, best_per = longest;
-  for (int64_t split = 1; split <= std::max<int64_t>(1, longest / kMinTiles); split += 1 + split / 8) {
-    int64_t per = (longest + split - 1) / split;
-    if (split > 1) per += per & 1;  // whole 64-key tiles
-    int64_t records;
-    const int64_t rounds = load(per, &records);
     if (records > cap) continue;
-    const int64_t cost = rounds * (per + kFixed) + (records ? kJoin : 0);
-    if (split == 1 || cost < best) {
+    // workgroups with work, per CU of the fullest XCD
+    const float load = (float)((units + kXcds - 1) / kXcds) * rt * (seen / whole);
+    const int on_cu = std::max(1, (int)std::ceil(load * kXcds / g.n_cu));
+    const int rounds = (on_cu + per_cu - 1) / per_cu;
+    const float cost = rounds * (kStartUs + per * tile_us * (std::min(on_cu, per_cu) > 1 ? kSharedCu : 1.f)) +
+                       (records ? kJoinUs + records * record_mb * kRecordUs : 0.f);
+    if (k == 0 || cost < best) {
       best = cost;
       best_per = per;
     }
@@ -815,8 +832,8 @@ void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int tile_rows, size
   int64_t rec = 0, at = 0;
   for (int i = 0; i < n_items; ++i) {
     mi::TreeItem& it = p.item[i];
-    it.tiles_per_split = (int32_t)std::min<int64_t>(best_per, tiles_of(it));
-    it.n_split = (int32_t)((tiles_of(it) + it.tiles_per_split - 1) / it.tiles_per_split);
+    it.tiles_per_split = std::min(best_per, tiles[i]);
+    it.n_split = (tiles[i] + it.tiles_per_split - 1) / it.tiles_per_split;
     it.rec0 = (int32_t)rec;
     it.xcd0 = (uint32_t)(at % kXcds);
     if (it.n_split > 1) rec += (int64_t)p.n_head_kv * it.n_rt * it.n_split;
@@ -892,7 +909,7 @@ int run_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* masks, int n
       most = std::max(most, a->n_tokens * a->n_rep);
     }
     const int tile_rows = mi::tree_tile_rows(most);
-    plan_tree(p, cnt, r0.head_dim, tile_rows, ws->part_bytes);
+    plan_tree(p, cnt, r0.head_dim, elt, tile_rows, ws->part_bytes);
     hipError_t e = mi::launch_tree(p, cnt, r0.head_dim, elt, tile_rows, stream);
     if (e != hipSuccess) return hip_fail(e, "tree attention launch");
     base += cnt;

@@ -152,6 +152,11 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (TreeCfg<D, KT>::WAVES_PER_SIMD)
       }
     }
   };
+  if (tile0 >= tile1 && n_split > 1) {  // no key for these rows: nothing to join
+    float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * n_rt + rt) * n_split + sp) * (ROWS * (D + 2));
+    if (threadIdx.x < 2 * ROWS) rec[ROWS * D + threadIdx.x] = threadIdx.x < ROWS ? -INFINITY : 0.f;
+    return;
+  }
   int tile = tile0 + wave;
   if (tile < tile1) {
     load_k(tile);
@@ -502,18 +507,20 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (TreeCfg<D, KT>::WAVES_PER_SIMD)
 // running maximum, kInFlight of them on their way at once; the slices meet in
 // LDS in order. The records were just written and come from the caches, so the
 // time is their latency: few records in turn per wave is what counts.
+constexpr int kJoinInFlight = 8, kJoinSlices = 16;
+
 template <int D>
-__global__ __launch_bounds__(256) void tree_combine_kernel(const TreeParams p, int tile_rows, int slices) {
-  constexpr int kInFlight = 4;
-  __shared__ f32x4 part[4][kWave];
-  __shared__ f32x2 ml[4][kWave];
+__global__ __launch_bounds__(kJoinSlices* kWave) void tree_combine_kernel(const TreeParams p, int tile_rows, int slices) {
+  constexpr int kInFlight = kJoinInFlight;
+  __shared__ f32x4 part[kJoinSlices][kWave];
+  __shared__ f32x2 ml[kJoinSlices][kWave];
   const TreeItem& it = p.item[blockIdx.y];
   const int rows = it.n_tokens * p.n_rep, n_split = it.n_split;
   if (n_split <= 1) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int slice = wave % slices;
   const int groups = (rows + 31) / 32;  // of 32 rows, per KV head
-  const int unit = blockIdx.x * (4 / slices) + wave / slices;
+  const int unit = blockIdx.x * ((int)blockDim.x / kWave / slices) + wave / slices;
   const int chunk = unit % (D / 8), grp = unit / (D / 8) % groups, g = unit / (D / 8) / groups;
   const bool valid = g < p.n_head_kv;
   const int64_t rec_floats = (int64_t)tile_rows * (D + 2);
@@ -540,7 +547,8 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const TreeParams p, i
       const float mn = fmaxf(mx, ms[u]);
       const float mu = mn == -INFINITY ? 0.f : mn;
       const float a = fast_exp2(mx - mu), b = fast_exp2(ms[u] - mu);
-      acc = acc * a + os[u] * b;
+      // (a split without a key for the row may have left its sums unwritten)
+      acc = acc * a + (ms[u] == -INFINITY ? f32x4{0.f, 0.f, 0.f, 0.f} : os[u] * b);
       l = l * a + ls[u] * b;
       mx = mn;
     }
@@ -565,7 +573,8 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(const TreeParams p, i
   }
   const int r = grp * 32 + lane % 32;
   if (!valid || r >= rows) return;
-  const float inv = mx == -INFINITY ? 0.f : 1.f / l;
+  // (no key at all: zeros; every score NaN: the sum is)
+  const float inv = mx == -INFINITY && l == 0.f ? 0.f : 1.f / l;
   const int t = r / p.n_rep, h = g * p.n_rep + r % p.n_rep;
   gstore(reinterpret_cast<char*>(it.out) + (int64_t)t * p.o_s2 + (int64_t)h * p.o_s1 + 32 * chunk + 16 * (lane / 32),
          acc * inv);
@@ -601,11 +610,13 @@ hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, 
                        : head_dim == 64 ? launch_narrow<64>(p, grid, elt, stream)
                                         : launch_narrow<128>(p, grid, elt, stream);
   if (e != hipSuccess || units == 0) return e;
-  // slices: about four records each
-  const int slices = splits > 8 ? 4 : splits > 4 ? 2 : 1;
-  const dim3 cgrid((unsigned)((units * slices + 3) / 4), n_items);
-  if (head_dim == 64) hipLaunchKernelGGL(tree_combine_kernel<64>, cgrid, dim3(256), 0, stream, p, tile_rows, slices);
-  else hipLaunchKernelGGL(tree_combine_kernel<128>, cgrid, dim3(256), 0, stream, p, tile_rows, slices);
+  // slices: one batch of records in flight each, as far as a workgroup goes
+  int slices = 1;
+  while (slices < kJoinSlices && slices * kJoinInFlight < splits) slices *= 2;
+  const int waves = std::max(4, slices);
+  const dim3 cgrid((unsigned)((units * slices + waves - 1) / waves), n_items);
+  if (head_dim == 64) hipLaunchKernelGGL(tree_combine_kernel<64>, cgrid, dim3(waves * kWave), 0, stream, p, tile_rows, slices);
+  else hipLaunchKernelGGL(tree_combine_kernel<128>, cgrid, dim3(waves * kWave), 0, stream, p, tile_rows, slices);
   return hipGetLastError();
 }
 

@@ -118,6 +118,11 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
   const int key_begin = sp * it.tiles_per_split * kTreeTile;
   const int key_end = min(lim, key_begin + it.tiles_per_split * kTreeTile);
   const bool active = row0 + 32 * wave < rows;  // the wave has rows
+  if (key_begin >= key_end && n_split > 1) {  // no key for these rows: nothing to join
+    float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * n_rt + rt) * n_split + sp) * (ROWS * (D + 2));
+    for (int i = tid; i < 2 * ROWS; i += THREADS) rec[ROWS * D + i] = i < ROWS ? -INFINITY : 0.f;
+    return;
+  }
 
   // ---- fetching a tile --------------------------------------------------------
   // Thread t takes slots t and t + 256 of the tile's rows (a row's slots are in
