@@ -770,25 +770,32 @@ int run_prefill(const mi_hip_attn_args* a, const Resolved& r, hipStream_t stream
 // head, split) brings n_rt workgroups, one per row tile, to one XCD; units go to
 // the XCDs in turn through all items. What a number of tiles per split costs
 // follows what the kernels were measured to take (us; one workgroup alone on
-// its CU): kTileUs per key tile, kStartUs besides, 1.7 times the tiles when two
-// share a CU; records that are to be joined kJoinUs for the second launch and
-// kRecordUs per MB. Measured against this, best of all splits: a 25-token tree
-// over 4107 F16 keys (28/4 heads of 128) 20.0 us at 6 tiles (4: 22.3, 12: 23.4,
-// all in one: 136), one token over 32000 (14/2 heads of 64) 12.7 at 8 (4: 15.8,
-// 32: 14.4), over 500 7.8 unsplit (4: 11.0), a 64-token tree over 16000 F32 keys
+// its CU): kTileUs per key tile, kStartUs besides, kSharedCu times the tiles when
+// several share a CU; records that are to be joined kJoinUs for the second launch
+// and kRecordUs per MB. Measured with every split (us a call): a 25-token tree
+// over 4107 F16 keys (28/4 heads of 128) 20.0 at 6 tiles (4: 22.3, 12: 23.4, all
+// in one: 136), one token over 32000 (14/2 heads of 64) 12.5 at 8 (4: 16.2, 32:
+// 13.4), over 500 8.0 unsplit (4: 10.1), 24 times one over 4095 8-bit keys (28/4
+// of 128) 30.2 at 28 (12: 37.5, 64: 36.9), a 64-token tree over 16000 F32 keys
 // (28/4 of 128) 91 at 32 (16: 101, 64: 166).
-constexpr float kTileUs[2][3][2] = {
+constexpr float kTileUs[3][3][2] = {
     // head_dim 64, 128 of 8-bit, F16, F32 caches
+    {{0.17f, 0.37f}, {0.14f, 0.28f}, {0.33f, 0.66f}},  // up to 16 rows
     {{0.26f, 0.48f}, {0.16f, 0.37f}, {0.45f, 1.06f}},  // up to 32 rows
     {{0.84f, 1.42f}, {0.55f, 1.00f}, {1.20f, 2.40f}},  // tiles of 128 rows
 };
-constexpr float kStartUs = 6.f, kJoinUs = 4.f, kRecordUs = 0.25f, kSharedCu = 1.7f;
+constexpr float kStartUs = 6.f, kJoinUs = 4.f, kRecordUs = 0.25f;
+// by the same three kinds: workgroups that a CU holds (registers) for head_dim 64
+// and 128, and what the tiles take when it holds more than one
+constexpr int kPerCu[3][2] = {{3, 2}, {2, 1}, {2, 2}};
+constexpr float kSharedCu[3] = {2.0f, 1.7f, 1.7f};
 
-void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, size_t part_bytes) {
+void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int elt, int rows, int tile_rows, size_t part_bytes) {
   constexpr int kXcds = 8;
   const bool wide = tile_rows > 32;
-  const int per_cu = head_dim == 128 && (!wide || elt == 4) ? 1 : 2;  // workgroups (registers)
-  const float tile_us = kTileUs[wide][elt == 1 ? 0 : elt == 2 ? 1 : 2][head_dim == 128];
+  const int kind = wide ? 2 : rows > 16;
+  const int per_cu = wide && elt == 4 && head_dim == 128 ? 1 : kPerCu[kind][head_dim == 128];
+  const float tile_us = kTileUs[kind][elt == 1 ? 0 : elt == 2 ? 1 : 2][head_dim == 128];
   const float record_mb = mi::tree_record_floats(head_dim, tile_rows) * sizeof(float) * 1e-6f;
   const int64_t cap = (int64_t)(part_bytes / (mi::tree_record_floats(head_dim, tile_rows) * sizeof(float)));
   // a workgroup's least: a tile for each wave, or (wide) one tile of its own
@@ -822,7 +829,7 @@ void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int elt, int tile_r
     const float load = (float)((units + kXcds - 1) / kXcds) * rt * (seen / whole);
     const int on_cu = std::max(1, (int)std::ceil(load * kXcds / g.n_cu));
     const int rounds = (on_cu + per_cu - 1) / per_cu;
-    const float cost = rounds * (kStartUs + per * tile_us * (std::min(on_cu, per_cu) > 1 ? kSharedCu : 1.f)) +
+    const float cost = rounds * (kStartUs + per * tile_us * (std::min(on_cu, per_cu) > 1 ? kSharedCu[kind] : 1.f)) +
                        (records ? kJoinUs + records * record_mb * kRecordUs : 0.f);
     if (k == 0 || cost < best) {
       best = cost;
@@ -909,7 +916,7 @@ int run_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* masks, int n
       most = std::max(most, a->n_tokens * a->n_rep);
     }
     const int tile_rows = mi::tree_tile_rows(most);
-    plan_tree(p, cnt, r0.head_dim, elt, tile_rows, ws->part_bytes);
+    plan_tree(p, cnt, r0.head_dim, elt, most, tile_rows, ws->part_bytes);
     hipError_t e = mi::launch_tree(p, cnt, r0.head_dim, elt, tile_rows, stream);
     if (e != hipSuccess) return hip_fail(e, "tree attention launch");
     base += cnt;

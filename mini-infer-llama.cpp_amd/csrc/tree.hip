@@ -17,21 +17,23 @@
 // record in the workspace that tree_combine_kernel joins (a second launch, so
 // that neither needs a counter and both may be captured into a graph).
 //
-// This kernel: row tiles of 32, for calls that need no more. Its waves take the
-// split's key tiles in turn, K and V straight to registers, and meet in LDS at
-// the end. (More rows: tree_wide.hip.)
+// This kernel: one tile of 16 or 32 rows, for calls that need no more. Its waves
+// take the split's key tiles in turn, K and V straight to registers, and meet in
+// LDS at the end. (More rows: tree_wide.hip.)
 //
-// Per key tile (lane = (c = lane % 32, kh = lane / 32)), 32x32 MFMAs:
+// Per key tile of 32 (lane = (c = lane % 16, q = lane / 16)), 16x16 MFMAs:
 //   S^T = K . Q^T: A is K (key c), B the queries (row c); a lane ends up with
-//   the 16 keys 8 (i / 4) + 4 kh + i % 4 of row c, so the softmax runs within
-//   lanes but for one exchange between lane and lane ^ 32, and P is already
-//   the B operand of O^T += V^T . P^T. V's A operand is loaded as rows: lane
-//   (c, kh) takes the NDB = D / 32 consecutive dims NDB c .. of its 16 keys,
-//   so row c of output block db is dim NDB c + db.
+//   keys 4 q + j and 16 + 4 q + j (j < 4) of row c, so the softmax runs within
+//   lanes but for an exchange between the four lanes of a row, and P is already
+//   the B operand of O^T += V^T . P^T. V's A operand is loaded as rows: a lane
+//   takes the NE = D / 16 consecutive dims NE c .. of its eight keys, so row c of
+//   output block db is dim NE c + db.
+// (The wide kernel does the same with 32x32 MFMAs: lane = (c = lane % 32, kh =
+// lane / 32), a lane has the 16 keys 8 (i / 4) + 4 kh + i % 4 of row c.)
 //
-// Products. F32 cache: v_mfma_f32_32x32x2f32. F16 and 8-bit caches: the cache
+// Products. F32 cache: v_mfma_f32_16x16x4f32. F16 and 8-bit caches: the cache
 // operand is exact in f16, the queries and the probabilities are f16 pairs
-// hi = RNE(x), lo = RNE(x - hi), two v_mfma_f32_32x32x16_f16 a step. So that
+// hi = RNE(x), lo = RNE(x - hi), two v_mfma_f32_16x16x32_f16 a step. So that
 // lo stays normal, each query row is scaled by the power of two that puts its
 // largest element in [2^13, 2^14) (undone in the exponent's multiply-add), and
 // the probabilities are 2^(s - ref) for a reference that keeps the largest
@@ -40,6 +42,13 @@
 //   8-bit K: a row's scales (one per 32 dims) multiply the S^T of their own
 //   32 dims. 8-bit V: the row's one scale multiplies the probability; ref keeps
 //   the largest such product in that range.
+//
+// Bound: each byte of the cache comes from memory once, 24 sequences of one token
+// over 4095 F16 keys (28/4 heads of 128) at 5.2 TB/s (38.8 us with the join); over
+// few keys the start, a tile's chain of loads, products and exponentials and the
+// join's launch (one token over 4000: 10.6 us). Rows beyond the group's are work
+// for nothing: with 32x32 MFMAs, whose tile is 32 rows, that call took 57 us, and
+// twice the registers let one workgroup less onto a CU.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -48,57 +57,88 @@
 
 namespace mi {
 
-// KT: float, _Float16 or int8_t.
-template <int D, typename KT>
+namespace {
+
+constexpr int kTreeRows = 32;  // rows of this kernel's records
+
+__device__ inline f32x4 mfma16_f16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x4 mfma16_f32(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// Over the four lanes that share lane % 16. v_permlane16_swap exchanges the odd
+// rows of 16 lanes of one operand with the even rows of the other, so two copies
+// of x become x of the even and of the odd row of the pair. (s_nop: as in swap32.)
+__device__ inline void swap16(float x, float& a, float& b) {
+  float y = x;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  a = x;
+  b = y;
+}
+__device__ inline float max_quarters(float x) {
+  float a, b;
+  swap16(x, a, b);
+  return max32(fmaxf(a, b));
+}
+__device__ inline float sum_quarters(float x) {
+  float a, b;
+  swap16(x, a, b);
+  return sum32(a + b);
+}
+
+// Bits 4 q .. 4 q + 3 and 16 + 4 q .. of a tile's 32 keys: the eight of a lane.
+__device__ inline unsigned slots_of(unsigned keys, int q) {
+  return (keys >> (4 * q) & 0xfu) | (keys >> (16 + 4 * q) & 0xfu) << 4;
+}
+
+}  // namespace
+
+// KT: float, _Float16 or int8_t; RT: 16-row tiles of queries.
+template <int D, typename KT, int RT>
 struct TreeCfg {
   static constexpr int ELT = (int)sizeof(KT);
   static constexpr bool Q8 = ELT == 1, F32 = ELT == 4;
-  static constexpr int NDB = D / 32;             // output blocks of 32 dims; scales per 8-bit K row
-  static constexpr int ROWS = 32;
-  static constexpr int KW = D * ELT / 8;         // 32-bit words of K per lane and tile
-  static constexpr int VW = NDB * ELT >= 4 ? NDB * ELT / 4 : 1;  // words of V per lane and key
-  static constexpr int XS = 36;                  // exchange row stride (floats)
-  static constexpr int L_X = 0;                  // waves' outputs of one 32-dim block
+  static constexpr int NB = D / 32;              // 32-dim blocks (of K; scales per 8-bit K row)
+  static constexpr int NE = D / 16;              // V dims per lane and key; output blocks of 16 dims
+  static constexpr int ROWS = 16 * RT;
+  static constexpr int KB = F32 ? 2 * NB : NB;   // K loads per 16 keys
+  static constexpr int KW = F32 || ELT == 2 ? 4 : 2;  // words of one
+  static constexpr int VW = NE * ELT / 4;        // words of V per lane and key
+  static constexpr int XS = D + 4;               // exchange row stride (floats)
   static constexpr int L_ML = kTreeWaves * ROWS * XS * 4;  // reference, sum per wave and row
   static constexpr int LDS = L_ML + kTreeWaves * ROWS * 2 * 4;
   // While the keys stream, a wave keeps the tile's scales in its own part of
-  // the exchange area: NDB blocks of 32 K scales, 32 V scales, 32 exponents.
-  static constexpr int SC = (NDB + 2) * 32 * 4;
+  // the exchange area: NB blocks of 32 K scales, 32 V scales, 32 exponents.
+  static constexpr int SC = (NB + 2) * 32 * 4;
   static_assert(SC <= ROWS * XS * 4, "scales fit a wave's exchange area");
-  // head_dim 128 takes more registers than two workgroups per CU leave.
-  static constexpr int WAVES_PER_SIMD = D == 64 ? 2 : 1;
+  // head_dim 128, two tiles: more registers than two workgroups on a CU leave.
+  static constexpr int WAVES_PER_SIMD = D == 128 && RT == 2 ? 1 : 2;
 };
 
-template <int D, typename KT>
-__global__ __launch_bounds__(kTreeWaves* kWave, (TreeCfg<D, KT>::WAVES_PER_SIMD)) void tree_kernel(const TreeParams p) {
-  typedef TreeCfg<D, KT> C;
-  constexpr int NDB = C::NDB, ROWS = C::ROWS, ELT = C::ELT, KW = C::KW, VW = C::VW;
+template <int D, typename KT, int RT>
+__global__ __launch_bounds__(kTreeWaves* kWave, (TreeCfg<D, KT, RT>::WAVES_PER_SIMD)) void tree_kernel(const TreeParams p) {
+  typedef TreeCfg<D, KT, RT> C;
+  constexpr int NB = C::NB, NE = C::NE, ROWS = C::ROWS, ELT = C::ELT, KB = C::KB, KW = C::KW, VW = C::VW;
   constexpr bool Q8 = C::Q8, F32 = C::F32;
-  __shared__ __attribute__((aligned(16))) char lds_raw[C::LDS];
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   lds_t* const lds = (lds_t*)lds_raw;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int c = lane & 31, kh = lane >> 5;
+  const int c = lane & 15, q4 = lane >> 4;
 
-  // Workgroup -> (KV head, split) unit and row tile. The row tiles of a unit
-  // read the same keys, so they are numbered 8 apart: workgroups go to the 8
-  // XCDs in turn, and theirs then share an L2. Later row tiles of a causal
-  // chunk see more keys, so they come first.
+  // Workgroup -> (KV head, split) unit; units go to the 8 XCDs in turn. (One row
+  // tile: calls of more rows take the wide kernel.)
   const TreeItem& it = p.item[blockIdx.y];
-  const int n_rt = it.n_rt, n_split = it.n_split;
-  const int y = blockIdx.x / 8;
-  const int rt = n_rt - 1 - y % n_rt;
-  const int unit = (y / n_rt) * 8 + (int)((blockIdx.x - it.xcd0) % 8);
+  const int n_split = it.n_split;
+  const int unit = (blockIdx.x / 8) * 8 + (int)((blockIdx.x - it.xcd0) % 8);
   if (unit >= p.n_head_kv * n_split) return;
   const int g = unit / n_split, sp = unit % n_split;
   const int n_past = it.n_past, n_kv = n_past + it.n_tokens;
   const int rows = it.n_tokens * p.n_rep;
-  const int row0 = rt * ROWS;
-  // keys that some row of the tile may see
-  const int last_token = min(row0 + ROWS - 1, rows - 1) / p.n_rep;
-  const int lim = it.mask ? n_kv : min(n_kv, n_past + last_token + 1);
   const int tile0 = sp * it.tiles_per_split;
-  const int tile1 = min(tile0 + it.tiles_per_split, (lim + kTreeTile - 1) / kTreeTile);
+  const int tile1 = min(tile0 + it.tiles_per_split, (n_kv + kTreeTile - 1) / kTreeTile);
 
   // ---- loads of a key tile --------------------------------------------------
   // The descriptors start at the tile's first row (64-bit), so a cache of any
@@ -107,27 +147,37 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (TreeCfg<D, KT>::WAVES_PER_SIMD)
   const char* const kbase = it.k + (int64_t)g * p.k_s1;
   const char* const vbase = it.v + (int64_t)g * p.v_s1;
   const int ks2 = (int)p.k_s2, vs2 = (int)p.v_s2;
-  unsigned kw[KW], vw[16 * VW], ksc = 0, vsc = 0;
-  const unsigned ko = (unsigned)(c * ks2 + 16 * kh);
-  const unsigned vo = (unsigned)(4 * kh * vs2 + c * NDB * ELT);
+  unsigned kw[2][KB][KW], vw[8][VW], ksc = 0, vsc = 0;
+  const unsigned ko = (unsigned)(c * ks2 + 4 * KW * q4);
+  const unsigned vo = (unsigned)(4 * q4 * vs2 + c * NE * ELT);
   lds_t* const sc_lds = lds + wave * ROWS * C::XS * 4;
+  const int c32 = lane & 31, half = lane >> 5;
   auto load_k = [&](int tile) __attribute__((always_inline)) {
     const int key0 = tile * kTreeTile;
     const int n = min(n_kv - key0, kTreeTile);
     const rsrc_t r = make_rsrc(kbase + (int64_t)key0 * ks2, (unsigned)((n - 1) * ks2 + D * ELT));
 #pragma unroll
-    for (int s = 0; s < KW / 4; ++s) {
-      const u32x4 x = buf_b128(r, ko + 32 * s);
+    for (int hk = 0; hk < 2; ++hk)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kw[4 * s + j] = x[j];
-    }
+      for (int b = 0; b < KB; ++b) {
+        const unsigned at = ko + (unsigned)(16 * hk * ks2) + 16 * KW * b;
+        if constexpr (KW == 4) {
+          const u32x4 x = buf_b128(r, at);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kw[hk][b][j] = x[j];
+        } else {
+          const u32x2 x = buf_b64(r, at);
+          kw[hk][b][0] = x[0];
+          kw[hk][b][1] = x[1];
+        }
+      }
     if constexpr (Q8) {
-      // the scales of key c: lane half kh takes half of the K row's
+      // the scales of key lane % 32: each half of the wave takes half of the K row's
       const int64_t at = (int64_t)key0 * p.n_head_kv + g;
-      const rsrc_t rk = make_rsrc(it.k_scale + at * (2 * NDB), (unsigned)((n - 1) * p.n_head_kv * 2 * NDB + 2 * NDB));
-      ksc = NDB == 4 ? buf_b32(rk, (unsigned)(c * p.n_head_kv * 8 + 4 * kh)) : buf_b16(rk, (unsigned)(c * p.n_head_kv * 4 + 2 * kh));
+      const rsrc_t rk = make_rsrc(it.k_scale + at * (2 * NB), (unsigned)((n - 1) * p.n_head_kv * 2 * NB + 2 * NB));
+      ksc = NB == 4 ? buf_b32(rk, (unsigned)(c32 * p.n_head_kv * 8 + 4 * half)) : buf_b16(rk, (unsigned)(c32 * p.n_head_kv * 4 + 2 * half));
       const rsrc_t rv = make_rsrc(it.v_scale + at * 2, (unsigned)((n - 1) * p.n_head_kv * 2 + 2));
-      vsc = buf_b16(rv, (unsigned)(c * p.n_head_kv * 2));
+      vsc = buf_b16(rv, (unsigned)(c32 * p.n_head_kv * 2));
     }
   };
   auto load_v = [&](int tile) __attribute__((always_inline)) {
@@ -135,369 +185,396 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (TreeCfg<D, KT>::WAVES_PER_SIMD)
     const int n = min(n_kv - key0, kTreeTile);
     const rsrc_t r = make_rsrc(vbase + (int64_t)key0 * vs2, (unsigned)((n - 1) * vs2 + D * ELT));
 #pragma unroll
-    for (int t = 0; t < 16; ++t) {
-      const unsigned at = vo + (unsigned)((8 * (t >> 2) + (t & 3)) * vs2);
-      if constexpr (NDB * ELT == 16) {
-        const u32x4 x = buf_b128(r, at);
+    for (int j = 0; j < 8; ++j) {  // keys 16 (j / 4) + 4 q4 + j % 4
+      const unsigned at = vo + (unsigned)((16 * (j / 4) + j % 4) * vs2);
+      if constexpr (VW >= 4) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) vw[4 * t + j] = x[j];
-      } else if constexpr (NDB * ELT == 8) {
+        for (int w = 0; w < VW; w += 4) {
+          const u32x4 x = buf_b128(r, at + 4 * w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vw[j][w + i] = x[i];
+        }
+      } else if constexpr (VW == 2) {
         const u32x2 x = buf_b64(r, at);
-        vw[2 * t] = x[0];
-        vw[2 * t + 1] = x[1];
-      } else if constexpr (NDB * ELT == 4) {
-        vw[t] = buf_b32(r, at);
+        vw[j][0] = x[0];
+        vw[j][1] = x[1];
       } else {
-        vw[t] = buf_b16(r, at);
+        vw[j][0] = buf_b32(r, at);
       }
     }
   };
-  if (tile0 >= tile1 && n_split > 1) {  // no key for these rows: nothing to join
-    float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * n_rt + rt) * n_split + sp) * (ROWS * (D + 2));
-    if (threadIdx.x < 2 * ROWS) rec[ROWS * D + threadIdx.x] = threadIdx.x < ROWS ? -INFINITY : 0.f;
-    return;
-  }
   int tile = tile0 + wave;
   if (tile < tile1) {
     load_k(tile);
     load_v(tile);
   }
 
-  // ---- queries ------------------------------------------------------------
-  // Dims of B's step s, lane half kh, element j (A's are loaded the same way):
-  // F32 8 (s / 4) + 4 kh + s % 4; F16 16 s + 8 kh + j; 8-bit
-  // 32 (s / 2) + 16 kh + 8 (s % 2) + j. Each is 16 consecutive bytes of K.
-  float qf[F32 ? D / 2 : 1];
-  f16x8 qh[F32 ? 1 : D / 16], ql[F32 ? 1 : D / 16];
-  float unscale = 1.f;
-  const bool valid = row0 + c < rows;
-  const int token = valid ? (row0 + c) / p.n_rep : 0;
-  {
-    const int h = g * p.n_rep + (valid ? row0 + c - token * p.n_rep : 0);
-    const char* const qp = reinterpret_cast<const char*>(it.q) + (int64_t)token * p.q_s2 + (int64_t)h * p.q_s1;
+  // ---- queries: row c of tile i; dims as K's ------------------------------------
+  float qf[F32 ? RT : 1][F32 ? D / 4 : 1];
+  f16x8 qh[F32 ? 1 : RT][F32 ? 1 : NB], ql[F32 ? 1 : RT][F32 ? 1 : NB];
+  float unscale[RT];
+  int token[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int r = 16 * i + c;
+    const bool valid = r < rows;
+    token[i] = valid ? r / p.n_rep : 0;
+    unscale[i] = 1.f;
+    const int h = g * p.n_rep + (valid ? r - token[i] * p.n_rep : 0);
+    const char* const qp = reinterpret_cast<const char*>(it.q) + (int64_t)token[i] * p.q_s2 + (int64_t)h * p.q_s1;
     if constexpr (F32) {
 #pragma unroll
-      for (int s = 0; s < D / 2; s += 4) {
-        const f32x4 x = gload<f32x4>(qp + 4 * (2 * s + 4 * kh));
+      for (int s = 0; s < D / 4; s += 4) {  // dims 4 s + 4 q4 + j
+        const f32x4 x = gload<f32x4>(qp + 4 * (4 * s + 4 * q4));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) qf[s + j] = valid ? x[j] * p.scale_log2e : 0.f;
+        for (int j = 0; j < 4; ++j) qf[i][s + j] = valid ? x[j] * p.scale_log2e : 0.f;
       }
     } else {
-      float x[D / 2];
-      float amax = 0.f;
+      float x[D / 4], amax = 0.f;
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        const int dim = Q8 ? 32 * (s / 2) + 16 * kh + 8 * (s % 2) : 16 * s + 8 * kh;
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const f32x4 v = gload<f32x4>(qp + 4 * (dim + 4 * e));
+          const f32x4 v = gload<f32x4>(qp + 4 * (32 * b + 8 * q4 + 4 * e));
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            x[8 * s + 4 * e + j] = valid ? v[j] * p.scale_log2e : 0.f;
-            amax = fmaxf(amax, fabsf(x[8 * s + 4 * e + j]));
+            x[8 * b + 4 * e + j] = valid ? v[j] * p.scale_log2e : 0.f;
+            amax = fmaxf(amax, fabsf(x[8 * b + 4 * e + j]));
           }
         }
-      }
-      amax = max32(amax);
+      amax = max_quarters(amax);
       int qexp = 0;
       if (amax > 0.f && amax < INFINITY) qexp = max(ilogbf(amax) - 13, -100);
-      unscale = ldexpf(Q8 ? kByteUnscale : 1.f, qexp);
+      unscale[i] = ldexpf(Q8 ? kByteUnscale : 1.f, qexp);
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s)
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           f16x2 hi, lo;
-          split2(ldexpf(x[8 * s + j], -qexp), ldexpf(x[8 * s + j + 1], -qexp), hi, lo);
-          qh[s][j] = hi[0];
-          qh[s][j + 1] = hi[1];
-          ql[s][j] = lo[0];
-          ql[s][j + 1] = lo[1];
+          split2(ldexpf(x[8 * b + j], -qexp), ldexpf(x[8 * b + j + 1], -qexp), hi, lo);
+          qh[i][b][j] = hi[0];
+          qh[i][b][j + 1] = hi[1];
+          ql[i][b][j] = lo[0];
+          ql[i][b][j + 1] = lo[1];
         }
     }
   }
 
   // ---- state --------------------------------------------------------------
-  floatx16 o[NDB];
-  float ref = -INFINITY, l = 0.f;
+  f32x4 o[RT][NE];
+  float ref[RT], l[RT];
 #pragma unroll
-  for (int db = 0; db < NDB; ++db) o[db] = (floatx16)(0.f);
+  for (int i = 0; i < RT; ++i) {
+    ref[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int db = 0; db < NE; ++db) o[i][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 
   for (; tile < tile1; tile += kTreeWaves) {
     const int key0 = tile * kTreeTile;
     const int next = tile + kTreeWaves;
-    // ---- S^T = K . Q^T ------------------------------------------------------
-    floatx16 s = (floatx16)(0.f);
-    f32x4 vfac[4], vexp[4];  // 8-bit: V scales of the lane's keys and their exponents
-    if constexpr (F32) {
-#pragma unroll
-      for (int st = 0; st < D / 2; ++st) s = mfma_f32(__builtin_bit_cast(float, kw[st]), qf[st], s);
-    } else if constexpr (!Q8) {
-#pragma unroll
-      for (int st = 0; st < D / 16; ++st) {
-        const f16x8 k8 = __builtin_bit_cast(f16x8, u32x4{kw[4 * st], kw[4 * st + 1], kw[4 * st + 2], kw[4 * st + 3]});
-        s = mfma_f16(k8, ql[st], s);
-        s = mfma_f16(k8, qh[st], s);
-      }
-    } else {
-      // the scales, to where each lane can read those of its own 16 keys
+    // ---- S^T = K . Q^T: s[i][4 hk + j] is key 16 hk + 4 q4 + j of row c ----------
+    float s[RT][8];
+    f32x4 vfac[2], vexp[2];  // 8-bit: V scales of the lane's keys and their exponents
+    if constexpr (Q8) {
+      // the scales, to where each lane can read those of its own keys
       auto h2f = [](unsigned x) { return (float)__builtin_bit_cast(_Float16, (unsigned short)x); };
-      if constexpr (NDB == 4) {
-        lds_store<float>(sc_lds + (64 * kh + c) * 4, h2f(ksc & 0xffffu));
-        lds_store<float>(sc_lds + (64 * kh + 32 + c) * 4, h2f(ksc >> 16));
+      if constexpr (NB == 4) {
+        lds_store<float>(sc_lds + (64 * half + c32) * 4, h2f(ksc & 0xffffu));
+        lds_store<float>(sc_lds + (64 * half + 32 + c32) * 4, h2f(ksc >> 16));
       } else {
-        lds_store<float>(sc_lds + (32 * kh + c) * 4, h2f(ksc));
+        lds_store<float>(sc_lds + (32 * half + c32) * 4, h2f(ksc));
       }
       const float v = h2f(vsc);
-      if (kh == 0) {
-        lds_store<float>(sc_lds + (32 * NDB + c) * 4, v);
-        lds_store<float>(sc_lds + (32 * NDB + 32 + c) * 4, (float)scale_exponent(v < INFINITY ? v : 0.f));
+      if (half == 0) {
+        lds_store<float>(sc_lds + (32 * NB + c32) * 4, v);
+        lds_store<float>(sc_lds + (32 * NB + 32 + c32) * 4, (float)scale_exponent(v < INFINITY ? v : 0.f));
       }
       wave_lds_fence();
+    }
 #pragma unroll
-      for (int b = 0; b < NDB; ++b) {
-        floatx16 part = (floatx16)(0.f);
+    for (int hk = 0; hk < 2; ++hk) {
+      f32x4 acc[RT];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const unsigned w0 = kw[4 * b + 2 * e] ^ 0x80808080u, w1 = kw[4 * b + 2 * e + 1] ^ 0x80808080u;
-          const f16x2 x0 = bytes_f16<0, 1>(w0, w0), x1 = bytes_f16<2, 3>(w0, w0);
-          const f16x2 x2 = bytes_f16<0, 1>(w1, w1), x3 = bytes_f16<2, 3>(w1, w1);
-          const f16x8 k8 = {x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
-          part = mfma_f16(k8, ql[2 * b + e], part);
-          part = mfma_f16(k8, qh[2 * b + e], part);
-        }
+      for (int i = 0; i < RT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (F32) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 sc = lds_load<f32x4>(sc_lds + (32 * b + 8 * q + 4 * kh) * 4);
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[4 * q + j] = fmaf(part[4 * q + j], sc[j], s[4 * q + j]);
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+              acc[i] = mfma16_f32(__builtin_bit_cast(float, kw[hk][b][j]), qf[i][4 * b + j], acc[i]);
+      } else {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          f16x8 k8;
+          if constexpr (Q8) {
+            const unsigned w0 = kw[hk][b][0] ^ 0x80808080u, w1 = kw[hk][b][1] ^ 0x80808080u;
+            const f16x2 x0 = bytes_f16<0, 1>(w0, w0), x1 = bytes_f16<2, 3>(w0, w0);
+            const f16x2 x2 = bytes_f16<0, 1>(w1, w1), x3 = bytes_f16<2, 3>(w1, w1);
+            k8 = f16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+          } else {
+            k8 = __builtin_bit_cast(f16x8, u32x4{kw[hk][b][0], kw[hk][b][1], kw[hk][b][2], kw[hk][b][3]});
+          }
+          if constexpr (Q8) {
+            const f32x4 sc = lds_load<f32x4>(sc_lds + (32 * b + 16 * hk + 4 * q4) * 4);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+              f32x4 part = mfma16_f16(k8, ql[i][b], f32x4{0.f, 0.f, 0.f, 0.f});
+              part = mfma16_f16(k8, qh[i][b], part);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(part[j], sc[j], acc[i][j]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+              acc[i] = mfma16_f16(k8, ql[i][b], acc[i]);
+              acc[i] = mfma16_f16(k8, qh[i][b], acc[i]);
+            }
+          }
         }
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        vfac[q] = lds_load<f32x4>(sc_lds + (32 * NDB + 8 * q + 4 * kh) * 4);
-        vexp[q] = lds_load<f32x4>(sc_lds + (32 * NDB + 32 + 8 * q + 4 * kh) * 4);
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][4 * hk + j] = acc[i][j];
+    }
+    if constexpr (Q8) {
+#pragma unroll
+      for (int hk = 0; hk < 2; ++hk) {
+        vfac[hk] = lds_load<f32x4>(sc_lds + (32 * NB + 16 * hk + 4 * q4) * 4);
+        vexp[hk] = lds_load<f32x4>(sc_lds + (32 * NB + 32 + 16 * hk + 4 * q4) * 4);
       }
       wave_lds_fence();  // the scales are read before the next tile's are written
     }
     if (next < tile1) load_k(next);
 
     // ---- mask -----------------------------------------------------------------
-    unsigned vis = ~0u;
+    // bit 4 hk + j of vis: the row sees the lane's key 16 hk + 4 q4 + j
+    unsigned row_vis[RT], vis[RT];
     const bool masked = key0 + kTreeTile > n_past;  // a tile of drafted keys
     if (masked) {
-      vis = visible_bits(it, token, key0);
-      const unsigned mine = vis >> (4 * kh);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = mine >> (8 * (e >> 2) + (e & 3)) & 1u ? s[e] : -INFINITY;
+      for (int i = 0; i < RT; ++i) {
+        row_vis[i] = visible_bits(it, token[i], key0);
+        vis[i] = slots_of(row_vis[i], q4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[i][e] = vis[i] >> e & 1u ? s[i][e] : -INFINITY;
+      }
     }
 
     // ---- softmax, relative to ref -----------------------------------------------
-    float top;
-    if constexpr (Q8) {  // of the probability times the V row's scale
-      floatx16 x;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = fmaf(s[e], unscale, vexp[e >> 2][e & 3]);
-      top = max32(max16(x, -INFINITY));
-    } else {
-      top = max32(max16(s, -INFINITY)) * unscale;
-    }
-    const float alpha = move_ref(ref, top);
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0ull) {
-      l *= alpha;
+    for (int i = 0; i < RT; ++i) {
+      float top = -INFINITY;
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) o[db] *= alpha;
-    }
-    const float at = ref == -INFINITY ? 0.f : ref;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int e = 0; e < 8; e += 2) {
+        // (8-bit: of the probability times the V row's scale)
+        const float a = Q8 ? fmaf(s[i][e], unscale[i], vexp[e / 4][e % 4]) : s[i][e];
+        const float b = Q8 ? fmaf(s[i][e + 1], unscale[i], vexp[e / 4][e % 4 + 1]) : s[i][e + 1];
+        top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, a), b);
+      }
+      const float alpha = move_ref(ref[i], max_quarters(top) * (Q8 ? 1.f : unscale[i]));
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0ull) {
+        l[i] *= alpha;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      s[e] = fast_exp2(fmaf(s[e], unscale, -at));
-      sum[e & 3] += s[e];
-    }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    if constexpr (Q8) {
+        for (int db = 0; db < NE; ++db) o[i][db] *= alpha;
+      }
+      const float at = ref[i] == -INFINITY ? 0.f : ref[i];
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] *= vfac[e >> 2][e & 3];
-      if (masked) {  // (a scale may not be finite: 0 times it is not 0)
-        const unsigned mine = vis >> (4 * kh);
+      for (int e = 0; e < 8; ++e) {
+        s[i][e] = fast_exp2(fmaf(s[i][e], unscale[i], -at));
+        sum[e & 1] += s[i][e];
+        if constexpr (Q8) s[i][e] *= vfac[e / 4][e % 4];
+      }
+      l[i] += sum[0] + sum[1];
+      if constexpr (Q8) {
+        if (masked) {  // (a scale may not be finite: 0 times it is not 0)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = mine >> (8 * (e >> 2) + (e & 3)) & 1u ? s[e] : 0.f;
+          for (int e = 0; e < 8; ++e) s[i][e] = vis[i] >> e & 1u ? s[i][e] : 0.f;
+        }
       }
     }
 
     // ---- values that are not finite, in a tile that some rows do not see --------
     // Their products with a masked key's probability of 0 would not be 0: they
     // are taken as zeros, and the rows that do see them get NaN there.
-    unsigned nf[NDB];  // bit t: the lane's key t, dim NDB c + db
+    unsigned nf[NE];  // bit j: the lane's key j, dim NE c + db
     bool any_nf = false;
     if constexpr (!Q8) {
       if (masked) {
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) nf[db] = 0u;
+        for (int db = 0; db < NE; ++db) nf[db] = 0u;
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
+        for (int j = 0; j < 8; ++j) {
 #pragma unroll
           for (int w = 0; w < VW; ++w) {
             if constexpr (F32) {
-              if (not_finite(__builtin_bit_cast(float, vw[VW * t + w]))) {
-                nf[w] |= 1u << t;
-                vw[VW * t + w] = 0u;
+              if (not_finite(__builtin_bit_cast(float, vw[j][w]))) {
+                nf[w] |= 1u << j;
+                vw[j][w] = 0u;
               }
             } else {
-              const unsigned b = not_finite2(vw[VW * t + w]);
-              nf[2 * w] |= (b & 1u) << t;
-              nf[2 * w + 1] |= (b >> 1) << t;
-              vw[VW * t + w] &= (b & 1u ? 0u : 0xffffu) | (b & 2u ? 0u : 0xffff0000u);
+              const unsigned b = not_finite2(vw[j][w]);
+              nf[2 * w] |= (b & 1u) << j;
+              nf[2 * w + 1] |= (b >> 1) << j;
+              vw[j][w] &= (b & 1u ? 0u : 0xffffu) | (b & 2u ? 0u : 0xffff0000u);
             }
           }
         }
         unsigned all = 0u;
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) all |= nf[db];
+        for (int db = 0; db < NE; ++db) all |= nf[db];
         any_nf = __builtin_amdgcn_ballot_w64(all != 0u) != 0ull;
       }
     }
 
-    // ---- O^T += V^T . P^T -----------------------------------------------------
+    // ---- O^T += V^T . P^T: o[i][db][j] is dim NE (4 q4 + j) + db of row c ----------
     if constexpr (F32) {
 #pragma unroll
-      for (int t = 0; t < 16; ++t)
+      for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) o[db] = mfma_f32(__builtin_bit_cast(float, vw[VW * t + db]), s[t], o[db]);
+        for (int db = 0; db < NE; ++db)
+#pragma unroll
+          for (int i = 0; i < RT; ++i) o[i][db] = mfma16_f32(__builtin_bit_cast(float, vw[j][db]), s[i][j], o[i][db]);
     } else {
+      f16x8 ph[RT], pl[RT];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        f16x8 ph, pl;
+      for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           f16x2 hi, lo;
-          split2(s[8 * u + j], s[8 * u + j + 1], hi, lo);
-          ph[j] = hi[0];
-          ph[j + 1] = hi[1];
-          pl[j] = lo[0];
-          pl[j + 1] = lo[1];
+          split2(s[i][j], s[i][j + 1], hi, lo);
+          ph[i][j] = hi[0];
+          ph[i][j + 1] = hi[1];
+          pl[i][j] = lo[0];
+          pl[i][j + 1] = lo[1];
+        }
+      if constexpr (Q8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vw[j][w] ^= 0x80808080u;
+      }
+#pragma unroll
+      for (int db = 0; db < NE; ++db) {
+        f16x8 v8;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          f16x2 x;
+          if constexpr (Q8) {
+            const unsigned w0 = vw[j][db / 4], w1 = vw[j + 1][db / 4];
+            x = db % 4 == 0 ? bytes_f16<0, 4>(w1, w0) : db % 4 == 1 ? bytes_f16<1, 5>(w1, w0)
+              : db % 4 == 2 ? bytes_f16<2, 6>(w1, w0) : bytes_f16<3, 7>(w1, w0);
+          } else {
+            x = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(vw[j + 1][db / 2], vw[j][db / 2],
+                                                                db & 1 ? 0x07060302u : 0x05040100u));
+          }
+          v8[j] = x[0];
+          v8[j + 1] = x[1];
         }
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          f16x8 v8;
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            const int t = 8 * u + j;
-            f16x2 x;
-            if constexpr (Q8) {
-              const unsigned w0 = vw[t] ^ 0x80808080u, w1 = vw[t + 1] ^ 0x80808080u;
-              x = db == 0 ? bytes_f16<0, 4>(w1, w0) : db == 1 ? bytes_f16<1, 5>(w1, w0)
-                : db == 2 ? bytes_f16<2, 6>(w1, w0) : bytes_f16<3, 7>(w1, w0);
-            } else {
-              const unsigned w0 = vw[VW * t + db / 2], w1 = vw[VW * (t + 1) + db / 2];
-              x = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(w1, w0, db & 1 ? 0x07060302u : 0x05040100u));
-            }
-            v8[j] = x[0];
-            v8[j + 1] = x[1];
-          }
-          o[db] = mfma_f16(v8, pl, o[db]);
-          o[db] = mfma_f16(v8, ph, o[db]);
+        for (int i = 0; i < RT; ++i) {
+          o[i][db] = mfma16_f16(v8, pl[i], o[i][db]);
+          o[i][db] = mfma16_f16(v8, ph[i], o[i][db]);
         }
       }
     }
     if constexpr (!Q8) {
       if (masked && any_nf) {
         for (int src = 0; src < kWave; ++src) {  // the lane that holds the values
-          const int sc = src & 31, sh = src >> 5;
-          unsigned bits[NDB], some = 0u;
+          const int sc = src & 15, sq = src >> 4;
+          unsigned bits[NE], some = 0u;
 #pragma unroll
-          for (int db = 0; db < NDB; ++db) {
+          for (int db = 0; db < NE; ++db) {
             bits[db] = (unsigned)__builtin_amdgcn_readlane((int)nf[db], src);
             some |= bits[db];
           }
           if (some == 0u) continue;
-          const unsigned x = vis >> (4 * sh);  // the row's sight of that lane's keys, bit t
-          const unsigned seen = (x & 0xfu) | (x >> 4 & 0xf0u) | (x >> 8 & 0xf00u) | (x >> 12 & 0xf000u);
 #pragma unroll
-          for (int db = 0; db < NDB; ++db)
+          for (int i = 0; i < RT; ++i) {
+            const unsigned seen = slots_of(row_vis[i], sq);
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if ((bits[db] & seen) != 0u && 8 * (e >> 2) + 4 * kh + (e & 3) == sc) o[db][e] = NAN;
+            for (int db = 0; db < NE; ++db)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if ((bits[db] & seen) != 0u && 4 * q4 + j == sc) o[i][db][j] = NAN;
+          }
         }
       }
     }
     if (next < tile1) load_v(next);
   }
 
-  // ---- the waves' parts ---------------------------------------------------------
+  // ---- the waves' parts, through LDS -----------------------------------------------
   wave_lds_fence();
-  const float ls = sum32(l);
-  if (kh == 0) {
-    lds_store<float>(lds + C::L_ML + ((wave * ROWS + c) * 2) * 4, ref);
-    lds_store<float>(lds + C::L_ML + ((wave * ROWS + c) * 2 + 1) * 4, ls);
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const float lt = sum_quarters(l[i]);
+    if (q4 == 0) lds_store<f32x2>(lds + C::L_ML + ((wave * ROWS + 16 * i + c) * 2) * 4, f32x2{ref[i], lt});
   }
   __syncthreads();
-  float mt = -INFINITY, lt = 0.f;
-  {
-    constexpr float unit_o = Q8 ? kByteUnscale : 1.f;  // of the values' 2^-10
+  constexpr float unit_o = Q8 ? kByteUnscale : 1.f;  // of the values' 2^-10
+  float mt[RT], lt[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
     f32x2 ml[kTreeWaves];
+    mt[i] = -INFINITY;
+    lt[i] = 0.f;
 #pragma unroll
     for (int w = 0; w < kTreeWaves; ++w) {
-      ml[w] = lds_load<f32x2>(lds + C::L_ML + ((w * ROWS + c) * 2) * 4);
-      mt = fmaxf(mt, ml[w][0]);
+      ml[w] = lds_load<f32x2>(lds + C::L_ML + ((w * ROWS + 16 * i + c) * 2) * 4);
+      mt[i] = fmaxf(mt[i], ml[w][0]);
     }
-    const float mu = mt == -INFINITY ? 0.f : mt;
+    const float mu = mt[i] == -INFINITY ? 0.f : mt[i];
 #pragma unroll
-    for (int w = 0; w < kTreeWaves; ++w) lt += ml[w][1] * fast_exp2(ml[w][0] - mu);
-    const float wt = fast_exp2(ref - mu) * unit_o;
+    for (int w = 0; w < kTreeWaves; ++w) lt[i] += ml[w][1] * fast_exp2(ml[w][0] - mu);
+    const float wt = fast_exp2(ref[i] - mu) * unit_o;
 #pragma unroll
-    for (int db = 0; db < NDB; ++db) o[db] *= wt;
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int db = 0; db < NE; db += 4)
+        lds_store<f32x4>(lds + ((wave * ROWS + 16 * i + c) * C::XS + NE * (4 * q4 + j) + db) * 4,
+                         f32x4{o[i][db][j], o[i][db + 1][j], o[i][db + 2][j], o[i][db + 3][j]} * wt);
   }
-  // One 32-dim block at a time through LDS; a thread sums the waves' parts of
-  // its (row, column) pairs.
-  constexpr int PER = ROWS * 32 / (kTreeWaves * kWave);
-  float acc[PER][NDB];
-#pragma unroll
-  for (int db = 0; db < NDB; ++db) {
-    if (db > 0) __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      lds_store<f32x4>(lds + ((wave * ROWS + c) * C::XS + 8 * q + 4 * kh) * 4,
-                       f32x4{o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]});
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int idx = e * kTreeWaves * kWave + threadIdx.x;
-      float x = 0.f;
-#pragma unroll
-      for (int w = 0; w < kTreeWaves; ++w) x += lds_load<float>(lds + ((w * ROWS + idx / 32) * C::XS + idx % 32) * 4);
-      acc[e][db] = x;
-    }
-  }
-  if (n_split > 1) {
-    float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * n_rt + rt) * n_split + sp) * (ROWS * (D + 2));
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int idx = e * kTreeWaves * kWave + threadIdx.x;
-      if (row0 + idx / 32 >= rows) continue;
-      float* const w = rec + tree_record_at(D, idx / 32, (NDB * (idx % 32)) & ~3);
-      if constexpr (NDB == 4) gstore(w, f32x4{acc[e][0], acc[e][1], acc[e][2], acc[e][3]});
-      else gstore(w + 2 * (idx % 2), f32x2{acc[e][0], acc[e][1]});
-    }
-    if (wave == 0 && kh == 0) {
-      rec[ROWS * D + c] = mt;
-      rec[ROWS * D + ROWS + c] = lt;
-    }
-    return;
-  }
-  // the rows' sums to where the storing threads read them
-  if (wave == 0 && kh == 0) lds_store<float>(lds + C::L_ML + c * 4, mt == -INFINITY ? 0.f : 1.f / lt);
   __syncthreads();
+  float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)g * n_split + sp) * (kTreeRows * (D + 2));
+  if (n_split > 1) {
+    if (wave == 0 && q4 == 0) {
 #pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    const int idx = e * kTreeWaves * kWave + threadIdx.x;
-    const int r = row0 + idx / 32;
+      for (int i = 0; i < RT; ++i) {
+        rec[kTreeRows * D + 16 * i + c] = mt[i];
+        rec[kTreeRows * D + kTreeRows + 16 * i + c] = lt[i];
+      }
+    }
+  } else {
+    // the rows' factors to where the storing threads read them (where the waves'
+    // references lay: every wave has read them)
+    if (wave == 0 && q4 == 0) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+        lds_store<float>(lds + C::L_ML + (16 * i + c) * 4, mt[i] == -INFINITY && lt[i] == 0.f ? 0.f : 1.f / lt[i]);
+    }
+    __syncthreads();
+  }
+  // thread: four dims of a row
+#pragma unroll
+  for (int e = 0; e < ROWS * D / 4; e += kTreeWaves * kWave) {
+    const int idx = e + threadIdx.x, r = idx / (D / 4), d = 4 * (idx % (D / 4));
     if (r >= rows) continue;
-    const float inv = lds_load<float>(lds + C::L_ML + (idx / 32) * 4);
-    const int t = r / p.n_rep, h = g * p.n_rep + r % p.n_rep;
-    char* const w = reinterpret_cast<char*>(it.out) + (int64_t)t * p.o_s2 + (int64_t)h * p.o_s1 + 4 * NDB * (idx % 32);
-    if constexpr (NDB == 4) gstore(w, f32x4{acc[e][0] * inv, acc[e][1] * inv, acc[e][2] * inv, acc[e][3] * inv});
-    else gstore(w, f32x2{acc[e][0] * inv, acc[e][1] * inv});
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; ++w) x += lds_load<f32x4>(lds + ((w * ROWS + r) * C::XS + d) * 4);
+    if (n_split > 1) {
+      put_record(rec + tree_record_at(D, r, d), x);
+    } else {
+      const int t = r / p.n_rep, h = g * p.n_rep + r - t * p.n_rep;
+      gstore(reinterpret_cast<char*>(it.out) + (int64_t)t * p.o_s2 + (int64_t)h * p.o_s1 + 4 * d,
+             x * lds_load<float>(lds + C::L_ML + r * 4));
+    }
   }
 }
 
@@ -586,20 +663,31 @@ int tree_tile_rows(int rows) { return rows <= 32 ? 32 : 128; }
 
 size_t tree_record_floats(int head_dim, int tile_rows) { return (size_t)tile_rows * (head_dim + 2); }
 
-template <int D>
-static hipError_t launch_narrow(const TreeParams& p, dim3 grid, int elt, hipStream_t stream) {
-  if (elt == 1) hipLaunchKernelGGL((tree_kernel<D, int8_t>), grid, dim3(kTreeWaves * kWave), 0, stream, p);
-  else if (elt == 2) hipLaunchKernelGGL((tree_kernel<D, _Float16>), grid, dim3(kTreeWaves * kWave), 0, stream, p);
-  else hipLaunchKernelGGL((tree_kernel<D, float>), grid, dim3(kTreeWaves * kWave), 0, stream, p);
+template <int D, typename KT, int RT>
+static hipError_t launch_narrow_t(const TreeParams& p, dim3 grid, hipStream_t stream) {
+  typedef TreeCfg<D, KT, RT> C;
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&tree_kernel<D, KT, RT>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+  if (attr != hipSuccess) return attr;
+  hipLaunchKernelGGL((tree_kernel<D, KT, RT>), grid, dim3(kTreeWaves * kWave), C::LDS, stream, p);
   return hipGetLastError();
+}
+
+// 16 rows where they are enough: half the products and vector instructions.
+template <int D>
+static hipError_t launch_narrow(const TreeParams& p, dim3 grid, int elt, bool two, hipStream_t stream) {
+  if (elt == 1) return two ? launch_narrow_t<D, int8_t, 2>(p, grid, stream) : launch_narrow_t<D, int8_t, 1>(p, grid, stream);
+  if (elt == 2) return two ? launch_narrow_t<D, _Float16, 2>(p, grid, stream) : launch_narrow_t<D, _Float16, 1>(p, grid, stream);
+  return two ? launch_narrow_t<D, float, 2>(p, grid, stream) : launch_narrow_t<D, float, 1>(p, grid, stream);
 }
 
 hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, hipStream_t stream) {
   unsigned gx = 0;
   int64_t units = 0;  // waves' worth of records to join, of the largest item
-  int splits = 1;
+  int splits = 1, most = 0;
   for (int i = 0; i < n_items; ++i) {
     const TreeItem& it = p.item[i];
+    most = std::max(most, it.n_tokens * p.n_rep);
     gx = std::max(gx, ((unsigned)p.n_head_kv * it.n_split + 7) / 8 * 8 * (unsigned)it.n_rt);
     if (it.n_split > 1)
       units = std::max(units, ((int64_t)it.n_tokens * p.n_rep + 31) / 32 * p.n_head_kv * (head_dim / 8));
@@ -607,8 +695,8 @@ hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, 
   }
   const dim3 grid(gx, n_items);
   const hipError_t e = tile_rows == 128  ? launch_tree_wide(p, grid, head_dim, elt, stream)
-                       : head_dim == 64 ? launch_narrow<64>(p, grid, elt, stream)
-                                        : launch_narrow<128>(p, grid, elt, stream);
+                       : head_dim == 64 ? launch_narrow<64>(p, grid, elt, most > 16, stream)
+                                        : launch_narrow<128>(p, grid, elt, most > 16, stream);
   if (e != hipSuccess || units == 0) return e;
   // slices: one batch of records in flight each, as far as a workgroup goes
   int slices = 1;
