@@ -35,6 +35,12 @@ constexpr int kThreads = 256;
 constexpr int kSmallChunk = 4 * kThreads, kChunk = 8 * kThreads;
 constexpr int64_t kFewPerCu = 4;
 
+// A row may start at any multiple of 4 bytes (an odd vocabulary); loads and stores
+// of four take that as they are.
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+__device__ inline f32x4 load4(const char* p) { return *(const __attribute__((address_space(1))) f32x4_any*)p; }
+__device__ inline void store4(char* p, f32x4 v) { *(__attribute__((address_space(1))) f32x4_any*)p = v; }
+
 // Larger for the larger value, and for the lower token among equal values; 0
 // for what is never chosen.
 __device__ inline uint64_t key_of(float v, int t) {
@@ -72,7 +78,6 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) 
   const char* const in = p.in + row * p.in_nb + 4 * (int64_t)base;
   char* const out = p.out + row * p.out_nb + 4 * (int64_t)base;
   const char* const mask = p.mask ? p.mask + row * p.mask_nb + base / 8 : nullptr;
-  const bool vec = ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
 
   // Group k of thread tid: logits 4 (tid + 256 k) .. of the chunk.
   float x[PER][4];
@@ -81,8 +86,8 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) 
   for (int k = 0; k < PER; ++k) {
     const int i = 4 * (tid + kThreads * k);
     allow[k] = ~0u;
-    if (vec && i + 4 <= n) {
-      const f32x4 v = gload<f32x4>(in + 4 * i);
+    if (i + 4 <= n) {
+      const f32x4 v = load4(in + 4 * i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[k][j] = v[j];
     } else {
@@ -160,8 +165,8 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) 
         top = key > top ? key : top;
       }
     }
-    if (vec && i + 4 <= n) {
-      gstore(out + 4 * i, f32x4{x[k][0], x[k][1], x[k][2], x[k][3]});
+    if (i + 4 <= n) {
+      store4(out + 4 * i, f32x4{x[k][0], x[k][1], x[k][2], x[k][3]});
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
