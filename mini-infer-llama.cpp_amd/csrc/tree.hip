@@ -37,7 +37,8 @@
 // lo stays normal, each query row is scaled by the power of two that puts its
 // largest element in [2^13, 2^14) (undone in the exponent's multiply-add), and
 // the probabilities are 2^(s - ref) for a reference that keeps the largest
-// between 2^6 and 2^14 (move_ref; the division by their sum undoes it): 2^-22
+// between 2^6 and 2^14 (move_ref; the division by their sum undoes it; with an
+// F32 cache 2^-14 times that, since its values may be of any size): 2^-22
 // relative to the row's largest element.
 //   8-bit K: a row's scales (one per 32 dims) multiply the S^T of their own
 //   32 dims. 8-bit V: the row's one scale multiplies the probability; ref keeps
@@ -382,7 +383,8 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (TreeCfg<D, KT, RT>::WAVES_PER_S
 #pragma unroll
         for (int db = 0; db < NE; ++db) o[i][db] *= alpha;
       }
-      const float at = ref[i] == -INFINITY ? 0.f : ref[i];
+      // (F32: probabilities up to 1, so that no product with a value leaves float's range)
+      const float at = ref[i] == -INFINITY ? 0.f : ref[i] + (F32 ? kRefMost : 0.f);
       float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -658,7 +660,8 @@ __global__ __launch_bounds__(kJoinSlices* kWave) void tree_combine_kernel(const 
 }
 
 // The kernel that streams keys to registers for up to 32 rows, else the wide
-// kernel (tree_wide.hip), whose waves without rows only fetch.
+// kernel (tree_wide.hip), whose waves without rows only fetch. Eight times 28 rows
+// over 4000 8-bit keys of 128 (us): 20.9, wide 32.6; F16 keys of 64 12.2, 13.6.
 int tree_tile_rows(int rows) { return rows <= 32 ? 32 : 128; }
 
 size_t tree_record_floats(int head_dim, int tile_rows) { return (size_t)tile_rows * (head_dim + 2); }
@@ -673,7 +676,8 @@ static hipError_t launch_narrow_t(const TreeParams& p, dim3 grid, hipStream_t st
   return hipGetLastError();
 }
 
-// 16 rows where they are enough: half the products and vector instructions.
+// 16 rows where they are enough: half the products and vector instructions. 24
+// times 14 rows over 3000 8-bit keys of 64 (us): 14.6, with two tiles 19.2.
 template <int D>
 static hipError_t launch_narrow(const TreeParams& p, dim3 grid, int elt, bool two, hipStream_t stream) {
   if (elt == 1) return two ? launch_narrow_t<D, int8_t, 2>(p, grid, stream) : launch_narrow_t<D, int8_t, 1>(p, grid, stream);

@@ -94,9 +94,11 @@ __device__ inline float max16(const floatx16& s, float x) {
 // what it scales), and then to 2^6 for the largest seen: rows move after their
 // first tile hardly ever, so that what has been summed is hardly ever rescaled.
 // `top`: the tile's largest score (plus the V scales' exponent). Returns the
-// factor of what has been summed.
+// factor of what has been summed. (No contraction: `top` may be a product that
+// is -inf, and fused with ref = -inf it would be compared before it is rounded.)
 constexpr float kRefMost = 14.f, kRefNew = 6.f;
 __device__ inline float move_ref(float& ref, float top) {
+#pragma clang fp contract(off)
   if (!(top - ref > kRefMost)) return 1.f;
   const float now = top - kRefNew, alpha = fast_exp2(ref - now);
   ref = now;
