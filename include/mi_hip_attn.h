@@ -86,7 +86,8 @@ int mi_hip_set_alloc_limit(uint64_t bytes);
 
 /* The split-KV decode kernel's scratch: one partial-result record per
  * workgroup, per-group counters (dynamic sub-tile claims, merge election,
- * arrivals) and status words. Launches that share a workspace must be
+ * arrivals) and status words; and the parts that mi_hip_attn_tree and
+ * mi_hip_logits_adjust join. Launches that share a workspace must be
  * ordered (one stream, or synchronised); launches on different workspaces may
  * run concurrently. Every KV cache owns one (mi_hip_kv_workspace); callers
  * that attend over explicit tensors create their own, or fall back to the
@@ -374,9 +375,10 @@ typedef struct mi_hip_tree_mask {
  * query j sees of scale q_j.k_t, times v_t. F32, F16 and 8-bit caches; items
  * share the head shape, element type and scale, n_past and n_tokens may differ.
  * masks: one per item, or NULL (every item a chain). A query that sees no key
- * gives zeros, and so does one whose every score is -inf. What lies in rows that
- * a query does not see never shows in its output, infinities and NaN included;
- * an infinite or NaN value in a V row that it sees may give NaN for infinity.
+ * gives zeros, and so does one whose every score is below float's range. What
+ * lies in rows that a query does not see never shows in its output, infinities
+ * and NaN included; an infinite value in a row that it sees may give NaN for
+ * infinity, and so may a score above float's range.
  * Scratch for joining the parts of long caches: ws of the first item, else its
  * cache's workspace, else the library default; calls that share one must be
  * ordered. Nothing is kept in it between calls, so unlike the other decode entry
@@ -464,10 +466,10 @@ int mi_hip_rope_append(const mi_hip_rope_args* args);
  * tokens at positions of their own. Per row x of Q and K (one head of one
  * token): y = x / sqrt(mean(x^2) + eps) * w where the norm's weights are given,
  * then the rotation of MI_OP_ROPE at the token's position (the angle is one
- * float product, position * frequency); Q into q_out (which may equal q), K and
- * V into the cache rows n_past + token. Without weights, pos and freq the
- * results of mi_hip_rope_append. Any cache type. No counterpart in the
- * reference. */
+ * float product, position * frequency); Q into q_out (which may equal q, with
+ * the same strides), K and V into the cache rows n_past + token. Without
+ * weights, pos and freq the results of mi_hip_rope_append. Any cache type. May
+ * be captured into a graph. No counterpart in the reference. */
 typedef struct mi_hip_norm_rope_args {
   mi_hip_kv* kv;
   int32_t layer;

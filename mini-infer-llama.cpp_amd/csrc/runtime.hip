@@ -1830,6 +1830,9 @@ int mi_hip_norm_rope_append(const mi_hip_norm_rope_args* a) {
                   kv->d.n_head_kv);
     if (!strides4(a->q_nb) || !strides4(a->q_out_nb))
       return fail(MI_HIP_E_INVALID, "Q strides must be multiples of 4 bytes");
+    if (a->q == a->q_out && (a->q_nb[0] != a->q_out_nb[0] || (a->n_head > 1 && a->q_nb[1] != a->q_out_nb[1]) ||
+                             (a->n_tokens > 1 && a->q_nb[2] != a->q_out_nb[2])))
+      return fail(MI_HIP_E_INVALID, "in place, q and q_out must have the same strides");
   }
   if (!strides4(a->k_nb) || !strides4(a->v_nb))
     return fail(MI_HIP_E_INVALID, "K/V strides must be multiples of 4 bytes");
