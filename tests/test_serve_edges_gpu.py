@@ -83,6 +83,24 @@ def test_huge_rows_that_other_queries_see(hip, stream, cache, d, rep, t):
 
 
 @pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rep,t", KERNELS)
+def test_rows_of_very_different_sizes(hip, stream, cache, d, rep, t):
+    # K and V rows that grow and shrink by powers of ten from row to row; per element within the tolerance of
+    # the largest V row that the query sees
+    rng = np.random.default_rng([d, rep, t, 4])
+    hkv, n_past = 2, 400
+    n = n_past + t
+    lo, hi = {"f32": (-12, 12), "f16": (-3, 4), "q8": (-5, 6)}[cache]
+    k = rng.standard_normal((n + 1, hkv, d)) * 10.0 ** rng.integers(-3, 1, (n + 1, hkv, 1))
+    v = rng.standard_normal((n + 1, hkv, d)) * 10.0 ** rng.integers(lo, hi, (n + 1, hkv, 1))
+    s = Seq(hip, rng, cache, d, hkv, rep, n_past, t, None, spare=1, k=k.astype(np.float32), v=v.astype(np.float32))
+    run(hip, [s], stream)
+    s.check(f"{cache} {d} {rep} {t}")
+    s.close()
+
+
+@pytest.mark.parametrize("cache", CACHES)
 @pytest.mark.parametrize("rep,t", KERNELS)
 def test_queries_that_are_not_finite_and_scores_below_the_range(hip, stream, cache, rep, t):
     rng = np.random.default_rng([rep, t, 2])
