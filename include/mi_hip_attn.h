@@ -508,7 +508,8 @@ int mi_hip_norm_rope_append(const mi_hip_norm_rope_args* args);
  * src/model_qwen2.cpp:690-700), -1 if every y is -inf or NaN. All pointers are
  * device memory; offsets have n_rows + 1 entries, row r's list is
  * [off[r], off[r + 1]). Ids outside [0, n_vocab) in the lists are passed over.
- * May be captured into a graph. No counterpart in the reference. */
+ * Calls for ids that share a workspace must be ordered. May be captured into a
+ * graph. No counterpart in the reference. */
 typedef struct mi_hip_logits_args {
   const float* logits;
   size_t nb;                /* bytes between rows */

@@ -144,6 +144,10 @@ struct NormRope {
 };
 hipError_t launch_norm_rope(const NormRope& p, hipStream_t stream);
 
+// Arrival counters of a workspace, kArrivalWords apart: counters in one line are
+// counted one after the other in memory (64 rows of logits: 53 us, 27 apart).
+constexpr int kArrivals = 1024, kArrivalWords = 64;
+
 // logits.hip. One row per sequence or tree node; the lists' offsets have
 // n_rows + 1 entries.
 struct LogitsAdjust {
@@ -159,7 +163,8 @@ struct LogitsAdjust {
   const char* mask;        // bit t of a row's 32-bit words: token t is allowed; null: all
   int64_t mask_nb;
   int32_t* ids;            // greedy ids; null: not asked for
-  uint64_t* part;          // scratch for ids: logits_chunks(n_vocab) words a row
+  uint64_t* part;          // scratch for ids: logits_chunks(n_vocab) words a row,
+  unsigned* arrived;       // and a counter, zero before and after the launch
   int32_t n_vocab, n_rows;
 };
 int logits_chunks(int n_vocab);

@@ -12,8 +12,8 @@
 // counts the history's tokens that lie in the chunk in LDS (whole numbers, so the
 // atomics' order does not show) and one wave adds up the biases; then each logit
 // is finished, stored, and the chunk's best kept as one 64-bit key (value order,
-// then lower token). A second kernel takes the row's best. Each logit is read
-// and written once; a row's history is read by every chunk of the row, from the
+// then lower token); the row's last workgroup takes the best of those. Each logit
+// is read and written once; a row's history is read by every chunk of the row, from the
 // caches. Bound: memory for many rows, the chain of dependent loads (offsets,
 // history, LDS) for few; there the chunks are smaller, so that more workgroups
 // share a row.
@@ -31,7 +31,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // before the stores were nontemporal: 29.7 us;
 // 4096 a chunk 35.0, 1024, where the histories are read twice as often, 34.7).
 // Chunks of 1024 while a launch has at most four of them per CU: in a graph, one
-// row of 151936 6.3 us (2048: 6.9), 4 rows 7.0 (7.4), 16 rows 10.2 (8.8).
+// row of 32000 5.5 us (2048: 6.4), 16 rows 6.1 (6.9); of 151936 7.1 and 8.6 either
+// way, where more workgroups take longer to be counted.
 constexpr int kThreads = 256;
 constexpr int kSmallChunk = 4 * kThreads, kChunk = 8 * kThreads;
 constexpr int64_t kFewPerCu = 4;
@@ -41,7 +42,7 @@ constexpr int64_t kFewPerCu = 4;
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 __device__ inline f32x4 load4(const char* p) { return *(const __attribute__((address_space(1))) f32x4_any*)p; }
 // (The logits are not read again here: nontemporal, so that a launch does not end
-// by writing its XCDs' L2s back. 48 rows of 151936: 14.9 -> 11.5 us.)
+// by writing its XCDs' L2s back. 48 rows of 151936: 11.7 us instead of 14.9.)
 __device__ inline void store4(char* p, f32x4 v) {
   __builtin_nontemporal_store((f32x4_any)v, (__attribute__((address_space(1))) f32x4_any*)p);
 }
@@ -182,22 +183,32 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) 
   top = wave_max_u64(top);
   if (lane == 0) best[tid / kWave] = top;
   __syncthreads();
-  if (tid == 0) {
+  // The last workgroup of the row to get here takes the best of its chunks, whose
+  // keys are in memory before they are counted: agent-scope stores go through the
+  // L2, and the wave waits for its own. (With a second launch for this, us a call:
+  // one row of 151936 10.1 instead of 7.9, 48 rows 11.7 instead of 11.1; in a graph
+  // 6.2 instead of 7.1, one row of 32000 5.6 instead of 5.5.)
+  if (tid >= kWave) return;
 #pragma unroll
-    for (int w = 1; w < kThreads / kWave; ++w) top = best[w] > top ? best[w] : top;
-    p.part[(int64_t)row * gridDim.x + blockIdx.x] = top;
+  for (int w = 0; w < kThreads / kWave; ++w) top = best[w] > top ? best[w] : top;
+  uint64_t* const part = p.part + (int64_t)row * gridDim.x;
+  unsigned before = 0;
+  if (lane == 0) {
+    __hip_atomic_store(part + blockIdx.x, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    wait_vmem<0>();
+    before = __hip_atomic_fetch_add(p.arrived + kArrivalWords * row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-}
-
-// One wave per row: the best of the row's chunks.
-__global__ __launch_bounds__(kWave) void logits_best_kernel(const uint64_t* part, int n_chunks, int32_t* ids) {
-  uint64_t top = 0ull;
-  for (int i = threadIdx.x; i < n_chunks; i += kWave) {
-    const uint64_t k = part[(int64_t)blockIdx.x * n_chunks + i];
+  if (__builtin_amdgcn_readfirstlane((int)before) != (int)gridDim.x - 1) return;
+  top = 0ull;
+  for (int i = lane; i < (int)gridDim.x; i += kWave) {
+    const uint64_t k = __hip_atomic_load(part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     top = k > top ? k : top;
   }
   top = wave_max_u64(top);
-  if (threadIdx.x == 0) ids[blockIdx.x] = top ? (int32_t)~(unsigned)top : -1;
+  if (lane == 0) {
+    p.ids[row] = top ? (int32_t)~(unsigned)top : -1;
+    __hip_atomic_store(p.arrived + kArrivalWords * row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
 }
 
 int logits_chunks(int n_vocab) { return (n_vocab + kSmallChunk - 1) / kSmallChunk; }
@@ -208,9 +219,6 @@ hipError_t launch_logits_adjust(const LogitsAdjust& p, int n_cu, hipStream_t str
   const int chunk = small ? kSmallChunk : kChunk, chunks = (p.n_vocab + chunk - 1) / chunk;
   if (small) hipLaunchKernelGGL(logits_kernel<kSmallChunk>, dim3(chunks, p.n_rows), dim3(kThreads), 0, stream, p);
   else hipLaunchKernelGGL(logits_kernel<kChunk>, dim3(chunks, p.n_rows), dim3(kThreads), 0, stream, p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || !p.ids) return e;
-  hipLaunchKernelGGL(logits_best_kernel, dim3(p.n_rows), dim3(kWave), 0, stream, p.part, chunks, p.ids);
   return hipGetLastError();
 }
 

@@ -328,12 +328,13 @@ bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) %
 }  // namespace
 
 // ---------------------------------------------------------------------------
-// Decode workspace: [status words][two counter sets][records][parts], each
-// 256-byte aligned. Zeroed once at creation; afterwards the kernels keep the
-// counter sets zero between launches (see decode.hip) and the epoch stamps
-// make stale records recognisable. The parts belong to the launches that keep
-// nothing between calls (tree attention's split records, the logits' chunk
-// maxima): each writes what it then reads.
+// Decode workspace: [status words][two counter sets][records][arrival counters]
+// [parts], each 256-byte aligned. Zeroed once at creation; afterwards the kernels
+// keep the counter sets zero between launches (see decode.hip) and the epoch
+// stamps make stale records recognisable. Arrival counters and parts belong to
+// the launches that keep nothing between calls (tree attention's split records,
+// the logits' chunk maxima): each writes the parts that it then reads, and
+// leaves at zero the counters that it uses.
 // ---------------------------------------------------------------------------
 struct mi_hip_workspace {
   int groups = 0;           // groups one launch may have (counter-set capacity)
@@ -345,6 +346,7 @@ struct mi_hip_workspace {
   float* rec = nullptr;
   size_t part_bytes = 0;    // capacity of the parts (0: none)
   char* part = nullptr;
+  unsigned* arrived = nullptr;  // kArrivals counters of the launches that join parts
   std::mutex mu;
   uint32_t epoch = 0;       // stamp of the last launch
   int dirty[2] = {0, 0};    // counter set s: groups [0, dirty[s]) the last launch on it used
@@ -367,11 +369,13 @@ size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 size_t ws_counter_bytes(int groups) { return 2 * (size_t)groups * mi::kCtrInts * sizeof(unsigned); }
 
+constexpr size_t kArrivalBytes = (size_t)mi::kArrivals * mi::kArrivalWords * sizeof(unsigned);
+
 // Bytes of a workspace covering `groups` groups, `rec_bytes` of records and
 // `part_bytes` of parts.
 size_t ws_total_bytes(int groups, size_t rec_bytes, size_t part_bytes) {
   return kWsAlign + round_up(ws_counter_bytes(groups), kWsAlign) + round_up(rec_bytes, kWsAlign) +
-         round_up(part_bytes, kWsAlign);
+         (part_bytes ? kArrivalBytes + round_up(part_bytes, kWsAlign) : 0);
 }
 
 // Bytes of parts that let a tree-attention launch split its keys over
@@ -393,7 +397,10 @@ void ws_layout(mi_hip_workspace* ws, char* base, int groups, size_t rec_bytes, s
   ws->cnt = reinterpret_cast<unsigned*>(base + kWsAlign);
   char* const rec = base + kWsAlign + round_up(ws_counter_bytes(groups), kWsAlign);
   ws->rec = reinterpret_cast<float*>(rec);
-  ws->part = part_bytes ? rec + round_up(rec_bytes, kWsAlign) : nullptr;
+  if (part_bytes) {
+    ws->arrived = reinterpret_cast<unsigned*>(rec + round_up(rec_bytes, kWsAlign));
+    ws->part = reinterpret_cast<char*>(ws->arrived) + kArrivalBytes;
+  }
 }
 
 // Groups and record bytes that cover every decode launch of a head shape: up
@@ -1894,9 +1901,9 @@ int mi_hip_logits_adjust(const mi_hip_logits_args* a) {
   if (rc) return rc;
   mi_hip_workspace* const ws = a->ws ? a->ws : g.default_ws;
   if (!ws) return fail(MI_HIP_E_STATE, "no workspace (the library default is gone)");
-  // as many rows a launch as their chunks' maxima have room for (and the grid)
+  // as many rows a launch as their chunks' maxima and counters have room for (and the grid)
   const int64_t row_part = (int64_t)mi::logits_chunks(a->n_vocab) * 8;
-  const int64_t most = std::min<int64_t>(65535, a->ids ? (int64_t)ws->part_bytes / row_part : 65535);
+  const int64_t most = a->ids ? std::min<int64_t>(mi::kArrivals, (int64_t)ws->part_bytes / row_part) : 65535;
   if (most < 1) return fail(MI_HIP_E_UNSUPPORTED, "n_vocab %d: the workspace does not hold one row's parts", a->n_vocab);
   mi::LogitsAdjust p{};
   p.in_nb = (int64_t)a->nb;
@@ -1906,6 +1913,7 @@ int mi_hip_logits_adjust(const mi_hip_logits_args* a) {
   p.bias = a->bias;
   p.mask_nb = (int64_t)a->mask_nb;
   p.part = reinterpret_cast<uint64_t*>(ws->part);
+  p.arrived = ws->arrived;
   p.n_vocab = a->n_vocab;
   for (int64_t r = 0; r < a->n_rows; r += most) {
     p.n_rows = (int32_t)std::min(most, a->n_rows - r);

@@ -157,6 +157,27 @@ def test_two_calls_at_once_on_their_own_workspaces(hip, stream):
     hip.check(hip.mi_hip_workspace_destroy(ws[0]))
 
 
+def test_ids_of_two_calls_at_once_on_their_own_workspaces(hip, stream):
+    import torch
+    rng = np.random.default_rng(7)
+    ws = [hip.workspace_create(1, 1, 64) for _ in range(2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    xs = [dev(rng.standard_normal(s).astype(np.float32)) for s in ((3, 151936), (40, 33000))]
+    outs = [torch.empty_like(x) for x in xs]
+    ids = [torch.full((20, len(x)), -5, device="cuda", dtype=torch.int32) for x in xs]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for x, out, d, w, st in zip(xs, outs, ids, ws, streams):
+            a = mh.logits_args(x, out, st.cuda_stream, ids=d[i])
+            a.ws = w
+            hip.check(hip.mi_hip_logits_adjust(ctypes.byref(a)))
+    torch.cuda.synchronize()
+    for x, d in zip(xs, ids):
+        assert torch.equal(d, x.argmax(1).to(torch.int32).expand(20, -1))
+    for w in ws:
+        hip.check(hip.mi_hip_workspace_destroy(w))
+
+
 @pytest.mark.parametrize("kind", [mh.MI_TYPE_F32, mh.MI_TYPE_F16, mh.MI_HIP_TYPE_Q8])
 def test_a_captured_step_replays(hip, stream, kind):
     # norms and RoPE with append, attention, the kept rows and a read back in one graph, replayed with
