@@ -14,8 +14,9 @@
 // cut into row tiles (row r is token r / n_rep, head r % n_rep of the group),
 // the keys into splits of whole 32-key tiles. A workgroup owns (item, KV head,
 // row tile, split). With one split its result is the output, otherwise it is a
-// record in the workspace that tree_combine_kernel joins (a second launch, so
-// that neither needs a counter and both may be captured into a graph).
+// record in the workspace that tree_combine_kernel joins: a second launch, since
+// a group's last workgroup takes longer for its records from other XCDs than a
+// launch does (one token over 4000 keys of 64: 20.5 us instead of 11.3).
 //
 // This kernel: one tile of 16 or 32 rows, for calls that need no more. Its waves
 // take the split's key tiles in turn, K and V straight to registers, and meet in
