@@ -121,6 +121,7 @@ struct TreeItem {
   int32_t n_split;          // key splits (1: no records, the kernel writes the output)
   int32_t tiles_per_split;  // key tiles (where there is more than one split: whole tiles of the kernel)
   int32_t rec0;             // the item's first record
+  int32_t unit_rt;          // row tiles per unit: n_rt over the units' parts, rounded up
   uint32_t xcd0;            // XCD of the item's first unit (their units go to the 8 XCDs in turn)
 };
 
@@ -130,6 +131,7 @@ struct TreeParams {
   int32_t n_rep, n_head_kv;
   float scale_log2e;
   float* rec;  // records of the items with more than one split
+  int32_t row_shift;  // 2^row_shift units per KV head and split: the row tiles in turn
   TreeItem item[kTreeMaxItems];  // grid row y serves item y
 };
 static_assert(sizeof(TreeParams) <= 4096 - 64, "kernel arguments");

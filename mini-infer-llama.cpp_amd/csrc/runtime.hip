@@ -774,28 +774,29 @@ int run_prefill(const mi_hip_attn_args* a, const Resolved& r, hipStream_t stream
 }
 
 // Tree attention: how many key tiles one workgroup takes. A unit (item, KV
-// head, split) brings n_rt workgroups, one per row tile, to one XCD; units go to
-// the XCDs in turn through all items. What a number of tiles per split costs
-// follows what the kernels were measured to take (us; one workgroup alone on
-// its CU): kTileUs per key tile, kStartUs besides, kSharedCu times the tiles when
-// several share a CU; records that are to be joined kJoinUs for the second launch
-// and kRecordUs per MB. Measured with every split (us a call): a 25-token tree
-// over 4107 F16 keys (28/4 heads of 128) 20.0 at 6 tiles (4: 22.3, 12: 23.4, all
-// in one: 136), one token over 32000 (14/2 heads of 64) 12.5 at 8 (4: 16.2, 32:
-// 13.4), over 500 8.0 unsplit (4: 10.1), 24 times one over 4095 8-bit keys (28/4
-// of 128) 30.2 at 28 (12: 37.5, 64: 36.9), a 64-token tree over 16000 F32 keys
-// (28/4 of 128) 91 at 32 (16: 101, 64: 166).
+// head, split, part of the row tiles) brings its workgroups, one per row tile, to
+// one XCD; units go to the XCDs in turn through all items. What a number of tiles per split costs
+// follows what the kernels take (us): kTileUs per key tile, kStartUs besides,
+// kSharedCu times the tiles when several workgroups share a CU; records that are
+// to be joined kJoinUs for the second launch and kRecordUs per MB. The figures
+// are fitted to calls measured with every split, 84 shapes of 128 rows and more
+// and 72 of up to 16: the chosen split is 1 and 2% slower than the best, on the
+// average. Some (us a call): a 25-token tree over 4107 F16 keys (28/4 heads of
+// 128) 20.7 at 6 tiles (4: 23.6, 12: 23.4, all in one: 139), 1024 tokens after
+// 1337 91 at 40 to 64 (unsplit: 122) with an 8-bit cache, one token over 32000
+// F16 keys (14/2 heads of 64) 12.5 at 8 (4: 16.2, 32: 13.4), over 500 8.0 unsplit
+// (4: 10.1).
 constexpr float kTileUs[3][3][2] = {
     // head_dim 64, 128 of 8-bit, F16, F32 caches
     {{0.17f, 0.37f}, {0.14f, 0.28f}, {0.33f, 0.66f}},  // up to 16 rows
     {{0.26f, 0.48f}, {0.16f, 0.37f}, {0.45f, 1.06f}},  // up to 32 rows
-    {{0.84f, 1.42f}, {0.55f, 1.00f}, {1.20f, 2.40f}},  // tiles of 128 rows
+    {{0.76f, 1.28f}, {0.50f, 0.90f}, {1.08f, 2.16f}},  // tiles of 128 rows
 };
 constexpr float kStartUs = 6.f, kJoinUs = 4.f, kRecordUs = 0.25f;
 // by the same three kinds: workgroups that a CU holds (registers) for head_dim 64
 // and 128, and what the tiles take when it holds more than one
 constexpr int kPerCu[3][2] = {{3, 2}, {2, 1}, {2, 2}};
-constexpr float kSharedCu[3] = {2.0f, 1.7f, 1.7f};
+constexpr float kSharedCu[3] = {2.0f, 1.7f, 1.4f};
 
 void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int elt, int rows, int tile_rows, size_t part_bytes) {
   constexpr int kXcds = 8;
@@ -818,6 +819,13 @@ void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int elt, int rows, 
     whole += all;
     seen += it.mask ? all : (float)it.n_rt * (tiles[i] - 0.5f * it.n_tokens / mi::kTreeTile);
   }
+  // Few units (KV heads times splits) of many row tiles: parts of the row tiles,
+  // up to as many as make every XCD's share the same.
+  auto row_shift = [](int64_t units, int rt) {
+    int shift = 0;
+    while ((units << shift) % kXcds != 0 && 2 << shift <= rt) ++shift;
+    return shift;
+  };
   float best = 0.f;
   int best_per = longest;
   // all in one, then 1, 2, .. 7, 8, 10, 12, 14, 16, 20, .. times the least
@@ -832,15 +840,19 @@ void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int elt, int rows, 
       rt = std::max(rt, p.item[i].n_rt);
     }
     if (records > cap) continue;
-    // workgroups with work, per CU of the fullest XCD
-    const float load = (float)((units + kXcds - 1) / kXcds) * rt * (seen / whole);
-    const int on_cu = std::max(1, (int)std::ceil(load * kXcds / g.n_cu));
+    // workgroups per CU of the fullest XCD; where there are several, those of
+    // early tokens make up for those of late ones
+    const int shift = row_shift(units, rt), parts = 1 << shift;
+    const int64_t load = (units * parts + kXcds - 1) / kXcds * ((rt + parts - 1) / parts);
+    const int on_cu = (int)std::min<int64_t>(1 << 20, std::max<int64_t>(1, (load * kXcds + g.n_cu - 1) / g.n_cu));
     const int rounds = (on_cu + per_cu - 1) / per_cu;
-    const float cost = rounds * (kStartUs + per * tile_us * (std::min(on_cu, per_cu) > 1 ? kSharedCu[kind] : 1.f)) +
+    const float longer = (std::min(on_cu, per_cu) > 1 ? kSharedCu[kind] : 1.f) * (on_cu > 1 ? seen / whole : 1.f);
+    const float cost = rounds * (kStartUs + per * tile_us * longer) +
                        (records ? kJoinUs + records * record_mb * kRecordUs : 0.f);
     if (k == 0 || cost < best) {
       best = cost;
       best_per = per;
+      p.row_shift = shift;
     }
   }
   int64_t rec = 0, at = 0;
@@ -851,7 +863,8 @@ void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int elt, int rows, 
     it.rec0 = (int32_t)rec;
     it.xcd0 = (uint32_t)(at % kXcds);
     if (it.n_split > 1) rec += (int64_t)p.n_head_kv * it.n_rt * it.n_split;
-    at += (int64_t)p.n_head_kv * it.n_split;
+    it.unit_rt = (it.n_rt + (1 << p.row_shift) - 1) >> p.row_shift;
+    at += (int64_t)p.n_head_kv * it.n_split << p.row_shift;
   }
 }
 

@@ -693,7 +693,7 @@ hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, 
   for (int i = 0; i < n_items; ++i) {
     const TreeItem& it = p.item[i];
     most = std::max(most, it.n_tokens * p.n_rep);
-    gx = std::max(gx, ((unsigned)p.n_head_kv * it.n_split + 7) / 8 * 8 * (unsigned)it.n_rt);
+    gx = std::max(gx, (((unsigned)p.n_head_kv * it.n_split << p.row_shift) + 7) / 8 * 8 * (unsigned)it.unit_rt);
     if (it.n_split > 1)
       units = std::max(units, ((int64_t)it.n_tokens * p.n_rep + 31) / 32 * p.n_head_kv * (head_dim / 8));
     splits = std::max(splits, it.n_split);

@@ -102,21 +102,29 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int c = lane & 31, kh = lane >> 5;
 
-  // workgroup -> unit and row tile, as in tree_kernel
+  // Workgroup -> unit and row tile, as in tree_kernel: a unit is (KV head, split,
+  // every 2^row_shift-th row tile), its row tiles with the most keys come first.
   const TreeItem& it = p.item[blockIdx.y];
   const int n_rt = it.n_rt, n_split = it.n_split;
-  const int y = blockIdx.x / 8;
-  const int rt = n_rt - 1 - y % n_rt;
-  const int unit = (y / n_rt) * 8 + (int)((blockIdx.x - it.xcd0) % 8);
-  if (unit >= p.n_head_kv * n_split) return;
-  const int g = unit / n_split, sp = unit % n_split;
+  const int y = blockIdx.x / 8, yu = y / it.unit_rt;
+  const int unit = yu * 8 + (int)((blockIdx.x - it.xcd0) % 8);
+  const int gs = unit >> p.row_shift;
+  const int rt = n_rt - 1 - ((y - yu * it.unit_rt) << p.row_shift) - (unit - (gs << p.row_shift));
+  if (gs >= p.n_head_kv * n_split || rt < 0) return;
+  const int g = gs / n_split, sp = gs - g * n_split;
   const int n_past = it.n_past, n_kv = n_past + it.n_tokens;
   const int rows = it.n_tokens * p.n_rep;
   const int row0 = rt * ROWS;
   const int last_token = min(row0 + ROWS - 1, rows - 1) / p.n_rep;
   const int lim = it.mask ? n_kv : min(n_kv, n_past + last_token + 1);
-  const int key_begin = sp * it.tiles_per_split * kTreeTile;
-  const int key_end = min(lim, key_begin + it.tiles_per_split * kTreeTile);
+  // Each row tile cuts the keys that it sees into n_split parts (whole tiles), so
+  // that the units, and with them the XCDs, have the same work (2048 8-bit keys
+  // and as many tokens, 14/2 heads of 64: 87 -> 65 us; all row tiles of a unit on
+  // one XCD, that is with row_shift 0: 65 instead of 49).
+  const int tiles = (lim + TK - 1) / TK;
+  const int per_split = it.mask ? it.tiles_per_split * kTreeTile : (tiles + n_split - 1) / n_split * TK;
+  const int key_begin = min(sp * per_split, lim);
+  const int key_end = min(lim, key_begin + per_split);
   const bool active = row0 + 32 * wave < rows;  // the wave has rows
   if (key_begin >= key_end && n_split > 1) {  // no key for these rows: nothing to join
     float* const rec = p.rec + ((int64_t)it.rec0 + (int64_t)(g * n_rt + rt) * n_split + sp) * (ROWS * (D + 2));
