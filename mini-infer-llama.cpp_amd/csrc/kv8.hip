@@ -15,7 +15,10 @@
 // (max |x| > 8319008), reads back as NaN.
 //
 // Every kernel here reads each input once and writes each output once; the
-// arithmetic is far below what the memory takes.
+// arithmetic is far below what the memory takes. 16384 positions of 4 heads of
+// 128, us a kernel: K quantised 10.4 (42 MB, 4.1 TB/s), V 9.3, read back as F16
+// 6.0 (26 MB, 4.2 TB/s); norms, RoPE and append of 4096 tokens, 28/4 heads of 128,
+// F16 cache 24.2 (143 MB, 5.9 TB/s); a few rows 2 to 4, a launch's own time.
 #include <cmath>
 #include <type_traits>
 
@@ -322,6 +325,7 @@ hipError_t launch_kv_read(const CacheView& c, int which, int pos0, int n_tokens,
   return hipGetLastError();
 }
 
+// Bound: one read's latency per eight rows (6 of 25 rows, 14/2 heads of 64: 3.4 us).
 // Two bytes of one position's plane per thread, the kept rows in order: row
 // n_past + i is written after it has been read (as some idx[j] <= i, j <= i),
 // by the same thread, so the move may overlap itself. kInFlight rows are read

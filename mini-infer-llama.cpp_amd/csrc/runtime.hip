@@ -426,7 +426,8 @@ int ws_create(int groups, size_t rec_bytes, size_t part_bytes, mi_hip_workspace*
     delete ws;
     return rc;
   }
-  hipError_t e = hipMemset(p, 0, bytes);  // counters zero, record stamps 0 (no launch's epoch)
+  // counters zero, record stamps 0 (no launch's epoch); the parts need nothing
+  hipError_t e = hipMemset(p, 0, bytes - round_up(part_bytes, kWsAlign));
   if (e == hipSuccess) e = hipDeviceSynchronize();
   if (e != hipSuccess) {
     dev_free(p, bytes);
@@ -775,13 +776,13 @@ int run_prefill(const mi_hip_attn_args* a, const Resolved& r, hipStream_t stream
 
 // Tree attention: how many key tiles one workgroup takes. A unit (item, KV
 // head, split, part of the row tiles) brings its workgroups, one per row tile, to
-// one XCD; units go to the XCDs in turn through all items. What a number of tiles per split costs
-// follows what the kernels take (us): kTileUs per key tile, kStartUs besides,
-// kSharedCu times the tiles when several workgroups share a CU; records that are
-// to be joined kJoinUs for the second launch and kRecordUs per MB. The figures
-// are fitted to calls measured with every split, 84 shapes of 128 rows and more
-// and 72 of up to 16: the chosen split is 1 and 2% slower than the best, on the
-// average. Some (us a call): a 25-token tree over 4107 F16 keys (28/4 heads of
+// one XCD; units go to the XCDs in turn through all items. What a number of tiles
+// per split costs follows what the kernels take (us): kTileUs per key tile,
+// kStartUs besides, kSharedCu times the tiles when several workgroups share a CU;
+// records that are to be joined kJoinUs for the second launch and kRecordUs per
+// MB. The figures are fitted to calls measured with every split, 84 shapes of more
+// than 32 rows and 72 of up to 16: the chosen split is 1 and 2% slower than the
+// best, on the average. Some (us a call): a 25-token tree over 4107 F16 keys (28/4 heads of
 // 128) 20.7 at 6 tiles (4: 23.6, 12: 23.4, all in one: 139), 1024 tokens after
 // 1337 91 at 40 to 64 (unsplit: 122) with an 8-bit cache, one token over 32000
 // F16 keys (14/2 heads of 64) 12.5 at 8 (4: 16.2, 32: 13.4), over 500 8.0 unsplit
