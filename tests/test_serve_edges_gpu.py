@@ -137,6 +137,21 @@ def test_groups_at_the_borders_between_the_kernels(hip, stream, cache, d, hkv, r
     s.close()
 
 
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("d,hkv,rep,items", [  # n_past, tokens and mask of each item
+    (64, 1, 7, [(0, 500, "chain")]), (64, 1, 7, [(900, 300, "random")]), (128, 4, 7, [(70, 260, "chain")]),
+    (128, 3, 5, [(0, 300, "chain"), (1000, 1, "chain"), (33, 90, "tree"), (5, 450, "chain"), (2000, 40, "random")]),
+    (64, 2, 7, [(1500, 400, "chain"), (0, 130, "all"), (257, 19, "chain")])])
+def test_many_row_tiles_and_mixed_batches(hip, stream, cache, d, hkv, rep, items):
+    # row tiles that cut their own keys, dealt in parts where a call has few (KV head, split) units
+    rng = np.random.default_rng([d, hkv, rep, len(items)])
+    seqs = [Seq(hip, rng, cache, d, hkv, rep, n_past, t, make_bits(rng, kind, t)) for n_past, t, kind in items]
+    run(hip, seqs, stream)
+    for i, s in enumerate(seqs):
+        s.check(f"item {i} {items[i]}")
+        s.close()
+
+
 def test_two_calls_at_once_on_their_own_workspaces(hip, stream):
     import torch
     rng = np.random.default_rng(3)
