@@ -13,8 +13,8 @@
 // atomics' order does not show) and one wave adds up the biases; then each logit
 // is finished, stored, and the chunk's best kept as one 64-bit key (value order,
 // then lower token); the row's last workgroup takes the best of those. Each logit
-// is read and written once; a row's history is read by every chunk of the row, from the
-// caches. Bound: memory for many rows, the chain of dependent loads (offsets,
+// is read and written once; a row's history is read by every chunk of the row, from
+// the caches. Bound: memory for many rows, the chain of dependent loads (offsets,
 // history, LDS) for few; there the chunks are smaller, so that more workgroups
 // share a row.
 #include "attn_common.h"
@@ -26,15 +26,12 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// Chunks of 2048: 16 KB of LDS, so that eight workgroups fit a CU and their
-// chains of loads overlap (64 rows of 151936 with histories, biases and a mask,
-// before the stores were nontemporal: 29.7 us;
-// 4096 a chunk 35.0, 1024, where the histories are read twice as often, 34.7).
-// Chunks of 1024 while a launch has at most four of them per CU: in a graph, one
-// row of 32000 5.5 us (2048: 6.4), 16 rows 6.1 (6.9); of 151936 7.1 and 8.6 either
-// way, where more workgroups take longer to be counted.
-constexpr int kThreads = 256;
-constexpr int kSmallChunk = 4 * kThreads, kChunk = 8 * kThreads;
+// Chunks of 2048 logits; of 4096 and 512 threads where rows have histories, which
+// every chunk reads (64 rows of 151936 with histories, biases and a mask 24.9 us,
+// by 2048 26.5; 48 rows without lists 12.7, by 2048 11.3); of 1024 while a launch
+// has at most four of them per CU (in a graph, one row of 32000 5.5 us, by 2048
+// 6.4, 16 rows 6.1 and 6.9; of 151936 7.1 and 8.6 either way, where more workgroups
+// take longer to be counted).
 constexpr int64_t kFewPerCu = 4;
 
 // A row may start at any multiple of 4 bytes (an odd vocabulary); loads and stores
@@ -68,13 +65,13 @@ __device__ inline uint64_t wave_max_u64(uint64_t x) {
 
 }  // namespace
 
-template <int CHUNK>
-__global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) {
-  constexpr int PER = CHUNK / (4 * kThreads);  // groups of four logits per thread
+template <int CHUNK, int THREADS>
+__global__ __launch_bounds__(THREADS) void logits_kernel(const LogitsAdjust p) {
+  constexpr int PER = CHUNK / (4 * THREADS);  // groups of four logits per thread
   constexpr int kInFlight = 8;                 // history ids per thread
   __shared__ __attribute__((aligned(16))) unsigned count[CHUNK];
   __shared__ __attribute__((aligned(16))) float bias[CHUNK];
-  __shared__ uint64_t best[kThreads / kWave];
+  __shared__ uint64_t best[THREADS / kWave];
   const int row = blockIdx.y, base = blockIdx.x * CHUNK;
   const int n = min(CHUNK, p.n_vocab - base);
   const int tid = threadIdx.x, lane = tid % kWave;
@@ -85,12 +82,28 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) 
   char* const out = p.out + row * p.out_nb + 4 * (int64_t)base;
   const char* const mask = p.mask ? p.mask + row * p.mask_nb + base / 8 : nullptr;
 
-  // Group k of thread tid: logits 4 (tid + 256 k) .. of the chunk.
+      // The lists' first loads, then the logits': loads come back in order, and the
+  // lists are worked on while the logits are on their way.
+  unsigned at[kInFlight], bat = ~0u;
+  float bval = 0.f;
+  auto read_hist = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+      at[u] = i + u * THREADS < h1 ? (unsigned)p.hist[i + u * THREADS] - (unsigned)base : ~0u;
+  };
+  auto read_bias = [&](int i) __attribute__((always_inline)) {
+    bat = i < b1 ? (unsigned)p.bias_id[i] - (unsigned)base : ~0u;
+    bval = i < b1 ? p.bias[i] : 0.f;
+  };
+  if (counts) read_hist(h0 + tid);
+  if (biases && tid < kWave) read_bias(b0 + lane);
+
+  // Group k of thread tid: logits 4 (tid + THREADS k) .. of the chunk.
   float x[PER][4];
   unsigned allow[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int i = 4 * (tid + kThreads * k);
+    const int i = 4 * (tid + THREADS * k);
     allow[k] = ~0u;
     if (i + 4 <= n) {
       const f32x4 v = load4(in + 4 * i);
@@ -103,22 +116,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) 
     if (mask && i < n) allow[k] = gload<unsigned>(mask + (i / 32) * 4) >> (i % 32);
   }
   if (counts || biases) {
-    // (the lists' first loads are on their way while LDS is cleared)
-    unsigned at[kInFlight];
-    auto read_hist = [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-        at[u] = i + u * kThreads < h1 ? (unsigned)p.hist[i + u * kThreads] - (unsigned)base : ~0u;
-    };
-    unsigned bat = ~0u;
-    float bval = 0.f;
-    auto read_bias = [&](int i) __attribute__((always_inline)) {
-      bat = i < b1 ? (unsigned)p.bias_id[i] - (unsigned)base : ~0u;
-      bval = i < b1 ? p.bias[i] : 0.f;
-    };
-    read_hist(h0 + tid);
-    if (tid < kWave) read_bias(b0 + lane);
-    for (int i = 4 * tid; i < CHUNK; i += 4 * kThreads) {
+    for (int i = 4 * tid; i < CHUNK; i += 4 * THREADS) {
       *reinterpret_cast<f32x4*>(count + i) = f32x4{0.f, 0.f, 0.f, 0.f};
       *reinterpret_cast<f32x4*>(bias + i) = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -127,7 +125,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) 
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u)
         if (at[u] < (unsigned)n) atomicAdd(&count[at[u]], 1u);
-      i += kInFlight * kThreads;
+      i += kInFlight * THREADS;
       if (i < h1) read_hist(i);
     }
     // One wave adds the biases, lane by lane, so that a token that is listed
@@ -154,7 +152,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) 
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
 #pragma clang fp contract(off)
-    const int i = 4 * (tid + kThreads * k);
+    const int i = 4 * (tid + THREADS * k);
     if (i >= n) break;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -190,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) 
   // 6.2 instead of 7.1, one row of 32000 5.6 instead of 5.5.)
   if (tid >= kWave) return;
 #pragma unroll
-  for (int w = 0; w < kThreads / kWave; ++w) top = best[w] > top ? best[w] : top;
+  for (int w = 0; w < THREADS / kWave; ++w) top = best[w] > top ? best[w] : top;
   uint64_t* const part = p.part + (int64_t)row * gridDim.x;
   unsigned before = 0;
   if (lane == 0) {
@@ -211,15 +209,18 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(const LogitsAdjust p) 
   }
 }
 
-int logits_chunks(int n_vocab) { return (n_vocab + kSmallChunk - 1) / kSmallChunk; }
+int logits_chunks(int n_vocab) { return (n_vocab + 1023) / 1024; }
+
+template <int CHUNK, int THREADS>
+static hipError_t launch_logits(const LogitsAdjust& p, hipStream_t stream) {
+  const dim3 grid((unsigned)((p.n_vocab + CHUNK - 1) / CHUNK), (unsigned)p.n_rows);
+  hipLaunchKernelGGL((logits_kernel<CHUNK, THREADS>), grid, dim3(THREADS), 0, stream, p);
+  return hipGetLastError();
+}
 
 hipError_t launch_logits_adjust(const LogitsAdjust& p, int n_cu, hipStream_t stream) {
-  // small chunks while they leave at most a few workgroups per CU
-  const bool small = (int64_t)logits_chunks(p.n_vocab) * p.n_rows <= kFewPerCu * n_cu;
-  const int chunk = small ? kSmallChunk : kChunk, chunks = (p.n_vocab + chunk - 1) / chunk;
-  if (small) hipLaunchKernelGGL(logits_kernel<kSmallChunk>, dim3(chunks, p.n_rows), dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL(logits_kernel<kChunk>, dim3(chunks, p.n_rows), dim3(kThreads), 0, stream, p);
-  return hipGetLastError();
+  if ((int64_t)logits_chunks(p.n_vocab) * p.n_rows <= kFewPerCu * n_cu) return launch_logits<1024, 256>(p, stream);
+  return p.hist ? launch_logits<4096, 512>(p, stream) : launch_logits<2048, 256>(p, stream);
 }
 
 }  // namespace mi
