@@ -354,12 +354,14 @@ class Lib:
 
     def kv_write(self, kv, layer, which, pos0, src, stream):
         """Rows of an F32 device tensor (n_tokens, n_head_kv, head_dim) into K (which 0) or V (1)."""
+        _expect(_kind(src) == MI_TYPE_F32, "src: float32")
         self.check(self.so.mi_hip_kv_write(kv, layer, which, pos0, src.shape[0], src.data_ptr(),
                                            _Strides(*nb3_of(src)), 1, stream))
 
     def kv_read(self, kv, layer, which, pos0, dst, stream):
         """Cache rows into a device tensor (n_tokens, n_head_kv, head_dim), F32 or F16."""
-        kind = MI_TYPE_F16 if dst.element_size() == 2 else MI_TYPE_F32
+        kind = _kind(dst)
+        _expect(kind is not None, "dst: float32 or float16")
         self.check(self.so.mi_hip_kv_read(kv, layer, which, pos0, dst.shape[0], dst.data_ptr(), kind,
                                           _Strides(*nb3_of(dst)), stream))
 
@@ -376,6 +378,22 @@ def lib():
     if _lib is None:
         _lib = Lib()
     return _lib
+
+
+_kinds = {}
+
+
+def _kind(t):
+    """The element type of a torch tensor: MI_TYPE_F32, MI_TYPE_F16 or None."""
+    if not _kinds:
+        import torch
+        _kinds.update({torch.float32: MI_TYPE_F32, torch.float16: MI_TYPE_F16})
+    return _kinds.get(t.dtype)
+
+
+def _expect(ok, what):
+    if not ok:
+        raise ValueError(what)
 
 
 def nb3_of(t):
@@ -438,6 +456,15 @@ def norm_rope_args(kv, layer, n_past, n_dims, freq_base, stream, k, v, q=None, q
                    q_norm=None, k_norm=None, eps=0.0):
     """Builds NormRopeArgs from torch tensors as rope_args does; pos (n_tokens, int32) and the
     norms' weights (head_dim) are device tensors, freq n_dims / 2 floats on the host."""
+    for t in (k, v, q, q_out, q_norm, k_norm):
+        _expect(t is None or _kind(t) == MI_TYPE_F32, "q, k, v and the norms' weights: float32")
+    _expect(v.shape == k.shape and (q is None or q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2]) and
+            (q is None or q_out is None or q_out.shape == q.shape), "q, k, v: shapes of the same tokens and head_dim")
+    _expect(all(w is None or (w.numel() == k.shape[2] and w.is_contiguous()) for w in (q_norm, k_norm)),
+            "q_norm, k_norm: head_dim weights")
+    _expect(pos is None or (pos.element_size() == 4 and pos.numel() >= k.shape[0] and pos.is_contiguous()),
+            "pos: an int32 position for each token")
+    _expect(freq is None or len(freq) == n_dims // 2, "freq: n_dims / 2 frequencies")
     a = NormRopeArgs()
     a.kv, a.layer, a.n_past, a.n_dims = kv, layer, n_past, n_dims
     a.freq_base, a.eps = freq_base, eps
@@ -463,6 +490,8 @@ def norm_rope_args(kv, layer, n_past, n_dims, freq_base, stream, k, v, q=None, q
 def tree_masks(bits):
     """An array of TreeMask from one device tensor of 64-bit words (n_tokens, words) per item, or
     None for an item whose tokens are a chain."""
+    _expect(all(b is None or (b.element_size() == 8 and b.dim() == 2 and b.stride(1) == 1) for b in bits),
+            "bits: rows of 64-bit words")
     return (TreeMask * len(bits))(*[TreeMask() if b is None else TreeMask(b.data_ptr(), b.stride(0) * 8)
                                     for b in bits])
 
@@ -471,8 +500,20 @@ def logits_args(logits, out, stream, penalties=None, hist=None, hist_off=None, b
                 bias_off=None, mask=None, ids=None, ws=None):
     """Builds LogitsArgs from device tensors: logits and out (n_rows, n_vocab), penalties
     (n_rows, 3), int32 lists and offsets, mask (n_rows, words) of 32 bits or one row for all."""
+    rows, vocab = logits.shape
+    _expect(out.shape == logits.shape and all(_kind(t) == MI_TYPE_F32 and (t.stride(1) == 1 or vocab == 1)
+                                              for t in (logits, out)), "logits, out: float32 rows (n_rows, n_vocab)")
+    for t in (penalties, hist, hist_off, bias_id, bias, bias_off, ids):
+        _expect(t is None or (t.element_size() == 4 and t.is_contiguous()), "lists: contiguous, 32 bits an element")
+    _expect(penalties is None or penalties.numel() == 3 * rows, "penalties: three for each row")
+    _expect(all(t is None or t.numel() == rows + 1 for t in (hist_off, bias_off)), "offsets: n_rows + 1")
+    _expect(ids is None or ids.numel() >= rows, "ids: one for each row")
+    _expect((bias is None) == (bias_id is None) and (bias is None or bias.numel() == bias_id.numel()),
+            "bias: a value for each id")
+    _expect(mask is None or (mask.element_size() == 4 and mask.shape[0] in (1, rows) and mask.stride(1) == 1 and
+                             mask.shape[1] >= (vocab + 31) // 32), "mask: rows of n_vocab bits in 32-bit words")
     a = LogitsArgs()
-    a.n_rows, a.n_vocab = logits.shape
+    a.n_rows, a.n_vocab = rows, vocab
     a.logits, a.nb = logits.data_ptr(), logits.stride(0) * 4
     a.out, a.out_nb = out.data_ptr(), out.stride(0) * 4
     for name, t in (("penalties", penalties), ("hist", hist), ("hist_off", hist_off), ("bias_id", bias_id),

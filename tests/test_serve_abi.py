@@ -71,3 +71,37 @@ def test_cache_handles(lib):
     assert lib.mi_hip_norm_rope_append(None) == 1
     a = mh.NormRopeArgs()
     assert lib.mi_hip_norm_rope_append(ctypes.byref(a)) == 1 and "NULL" in lib.last_error()
+
+
+def test_builders_refuse_what_does_not_fit(lib):
+    import torch
+    f = torch.zeros
+    q, k, v = f(3, 4, 64), f(3, 2, 64), f(3, 2, 64)
+    i32 = torch.int32
+    mh.norm_rope_args(None, 0, 0, 64, 1e4, None, k, v, q=q, pos=f(3, dtype=i32), q_norm=f(64), k_norm=f(64), freq=[1.0] * 32)
+    for kw in (dict(q=q.half()), dict(q=q[:2]), dict(q=q[..., :32]), dict(q=q, q_out=q[:, :2]), dict(q_norm=f(32)),
+               dict(k_norm=f(128)[::2]), dict(pos=f(2, dtype=i32)), dict(pos=f(3, dtype=torch.int64)), dict(freq=[1.0] * 31)):
+        with pytest.raises(ValueError):
+            mh.norm_rope_args(None, 0, 0, 64, 1e4, None, k, v, **kw)
+    with pytest.raises(ValueError):
+        mh.norm_rope_args(None, 0, 0, 64, 1e4, None, k, v.half())
+    mh.tree_masks([None, f(5, 1, dtype=torch.int64), f(5, 3, dtype=torch.int64)[:, :1]])
+    for bad in (f(5, 2, dtype=i32), f(5, dtype=torch.int64), f(2, 5, dtype=torch.int64).t()):
+        with pytest.raises(ValueError):
+            mh.tree_masks([bad])
+    x, words = f(4, 100), f(4, 4, dtype=i32)
+    off = f(5, dtype=i32)
+    mh.logits_args(x, x, None, penalties=f(4, 3), hist=f(7, dtype=i32), hist_off=off, bias_id=f(2, dtype=i32), bias=f(2),
+                   bias_off=off, mask=words, ids=f(4, dtype=i32))
+    for kw in (dict(out=f(4, 99)), dict(out=x.half()), dict(out=f(100, 4).t()), dict(penalties=f(3, 3)),
+               dict(hist_off=off[:4]), dict(hist=f(7, dtype=torch.int64)), dict(bias=f(2)),
+               dict(bias=f(2), bias_id=f(3, dtype=i32)), dict(mask=words[:3]), dict(mask=words[:, :3]),
+               dict(mask=words.to(torch.int64)), dict(ids=f(3, dtype=i32))):
+        with pytest.raises(ValueError):
+            mh.logits_args(x, kw.pop("out", x), None, **kw)
+    for call in (lambda t: lib.kv_write(None, 0, 0, 0, t, None), lambda t: lib.kv_read(None, 0, 0, 0, t, None)):
+        for bad in (k.double(), k.bfloat16(), k.to(torch.int16)):
+            with pytest.raises(ValueError):
+                call(bad)
+    with pytest.raises(ValueError):
+        lib.kv_write(None, 0, 0, 0, k.half(), None)
