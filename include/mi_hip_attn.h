@@ -103,7 +103,8 @@ typedef struct mi_hip_workspace_desc {
 } mi_hip_workspace_desc;
 
 /* One device allocation covering any decode launch of up to 32 items of this
- * head shape (mi_hip_attn_decode_batch's limit per launch). */
+ * head shape (mi_hip_attn_decode_batch's limit per launch) and, with 17 MB (head_dim
+ * 64) or 34 MB of parts, any call of mi_hip_attn_tree and mi_hip_logits_adjust. */
 int mi_hip_workspace_create(const mi_hip_workspace_desc* desc, mi_hip_workspace** out);
 int mi_hip_workspace_destroy(mi_hip_workspace* ws);
 
@@ -229,7 +230,8 @@ typedef struct mi_hip_kv_desc {
  * [head_dim, n_head_kv, n_ctx] (position-major, the layout of
  * src/model_qwen2.cpp:564-577), plus the host-node staging buffer (sized for
  * n_ctx) and the cache's own decode workspace (covering a decode launch of up
- * to 32 items of this head shape). Nothing is allocated afterwards.
+ * to 32 items of this head shape, and the parts of mi_hip_attn_tree: 17 MB at
+ * head_dim 64, 34 MB at 128). Nothing is allocated afterwards.
  * Replaces mi_kv_cache_init's host KV context (src/model_qwen2.cpp:564-577). */
 int mi_hip_kv_create(const mi_hip_kv_desc* desc, mi_hip_kv** out);
 int mi_hip_kv_destroy(mi_hip_kv* kv);
