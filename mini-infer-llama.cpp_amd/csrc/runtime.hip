@@ -832,19 +832,25 @@ void plan_tree(mi::TreeParams& p, int n_items, int head_dim, int elt, int rows, 
   // all in one, then 1, 2, .. 7, 8, 10, 12, 14, 16, 20, .. times the least
   for (int k = 0; k * least < longest; k += k < 8 ? 1 : 1 << (29 - __builtin_clz((unsigned)k))) {
     const int per = k == 0 ? longest : k * least;
-    int64_t records = 0, units = 0;
+    int64_t records = 0, units = 0, most_units = 0;
     int rt = 1;
     for (int i = 0; i < n_items; ++i) {
       const int n = (tiles[i] + per - 1) / per * p.n_head_kv;
       units += n;
+      most_units = std::max<int64_t>(most_units, n);
       if (n > p.n_head_kv) records += (int64_t)n * p.item[i].n_rt;
       rt = std::max(rt, p.item[i].n_rt);
     }
     if (records > cap) continue;
-    // workgroups per CU of the fullest XCD; where there are several, those of
-    // early tokens make up for those of late ones
+    // Workgroups per CU of the fullest XCD. The grid gives every item as many as the
+    // longest has; those without work are gone at once, but until then they put
+    // others together on a CU, while another has none: up to 1.4 times the units
+    // (eight times one token after up to 9000, F16, 28/4 heads of 128: 27 us with
+    // 256 workgroups in all, 33 with 320 of which 256 have work). Where a CU has
+    // several, those of early tokens make up for those of late ones.
     const int shift = row_shift(units, rt), parts = 1 << shift;
-    const int64_t load = (units * parts + kXcds - 1) / kXcds * ((rt + parts - 1) / parts);
+    const int64_t octets = (units * parts + kXcds - 1) / kXcds, grid = (most_units * parts + kXcds - 1) / kXcds * n_items;
+    const int64_t load = std::min(std::max(octets, grid), (int64_t)(1.4f * octets)) * ((rt + parts - 1) / parts);
     const int on_cu = (int)std::min<int64_t>(1 << 20, std::max<int64_t>(1, (load * kXcds + g.n_cu - 1) / g.n_cu));
     const int rounds = (on_cu + per_cu - 1) / per_cu;
     const float longer = (std::min(on_cu, per_cu) > 1 ? kSharedCu[kind] : 1.f) * (on_cu > 1 ? seen / whole : 1.f);
