@@ -46,8 +46,8 @@
 //   the largest such product in that range.
 //
 // Bound: each byte of the cache comes from memory once, 24 sequences of one token
-// over 4095 F16 keys (28/4 heads of 128) at 5.2 TB/s (38.8 us with the join); over
-// few keys the start, a tile's chain of loads, products and exponentials and the
+// over 2788 to 4096 F16 keys (28/4 heads of 128, 170 MB) at 5.1 TB/s, 33.0 us with
+// the join; over few keys the start, a tile's chain of loads, products and exponentials and the
 // join's launch (one token over 4000: 10.6 us). Rows beyond the group's are work
 // for nothing: with 32x32 MFMAs, whose tile is 32 rows, that call took 57 us, and
 // twice the registers let one workgroup less onto a CU.

@@ -27,8 +27,8 @@
 // Bound: issue slots. Per 32 keys and 32 rows of 128 over an 8-bit cache a wave has
 // 32 matrix instructions (1024 cycles) and 266 others (1064, and 16 exponentials
 // at a quarter of the rate); two waves share a SIMD, whose two pipes are busy 92%
-// of the waves' time added up. Four 64-token trees over 16384 8-bit keys (28/4
-// heads of 128): 146 us, 717 TFLOP/s of f16 products, of the 1106 that a large
+// of the waves' time added up. Four 64-token trees over 12304 to 16384 8-bit
+// keys (28/4 heads of 128): 146 us, 717 TFLOP/s of f16 products, of the 1106 that a large
 // product reaches. Fetching two tiles ahead, and the softmax of one tile beside the
 // products of the next, took as long: the registers they need spill or the LDS
 // latency shows. Few keys: the start (about 6 us) and the join.
