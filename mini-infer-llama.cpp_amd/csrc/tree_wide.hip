@@ -91,8 +91,13 @@ struct WideCfg {
   // exponents (f16 [TK]).
   static constexpr int L_SC = 4 * TILE;
   static constexpr int SC_K = 0, SC_V = Q8 ? NDB * TK * 2 : TK * 4, SC_E = SC_V + TK * 4, SC = SC_E + TK * 2;
-  static constexpr int L_NF = L_SC + (ELT == 2 ? 0 : 2 * SC);  // per buffer: the last tile with values that are not finite
-  static constexpr int LDS = L_NF + 16;
+  // Per buffer and wave: the last tile in which the wave fetched values that are not
+  // finite. Each wave sets up and writes its own words, in order; the others read
+  // them behind the barrier that ends the fetch.
+  static constexpr int L_NF = L_SC + (ELT == 2 ? 0 : 2 * SC);
+  static constexpr int NF = 4 * kTreeWaves;  // bytes of a buffer's
+  static constexpr int LDS = L_NF + 2 * NF;
+  static_assert(L_NF % 16 == 0, "a buffer's words are read at once");
   // F32 tiles at head_dim 128 take more registers than two workgroups per CU
   // leave each other.
   static constexpr int WAVES_PER_SIMD = D == 128 && F32 ? 1 : 2;
@@ -222,6 +227,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
     return max_lanes<NSLOT>(most);
   };
   constexpr int VSWZ = NSLOT >= 16 ? 3 : 1;  // rows of 128 bytes: two of them span the banks
+  lds_t* const nf = lds + C::L_NF + 4 * wave;  // the wave's word of buffer 0
   // In a tile that some rows do not see, V values (8-bit: scales) that are not
   // finite become zeros, since a masked key's probability of 0 times them would
   // not be 0, and the tile is marked for the rows that do see them.
@@ -261,7 +267,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
               vw[i][j] &= (b & 1u ? 0u : 0xffffu) | (b & 2u ? 0u : 0xffff0000u);
             }
           }
-          if (any) lds_store<int>(lds + C::L_NF + 4 * buf, key0);
+          if (any) lds_store<int>(nf + C::NF * buf, key0);
         }
       }
       widen(vw[i], e, x);
@@ -275,7 +281,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
         float v = (float)__builtin_bit_cast(_Float16, (unsigned short)scw);
         const bool finite = v < INFINITY;  // (scales are not negative)
         if (masked && !finite) {
-          lds_store<int>(lds + C::L_NF + 4 * buf, key0);
+          lds_store<int>(nf + C::NF * buf, key0);
           v = 0.f;
         }
         lds_store<float>(sc + C::SC_V + 4 * sc_key, v);
@@ -283,7 +289,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
       }
     }
   };
-  if (tid < 2) lds_store<int>(lds + C::L_NF + 4 * tid, -1);
+  if (lane < 2) lds_store<int>(nf + C::NF * lane, -1);
   if (key_begin < key_end) fetch(key_begin);
 
   // ---- queries: row c of the wave's 32, dims 16 s + 8 kh + j of step s -----------
@@ -492,7 +498,13 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
     }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     // rows that see a value which is not finite get NaN in its dim (8-bit: in all)
-    if (masked && lds_load<int>(lds + C::L_NF + 4 * buf) == key0) {
+    static_assert(kTreeWaves == 4, "a word for each wave");
+    bool marked = false;
+    if (masked) {
+      const i32x4 m = lds_load<i32x4>(lds + C::L_NF + C::NF * buf);
+      marked = m[0] == key0 || m[1] == key0 || m[2] == key0 || m[3] == key0;
+    }
+    if (marked) {
       const int n = min(n_kv - key0, TK);
       for (int t = 0; t < n; ++t) {
         unsigned word = vis[0];
