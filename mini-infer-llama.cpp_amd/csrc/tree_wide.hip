@@ -11,7 +11,7 @@
 //
 // F32 caches: a row of K or V becomes f16 pairs of its values times 2^-e, the
 // power of two that brings its largest into [2^14, 2^15), so a value is at most
-// 2^-22 of itself or 2^-39 of the row's largest off, and a product of pairs is
+// 2^-22 of itself or 2^-39 of the row's largest off (V: or 2^-115), and a product of pairs is
 // hi.lo + lo.hi + hi.hi (three v_mfma_f32_32x32x16_f16, 5 times the rate of
 // v_mfma_f32_32x32x2f32). K's exponent is added to its scores, V's belongs to
 // the probability like the scale of an 8-bit row.
@@ -53,12 +53,12 @@ __device__ inline u32x2 lds_transposed(const lds_t* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
 }
 
-// The exponents of F32 rows: 2^-e times the row's largest lies in [2^14, 2^15).
-// Not below -90: the probabilities of a row are relative to what includes e
+// The exponents of F32 rows: 2^-e times the row's largest lies in [2^14, 2^15)
+// (below it for a row without a normal number, whose values 2^-e times are exact).
+__device__ inline int row_exponent(float most) { return (int)(__builtin_bit_cast(unsigned, most) >> 23) - 127 - 14; }
+// V's, not below -90: the probabilities of a row are relative to what includes e
 // (move_ref), and their sum has to stay in float's range.
-__device__ inline int row_exponent(float most) {
-  return max((int)(__builtin_bit_cast(unsigned, most) >> 23) - 127 - 14, -90);
-}
+constexpr int kLeastVExponent = -90;
 
 // Maximum over aligned groups of N = 8 or 16 lanes.
 template <int N>
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
       for (int pl = 0; pl < PL; ++pl)
         lds_store<u32x4>(lds + C::L_K + buf * C::TILE + pl * PLANE + r * (2 * D) + 16 * (s ^ swz<NSLOT>(r)), x[pl]);
       if constexpr (F32) {
-        e = row_exponent(row_most(vw[i]));
+        e = max(row_exponent(row_most(vw[i])), kLeastVExponent);
         lds_store<float>(sc + C::SC_V + 4 * r, ldexpf(1.f, e));
         lds_store<_Float16>(sc + C::SC_E + 2 * r, (_Float16)e);
       }
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
       }
     if (key_begin < key_end) put(0, key_begin);  // (under the queries' loads)
     amax = max32(amax);
-    if (amax > 0.f && amax < INFINITY) qexp = max(ilogbf(amax) - 13, -100);
+    if (amax > 0.f && amax < INFINITY) qexp = F32 ? ilogbf(amax) - 13 : max(ilogbf(amax) - 13, -100);
 #pragma unroll
     for (int s = 0; s < D / 16; ++s)
 #pragma unroll

@@ -41,3 +41,18 @@ def test_marks_of_first_tiles_in_many_workgroups(hip, stream, cache, d):
             assert np.all(np.abs(got - want)[~bad] <= 2.0 ** -21 * np.abs(want[~bad]).max())
     for s in seqs:
         s.close()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rep,t", [(3, 10), (4, 24)])  # 30 rows per KV head, 96
+@pytest.mark.parametrize("qmul,kmul", [(1e36, 1e-36), (1e30, 1e-30), (1e-36, 1e36), (1e-30, 1e30)])
+def test_small_keys_and_small_queries(hip, stream, d, rep, t, qmul, kmul):
+    # an F32 cache: scores of ordinary size from keys or queries at the ends of float's range
+    rng = np.random.default_rng([d, rep, t, 21])
+    hkv, n_past = 2, 200
+    n = n_past + t
+    k = (rng.standard_normal((n + 1, hkv, d)) * kmul).astype(np.float32)
+    s = Seq(hip, rng, "f32", d, hkv, rep, n_past, t, None, spare=1, qmul=qmul, k=k)
+    run(hip, [s], stream)
+    s.check(f"{d} {rep} {t} {qmul} {kmul}")
+    s.close()
