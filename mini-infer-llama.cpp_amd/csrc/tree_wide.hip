@@ -11,7 +11,7 @@
 //
 // F32 caches: a row of K or V becomes f16 pairs of its values times 2^-e, the
 // power of two that brings its largest into [2^14, 2^15), so a value is at most
-// 2^-22 of itself or 2^-39 of the row's largest off (V: or 2^-115), and a product of pairs is
+// 2^-22 of itself or 2^-39 of the row's largest off (V: or 2^-124), and a product of pairs is
 // hi.lo + lo.hi + hi.hi (three v_mfma_f32_32x32x16_f16, 5 times the rate of
 // v_mfma_f32_32x32x2f32). K's exponent is added to its scores, V's belongs to
 // the probability like the scale of an 8-bit row.
@@ -56,9 +56,12 @@ __device__ inline u32x2 lds_transposed(const lds_t* p) {
 // The exponents of F32 rows: 2^-e times the row's largest lies in [2^14, 2^15)
 // (below it for a row without a normal number, whose values 2^-e times are exact).
 __device__ inline int row_exponent(float most) { return (int)(__builtin_bit_cast(unsigned, most) >> 23) - 127 - 14; }
-// V's, not below -90: the probabilities of a row are relative to what includes e
-// (move_ref), and their sum has to stay in float's range.
-constexpr int kLeastVExponent = -90;
+// V's: the probabilities of a row are relative to what includes e (move_ref), and
+// their sum has to stay in float's range, so there e counts as -90 at least. Rows
+// below that still take a smaller e, as the products p 2^e have 2^9 to spare before
+// their pairs are less exact than 2^-22; values below 2^-102 are then at most
+// 2^-124 off, as a probability times one is.
+constexpr int kLeastVExponent = -99, kLeastRefExponent = -90;
 
 // Maximum over aligned groups of N = 8 or 16 lanes.
 template <int N>
@@ -250,7 +253,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
       if constexpr (F32) {
         e = max(row_exponent(row_most(vw[i])), kLeastVExponent);
         lds_store<float>(sc + C::SC_V + 4 * r, ldexpf(1.f, e));
-        lds_store<_Float16>(sc + C::SC_E + 2 * r, (_Float16)e);
+        lds_store<_Float16>(sc + C::SC_E + 2 * r, (_Float16)max(e, kLeastRefExponent));
       }
       if constexpr (!Q8) {
         if (masked) {

@@ -56,3 +56,31 @@ def test_small_keys_and_small_queries(hip, stream, d, rep, t, qmul, kmul):
     run(hip, [s], stream)
     s.check(f"{d} {rep} {t} {qmul} {kmul}")
     s.close()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rep,t", [(3, 10), (4, 24)])  # 30 rows per KV head, 96
+@pytest.mark.parametrize("vmul", [1e-26, 1e-30, 1e-33, 1e-36])
+def test_small_values(hip, stream, d, rep, t, vmul):
+    # an F32 cache whose V rows are all small. A query that sees one key gives its V row: at most 2^-21 of the
+    # row's largest off (values and probabilities as pairs, 2^-22 each, and a few roundings of 2^-24 that cancel
+    # no digits: 2^-20 with them), or 2^-123 (the resolution 2^-124 of values below 2^-102, and the
+    # probability's as much)
+    rng = np.random.default_rng([d, rep, t, 22])
+    hkv, n_past = 2, 33
+    n = n_past + t
+    v = (rng.standard_normal((n + 1, hkv, d)) * vmul).astype(np.float32)
+    s = Seq(hip, rng, "f32", d, hkv, rep, n_past, t, None, spare=1, v=v)
+    run(hip, [s], stream)
+    got = s.out.cpu().numpy().astype(np.float64)
+    seen = ref.visible(n_past, t, None)
+    want = ref.attention(s.q, s.k, s.v, seen, s.scale)
+    assert np.abs(got - want).max() <= ref.attention_tolerance(s.q, s.k, s.v, seen, s.scale) + 2.0 ** -123
+    s.close()
+    bits = np.array([[1 << j] for j in range(t)], np.uint64)
+    one = Seq(hip, rng, "f32", d, hkv, rep, 0, t, bits, spare=1, v=v[n_past:].copy())
+    run(hip, [one], stream)
+    want = np.repeat(one.v.astype(np.float64), rep, 1)
+    tol = 2.0 ** -20 * np.abs(want).max(-1, keepdims=True) + 2.0 ** -123
+    assert np.all(np.abs(one.out.cpu().numpy() - want) <= tol)
+    one.close()
