@@ -366,10 +366,11 @@ hipError_t launch_kv_keep(const KvKeep& p, hipStream_t stream) {
 // and sine in double, rounded): pair (i, i + n_dims / 2) of the first n_dims.
 //
 // A wave per row, any strides and n_dims: the row passes through LDS so that a
-// lane finds its dims' partners.
+// lane finds its dims' partners. K on its way to an 8-bit cache stays in double
+// precision until it is quantised, as in the form for aligned rows below.
 template <int E>
 __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
-  __shared__ float rows[4][64 * E];
+  __shared__ double rows[4][64 * E];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int hkv = p.cache.n_head_kv, per_tok = p.n_head + 2 * hkv;
   const int64_t r = (int64_t)blockIdx.x * 4 + wave;
@@ -385,6 +386,10 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
 #pragma unroll
   for (int i = 0; i < E; ++i) x[i] = ldf(src, so + (lane + 64 * i) * nb[0]);
   if (kind < 2) {
+    const bool exact = kind == 1 && p.cache.elt == 1;
+    double y[E];  // the row where it is not rounded on the way
+#pragma unroll
+    for (int i = 0; i < E; ++i) y[i] = x[i];
     const float* const w = kind == 0 ? p.q_norm : p.k_norm;
     if (w) {
       double ss = 0.0;  // (in double in any case: this is not the fast form)
@@ -392,11 +397,15 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
       for (int i = 0; i < E; ++i) ss += (double)x[i] * x[i];
       const double inv = 1.0 / sqrt(group_sum<64>(ss) / (64 * E) + (double)p.eps);
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = (float)(x[i] * inv) * gload<float>(w + lane + 64 * i);
+      for (int i = 0; i < E; ++i) {
+        const float wi = gload<float>(w + lane + 64 * i);
+        y[i] = x[i] * inv * wi;
+        x[i] = (float)(x[i] * inv) * wi;
+      }
     }
-    float* const row = rows[wave];
+    double* const row = rows[wave];
 #pragma unroll
-    for (int i = 0; i < E; ++i) row[lane + 64 * i] = x[i];
+    for (int i = 0; i < E; ++i) row[lane + 64 * i] = exact ? y[i] : x[i];
     wave_lds_fence();
     const int half = p.n_dims / 2;
     const int pos = p.pos ? gload<int>(p.pos + t) : p.n_past + t;
@@ -404,12 +413,17 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
     for (int i = 0; i < E; ++i) {
 #pragma clang fp contract(off)
       const int d = lane + 64 * i;
+      if (exact) x[i] = (float)y[i];
       if (d >= p.n_dims) continue;
       const int j = d < half ? d : d - half;
       double s, c;
       sincos((double)((float)pos * p.freq[j]), &s, &c);
-      const float a = row[j], b = row[j + half];
-      x[i] = d < half ? a * (float)c - b * (float)s : a * (float)s + b * (float)c;
+      if (exact) {
+        x[i] = (float)(d < half ? row[j] * c - row[j + half] * s : row[j] * s + row[j + half] * c);
+      } else {
+        const float a = (float)row[j], b = (float)row[j + half];
+        x[i] = d < half ? a * (float)c - b * (float)s : a * (float)s + b * (float)c;
+      }
     }
   }
   if (kind == 0) {

@@ -8,7 +8,7 @@ import pytest
 
 import mi_hip_attn as mh
 import serve_ref as ref
-from test_kv8_gpu import dev, read
+from test_kv8_gpu import dev, tensor_at
 from test_tree_gpu import CACHES, Seq, run
 
 pytestmark = pytest.mark.gpu
@@ -84,3 +84,32 @@ def test_small_values(hip, stream, d, rep, t, vmul):
     tol = 2.0 ** -20 * np.abs(want).max(-1, keepdims=True) + 2.0 ** -123
     assert np.all(np.abs(one.out.cpu().numpy() - want) <= tol)
     one.close()
+
+
+@pytest.mark.parametrize("d,hkv,n_dims", [(64, 2, 64), (128, 3, 128), (64, 2, 20), (128, 1, 96)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_the_8_bit_keys_of_sources_of_any_alignment(hip, stream, d, hkv, n_dims, norm):
+    # K's 8-bit form is that of the float nearest to its 64-bit value, however the source's rows lie and
+    # whatever part of them is rotated. (The kernels' and the reference's 64-bit values differ by parts in 2^52,
+    # which moves a float, and then a whole number, once in far more values than these.)
+    import torch
+    rng = np.random.default_rng([d, n_dims, norm])
+    t = 2000
+    k = rng.standard_normal((t, hkv, d)).astype(np.float32) * 3
+    w = (1 + 0.3 * rng.standard_normal(d)).astype(np.float32)
+    f = (1e6 ** (-np.arange(0, n_dims, 2, dtype=np.float64) / n_dims)).astype(np.float32)
+    want = ref.norm_rope(k, w if norm else None, 1e-6, np.arange(t, dtype=np.int32), f).astype(np.float32)
+    want_q, want_scale = ref.quantize(want, 32)
+    apart = torch.full((t, hkv, d + 1), 9.0, device="cuda")  # rows that start at any 4 bytes
+    apart[:, :, :d] = dev(k)
+    dw = dev(w)
+    for dk in (dev(k), apart[:, :, :d]):
+        kv = hip.kv_create(1, t, hkv, d, hkv, mh.MI_HIP_TYPE_Q8)
+        a = mh.norm_rope_args(kv, 0, 0, n_dims, 1e6, stream, dk, dk, freq=f, k_norm=dw if norm else None, eps=1e-6)
+        hip.check(hip.mi_hip_norm_rope_append(ctypes.byref(a)))
+        torch.cuda.synchronize()
+        q = tensor_at(hip.kv_view(kv, 0, 0)[0], (t, hkv, d), "|i1").cpu().numpy()
+        scale = tensor_at(hip.kv_scales(kv, 0, 0)[0], (t, hkv, d // 32), "<f2").cpu().numpy()
+        assert np.array_equal(scale, want_scale)
+        assert np.array_equal(q, want_q.reshape(q.shape))
+        hip.check(hip.mi_hip_kv_destroy(kv))
