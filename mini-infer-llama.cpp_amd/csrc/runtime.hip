@@ -893,7 +893,7 @@ int run_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* masks, int n
     const int64_t row_bytes = (int64_t)r.head_dim * elt;
     if (r.k_s2 < row_bytes || r.v_s2 < row_bytes)
       return fail(MI_HIP_E_UNSUPPORTED, "item %d: position stride below one row", i);
-    if (32 * r.k_s2 > INT32_MAX || 32 * r.v_s2 > INT32_MAX)
+    if (r.k_s2 > INT32_MAX / 32 || r.v_s2 > INT32_MAX / 32)
       return fail(MI_HIP_E_UNSUPPORTED, "item %d: position stride above 2^26 bytes", i);
     if ((int64_t)a->n_past + a->n_tokens > INT32_MAX - 64 || (int64_t)a->n_tokens * a->n_head > (1 << 26))
       return fail(MI_HIP_E_UNSUPPORTED, "item %d: more than 2^26 query rows or 2^31 keys", i);

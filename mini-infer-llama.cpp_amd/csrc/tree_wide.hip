@@ -167,10 +167,12 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
   const char* const sc_src = Q8 ? (sc_k ? it.k_scale + 2 * (g * NDB + tid % NDB) : it.v_scale + 2 * g) : nullptr;
   auto fetch_rows = [&](const char* base, int s2, int key0, unsigned (&w)[PER][WORDS]) __attribute__((always_inline)) {
     const int n = min(n_kv - key0, TK);
-    const rsrc_t r = make_rsrc(base + (int64_t)key0 * s2, (unsigned)((n - 1) * s2 + D * ELT));
+    // (unsigned: 63 rows of up to 2^26 bytes pass 2^31)
+    const rsrc_t r = make_rsrc(base + (int64_t)key0 * s2, (unsigned)(n - 1) * (unsigned)s2 + D * ELT);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const unsigned at = (unsigned)(((tid + THREADS * i) / NSLOT) * s2 + 8 * ELT * ((tid + THREADS * i) % NSLOT));
+      const unsigned t = (unsigned)(tid + THREADS * i);
+      const unsigned at = t / NSLOT * (unsigned)s2 + 8 * ELT * (t % NSLOT);
       if constexpr (Q8) {
         const u32x2 a = buf_b64(r, at);
         w[i][0] = a[0];

@@ -113,3 +113,18 @@ def test_the_8_bit_keys_of_sources_of_any_alignment(hip, stream, d, hkv, n_dims,
         assert np.array_equal(scale, want_scale)
         assert np.array_equal(q, want_q.reshape(q.shape))
         hip.check(hip.mi_hip_kv_destroy(kv))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_tiles_whose_rows_pass_2_and_4_gib(hip, stream, d):
+    # positions 48 MiB apart: with 64 dims a tile of 64 keys is 3 GiB long
+    import torch
+    rng = np.random.default_rng([d, 23])
+    n_past, t, rep = 100, 12, 4
+    n = n_past + t
+    s = Seq(hip, rng, "f16", d, 1, rep, n_past, t, None, spare=0)
+    far = torch.empty((n, 24 << 20), device="cuda", dtype=torch.float16)
+    far[:, :d], far[:, d:2 * d] = s.dk[:, 0], s.dv[:, 0]
+    s.src = dict(k=far[:, None, :d], v=far[:, None, d:2 * d])
+    run(hip, [s], stream)
+    s.check("far rows")
