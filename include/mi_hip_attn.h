@@ -104,7 +104,11 @@ typedef struct mi_hip_workspace_desc {
 
 /* One device allocation covering any decode launch of up to 32 items of this
  * head shape (mi_hip_attn_decode_batch's limit per launch) and, with 17 MB (head_dim
- * 64) or 34 MB of parts, any call of mi_hip_attn_tree and mi_hip_logits_adjust. */
+ * 64) or 34 MB of parts, any call of mi_hip_attn_tree and mi_hip_logits_adjust. Where
+ * the allocation limit or the device has no room for the parts, a workspace (a cache's
+ * own and the default one too) is made without them: mi_hip_attn_tree then keeps each
+ * item's keys in one piece, which is slow over long caches, and
+ * mi_hip_logits_adjust refuses to give ids with it (MI_HIP_E_UNSUPPORTED). */
 int mi_hip_workspace_create(const mi_hip_workspace_desc* desc, mi_hip_workspace** out);
 int mi_hip_workspace_destroy(mi_hip_workspace* ws);
 

@@ -110,7 +110,10 @@ int dev_alloc(void** p, size_t bytes, const char* what) {
     return fail(MI_HIP_E_NOMEM, "%s: %zu bytes would exceed the allocation limit of %llu", what,
                 bytes, (unsigned long long)lim);
   hipError_t e = hipMalloc(p, bytes);
-  if (e != hipSuccess) return hip_fail(e, what);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();  // it is reported here, not by the next launch
+    return hip_fail(e, what);
+  }
   g.n_malloc++;
   const uint64_t now = g.live.fetch_add(bytes) + bytes;
   uint64_t pk = g.peak.load();
@@ -420,8 +423,14 @@ int ws_create(int groups, size_t rec_bytes, size_t part_bytes, mi_hip_workspace*
   mi_hip_workspace* ws = new (std::nothrow) mi_hip_workspace();
   if (!ws) return fail(MI_HIP_E_NOMEM, "host allocation failed");
   void* p = nullptr;
-  const size_t bytes = ws_total_bytes(groups, rec_bytes, part_bytes);
+  size_t bytes = ws_total_bytes(groups, rec_bytes, part_bytes);
   int rc = dev_alloc(&p, bytes, "decode workspace");
+  if (rc == MI_HIP_E_NOMEM && part_bytes) {
+    // the decode kernels need no parts: a workspace without them
+    part_bytes = 0;
+    bytes = ws_total_bytes(groups, rec_bytes, 0);
+    rc = dev_alloc(&p, bytes, "decode workspace");
+  }
   if (rc) {
     delete ws;
     return rc;
@@ -1924,7 +1933,9 @@ int mi_hip_logits_adjust(const mi_hip_logits_args* a) {
   // as many rows a launch as their chunks' maxima and counters have room for (and the grid)
   const int64_t row_part = (int64_t)mi::logits_chunks(a->n_vocab) * 8;
   const int64_t most = a->ids ? std::min<int64_t>(mi::kArrivals, (int64_t)ws->part_bytes / row_part) : 65535;
-  if (most < 1) return fail(MI_HIP_E_UNSUPPORTED, "n_vocab %d: the workspace does not hold one row's parts", a->n_vocab);
+  if (most < 1)
+    return fail(MI_HIP_E_UNSUPPORTED, "n_vocab %d: the workspace does not hold one row's parts (%zu bytes of parts)",
+                a->n_vocab, ws->part_bytes);
   mi::LogitsAdjust p{};
   p.in_nb = (int64_t)a->nb;
   p.out_nb = (int64_t)a->out_nb;

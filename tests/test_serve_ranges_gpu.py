@@ -128,3 +128,59 @@ def test_tiles_whose_rows_pass_2_and_4_gib(hip, stream, d):
     s.src = dict(k=far[:, None, :d], v=far[:, None, d:2 * d])
     run(hip, [s], stream)
     s.check("far rows")
+
+
+def test_caches_and_workspaces_where_a_limit_leaves_no_room_for_the_parts(hip, stream):
+    # made without them: attention then keeps every item's keys in one split, greedy ids are refused
+    import torch
+    rng = np.random.default_rng(24)
+    d, hkv, rep, n_past, t = 64, 2, 7, 700, 9
+    n = n_past + t
+    x = dev(rng.standard_normal((3, 5000)).astype(np.float32))
+    out, ids = torch.empty_like(x), torch.empty(3, device="cuda", dtype=torch.int32)
+    before = hip.alloc_stats().bytes_live
+    kv = hip.kv_create(1, n, hkv, d, hkv * rep, mh.MI_TYPE_F16)
+    whole = hip.alloc_stats().bytes_live - before
+    hip.check(hip.mi_hip_kv_destroy(kv))
+    ws = hip.workspace_create(hkv, hkv * rep, d)
+    ws_whole = hip.alloc_stats().bytes_live - before
+    hip.check(hip.mi_hip_workspace_destroy(ws))
+    try:
+        hip.check(hip.mi_hip_set_alloc_limit(before + whole - (1 << 20)))
+        kv = hip.kv_create(1, n, hkv, d, hkv * rep, mh.MI_TYPE_F16)
+        assert whole - (34 << 20) < hip.alloc_stats().bytes_live - before <= whole - (16 << 20)
+        hip.check(hip.mi_hip_set_alloc_limit(hip.alloc_stats().bytes_live + ws_whole - (1 << 20)))
+        ws = hip.workspace_create(hkv, hkv * rep, d)
+        # and a limit below what they need without parts still refuses
+        hip.check(hip.mi_hip_set_alloc_limit(hip.alloc_stats().bytes_live + 1000))
+        with pytest.raises(mh.MiHipError) as e:
+            hip.workspace_create(hkv, hkv * rep, d)
+        assert e.value.code == 4
+    finally:
+        hip.check(hip.mi_hip_set_alloc_limit(0))
+    bits, _ = ref.random_tree(rng, t)
+    s = Seq(hip, rng, "f16", d, hkv, rep, n_past, t, bits, spare=0)
+    for which, rows in ((0, s.dk), (1, s.dv)):
+        hip.kv_write(kv, 0, which, 0, rows.float(), stream)
+    s.src = dict(kv=kv, layer=0)
+    run(hip, [s], stream)
+    s.check("no parts")
+    s.out.fill_(float("nan"))
+    run(hip, [s], stream, ws)
+    s.check("no parts, own workspace")
+    # one token by the decode entry point, which needs none
+    one = Seq(hip, rng, "f16", d, hkv, rep, n - 1, 1, None, spare=0, k=s.k.astype(np.float32), v=s.v.astype(np.float32))
+    a = one.args(stream, ws)
+    hip.check(hip.mi_hip_attn_fwd(ctypes.byref(a)))
+    torch.cuda.synchronize()
+    want = ref.attention(one.q, one.k, one.v, ref.visible(n - 1, 1), one.scale)
+    assert np.abs(one.out.cpu().numpy() - want).max() <= 1e-2  # (an F16 cache's bar; conftest's TOL_F16)
+    a = mh.logits_args(x, out, stream, ids=ids, ws=ws)
+    assert hip.mi_hip_logits_adjust(ctypes.byref(a)) == 5
+    a = mh.logits_args(x, out, stream, ws=ws)
+    hip.check(hip.mi_hip_logits_adjust(ctypes.byref(a)))
+    torch.cuda.synchronize()
+    assert torch.equal(x, out)
+    hip.check(hip.mi_hip_workspace_destroy(ws))
+    hip.check(hip.mi_hip_kv_destroy(kv))
+    assert hip.alloc_stats().bytes_live == before
