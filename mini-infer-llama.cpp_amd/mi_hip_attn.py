@@ -50,6 +50,15 @@ class MiHipError(RuntimeError):
         self.code = code
 
 
+class KvHandle(int):
+    """A cache handle that knows the shape of the cache's rows."""
+
+    def __new__(cls, handle, n_head_kv, head_dim):
+        self = super().__new__(cls, handle)
+        self.rows = (n_head_kv, head_dim)
+        return self
+
+
 class MiTensor(ctypes.Structure):
     """ABI mirror of struct mi_tensor (src/tensor.h:122-160)."""
 
@@ -319,7 +328,7 @@ class Lib:
         d = KvDesc(n_layer, n_ctx, n_head_kv, head_dim, n_head, kv_type)
         h = ctypes.c_void_p()
         self.check(self.so.mi_hip_kv_create(ctypes.byref(d), ctypes.byref(h)))
-        return h.value
+        return KvHandle(h.value, n_head_kv, head_dim)
 
     def workspace_create(self, n_head_kv, n_head, head_dim):
         d = WorkspaceDesc(n_head_kv, n_head, head_dim)
@@ -355,15 +364,15 @@ class Lib:
     def kv_write(self, kv, layer, which, pos0, src, stream):
         """Rows of an F32 device tensor (n_tokens, n_head_kv, head_dim) into K (which 0) or V (1)."""
         _expect(_kind(src) == MI_TYPE_F32, "src: float32")
-        self.check(self.so.mi_hip_kv_write(kv, layer, which, pos0, src.shape[0], src.data_ptr(),
-                                           _Strides(*nb3_of(src)), 1, stream))
+        n, nb = _cache_rows(kv, src, 4)
+        self.check(self.so.mi_hip_kv_write(kv, layer, which, pos0, n, src.data_ptr(), nb, 1, stream))
 
     def kv_read(self, kv, layer, which, pos0, dst, stream):
         """Cache rows into a device tensor (n_tokens, n_head_kv, head_dim), F32 or F16."""
         kind = _kind(dst)
         _expect(kind is not None, "dst: float32 or float16")
-        self.check(self.so.mi_hip_kv_read(kv, layer, which, pos0, dst.shape[0], dst.data_ptr(), kind,
-                                          _Strides(*nb3_of(dst)), stream))
+        n, nb = _cache_rows(kv, dst, 4 if kind == MI_TYPE_F32 else 2)
+        self.check(self.so.mi_hip_kv_read(kv, layer, which, pos0, n, dst.data_ptr(), kind, nb, stream))
 
     def kv_keep(self, kv, n_past, idx, stream):
         """Rows n_past + idx[i] become rows n_past + i (idx: whole numbers on the host, increasing)."""
@@ -391,9 +400,34 @@ def _kind(t):
     return _kinds.get(t.dtype)
 
 
+def _is_int32(t):
+    return t.element_size() == 4 and not t.is_floating_point()
+
+
 def _expect(ok, what):
     if not ok:
         raise ValueError(what)
+
+
+def _rows_of(kv, shape):
+    # (a handle that is a plain number, or None, does not say its rows' shape)
+    rows = getattr(kv, "rows", None)
+    return len(shape) == 3 and (rows is None or (shape[1], shape[2]) == rows)
+
+
+def _cache_rows(kv, t, elt):
+    """Tokens and byte strides of a device tensor of rows of the cache."""
+    shape = t.shape
+    if not _rows_of(kv, shape):
+        raise ValueError("rows: shape (n_tokens, n_head_kv, head_dim) of the cache")
+    if not t.is_cuda:
+        raise ValueError("rows: device memory")
+    s2, s1, s0 = t.stride()
+    return shape[0], _Strides(s0 * elt, s1 * elt, s2 * elt)
+
+
+def _expect_one_device(*tensors):
+    _expect(len({t.device for t in tensors if t is not None}) <= 1, "tensors of one device")
 
 
 def nb3_of(t):
@@ -462,8 +496,10 @@ def norm_rope_args(kv, layer, n_past, n_dims, freq_base, stream, k, v, q=None, q
             (q is None or q_out is None or q_out.shape == q.shape), "q, k, v: shapes of the same tokens and head_dim")
     _expect(all(w is None or (w.numel() == k.shape[2] and w.is_contiguous()) for w in (q_norm, k_norm)),
             "q_norm, k_norm: head_dim weights")
-    _expect(pos is None or (pos.element_size() == 4 and pos.numel() >= k.shape[0] and pos.is_contiguous()),
+    _expect(_rows_of(kv, k.shape), "k, v: shape (n_tokens, n_head_kv, head_dim) of the cache")
+    _expect(pos is None or (_is_int32(pos) and pos.numel() >= k.shape[0] and pos.is_contiguous()),
             "pos: an int32 position for each token")
+    _expect_one_device(k, v, q, q_out, pos, q_norm, k_norm)
     _expect(freq is None or len(freq) == n_dims // 2, "freq: n_dims / 2 frequencies")
     a = NormRopeArgs()
     a.kv, a.layer, a.n_past, a.n_dims = kv, layer, n_past, n_dims
@@ -490,8 +526,9 @@ def norm_rope_args(kv, layer, n_past, n_dims, freq_base, stream, k, v, q=None, q
 def tree_masks(bits):
     """An array of TreeMask from one device tensor of 64-bit words (n_tokens, words) per item, or
     None for an item whose tokens are a chain."""
-    _expect(all(b is None or (b.element_size() == 8 and b.dim() == 2 and b.stride(1) == 1) for b in bits),
-            "bits: rows of 64-bit words")
+    _expect(all(b is None or (b.element_size() == 8 and not b.is_floating_point() and b.dim() == 2 and b.stride(1) == 1)
+                for b in bits), "bits: rows of 64-bit words")
+    _expect_one_device(*bits)
     return (TreeMask * len(bits))(*[TreeMask() if b is None else TreeMask(b.data_ptr(), b.stride(0) * 8)
                                     for b in bits])
 
@@ -503,15 +540,18 @@ def logits_args(logits, out, stream, penalties=None, hist=None, hist_off=None, b
     rows, vocab = logits.shape
     _expect(out.shape == logits.shape and all(_kind(t) == MI_TYPE_F32 and (t.stride(1) == 1 or vocab == 1)
                                               for t in (logits, out)), "logits, out: float32 rows (n_rows, n_vocab)")
-    for t in (penalties, hist, hist_off, bias_id, bias, bias_off, ids):
-        _expect(t is None or (t.element_size() == 4 and t.is_contiguous()), "lists: contiguous, 32 bits an element")
+    for t in (hist, hist_off, bias_id, bias_off, ids):
+        _expect(t is None or (_is_int32(t) and t.is_contiguous()), "hist, bias_id, offsets, ids: contiguous int32")
+    for t in (penalties, bias):
+        _expect(t is None or (_kind(t) == MI_TYPE_F32 and t.is_contiguous()), "penalties, bias: contiguous float32")
     _expect(penalties is None or penalties.numel() == 3 * rows, "penalties: three for each row")
     _expect(all(t is None or t.numel() == rows + 1 for t in (hist_off, bias_off)), "offsets: n_rows + 1")
     _expect(ids is None or ids.numel() >= rows, "ids: one for each row")
     _expect((bias is None) == (bias_id is None) and (bias is None or bias.numel() == bias_id.numel()),
             "bias: a value for each id")
-    _expect(mask is None or (mask.element_size() == 4 and mask.shape[0] in (1, rows) and mask.stride(1) == 1 and
+    _expect(mask is None or (_is_int32(mask) and mask.shape[0] in (1, rows) and mask.stride(1) == 1 and
                              mask.shape[1] >= (vocab + 31) // 32), "mask: rows of n_vocab bits in 32-bit words")
+    _expect_one_device(logits, out, penalties, hist, hist_off, bias_id, bias, bias_off, mask, ids)
     a = LogitsArgs()
     a.n_rows, a.n_vocab = rows, vocab
     a.logits, a.nb = logits.data_ptr(), logits.stride(0) * 4
