@@ -368,9 +368,10 @@ hipError_t launch_kv_keep(const KvKeep& p, hipStream_t stream) {
 // A wave per row, any strides and n_dims: the row passes through LDS so that a
 // lane finds its dims' partners. K on its way to an 8-bit cache stays in double
 // precision until it is quantised, as in the form for aligned rows below.
-template <int E>
+template <int E, bool Q8>
 __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
-  __shared__ double rows[4][64 * E];
+  __shared__ float rows[4][64 * E];
+  __shared__ double rows_d[Q8 ? 4 : 1][64 * E];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int hkv = p.cache.n_head_kv, per_tok = p.n_head + 2 * hkv;
   const int64_t r = (int64_t)blockIdx.x * 4 + wave;
@@ -386,11 +387,13 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
 #pragma unroll
   for (int i = 0; i < E; ++i) x[i] = ldf(src, so + (lane + 64 * i) * nb[0]);
   if (kind < 2) {
-    const bool exact = kind == 1 && p.cache.elt == 1;
-    double y[E];  // the row where it is not rounded on the way
-#pragma unroll
-    for (int i = 0; i < E; ++i) y[i] = x[i];
+    const bool exact = Q8 && kind == 1;
     const float* const w = kind == 0 ? p.q_norm : p.k_norm;
+    double y[E];  // the row where it is not rounded on the way
+    if (exact) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) y[i] = x[i];
+    }
     if (w) {
       double ss = 0.0;  // (in double in any case: this is not the fast form)
 #pragma unroll
@@ -399,13 +402,15 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const float wi = gload<float>(w + lane + 64 * i);
-        y[i] = x[i] * inv * wi;
-        x[i] = (float)(x[i] * inv) * wi;
+        if (exact) y[i] = y[i] * inv * wi;
+        else x[i] = (float)(x[i] * inv) * wi;
       }
     }
-    double* const row = rows[wave];
 #pragma unroll
-    for (int i = 0; i < E; ++i) row[lane + 64 * i] = exact ? y[i] : x[i];
+    for (int i = 0; i < E; ++i) {
+      if (exact) rows_d[Q8 ? wave : 0][lane + 64 * i] = y[i];
+      else rows[wave][lane + 64 * i] = x[i];
+    }
     wave_lds_fence();
     const int half = p.n_dims / 2;
     const int pos = p.pos ? gload<int>(p.pos + t) : p.n_past + t;
@@ -419,9 +424,10 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
       double s, c;
       sincos((double)((float)pos * p.freq[j]), &s, &c);
       if (exact) {
-        x[i] = (float)(d < half ? row[j] * c - row[j + half] * s : row[j] * s + row[j + half] * c);
+        const double a = rows_d[Q8 ? wave : 0][j], b = rows_d[Q8 ? wave : 0][j + half];
+        x[i] = (float)(d < half ? a * c - b * s : a * s + b * c);
       } else {
-        const float a = (float)row[j], b = (float)row[j + half];
+        const float a = rows[wave][j], b = rows[wave][j + half];
         x[i] = d < half ? a * (float)c - b * (float)s : a * (float)s + b * (float)c;
       }
     }
@@ -594,8 +600,14 @@ hipError_t launch_norm_rope(const NormRope& p, hipStream_t stream) {
   const int64_t rows = (int64_t)p.n_tokens * (p.n_head + 2 * p.cache.n_head_kv);
   if (rows == 0) return hipSuccess;
   const dim3 grid((unsigned)((rows + 3) / 4));
-  if (p.cache.head_dim == 64) hipLaunchKernelGGL(norm_rope_row_kernel<1>, grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL(norm_rope_row_kernel<2>, grid, dim3(256), 0, stream, p);
+  const bool q8 = p.cache.elt == 1;
+  if (p.cache.head_dim == 64) {
+    if (q8) hipLaunchKernelGGL((norm_rope_row_kernel<1, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((norm_rope_row_kernel<1, false>), grid, dim3(256), 0, stream, p);
+  } else {
+    if (q8) hipLaunchKernelGGL((norm_rope_row_kernel<2, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((norm_rope_row_kernel<2, false>), grid, dim3(256), 0, stream, p);
+  }
   return hipGetLastError();
 }
 
