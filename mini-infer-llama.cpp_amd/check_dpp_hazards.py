@@ -11,6 +11,12 @@ write of one of the instruction's VGPR operands in that window. Following the
 compiler's own conservative rule, every VGPR operand of the DPP instruction
 counts, not only the broadcast source.
 
+The same walk checks every vector instruction of inline asm (also multiply-adds
+that read f16, and swaps between lanes of a wave): what it reads must not come from
+a matrix instruction fewer than 19 wait states before (the longest any needs), nor
+from a transcendental one fewer than one; and the swaps' operands from no vector
+instruction fewer than two.
+
 Usage: python check_dpp_hazards.py file.s [...]   (exit status 1 on a finding)
 """
 import re
@@ -19,6 +25,8 @@ import sys
 _VREG = re.compile(r"\bv(\d+)\b|\bv\[(\d+):(\d+)\]")
 _DPP_MARK = ("row_newbcast", "quad_perm", "row_mirror", "row_half_mirror", "row_shl", "row_shr",
              "row_ror", "row_bcast", "wave_shl", "wave_shr", "wave_rol", "wave_ror")
+_TRANS = ("v_exp_", "v_log_", "v_rcp_", "v_rsq_", "v_sqrt_", "v_sin_", "v_cos_")
+_SWAPS = ("v_permlane16_swap", "v_permlane32_swap")
 _NO_VGPR_DEF = ("v_readlane", "v_readfirstlane", "v_cmp", "v_cmpx", "v_accvgpr_write")
 
 
@@ -38,10 +46,11 @@ def split_operands(rest):
 
 
 class Inst:
-    __slots__ = ("op", "text", "defs", "uses", "dpp", "wait", "target", "uncond", "line")
+    __slots__ = ("op", "text", "defs", "uses", "dpp", "wait", "target", "uncond", "line", "asm")
 
-    def __init__(self, op, rest, line):
+    def __init__(self, op, rest, line, asm=False):
         self.op = op
+        self.asm = asm and op.startswith("v_") and not op.startswith("v_mfma")
         self.text = rest
         self.line = line
         ops = split_operands(rest) if rest else []
@@ -67,7 +76,11 @@ class Inst:
 def parse_functions(path):
     funcs = {}
     cur = None
+    asm = False
     for ln, raw in enumerate(open(path), 1):
+        if "#ASMSTART" in raw or "#ASMEND" in raw:
+            asm = "#ASMSTART" in raw
+            continue
         line = raw.split(";", 1)[0].rstrip()
         if not line.strip():
             continue
@@ -85,11 +98,25 @@ def parse_functions(path):
         if s.startswith("."):
             continue
         parts = s.split(None, 1)
-        cur.append(Inst(parts[0], parts[1] if len(parts) > 1 else "", ln))
+        cur.append(Inst(parts[0], parts[1] if len(parts) > 1 else "", ln, asm))
     return funcs
 
 
-def check_function(name, items):
+def any_vector(inst):
+    return True
+
+
+def matrix(inst):
+    return inst.op.startswith("v_mfma")
+
+
+def transcendental(inst):
+    return inst.op.startswith(_TRANS)
+
+
+def walker(items):
+    """walk(i, regs, budget, seen, writes): the instruction of the kind `writes` that defines one of regs
+    within `budget` wait states before item i, or None."""
     # predecessors of each label: fall-through position and branch sites
     label_pos = {}
     for i, it in enumerate(items):
@@ -100,9 +127,7 @@ def check_function(name, items):
         if isinstance(it, Inst) and it.target is not None:
             branch_sites.setdefault(it.target, []).append(i)
 
-    findings = []
-
-    def walk(i, regs, budget, seen):
+    def walk(i, regs, budget, seen, writes=any_vector):
         # examine items before index i (exclusive) with `budget` wait states left
         j = i - 1
         while j >= 0:
@@ -112,7 +137,7 @@ def check_function(name, items):
                     key = (b, budget)
                     if key not in seen:
                         seen.add(key)
-                        r = walk_from_inst(b, regs, budget, seen)
+                        r = walk_from_inst(b, regs, budget, seen, writes)
                         if r:
                             return r
                 prev = j - 1
@@ -122,18 +147,25 @@ def check_function(name, items):
                     return None
                 j -= 1
                 continue
-            return walk_from_inst(j, regs, budget, seen)
+            return walk_from_inst(j, regs, budget, seen, writes)
         return None
 
-    def walk_from_inst(j, regs, budget, seen):
+    def walk_from_inst(j, regs, budget, seen, writes):
         it = items[j]
         if it.defs & regs:
-            return it
+            # (a write of another kind hides those before it)
+            return it if writes(it) else None
         budget -= it.wait
         if budget <= 0:
             return None
-        return walk(j, regs, budget, seen)
+        return walk(j, regs, budget, seen, writes)
 
+    return walk
+
+
+def check_function(name, items):
+    walk = walker(items)
+    findings = []
     for i, it in enumerate(items):
         if isinstance(it, Inst) and it.dpp and it.uses:
             hit = walk(i, it.uses, 2, set())
@@ -142,17 +174,33 @@ def check_function(name, items):
     return findings
 
 
+def check_asm_function(name, items):
+    walk = walker(items)
+    findings = []
+    for i, it in enumerate(items):
+        if not (isinstance(it, Inst) and it.asm):
+            continue
+        swap = it.op.startswith(_SWAPS)
+        reads = vregs(it.text if swap or "fmac" in it.op else it.text.partition(",")[2])
+        for writes, budget in ((matrix, 19), (transcendental, 1)) + (((any_vector, 2),) if swap else ()):
+            # one register at a time: a write of one does not hide the others'
+            hits = [walk(i, {r}, budget, set(), writes) for r in sorted(reads)]
+            findings += [(name, it, hit) for hit in hits if hit is not None]
+    return findings
+
+
 def main(paths):
     bad = []
-    n_dpp = 0
+    n_dpp = n_asm = 0
     for p in paths:
         for name, items in parse_functions(p).items():
             n_dpp += sum(1 for it in items if isinstance(it, Inst) and it.dpp)
-            bad += check_function(name, items)
+            n_asm += sum(1 for it in items if isinstance(it, Inst) and it.asm)
+            bad += check_function(name, items) + check_asm_function(name, items)
     for name, it, hit in bad:
         print(f"{name}: line {it.line}: {it.op} {it.text}\n    reads a VGPR written by line "
-              f"{hit.line}: {hit.op} {hit.text} (fewer than 2 wait states)")
-    print(f"checked {n_dpp} DPP instructions: {len(bad)} hazard(s)")
+              f"{hit.line}: {hit.op} {hit.text} (too few wait states)")
+    print(f"checked {n_dpp} DPP instructions and {n_asm} vector instructions of inline asm: {len(bad)} hazard(s)")
     return 1 if bad else 0
 
 
