@@ -94,13 +94,13 @@ size_t tree_record_floats(int head_dim, int tile_rows);
 // in tiles of tile_rows.
 hipError_t launch_tree(const TreeParams& p, int n_items, int head_dim, int elt, int tile_rows, hipStream_t stream);
 
-// tree_wide.hip: the kernel for tiles of 128 rows (F16 and 8-bit caches).
+// tree_wide.hip: the kernel for tiles of 128 rows (all cache types).
 hipError_t launch_tree_wide(const TreeParams& p, dim3 grid, int head_dim, int elt, hipStream_t stream);
 
 // kv8.hip -- rows on their way into and out of a cache.
 // A layer's K and V of a cache: element type by elt (4 F32, 2 F16, 1 8-bit
 // with its scales), byte strides of heads and positions; the scales' strides
-// follow from n_head_kv (see CacheRows in kv8.hip).
+// follow from n_head_kv (row_of and scale_of in kv8.hip).
 struct CacheView {
   char* t[2];      // K, V
   char* scale[2];  // 8-bit: f16 [head_dim / 32, n_head_kv, n_ctx], [n_head_kv, n_ctx]

@@ -18,7 +18,9 @@
 // arithmetic is far below what the memory takes. 16384 positions of 4 heads of
 // 128, us a kernel: K quantised 10.4 (42 MB, 4.1 TB/s), V 9.3, read back as F16
 // 6.0 (26 MB, 4.2 TB/s); norms, RoPE and append of 4096 tokens, 28/4 heads of 128,
-// F16 cache 24.2 (143 MB, 5.9 TB/s); a few rows 2 to 4, a launch's own time.
+// F16 cache 23.4, 8-bit 23.8 (143 MB, of which the launch before has left a part in
+// the memory-side cache; among other passes 32.1, 4.4 TB/s); a few rows 2 to 4, a
+// launch's own time.
 #include <cmath>
 #include <type_traits>
 
@@ -365,7 +367,10 @@ hipError_t launch_kv_keep(const KvKeep& p, hipStream_t stream) {
 // the rotation of rope.hip (angle = position * freq, one float product; cosine
 // and sine in double, rounded): pair (i, i + n_dims / 2) of the first n_dims.
 //
-// A wave per row, any strides and n_dims: the row passes through LDS so that a
+// A wave per row, any strides and n_dims, each lane with angles of its own in double
+// precision (4096 tokens of 28/4 heads of 128 with 96 dims rotated: 72.4 us, 8-bit
+// cache 80.9, where the form below, whose angles are once per token, takes 23 to 25
+// for all dims): the row passes through LDS so that a
 // lane finds its dims' partners. K on its way to an 8-bit cache stays in double
 // precision until it is quantised, as in the form for aligned rows below.
 template <int E, bool Q8>

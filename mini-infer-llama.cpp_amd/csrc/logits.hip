@@ -82,7 +82,7 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const LogitsAdjust p) {
   char* const out = p.out + row * p.out_nb + 4 * (int64_t)base;
   const char* const mask = p.mask ? p.mask + row * p.mask_nb + base / 8 : nullptr;
 
-      // The lists' first loads, then the logits': loads come back in order, and the
+  // The lists' first loads, then the logits': loads come back in order, and the
   // lists are worked on while the logits are on their way.
   unsigned at[kInFlight], bat = ~0u;
   float bval = 0.f;

@@ -14,9 +14,10 @@
 // cut into row tiles (row r is token r / n_rep, head r % n_rep of the group),
 // the keys into splits of whole 32-key tiles. A workgroup owns (item, KV head,
 // row tile, split). With one split its result is the output, otherwise it is a
-// record in the workspace that tree_combine_kernel joins: a second launch, since
-// a group's last workgroup takes longer for its records from other XCDs than a
-// launch does (one token over 4000 keys of 64: 20.5 us instead of 11.3).
+// record in the workspace that tree_combine_kernel joins: a second launch, 4 to 6
+// us of a split call. (Joined by a group's last workgroup instead, whose records
+// come from other XCDs, one token over 4000 keys of 64 took 20.5 us, not 11.3. A join
+// by all workgroups of the launch, as in decode.hip, has not been tried here.)
 //
 // This kernel: one tile of 16 or 32 rows, for calls that need no more. Its waves
 // take the split's key tiles in turn, K and V straight to registers, and meet in
@@ -45,12 +46,16 @@
 //   32 dims. 8-bit V: the row's one scale multiplies the probability; ref keeps
 //   the largest such product in that range.
 //
-// Bound: each byte of the cache comes from memory once, 24 sequences of one token
-// over 2788 to 4096 F16 keys (28/4 heads of 128, 170 MB) at 5.1 TB/s, 33.0 us with
-// the join; over few keys the start, a tile's chain of loads, products and exponentials and the
-// join's launch (one token over 4000: 10.6 us). Rows beyond the group's are work
-// for nothing: with 32x32 MFMAs, whose tile is 32 rows, that call took 57 us, and
-// twice the registers let one workgroup less onto a CU.
+// Bound: F16, memory, each byte of the cache once: 24 sequences of one token over
+// 2788 to 4096 keys (28/4 heads of 128, 170 MB) at 5.1 TB/s, 32.5 us with the join.
+// 8-bit caches are half the bytes and no faster: the same call 36.3 us, since four
+// values take about five instructions to widen, for 7 rows of 16 that are there; with
+// 14/2 heads of 64 14.4 us, F16 14.1: a row of 64 bytes is half a line, the other KV
+// head's half is fetched by another XCD (40 MB for the cache's 22). Over few keys the
+// start, a tile's chain of loads, products and exponentials and the join's launch (one
+// token over 4000: 10.6 us). Rows beyond the group's are work for nothing: with 32x32
+// MFMAs, whose tile is 32 rows, the F16 call of 128 dims took 57 us, and twice the
+// registers let one workgroup less onto a CU.
 #include <algorithm>
 
 #include "attn_common.h"

@@ -11,9 +11,10 @@
 //
 // F32 caches: a row of K or V becomes f16 pairs of its values times 2^-e, the
 // power of two that brings its largest into [2^14, 2^15), so a value is at most
-// 2^-22 of itself or 2^-39 of the row's largest off (V: or 2^-124), and a product of pairs is
-// hi.lo + lo.hi + hi.hi (three v_mfma_f32_32x32x16_f16, 5 times the rate of
-// v_mfma_f32_32x32x2f32). K's exponent is added to its scores, V's belongs to
+// 2^-22 of itself or 2^-39 of the row's largest off (V: or 2^-124), and a product
+// of pairs is hi.lo + lo.hi + hi.hi (three v_mfma_f32_32x32x16_f16, 5 times the
+// rate of v_mfma_f32_32x32x2f32): 22 bits an operand where up to 32 rows, which
+// those do not bound, take all 24. K's exponent is added to its scores, V's belongs to
 // the probability like the scale of an 8-bit row.
 //
 // LDS rows are a key's D f16 values in 16-byte slots, permuted by row so that
@@ -24,10 +25,11 @@
 // a lane's V operand are those of its S^T registers, so P needs no exchange.
 // Operands are read one group of products ahead of their use.
 //
-// Bound: issue slots. Per 32 keys and 32 rows of 128 over an 8-bit cache a wave has
-// 32 matrix instructions (1024 cycles) and 266 others (1064, and 16 exponentials
-// at a quarter of the rate); two waves share a SIMD, whose two pipes are busy 92%
-// of the waves' time added up. Four 64-token trees over 12304 to 16384 8-bit
+// Bound: the matrix and the vector pipe, one after the other. Per 32 keys and 32
+// rows of 128 over an 8-bit cache a wave has 32 matrix instructions (1024 cycles) and
+// 266 others (1064, and 16 exponentials at a quarter of the rate); two waves share a
+// SIMD, whose matrix pipe is busy 43% of the time and whose vector pipe 52%: the two
+// waves hardly ever use them at once. Four 64-token trees over 12304 to 16384 8-bit
 // keys (28/4 heads of 128): 146 us, 717 TFLOP/s of f16 products, of the 1106 that a large
 // product reaches. Fetching two tiles ahead, and the softmax of one tile beside the
 // products of the next, took as long: the registers they need spill or the LDS
@@ -392,8 +394,10 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
         acc = mfma_f16(kf[i & 1][e][0], qh[st], acc);
       }
       if constexpr (Q8) {
+        // The scale products wait for the group's own matrix products. (Two parts in
+        // turn, of which one is in use: with one the compiler assigns registers
+        // otherwise, 1024 tokens after 1337, 14/2 heads of 64: 34.6 us instead of 33.9.)
         part[i & 1] = acc;
-        // the scale products of a group run under the next one's matrix products
         auto scale = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
