@@ -384,7 +384,13 @@ typedef struct mi_hip_tree_mask {
  * gives zeros, and so does one whose every score is below float's range. What
  * lies in rows that a query does not see never shows in its output, infinities
  * and NaN included; an infinite value in a row that it sees may give NaN for
- * infinity, and so may a score above float's range.
+ * infinity, and so may a score above float's range. Products: an F16 or 8-bit
+ * cache's values are taken as they are, queries and probabilities as two f16
+ * numbers each (22 bits); an F32 cache's and its queries are float products up to
+ * 32 query rows per KV head (n_tokens * n_rep of the largest of up to 32 items
+ * launched together), and two f16 numbers on both sides above that (a value at most
+ * 2^-22 of itself, 2^-39 of its row's largest, or 2^-124 in V, off). All sums are
+ * in float.
  * Scratch for joining the parts of long caches: ws of the first item, else its
  * cache's workspace, else the library default; calls that share one must be
  * ordered. Nothing is kept in it between calls, so unlike the other decode entry
