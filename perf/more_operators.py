@@ -191,7 +191,7 @@ def _tables_inputs(case, seed):
     ids = rng.permutation(n_pages)
     table = np.full((n, width), -1, np.int64)
     table[np.arange(width)[None, :] < held[:, None]] = ids[:held.sum()]
-    head = int(rng.randint(0, 1 << 20))
+    head = int(rng.randint(0, n_pages))
     ring = np.full(n_pages, -1, np.int64)
     ring[(head + np.arange(free)) % n_pages] = ids[held.sum():held.sum() + free]
     total = int(new.sum())
@@ -471,7 +471,9 @@ def _plain_tables(s):
     entry = table[sq, (pos // page).clamp_max(width - 1)].long()
     slots = torch.where(real & ~refused[sq], entry * page + pos % page, -1)
     i32 = torch.int32
-    return {"held": (held + take - give).to(i32), "ring_at": torch.stack((head + take.sum(), tail + give.sum())).to(i32),
+    head, tail = head + take.sum(), tail + give.sum()
+    laps = head // n_pages * n_pages
+    return {"held": (held + take - give).to(i32), "ring_at": torch.stack((head - laps, tail - laps)).to(i32),
             "n_kv": torch.where(refused, 0, cached + new).to(i32),
             "q_off": torch.cat((q_end.new_zeros(1), q_end)).to(i32), "slots": slots.to(i32), "pos": pos.to(i32),
             "seq": torch.where(real, seq, -1).to(i32), "refused": refused.sum()[None].to(i32), "table": table,
