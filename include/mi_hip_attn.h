@@ -240,6 +240,19 @@ typedef struct mi_hip_kv_desc {
 int mi_hip_kv_create(const mi_hip_kv_desc* desc, mi_hip_kv** out);
 int mi_hip_kv_destroy(mi_hip_kv* kv);
 
+/* A cache whose n_ctx rows are pages of `page_size` rows (a power of two of at
+ * least 16 that divides n_ctx), dealt out to sequences by block tables: row r of a
+ * layer is row r % page_size of page r / page_size, and a sequence's position t
+ * lies in row table[t / page_size] * page_size + t % page_size. mi_hip_paged_append
+ * fills it and mi_hip_attn_paged reads it; mi_hip_kv_write (device sources),
+ * mi_hip_kv_read, mi_hip_kv_view and mi_hip_kv_scales take a row where they say
+ * position. What reads a cache as one sequence refuses it (MI_HIP_E_UNSUPPORTED):
+ * the other attention entry points, mi_hip_rope_append, mi_hip_norm_rope_append,
+ * mi_hip_kv_keep and mi_hip_kv_bind. No staging for host nodes; its workspace is
+ * for the paged calls (parts of 34 MB at head_dim 64, 68 MB at 128). No counterpart
+ * in the reference. */
+int mi_hip_kv_create_paged(const mi_hip_kv_desc* desc, int32_t page_size, mi_hip_kv** out);
+
 /* The cache's own decode workspace (owned by the cache; do not destroy). */
 int mi_hip_kv_workspace(mi_hip_kv* kv, mi_hip_workspace** out);
 
@@ -400,6 +413,179 @@ typedef struct mi_hip_tree_mask {
  * No counterpart in the reference. */
 int mi_hip_attn_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* masks, int n_items,
                      void* stream);
+
+/* ---- many requests over a paged cache -------------------------------------- */
+
+/* A step's block tables, row and position of each token, from the requests'
+ * lengths, without a word from the host. All pointers are device memory, 4-byte
+ * aligned. Sequence i has n_cached[i] positions in the cache that stay, adds
+ * n_new[i] tokens, and holds the first held[i] entries of its row of table; it
+ * needs ceil((n_cached + n_new) / page_size) pages (0 for one that has ended).
+ * Free pages lie in ring, a queue of n_pages entries: ring_at = {head, tail}, 0 <=
+ * head < n_pages, those of head .. tail - 1 modulo n_pages are free. Pages that are
+ * missing come from the head, in the order of the sequences, pages held beyond the
+ * need go to the tail. A sequence is refused, and keeps its pages, if it takes
+ * pages and what it and those before it take is more than are free, if its need is
+ * more than max_pages, or if its tokens do not end within max_tokens. Written:
+ *   held_out, ring_at_out (may be held and ring_at), ring, and table, whose entries
+ *     behind a sequence's pages stay as they are;
+ *   n_kv[i]: n_cached + n_new, 0 if refused;
+ *   q_off[0 .. n_seq]: where each sequence's tokens begin, q_off[n_seq] their number;
+ *   slots[t], pos[t], seq[t]: token t's cache row (-1 if its sequence is refused or
+ *     its page is none), position and sequence; -1, 0 and -1 from q_off[n_seq] to
+ *     max_tokens (a batch that is padded). pos and seq may be NULL;
+ *   n_refused: how many sequences are refused, or NULL.
+ * Negative lengths count as 0. No other memory of the call may overlap what it
+ * writes. Calls on one pool must be ordered. May be captured into a graph. No
+ * counterpart in the reference. */
+typedef struct mi_hip_page_tables_args {
+  int32_t n_seq;
+  int32_t page_size;  /* a power of two of at least 16 */
+  int32_t n_pages;
+  int32_t max_pages;  /* entries of a row of table */
+  int32_t max_tokens; /* entries of slots, pos and seq */
+  const int32_t* n_cached;
+  const int32_t* n_new;
+  const int32_t* held;
+  int32_t* held_out;
+  int32_t* table;
+  size_t table_nb;    /* bytes between rows */
+  int32_t* ring;
+  const int32_t* ring_at;
+  int32_t* ring_at_out;
+  int32_t* n_kv;
+  int32_t* q_off;
+  int32_t* slots;
+  int32_t* pos;
+  int32_t* seq;
+  int32_t* n_refused;
+  void* stream;
+} mi_hip_page_tables_args;
+
+int mi_hip_page_tables(const mi_hip_page_tables_args* args);
+
+/* mi_hip_norm_rope_append into rows of a paged cache, with positions of one or
+ * several axes (time, height, width): pair j of a token's dims is turned by the
+ * float product pos[axis[j]][token] * frequency j. K and V go to the cache row
+ * slots[token]; those of a token whose slot is outside [0, n_ctx) are not stored
+ * (its Q is written). No two tokens may have the same slot. May be captured into a
+ * graph. No counterpart in the reference. */
+typedef struct mi_hip_paged_append_args {
+  mi_hip_kv* kv;        /* of mi_hip_kv_create_paged */
+  int32_t layer;
+  int32_t n_tokens;
+  const int32_t* slots; /* device, n_tokens cache rows */
+  int32_t n_dims;       /* rotated dims (even, <= head_dim) */
+  float freq_base;      /* frequencies freq_base^(-2p / n_dims), unless freq is given */
+  const float* freq;    /* host, n_dims / 2 frequencies, or NULL */
+  const int32_t* pos;   /* device, n_tokens positions of each axis */
+  size_t pos_nb;        /* bytes between axes */
+  int32_t n_axes;       /* 1 to 4 */
+  const int32_t* axis;  /* host, n_dims / 2 axes, or NULL: all of axis 0 */
+  float eps;
+  const float* q_norm;  /* device, head_dim weights, or NULL: no norm */
+  const float* k_norm;
+  int32_t n_head;       /* Q heads */
+  const float* q;       /* may be NULL (no Q) */
+  size_t q_nb[3];
+  float* q_out;         /* may be q, with the same strides */
+  size_t q_out_nb[3];
+  const float* k;
+  size_t k_nb[3];
+  const float* v;
+  size_t v_nb[3];
+  void* stream;
+} mi_hip_paged_append_args;
+
+int mi_hip_paged_append(const mi_hip_paged_append_args* args);
+
+/* Attention of each sequence's new tokens over its pages. Sequence i's queries are
+ * the rows q_off[i] .. q_off[i + 1] - 1 of q, its last positions: query j of them
+ * stands at n_kv[i] - (their number) + j and sees the positions up to its own. The
+ * lengths are read on the device, so a step needs no word from the host, and a
+ * captured call takes those of each replay. A query that sees no key gives zeros;
+ * rows of out outside every sequence stay as they are. What lies behind a query's
+ * position never shows in its output, infinities and NaN included. A position whose
+ * table entry is not in [0, n_ctx / page_size) has a row of NaN. Lengths count as
+ * clamped: q_off to [0, n_tokens], n_kv to [0, max_pages * page_size]; of a sequence
+ * with more than max_new queries the rest are left as they were. Products, sums and
+ * values that are not finite as in mi_hip_attn_tree, with the choice of kernel per
+ * sequence (n_rep times its queries up to 32, or more). The same bits on every
+ * run with the same lengths. Scratch for joining the parts of long sequences: ws,
+ * else the cache's own; calls that share one must be ordered. May be captured into
+ * a graph. No counterpart in the reference. */
+typedef struct mi_hip_attn_paged_args {
+  mi_hip_kv* kv;          /* of mi_hip_kv_create_paged */
+  int32_t layer;
+  int32_t n_seq;
+  int32_t n_tokens;       /* rows of q and out */
+  int32_t max_new;        /* most queries of a sequence (0: n_tokens) */
+  const int32_t* q_off;   /* device, n_seq + 1 */
+  const int32_t* n_kv;    /* device, n_seq: positions, the queries' own included */
+  const int32_t* table;   /* device, n_seq rows of max_pages page numbers */
+  size_t table_nb;        /* bytes between rows */
+  int32_t max_pages;
+  int32_t n_head;
+  const float* q;         /* device [head_dim, n_head, n_tokens] */
+  size_t q_nb[3];
+  float* out;
+  size_t out_nb[3];
+  float scale;
+  mi_hip_workspace* ws;
+  void* stream;
+} mi_hip_attn_paged_args;
+
+int mi_hip_attn_paged(const mi_hip_attn_paged_args* args);
+
+/* Verification of drafted tokens against the target's probabilities, so that the
+ * tokens that come out are distributed as if the target had drawn each. A sequence's
+ * nodes are the rows off[i] .. off[i + 1] - 1 (at most 1024; those behind are not
+ * looked at): node 0 is its last certain token, node c a drafted token[c] after node
+ * parent[c] < c (NULL: c - 1), and row c of logits is the target's after node c,
+ * p_c = softmax(logits / temperature), in 64 bits; temperature 0 has p_c one at the
+ * lowest of the largest logits. From node 0 on, the children of the node v that was
+ * accepted last are looked at in order; child c is accepted
+ *   draft NULL (tokens taken as certain): if u_c Z < p_v(token_c), Z = 1 less the
+ *     p_v of the children of v that were turned down (a token turned down before: never);
+ *   draft given (token_c was drawn from the probabilities in row c of draft; chains
+ *     only, parent NULL): if u_c draft_c(token_c) < p_v(token_c).
+ * When no child is left, the next token is drawn by u of node 0: the lowest t for
+ * which the sum of w up to t is above u times the sum of w, w = p_v without the
+ * tokens turned down, or max(p_v - draft_c, 0) for the turned down c. Written, for
+ * sequence i with row strides path_nb and tokens_nb:
+ *   n_path[i]: the accepted nodes, node 0 among them (1 .. max_path; where there are
+ *     max_path, the children of the last are not looked at), 0 for one without nodes;
+ *   path: their numbers in the sequence, as mi_hip_kv_keep takes them, then -1;
+ *   tokens: the accepted drafted tokens and the token drawn, n_path in all, then -1.
+ * The token drawn is -1 if its row has a NaN or a +infinity, or nothing but -infinity
+ * (then no child is accepted either); child tokens outside [0, n_vocab) are turned
+ * down. u is clamped to [0, 1). Scratch: ws, else the library default; calls that
+ * share one must be ordered. May be captured into a graph. No counterpart in the
+ * reference. */
+typedef struct mi_hip_verify_args {
+  const float* logits;      /* device, n_rows rows of n_vocab */
+  size_t nb;                /* bytes between rows */
+  int32_t n_vocab;
+  int32_t n_rows;
+  int32_t n_seq;
+  const int32_t* off;       /* device, n_seq + 1 */
+  const int32_t* token;     /* device, n_rows */
+  const int32_t* parent;    /* device, n_rows, or NULL */
+  const float* draft;       /* device, n_rows rows of n_vocab (those of node 0 are not read), or NULL */
+  size_t draft_nb;
+  const float* temperature; /* device, n_seq, or NULL: 1 */
+  const float* u;           /* device, n_rows numbers in [0, 1) */
+  int32_t max_path;         /* entries of a row of path and of tokens */
+  int32_t* n_path;          /* device, n_seq */
+  int32_t* path;
+  size_t path_nb;
+  int32_t* tokens;
+  size_t tokens_nb;
+  mi_hip_workspace* ws;
+  void* stream;
+} mi_hip_verify_args;
+
+int mi_hip_verify_draft(const mi_hip_verify_args* args);
 
 /* ---- node-level operators on device tensors ----------------------------- */
 /*

@@ -144,6 +144,79 @@ struct NormRope {
 };
 hipError_t launch_norm_rope(const NormRope& p, hipStream_t stream);
 
+// NormRope into rows of a paged cache, by positions of up to four axes.
+constexpr int kRopeAxes = 4;
+struct PagedRope : NormRope {
+  const int32_t* slots;  // device, a row for each token; outside [0, n_slots): not stored
+  int64_t pos_nb;        // bytes between axes
+  int32_t n_slots;
+  uint32_t axis[kRopeMaxPairs / 16];  // pair j's axis: bits 2 (j % 16) .. of word j / 16
+};
+hipError_t launch_paged_rope(const PagedRope& p, hipStream_t stream);
+
+// paged.hip. A step's block tables and slots (mi_hip_page_tables).
+struct PageTables {
+  const int32_t* n_cached;
+  const int32_t* n_new;
+  const int32_t* held;
+  int32_t* held_out;
+  char* table;
+  int64_t table_nb;
+  int32_t* ring;
+  const int32_t* ring_at;
+  int32_t* ring_at_out;
+  int32_t* n_kv;
+  int32_t* q_off;
+  int32_t* slots;
+  int32_t* pos;        // or null
+  int32_t* seq;        // or null
+  int32_t* n_refused;  // or null
+  int32_t n_seq, page_shift, n_pages, max_pages, max_tokens;
+};
+hipError_t launch_page_tables(const PageTables& p, hipStream_t stream);
+
+// paged_attn.hip. Attention over pages (mi_hip_attn_paged).
+struct PagedAttn {
+  CacheView cache;
+  const int32_t* q_off;
+  const int32_t* n_kv;
+  const char* table;
+  int64_t table_nb;
+  const char* q;
+  char* out;
+  int64_t q_s1, q_s2, o_s1, o_s2;
+  int32_t n_seq, n_tokens, max_new, max_kv, page_shift, n_pages, n_rep;
+  float scale_log2e;
+};
+hipError_t launch_paged_attn(const PagedAttn& p, hipStream_t stream);
+
+// verify.hip. Drafted tokens against the target's probabilities (mi_hip_verify_draft).
+constexpr int kVerifyMaxNodes = 1024;
+struct VerifyRow {
+  double sum;    // of the weights
+  float top;     // the largest logit; NaN: the row has a NaN or an infinity
+  int32_t best;  // its lowest token
+};
+struct Verify {
+  const char* logits;
+  int64_t nb;
+  const int32_t* off;
+  const int32_t* token;
+  const int32_t* parent;  // null: chains
+  const char* draft;      // null: tokens taken as certain
+  int64_t draft_nb;
+  const float* temperature;  // null: 1
+  const float* u;
+  int32_t* n_path;
+  char* path;
+  int64_t path_nb;
+  char* tokens;
+  int64_t tokens_nb;
+  VerifyRow* rows;  // scratch
+  int32_t n_vocab, n_rows, n_seq, max_path;
+};
+hipError_t launch_verify(const Verify& p, hipStream_t stream);
+
 // Arrival counters of a workspace, kArrivalWords apart: counters in one line are
 // counted one after the other in memory (64 rows of logits: 53 us, 27 apart).
 constexpr int kArrivals = 1024, kArrivalWords = 64;

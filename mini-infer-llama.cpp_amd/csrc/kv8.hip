@@ -367,14 +367,29 @@ hipError_t launch_kv_keep(const KvKeep& p, hipStream_t stream) {
 // the rotation of rope.hip (angle = position * freq, one float product; cosine
 // and sine in double, rounded): pair (i, i + n_dims / 2) of the first n_dims.
 //
+// P: NormRope (rows n_past + token of a cache, one position per token) or
+// PagedRope (rows by slots, positions by axes; a token without a row has its Q
+// written only).
+__device__ inline int position_of(const NormRope& p, int t, int) { return p.pos ? gload<int>(p.pos + t) : p.n_past + t; }
+__device__ inline int position_of(const PagedRope& p, int t, int pair) {
+  const unsigned axis = p.axis[pair / 16] >> (2 * (pair % 16)) & 3u;
+  return gload<int>(reinterpret_cast<const char*>(p.pos) + axis * p.pos_nb + 4 * (int64_t)t);
+}
+// The cache row of token t, -1 if it has none.
+__device__ inline int64_t cache_row(const NormRope& p, int t) { return (int64_t)p.n_past + t; }
+__device__ inline int64_t cache_row(const PagedRope& p, int t) {
+  const int slot = gload<int>(p.slots + t);
+  return (unsigned)slot < (unsigned)p.n_slots ? slot : -1;
+}
+
 // A wave per row, any strides and n_dims, each lane with angles of its own in double
 // precision (4096 tokens of 28/4 heads of 128 with 96 dims rotated: 72.4 us, 8-bit
 // cache 80.9, where the form below, whose angles are once per token, takes 23 to 25
 // for all dims): the row passes through LDS so that a
 // lane finds its dims' partners. K on its way to an 8-bit cache stays in double
 // precision until it is quantised, as in the form for aligned rows below.
-template <int E, bool Q8>
-__global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
+template <int E, bool Q8, typename P>
+__global__ __launch_bounds__(256) void norm_rope_row_kernel(const P p) {
   __shared__ float rows[4][64 * E];
   __shared__ double rows_d[Q8 ? 4 : 1][64 * E];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
@@ -418,7 +433,6 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
     }
     wave_lds_fence();
     const int half = p.n_dims / 2;
-    const int pos = p.pos ? gload<int>(p.pos + t) : p.n_past + t;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
 #pragma clang fp contract(off)
@@ -426,6 +440,7 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
       if (exact) x[i] = (float)y[i];
       if (d >= p.n_dims) continue;
       const int j = d < half ? d : d - half;
+      const int pos = position_of(p, t, j);
       double s, c;
       sincos((double)((float)pos * p.freq[j]), &s, &c);
       if (exact) {
@@ -442,7 +457,8 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
 #pragma unroll
     for (int i = 0; i < E; ++i) gstore<float>(o + (lane + 64 * i) * p.qo_nb[0], x[i]);
   } else {
-    store_row<E>(p.cache, kind - 1, (int64_t)p.n_past + t, h, lane, x);
+    const int64_t to = cache_row(p, t);
+    if (to >= 0) store_row<E>(p.cache, kind - 1, to, h, lane, x);
   }
 }
 
@@ -456,8 +472,8 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const NormRope p) {
 // it by a rounding.
 constexpr int kRopeTokens = 4;
 
-template <int D>
-__global__ __launch_bounds__(256) void norm_rope_kernel(const NormRope p, int tokens) {
+template <int D, typename P>
+__global__ __launch_bounds__(256) void norm_rope_kernel(const P p, int tokens) {
   constexpr int LANES = D / 8, HALF = D / 2;
   __shared__ float2 cs[kRopeTokens][HALF];
   __shared__ double cs_d[kRopeTokens][HALF][2];  // 8-bit caches
@@ -466,7 +482,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRope p, int to
   const bool q8 = p.cache.elt == 1;
   for (int i = threadIdx.x; i < nt * HALF; i += 256) {
     const int t = i / HALF, j = i % HALF;
-    const int pos = p.pos ? gload<int>(p.pos + t0 + t) : p.n_past + t0 + t;
+    const int pos = position_of(p, t0 + t, j);
     double sn, c;
     sincos((double)((float)pos * p.freq[j]), &sn, &c);
     cs[t][j] = float2{(float)c, (float)sn};
@@ -544,7 +560,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRope p, int to
       gstore(o + 4 * HALF, b);
       continue;
     }
-    const int64_t pos = (int64_t)p.n_past + t0 + t;
+    const int64_t pos = cache_row(p, t0 + t);
+    if (pos < 0) continue;
     char* const o = row_of(p.cache, kind - 1, pos, h);
     if (q8) {
       unsigned ma = 0, mb = 0;
@@ -585,7 +602,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRope p, int to
   }
 }
 
-hipError_t launch_norm_rope(const NormRope& p, hipStream_t stream) {
+template <typename P>
+static hipError_t launch_rope_rows(const P& p, hipStream_t stream) {
   const auto at16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
   if (p.n_dims == p.cache.head_dim && (!p.q || (rows_aligned(p.q, p.q_nb, 4) && rows_aligned(p.q_out, p.qo_nb, 4))) &&
       rows_aligned(p.k, p.k_nb, 4) && rows_aligned(p.v, p.v_nb, 4) && at16(p.q_norm) && at16(p.k_norm)) {
@@ -598,8 +616,8 @@ hipError_t launch_norm_rope(const NormRope& p, hipStream_t stream) {
     const bool few = p.n_tokens < 2 * 256 * kRopeTokens;
     const dim3 grid((unsigned)(few ? p.n_tokens : (p.n_tokens + kRopeTokens - 1) / kRopeTokens),
                     (unsigned)(few ? (per_tok + rows - 1) / rows : 1));
-    if (p.cache.head_dim == 64) hipLaunchKernelGGL(norm_rope_kernel<64>, grid, dim3(256), 0, stream, p, few ? 1 : kRopeTokens);
-    else hipLaunchKernelGGL(norm_rope_kernel<128>, grid, dim3(256), 0, stream, p, few ? 1 : kRopeTokens);
+    if (p.cache.head_dim == 64) hipLaunchKernelGGL((norm_rope_kernel<64, P>), grid, dim3(256), 0, stream, p, few ? 1 : kRopeTokens);
+    else hipLaunchKernelGGL((norm_rope_kernel<128, P>), grid, dim3(256), 0, stream, p, few ? 1 : kRopeTokens);
     return hipGetLastError();
   }
   const int64_t rows = (int64_t)p.n_tokens * (p.n_head + 2 * p.cache.n_head_kv);
@@ -607,13 +625,16 @@ hipError_t launch_norm_rope(const NormRope& p, hipStream_t stream) {
   const dim3 grid((unsigned)((rows + 3) / 4));
   const bool q8 = p.cache.elt == 1;
   if (p.cache.head_dim == 64) {
-    if (q8) hipLaunchKernelGGL((norm_rope_row_kernel<1, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((norm_rope_row_kernel<1, false>), grid, dim3(256), 0, stream, p);
+    if (q8) hipLaunchKernelGGL((norm_rope_row_kernel<1, true, P>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((norm_rope_row_kernel<1, false, P>), grid, dim3(256), 0, stream, p);
   } else {
-    if (q8) hipLaunchKernelGGL((norm_rope_row_kernel<2, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((norm_rope_row_kernel<2, false>), grid, dim3(256), 0, stream, p);
+    if (q8) hipLaunchKernelGGL((norm_rope_row_kernel<2, true, P>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((norm_rope_row_kernel<2, false, P>), grid, dim3(256), 0, stream, p);
   }
   return hipGetLastError();
 }
+
+hipError_t launch_norm_rope(const NormRope& p, hipStream_t stream) { return launch_rope_rows(p, stream); }
+hipError_t launch_paged_rope(const PagedRope& p, hipStream_t stream) { return launch_rope_rows(p, stream); }
 
 }  // namespace mi

@@ -508,6 +508,7 @@ struct mi_hip_kv {
   // scales (one per 32 dims) and V scales (one per row) scale_bytes apart.
   size_t scale_at[2] = {0, 0};  // of layer 0, from base
   size_t scale_bytes = 0;       // of one layer
+  int32_t page_size = 0;        // rows of a page; 0: one sequence's positions (no staging if paged)
 
   char* tensor(int layer, int which) const {
     return base + (size_t)(2 * layer + which) * tensor_bytes;
@@ -546,9 +547,26 @@ struct Resolved {
   int n_ctx;  // -1 when unknown (explicit tensors)
 };
 
+// Rows of a page: whole halves of a key tile, so that one page number serves 16 rows.
+constexpr int32_t kLeastPage = 16;
+
+// Refuses a paged cache where its rows would be taken as one sequence's.
+int check_unpaged(const mi_hip_kv* kv) {
+  if (kv->page_size > 0)
+    return fail(MI_HIP_E_UNSUPPORTED, "the cache is paged: its rows are not one sequence's positions");
+  return MI_HIP_OK;
+}
+
+int check_page_size(int32_t n) {
+  if (n < kLeastPage || (n & (n - 1)))
+    return fail(MI_HIP_E_UNSUPPORTED, "page_size %d: a power of two of at least %d", n, kLeastPage);
+  return MI_HIP_OK;
+}
+
 int resolve_kv(const mi_hip_attn_args* a, Resolved* r) {
   if (a->kv) {
     const mi_hip_kv* kv = a->kv;
+    if (int rc = check_unpaged(kv)) return rc;
     if (a->layer < 0 || a->layer >= kv->d.n_layer)
       return fail(MI_HIP_E_INVALID, "layer %d out of range [0, %d)", a->layer, kv->d.n_layer);
     r->k = kv->tensor(a->layer, 0);
@@ -1118,6 +1136,76 @@ int rt_bind() { return bind_device(); }
 int rt_n_cu() { return g.n_cu; }
 }  // namespace mi
 
+namespace {
+
+// freq[p] = base^(-2p / n_dims) for p < n_dims / 2, each a float powf exactly
+// as src/ops_cpu.cpp:289 evaluates it (the device then forms pos * freq[p]
+// with one rounded product, as the engine does).
+void rope_freqs(float* freq, int n_dims, float base) {
+  for (int p = 0; p < n_dims / 2; ++p) freq[p] = std::pow(base, -(float)(2 * p) / (float)n_dims);
+}
+
+int check_rope_dims(int n_dims, int head_dim) {
+  if (n_dims < 0 || n_dims % 2 || n_dims > head_dim || n_dims > 2 * mi::kRopeMaxPairs)
+    return fail(MI_HIP_E_UNSUPPORTED, "n_dims %d: must be even, in [0, head_dim = %d] and <= %d",
+                n_dims, head_dim, 2 * mi::kRopeMaxPairs);
+  return MI_HIP_OK;
+}
+
+bool strides4(const size_t nb[3]) { return nb[0] % 4 == 0 && nb[1] % 4 == 0 && nb[2] % 4 == 0; }
+
+// What the args of mi_hip_norm_rope_append and of mi_hip_paged_append have alike.
+template <typename Args>
+int check_norm_rope(const Args* a, const mi_hip_kv* kv) {
+  int rc;
+  if ((rc = check_rope_dims(a->n_dims, kv->d.head_dim))) return rc;
+  if ((a->q_norm || a->k_norm) && !(a->eps >= 0.f && std::isfinite(a->eps)))
+    return fail(MI_HIP_E_INVALID, "eps must be finite and >= 0");
+  if (a->q) {
+    if (!a->q_out) return fail(MI_HIP_E_INVALID, "q_out is NULL");
+    if (a->n_head <= 0 || a->n_head % kv->d.n_head_kv)
+      return fail(MI_HIP_E_INVALID, "n_head %d must be a positive multiple of n_head_kv %d", a->n_head,
+                  kv->d.n_head_kv);
+    if (!strides4(a->q_nb) || !strides4(a->q_out_nb))
+      return fail(MI_HIP_E_INVALID, "Q strides must be multiples of 4 bytes");
+    if (a->q == a->q_out && (a->q_nb[0] != a->q_out_nb[0] || (a->n_head > 1 && a->q_nb[1] != a->q_out_nb[1]) ||
+                             (a->n_tokens > 1 && a->q_nb[2] != a->q_out_nb[2])))
+      return fail(MI_HIP_E_INVALID, "in place, q and q_out must have the same strides");
+  }
+  if (!strides4(a->k_nb) || !strides4(a->v_nb))
+    return fail(MI_HIP_E_INVALID, "K/V strides must be multiples of 4 bytes");
+  for (const void* x : {(const void*)a->q, (const void*)a->q_out, (const void*)a->k, (const void*)a->v,
+                        (const void*)a->pos, (const void*)a->q_norm, (const void*)a->k_norm})
+    if (!aligned(x, 4)) return fail(MI_HIP_E_INVALID, "device pointers must be 4-byte aligned");
+  return MI_HIP_OK;
+}
+
+template <typename Args>
+void fill_norm_rope(const Args* a, const mi_hip_kv* kv, mi::NormRope& p) {
+  p.q = reinterpret_cast<const char*>(a->q);
+  p.q_out = reinterpret_cast<char*>(a->q_out);
+  p.k = reinterpret_cast<const char*>(a->k);
+  p.v = reinterpret_cast<const char*>(a->v);
+  p.pos = a->pos;
+  p.q_norm = a->q_norm;
+  p.k_norm = a->k_norm;
+  p.cache = kv->view(a->layer);
+  for (int i = 0; i < 3; ++i) {
+    p.q_nb[i] = (int64_t)a->q_nb[i];
+    p.qo_nb[i] = (int64_t)a->q_out_nb[i];
+    p.k_nb[i] = (int64_t)a->k_nb[i];
+    p.v_nb[i] = (int64_t)a->v_nb[i];
+  }
+  p.n_tokens = a->n_tokens;
+  p.n_head = a->q ? a->n_head : 0;
+  p.n_dims = a->n_dims;
+  p.eps = a->eps;
+  if (a->freq) std::copy(a->freq, a->freq + a->n_dims / 2, p.freq);
+  else rope_freqs(p.freq, a->n_dims, a->freq_base);
+}
+
+}  // namespace
+
 // ===========================================================================
 // C ABI
 // ===========================================================================
@@ -1248,7 +1336,8 @@ int mi_hip_set_alloc_limit(uint64_t bytes) {
   return MI_HIP_OK;
 }
 
-int mi_hip_kv_create(const mi_hip_kv_desc* d, mi_hip_kv** out) {
+// page_size 0: one sequence's positions, with staging for host nodes.
+static int kv_make(const mi_hip_kv_desc* d, int32_t page_size, mi_hip_kv** out) {
   if (!d || !out) return fail(MI_HIP_E_INVALID, "desc and out must be non-NULL");
   *out = nullptr;
   if (d->n_layer <= 0 || d->n_ctx <= 0 || d->n_head_kv <= 0 || d->n_head <= 0)
@@ -1261,6 +1350,8 @@ int mi_hip_kv_create(const mi_hip_kv_desc* d, mi_hip_kv** out) {
   if (d->type != MI_TYPE_F32 && d->type != MI_TYPE_F16 && d->type != MI_HIP_TYPE_Q8)
     return fail(MI_HIP_E_UNSUPPORTED, "cache type %d: F32 (0), F16 (1) or MI_HIP_TYPE_Q8 (%d)", d->type,
                 MI_HIP_TYPE_Q8);
+  if (page_size && d->n_ctx % page_size)
+    return fail(MI_HIP_E_INVALID, "n_ctx (%d) must be a multiple of page_size (%d)", d->n_ctx, page_size);
   int rc = bind_device();
   if (rc) return rc;
 
@@ -1281,8 +1372,11 @@ int mi_hip_kv_create(const mi_hip_kv_desc* d, mi_hip_kv** out) {
     kv->scale_bytes = plane[0] + plane[1];
     kv->bytes = kv->scale_at[0] + kv->scale_bytes * d->n_layer;
   }
-  kv->q_floats = (size_t)d->n_ctx * d->n_head * d->head_dim;
-  kv->row_floats = (size_t)d->n_ctx * d->n_head_kv * d->head_dim;
+  kv->page_size = page_size;
+  if (!page_size) {
+    kv->q_floats = (size_t)d->n_ctx * d->n_head * d->head_dim;
+    kv->row_floats = (size_t)d->n_ctx * d->n_head_kv * d->head_dim;
+  }
   kv->stage_bytes = (2 * kv->q_floats + kv->row_floats) * sizeof(float);
 
   void* p = nullptr;
@@ -1291,12 +1385,14 @@ int mi_hip_kv_create(const mi_hip_kv_desc* d, mi_hip_kv** out) {
     return rc;
   }
   kv->base = static_cast<char*>(p);
-  if ((rc = dev_alloc(&p, kv->stage_bytes, "KV staging"))) {
-    dev_free(kv->base, kv->bytes);
-    delete kv;
-    return rc;
+  if (kv->stage_bytes > 0) {
+    if ((rc = dev_alloc(&p, kv->stage_bytes, "KV staging"))) {
+      dev_free(kv->base, kv->bytes);
+      delete kv;
+      return rc;
+    }
+    kv->stage = static_cast<float*>(p);
   }
-  kv->stage = static_cast<float*>(p);
   hipError_t e = hipMemset(kv->base, 0, kv->bytes);
   if (e == hipSuccess) e = hipStreamCreateWithFlags(&kv->stream, hipStreamNonBlocking);
   if (e != hipSuccess) {
@@ -1305,10 +1401,10 @@ int mi_hip_kv_create(const mi_hip_kv_desc* d, mi_hip_kv** out) {
     delete kv;
     return hip_fail(e, "KV cache init");
   }
-  int groups;
-  size_t rec_bytes;
-  ws_capacity(d->n_head_kv, d->n_head / d->n_head_kv, d->head_dim, &groups, &rec_bytes);
-  if ((rc = ws_create(groups, rec_bytes, ws_part_bytes(d->head_dim), &kv->ws))) {
+  int groups = 1;  // (no decode launch of mi_hip_attn_fwd uses a paged cache's)
+  size_t rec_bytes = 0;
+  if (!page_size) ws_capacity(d->n_head_kv, d->n_head / d->n_head_kv, d->head_dim, &groups, &rec_bytes);
+  if ((rc = ws_create(groups, rec_bytes, (page_size ? 2 : 1) * ws_part_bytes(d->head_dim), &kv->ws))) {
     (void)hipStreamDestroy(kv->stream);
     dev_free(kv->stage, kv->stage_bytes);
     dev_free(kv->base, kv->bytes);
@@ -1317,6 +1413,13 @@ int mi_hip_kv_create(const mi_hip_kv_desc* d, mi_hip_kv** out) {
   }
   *out = kv;
   return MI_HIP_OK;
+}
+
+int mi_hip_kv_create(const mi_hip_kv_desc* d, mi_hip_kv** out) { return kv_make(d, 0, out); }
+
+int mi_hip_kv_create_paged(const mi_hip_kv_desc* d, int32_t page_size, mi_hip_kv** out) {
+  if (int rc = check_page_size(page_size)) return rc;
+  return kv_make(d, page_size, out);
 }
 
 int mi_hip_kv_destroy(mi_hip_kv* kv) {
@@ -1477,6 +1580,7 @@ int mi_hip_kv_write(mi_hip_kv* kv, int layer, int which, int pos0, int n_tokens,
   const char* dev_src = reinterpret_cast<const char*>(src);
   int64_t nb[3] = {(int64_t)src_nb[0], (int64_t)src_nb[1], (int64_t)src_nb[2]};
   if (!src_on_device) {
+    if (!kv->stage) return fail(MI_HIP_E_UNSUPPORTED, "a paged cache takes rows in device memory");
     // Host rows: one contiguous copy straight into an F32 cache, else via staging.
     const size_t bytes = (size_t)n_tokens * D * H * sizeof(float);
     if (src_contig && kv->elt == 4) {
@@ -1548,6 +1652,7 @@ int mi_hip_kv_read(mi_hip_kv* kv, int layer, int which, int pos0, int n_tokens, 
 
 int mi_hip_kv_keep(mi_hip_kv* kv, int n_past, const int32_t* idx, int n_idx, void* stream) {
   if (!kv || (n_idx > 0 && !idx)) return fail(MI_HIP_E_INVALID, "kv and idx must be non-NULL");
+  if (int rc = check_unpaged(kv)) return rc;
   if (n_idx < 0 || n_idx > mi::kKeepMax)
     return fail(MI_HIP_E_UNSUPPORTED, "n_idx %d: at most %d rows are kept", n_idx, mi::kKeepMax);
   if (n_past < 0 || n_past > kv->d.n_ctx)
@@ -1586,6 +1691,7 @@ int mi_hip_kv_bind(mi_hip_kv* kv, int layer, int which, const mi_tensor* host_kv
   if (!kv || !host_kv) return fail(MI_HIP_E_INVALID, "kv and host_kv must be non-NULL");
   if (layer < 0 || layer >= kv->d.n_layer || (which != 0 && which != 1))
     return fail(MI_HIP_E_INVALID, "layer %d / which %d out of range", layer, which);
+  if (int rc = check_unpaged(kv)) return rc;
   if (host_kv->ne[0] != kv->d.head_dim || host_kv->ne[1] != kv->d.n_head_kv ||
       host_kv->ne[2] > kv->d.n_ctx)
     return fail(MI_HIP_E_INVALID, "host tensor shape does not match the cache");
@@ -1724,26 +1830,6 @@ int mi_hip_op_softmax(mi_tensor* dst, void* stream) {
   return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "softmax launch");
 }
 
-namespace {
-
-// freq[p] = base^(-2p / n_dims) for p < n_dims / 2, each a float powf exactly
-// as src/ops_cpu.cpp:289 evaluates it (the device then forms pos * freq[p]
-// with one rounded product, as the engine does).
-void rope_freqs(float* freq, int n_dims, float base) {
-  for (int p = 0; p < n_dims / 2; ++p) freq[p] = std::pow(base, -(float)(2 * p) / (float)n_dims);
-}
-
-int check_rope_dims(int n_dims, int head_dim) {
-  if (n_dims < 0 || n_dims % 2 || n_dims > head_dim || n_dims > 2 * mi::kRopeMaxPairs)
-    return fail(MI_HIP_E_UNSUPPORTED, "n_dims %d: must be even, in [0, head_dim = %d] and <= %d",
-                n_dims, head_dim, 2 * mi::kRopeMaxPairs);
-  return MI_HIP_OK;
-}
-
-bool strides4(const size_t nb[3]) { return nb[0] % 4 == 0 && nb[1] % 4 == 0 && nb[2] % 4 == 0; }
-
-}  // namespace
-
 int mi_hip_op_rope(mi_tensor* dst, void* stream) {
   if (!dst || dst->op != MI_OP_ROPE) return fail(MI_HIP_E_INVALID, "dst is not a ROPE node");
   const mi_tensor* s = dst->src[0];
@@ -1780,6 +1866,7 @@ int mi_hip_op_rope(mi_tensor* dst, void* stream) {
 int mi_hip_rope_append(const mi_hip_rope_args* a) {
   if (!a || !a->kv || !a->k || !a->v) return fail(MI_HIP_E_INVALID, "args, kv, k and v must be non-NULL");
   const mi_hip_kv* kv = a->kv;
+  if (int rc = check_unpaged(kv)) return rc;
   if (a->layer < 0 || a->layer >= kv->d.n_layer)
     return fail(MI_HIP_E_INVALID, "layer %d out of range [0, %d)", a->layer, kv->d.n_layer);
   if (a->n_past < 0 || a->n_tokens < 0 || (int64_t)a->n_past + a->n_tokens > kv->d.n_ctx)
@@ -1850,57 +1937,210 @@ int mi_hip_rope_append(const mi_hip_rope_args* a) {
 int mi_hip_norm_rope_append(const mi_hip_norm_rope_args* a) {
   if (!a || !a->kv || !a->k || !a->v) return fail(MI_HIP_E_INVALID, "args, kv, k and v must be non-NULL");
   const mi_hip_kv* kv = a->kv;
+  if (int rc = check_unpaged(kv)) return rc;
   if (a->layer < 0 || a->layer >= kv->d.n_layer)
     return fail(MI_HIP_E_INVALID, "layer %d out of range [0, %d)", a->layer, kv->d.n_layer);
   if (a->n_past < 0 || a->n_tokens < 0 || (int64_t)a->n_past + a->n_tokens > kv->d.n_ctx)
     return fail(MI_HIP_E_INVALID, "rows [%d, %lld) outside [0, %d)", a->n_past, (long long)a->n_past + a->n_tokens,
                 kv->d.n_ctx);
   int rc;
-  if ((rc = check_rope_dims(a->n_dims, kv->d.head_dim))) return rc;
-  if ((a->q_norm || a->k_norm) && !(a->eps >= 0.f && std::isfinite(a->eps)))
-    return fail(MI_HIP_E_INVALID, "eps must be finite and >= 0");
-  if (a->q) {
-    if (!a->q_out) return fail(MI_HIP_E_INVALID, "q_out is NULL");
-    if (a->n_head <= 0 || a->n_head % kv->d.n_head_kv)
-      return fail(MI_HIP_E_INVALID, "n_head %d must be a positive multiple of n_head_kv %d", a->n_head,
-                  kv->d.n_head_kv);
-    if (!strides4(a->q_nb) || !strides4(a->q_out_nb))
-      return fail(MI_HIP_E_INVALID, "Q strides must be multiples of 4 bytes");
-    if (a->q == a->q_out && (a->q_nb[0] != a->q_out_nb[0] || (a->n_head > 1 && a->q_nb[1] != a->q_out_nb[1]) ||
-                             (a->n_tokens > 1 && a->q_nb[2] != a->q_out_nb[2])))
-      return fail(MI_HIP_E_INVALID, "in place, q and q_out must have the same strides");
-  }
-  if (!strides4(a->k_nb) || !strides4(a->v_nb))
-    return fail(MI_HIP_E_INVALID, "K/V strides must be multiples of 4 bytes");
-  for (const void* x : {(const void*)a->q, (const void*)a->q_out, (const void*)a->k, (const void*)a->v,
-                        (const void*)a->pos, (const void*)a->q_norm, (const void*)a->k_norm})
-    if (!aligned(x, 4)) return fail(MI_HIP_E_INVALID, "device pointers must be 4-byte aligned");
+  if ((rc = check_norm_rope(a, kv))) return rc;
   if (a->n_tokens == 0) return MI_HIP_OK;
   mi::NormRope p{};
-  p.q = reinterpret_cast<const char*>(a->q);
-  p.q_out = reinterpret_cast<char*>(a->q_out);
-  p.k = reinterpret_cast<const char*>(a->k);
-  p.v = reinterpret_cast<const char*>(a->v);
-  p.pos = a->pos;
-  p.q_norm = a->q_norm;
-  p.k_norm = a->k_norm;
-  p.cache = kv->view(a->layer);
-  for (int i = 0; i < 3; ++i) {
-    p.q_nb[i] = (int64_t)a->q_nb[i];
-    p.qo_nb[i] = (int64_t)a->q_out_nb[i];
-    p.k_nb[i] = (int64_t)a->k_nb[i];
-    p.v_nb[i] = (int64_t)a->v_nb[i];
-  }
-  p.n_tokens = a->n_tokens;
-  p.n_head = a->q ? a->n_head : 0;
+  fill_norm_rope(a, kv, p);
   p.n_past = a->n_past;
-  p.n_dims = a->n_dims;
-  p.eps = a->eps;
-  if (a->freq) std::copy(a->freq, a->freq + a->n_dims / 2, p.freq);
-  else rope_freqs(p.freq, a->n_dims, a->freq_base);
   if ((rc = bind_device())) return rc;
   hipError_t e = mi::launch_norm_rope(p, static_cast<hipStream_t>(a->stream));
   return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "norm rope append launch");
+}
+
+// ---------------------------------------------------------------------------
+// Many requests over a paged cache
+// ---------------------------------------------------------------------------
+int mi_hip_page_tables(const mi_hip_page_tables_args* a) {
+  if (!a) return fail(MI_HIP_E_INVALID, "args is NULL");
+  if (a->n_seq < 0 || a->max_tokens < 0) return fail(MI_HIP_E_INVALID, "n_seq and max_tokens must be >= 0");
+  if (a->n_pages < 1 || a->max_pages < 1) return fail(MI_HIP_E_INVALID, "n_pages and max_pages must be positive");
+  if (int rc = check_page_size(a->page_size)) return rc;
+  if ((int64_t)a->n_pages * a->page_size > INT32_MAX || (int64_t)a->max_pages * a->page_size > INT32_MAX - 64)
+    return fail(MI_HIP_E_UNSUPPORTED, "2^31 rows of the pool or of a sequence, or more");
+  const void* const each[] = {a->n_cached, a->n_new, a->held, a->held_out, a->table, a->n_kv};
+  for (const void* x : each)
+    if (a->n_seq > 0 && !x) return fail(MI_HIP_E_INVALID, "the sequences' arrays must be non-NULL");
+  if (!a->ring || !a->ring_at || !a->ring_at_out || !a->q_off || (a->max_tokens > 0 && !a->slots))
+    return fail(MI_HIP_E_INVALID, "ring, ring_at, ring_at_out, q_off and slots must be non-NULL");
+  for (const void* x : {each[0], each[1], each[2], each[3], each[4], each[5], (const void*)a->ring, (const void*)a->ring_at,
+                        (const void*)a->ring_at_out, (const void*)a->q_off, (const void*)a->slots, (const void*)a->pos,
+                        (const void*)a->seq, (const void*)a->n_refused})
+    if (!aligned(x, 4)) return fail(MI_HIP_E_INVALID, "device pointers must be 4-byte aligned");
+  if (a->table_nb % 4 || (a->n_seq > 1 && a->table_nb < 4 * (size_t)a->max_pages))
+    return fail(MI_HIP_E_INVALID, "table_nb must be a multiple of 4 and at least a row of %d entries", a->max_pages);
+  int rc = bind_device();
+  if (rc) return rc;
+  mi::PageTables p{};
+  p.n_cached = a->n_cached;
+  p.n_new = a->n_new;
+  p.held = a->held;
+  p.held_out = a->held_out;
+  p.table = reinterpret_cast<char*>(a->table);
+  p.table_nb = (int64_t)a->table_nb;
+  p.ring = a->ring;
+  p.ring_at = a->ring_at;
+  p.ring_at_out = a->ring_at_out;
+  p.n_kv = a->n_kv;
+  p.q_off = a->q_off;
+  p.slots = a->slots;
+  p.pos = a->pos;
+  p.seq = a->seq;
+  p.n_refused = a->n_refused;
+  p.n_seq = a->n_seq;
+  p.page_shift = __builtin_ctz((unsigned)a->page_size);
+  p.n_pages = a->n_pages;
+  p.max_pages = a->max_pages;
+  p.max_tokens = a->max_tokens;
+  hipError_t e = mi::launch_page_tables(p, static_cast<hipStream_t>(a->stream));
+  return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "page tables launch");
+}
+
+// A paged cache and one of its layers.
+static int check_paged(const mi_hip_kv* kv, int layer) {
+  if (!kv->page_size) return fail(MI_HIP_E_UNSUPPORTED, "the cache is not paged (mi_hip_kv_create_paged)");
+  if (layer < 0 || layer >= kv->d.n_layer)
+    return fail(MI_HIP_E_INVALID, "layer %d out of range [0, %d)", layer, kv->d.n_layer);
+  return MI_HIP_OK;
+}
+
+int mi_hip_paged_append(const mi_hip_paged_append_args* a) {
+  if (!a || !a->kv) return fail(MI_HIP_E_INVALID, "args and kv must be non-NULL");
+  const mi_hip_kv* kv = a->kv;
+  int rc;
+  if ((rc = check_paged(kv, a->layer))) return rc;
+  if (a->n_tokens < 0) return fail(MI_HIP_E_INVALID, "n_tokens must be >= 0");
+  if (a->n_tokens > 0 && (!a->k || !a->v || !a->slots || !a->pos))
+    return fail(MI_HIP_E_INVALID, "k, v, slots and pos must be non-NULL");
+  if (a->n_axes < 1 || a->n_axes > mi::kRopeAxes)
+    return fail(MI_HIP_E_UNSUPPORTED, "n_axes %d: 1 to %d", a->n_axes, mi::kRopeAxes);
+  if (a->pos_nb % 4 || !aligned(a->slots, 4))
+    return fail(MI_HIP_E_INVALID, "slots and the axes' positions must be 4-byte aligned");
+  if (a->n_axes > 1 && a->pos_nb < 4 * (size_t)a->n_tokens)
+    return fail(MI_HIP_E_INVALID, "pos_nb must be at least %d positions", a->n_tokens);
+  if ((rc = check_norm_rope(a, kv))) return rc;
+  for (int i = 0; a->axis && i < a->n_dims / 2; ++i)
+    if (a->axis[i] < 0 || a->axis[i] >= a->n_axes)
+      return fail(MI_HIP_E_INVALID, "axis[%d] = %d outside [0, %d)", i, a->axis[i], a->n_axes);
+  if (a->n_tokens == 0) return MI_HIP_OK;
+  mi::PagedRope p{};
+  fill_norm_rope(a, kv, p);
+  p.slots = a->slots;
+  p.pos_nb = (int64_t)a->pos_nb;
+  p.n_slots = kv->d.n_ctx;
+  for (int i = 0; a->axis && i < a->n_dims / 2; ++i) p.axis[i / 16] |= (uint32_t)a->axis[i] << 2 * (i % 16);
+  if ((rc = bind_device())) return rc;
+  hipError_t e = mi::launch_paged_rope(p, static_cast<hipStream_t>(a->stream));
+  return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "paged append launch");
+}
+
+int mi_hip_attn_paged(const mi_hip_attn_paged_args* a) {
+  if (!a || !a->kv) return fail(MI_HIP_E_INVALID, "args and kv must be non-NULL");
+  const mi_hip_kv* kv = a->kv;
+  int rc;
+  if ((rc = check_paged(kv, a->layer))) return rc;
+  if (a->n_seq < 0 || a->n_tokens < 0 || a->max_new < 0 || a->max_pages < 1)
+    return fail(MI_HIP_E_INVALID, "n_seq, n_tokens and max_new must be >= 0 and max_pages positive");
+  if (a->n_head <= 0 || a->n_head % kv->d.n_head_kv)
+    return fail(MI_HIP_E_INVALID, "n_head %d must be a positive multiple of n_head_kv %d", a->n_head, kv->d.n_head_kv);
+  if ((int64_t)a->n_tokens * a->n_head > (1 << 26) || (int64_t)a->max_pages * kv->page_size > INT32_MAX - 64 ||
+      a->n_seq > (1 << 20))
+    return fail(MI_HIP_E_UNSUPPORTED, "more than 2^26 query rows, 2^20 sequences or about 2^31 positions of one");
+  if (!std::isfinite(a->scale)) return fail(MI_HIP_E_INVALID, "scale must be finite");
+  if (!aligned(a->q_off, 4) || !aligned(a->n_kv, 4) || !aligned(a->table, 4))
+    return fail(MI_HIP_E_INVALID, "device pointers must be 4-byte aligned");
+  if (a->table_nb % 4 || (a->n_seq > 1 && a->table_nb < 4 * (size_t)a->max_pages))
+    return fail(MI_HIP_E_INVALID, "table_nb must be a multiple of 4 and at least a row of %d entries", a->max_pages);
+  if (a->n_tokens == 0 || a->n_seq == 0) return MI_HIP_OK;
+  if (!a->q_off || !a->n_kv || !a->table) return fail(MI_HIP_E_INVALID, "q_off, n_kv and table must be non-NULL");
+  if (!a->q || !a->out) return fail(MI_HIP_E_INVALID, "q and out must be device pointers");
+  if (a->q_nb[0] != 4 || a->out_nb[0] != 4)
+    return fail(MI_HIP_E_UNSUPPORTED, "q/out nb[0] must be 4 (head_dim contiguous)");
+  for (int i = 1; i < 3; ++i)
+    if (a->q_nb[i] % 16 || a->out_nb[i] % 16)
+      return fail(MI_HIP_E_UNSUPPORTED, "q/out nb[1], nb[2] must be multiples of 16 bytes");
+  if (!aligned(a->q, 16) || !aligned(a->out, 16)) return fail(MI_HIP_E_UNSUPPORTED, "q/out must be 16-byte aligned");
+  if ((rc = bind_device())) return rc;
+  mi::PagedAttn p{};
+  p.cache = kv->view(a->layer);
+  p.q_off = a->q_off;
+  p.n_kv = a->n_kv;
+  p.table = reinterpret_cast<const char*>(a->table);
+  p.table_nb = (int64_t)a->table_nb;
+  p.q = reinterpret_cast<const char*>(a->q);
+  p.out = reinterpret_cast<char*>(a->out);
+  p.q_s1 = (int64_t)a->q_nb[1];
+  p.q_s2 = (int64_t)a->q_nb[2];
+  p.o_s1 = (int64_t)a->out_nb[1];
+  p.o_s2 = (int64_t)a->out_nb[2];
+  p.n_seq = a->n_seq;
+  p.n_tokens = a->n_tokens;
+  p.max_new = a->max_new ? a->max_new : a->n_tokens;
+  p.max_kv = a->max_pages * kv->page_size;
+  p.page_shift = __builtin_ctz((unsigned)kv->page_size);
+  p.n_pages = kv->d.n_ctx / kv->page_size;
+  p.n_rep = a->n_head / kv->d.n_head_kv;
+  p.scale_log2e = a->scale * kLog2e;
+  hipError_t e = mi::launch_paged_attn(p, static_cast<hipStream_t>(a->stream));
+  return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "paged attention launch");
+}
+
+int mi_hip_verify_draft(const mi_hip_verify_args* a) {
+  if (!a) return fail(MI_HIP_E_INVALID, "args is NULL");
+  if (a->n_vocab <= 0 || a->n_rows < 0 || a->n_seq < 0 || a->max_path < 1)
+    return fail(MI_HIP_E_INVALID, "n_vocab and max_path must be positive, n_rows and n_seq >= 0");
+  if (a->n_vocab > INT32_MAX - (1 << 16)) return fail(MI_HIP_E_UNSUPPORTED, "n_vocab %d", a->n_vocab);
+  if ((a->n_seq > 0 && (!a->off || !a->n_path || !a->path || !a->tokens)) ||
+      (a->n_seq > 0 && a->n_rows > 0 && (!a->logits || !a->token || !a->u)))
+    return fail(MI_HIP_E_INVALID, "only parent, draft, temperature and ws may be NULL");
+  if (a->draft && a->parent) return fail(MI_HIP_E_UNSUPPORTED, "a draft's probabilities go with chains (parent NULL)");
+  const size_t row = 4 * (size_t)a->n_vocab;
+  if (a->nb % 4 || (a->n_rows > 1 && a->nb < row) ||
+      (a->draft && (a->draft_nb % 4 || (a->n_rows > 1 && a->draft_nb < row))))
+    return fail(MI_HIP_E_INVALID, "row strides must be multiples of 4 and at least %zu bytes", row);
+  const size_t out_row = 4 * (size_t)a->max_path;
+  if (a->path_nb % 4 || a->tokens_nb % 4 || (a->n_seq > 1 && (a->path_nb < out_row || a->tokens_nb < out_row)))
+    return fail(MI_HIP_E_INVALID, "path_nb and tokens_nb must be multiples of 4 and at least %zu bytes", out_row);
+  for (const void* x : {(const void*)a->logits, (const void*)a->off, (const void*)a->token, (const void*)a->parent,
+                        (const void*)a->draft, (const void*)a->temperature, (const void*)a->u, (const void*)a->n_path,
+                        (const void*)a->path, (const void*)a->tokens})
+    if (!aligned(x, 4)) return fail(MI_HIP_E_INVALID, "device pointers must be 4-byte aligned");
+  if (a->n_seq == 0) return MI_HIP_OK;
+  int rc = bind_device();
+  if (rc) return rc;
+  mi_hip_workspace* const ws = a->ws ? a->ws : g.default_ws;
+  if (!ws) return fail(MI_HIP_E_STATE, "no workspace (the library default is gone)");
+  if ((size_t)a->n_rows * sizeof(mi::VerifyRow) > ws->part_bytes)
+    return fail(MI_HIP_E_UNSUPPORTED, "n_rows %d: the workspace does not hold their parts (%zu bytes of parts)", a->n_rows,
+                ws->part_bytes);
+  mi::Verify p{};
+  p.logits = reinterpret_cast<const char*>(a->logits);
+  p.nb = (int64_t)a->nb;
+  p.off = a->off;
+  p.token = a->token;
+  p.parent = a->parent;
+  p.draft = reinterpret_cast<const char*>(a->draft);
+  p.draft_nb = (int64_t)a->draft_nb;
+  p.temperature = a->temperature;
+  p.u = a->u;
+  p.n_path = a->n_path;
+  p.path = reinterpret_cast<char*>(a->path);
+  p.path_nb = (int64_t)a->path_nb;
+  p.tokens = reinterpret_cast<char*>(a->tokens);
+  p.tokens_nb = (int64_t)a->tokens_nb;
+  p.rows = reinterpret_cast<mi::VerifyRow*>(ws->part);
+  p.n_vocab = a->n_vocab;
+  p.n_rows = a->n_rows;
+  p.n_seq = a->n_seq;
+  p.max_path = a->max_path;
+  hipError_t e = mi::launch_verify(p, static_cast<hipStream_t>(a->stream));
+  return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "verify launch");
 }
 
 int mi_hip_logits_adjust(const mi_hip_logits_args* a) {

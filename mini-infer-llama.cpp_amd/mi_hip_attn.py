@@ -205,6 +205,109 @@ class LogitsArgs(ctypes.Structure):
     ]
 
 
+class PageTablesArgs(ctypes.Structure):
+    _fields_ = [
+        ("n_seq", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("n_pages", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("max_tokens", ctypes.c_int32),
+        ("n_cached", ctypes.c_void_p),
+        ("n_new", ctypes.c_void_p),
+        ("held", ctypes.c_void_p),
+        ("held_out", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("table_nb", ctypes.c_size_t),
+        ("ring", ctypes.c_void_p),
+        ("ring_at", ctypes.c_void_p),
+        ("ring_at_out", ctypes.c_void_p),
+        ("n_kv", ctypes.c_void_p),
+        ("q_off", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("pos", ctypes.c_void_p),
+        ("seq", ctypes.c_void_p),
+        ("n_refused", ctypes.c_void_p),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("kv", ctypes.c_void_p),
+        ("layer", ctypes.c_int32),
+        ("n_tokens", ctypes.c_int32),
+        ("slots", ctypes.c_void_p),
+        ("n_dims", ctypes.c_int32),
+        ("freq_base", ctypes.c_float),
+        ("freq", ctypes.POINTER(ctypes.c_float)),
+        ("pos", ctypes.c_void_p),
+        ("pos_nb", ctypes.c_size_t),
+        ("n_axes", ctypes.c_int32),
+        ("axis", ctypes.POINTER(ctypes.c_int32)),
+        ("eps", ctypes.c_float),
+        ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p),
+        ("n_head", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("q_nb", ctypes.c_size_t * 3),
+        ("q_out", ctypes.c_void_p),
+        ("q_out_nb", ctypes.c_size_t * 3),
+        ("k", ctypes.c_void_p),
+        ("k_nb", ctypes.c_size_t * 3),
+        ("v", ctypes.c_void_p),
+        ("v_nb", ctypes.c_size_t * 3),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class AttnPagedArgs(ctypes.Structure):
+    _fields_ = [
+        ("kv", ctypes.c_void_p),
+        ("layer", ctypes.c_int32),
+        ("n_seq", ctypes.c_int32),
+        ("n_tokens", ctypes.c_int32),
+        ("max_new", ctypes.c_int32),
+        ("q_off", ctypes.c_void_p),
+        ("n_kv", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("table_nb", ctypes.c_size_t),
+        ("max_pages", ctypes.c_int32),
+        ("n_head", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("q_nb", ctypes.c_size_t * 3),
+        ("out", ctypes.c_void_p),
+        ("out_nb", ctypes.c_size_t * 3),
+        ("scale", ctypes.c_float),
+        ("ws", ctypes.c_void_p),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class VerifyArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("nb", ctypes.c_size_t),
+        ("n_vocab", ctypes.c_int32),
+        ("n_rows", ctypes.c_int32),
+        ("n_seq", ctypes.c_int32),
+        ("off", ctypes.c_void_p),
+        ("token", ctypes.c_void_p),
+        ("parent", ctypes.c_void_p),
+        ("draft", ctypes.c_void_p),
+        ("draft_nb", ctypes.c_size_t),
+        ("temperature", ctypes.c_void_p),
+        ("u", ctypes.c_void_p),
+        ("max_path", ctypes.c_int32),
+        ("n_path", ctypes.c_void_p),
+        ("path", ctypes.c_void_p),
+        ("path_nb", ctypes.c_size_t),
+        ("tokens", ctypes.c_void_p),
+        ("tokens_nb", ctypes.c_size_t),
+        ("ws", ctypes.c_void_p),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
 class Qwen2Hparams(ctypes.Structure):
     """ABI mirror of mi_hip_qwen2_hparams (include/mi_hip_qwen2.h)."""
     _fields_ = [("n_vocab", ctypes.c_int32), ("n_embd", ctypes.c_int32),
@@ -268,6 +371,11 @@ SIGNATURES = {
     "mi_hip_rope_append": ([ctypes.POINTER(RopeArgs)], _I),
     "mi_hip_norm_rope_append": ([ctypes.POINTER(NormRopeArgs)], _I),
     "mi_hip_logits_adjust": ([ctypes.POINTER(LogitsArgs)], _I),
+    "mi_hip_kv_create_paged": ([ctypes.POINTER(KvDesc), ctypes.c_int32, ctypes.POINTER(ctypes.c_void_p)], _I),
+    "mi_hip_page_tables": ([ctypes.POINTER(PageTablesArgs)], _I),
+    "mi_hip_paged_append": ([ctypes.POINTER(PagedAppendArgs)], _I),
+    "mi_hip_attn_paged": ([ctypes.POINTER(AttnPagedArgs)], _I),
+    "mi_hip_verify_draft": ([ctypes.POINTER(VerifyArgs)], _I),
     "mi_hip_memread": ([_P, ctypes.c_size_t, _P, ctypes.c_int32, _P], _I),
     "mi_hip_graph_prepare": ([ctypes.POINTER(MiCgraph)], _I),
     "mi_hip_compute_forward": ([ctypes.POINTER(MiTensor), _I, _I], _I),
@@ -328,6 +436,12 @@ class Lib:
         d = KvDesc(n_layer, n_ctx, n_head_kv, head_dim, n_head, kv_type)
         h = ctypes.c_void_p()
         self.check(self.so.mi_hip_kv_create(ctypes.byref(d), ctypes.byref(h)))
+        return KvHandle(h.value, n_head_kv, head_dim)
+
+    def kv_create_paged(self, n_layer, n_pages, page_size, n_head_kv, head_dim, n_head, kv_type=MI_TYPE_F32):
+        d = KvDesc(n_layer, n_pages * page_size, n_head_kv, head_dim, n_head, kv_type)
+        h = ctypes.c_void_p()
+        self.check(self.so.mi_hip_kv_create_paged(ctypes.byref(d), page_size, ctypes.byref(h)))
         return KvHandle(h.value, n_head_kv, head_dim)
 
     def workspace_create(self, n_head_kv, n_head, head_dim):
@@ -566,6 +680,119 @@ def logits_args(logits, out, stream, penalties=None, hist=None, hist_off=None, b
         a.hist_off = None
     if not a.bias_id:
         a.bias_off = a.bias = None
+    a.ws, a.stream = ws, stream
+    return a
+
+
+def _expect_ints(what, *tensors):
+    _expect(all(t is None or (_is_int32(t) and t.is_contiguous()) for t in tensors), what + ": contiguous int32")
+
+
+def _expect_table(table, n_seq):
+    _expect(_is_int32(table) and table.dim() == 2 and table.shape[0] == n_seq and
+            (table.stride(1) == 1 or table.shape[1] == 1 or n_seq == 0), "table: int32 rows (n_seq, max_pages)")
+
+
+def page_tables_args(page_size, n_cached, n_new, held, held_out, table, ring, ring_at, ring_at_out, n_kv, q_off, slots,
+                     stream, pos=None, seq=None, n_refused=None):
+    """Builds PageTablesArgs from int32 device tensors: n_cached, n_new, held, held_out and n_kv (n_seq),
+    q_off (n_seq + 1), table (n_seq, max_pages), ring (n_pages), ring_at and ring_at_out (2), slots, pos
+    and seq (max_tokens), n_refused (1)."""
+    n = n_cached.numel()
+    lists = (n_cached, n_new, held, held_out, ring, ring_at, ring_at_out, n_kv, q_off, slots, pos, seq, n_refused)
+    _expect_ints("lengths, ring, offsets, slots, pos, seq", *lists)
+    _expect(all(t.numel() == n for t in (n_new, held, held_out, n_kv)) and q_off.numel() == n + 1,
+            "n_new, held, held_out, n_kv: one for each sequence, q_off one more")
+    _expect(ring_at.numel() == 2 and ring_at_out.numel() == 2, "ring_at, ring_at_out: head and tail")
+    _expect(all(t is None or t.numel() == slots.numel() for t in (pos, seq)), "pos, seq: one for each slot")
+    _expect(n_refused is None or n_refused.numel() >= 1, "n_refused: one number")
+    _expect_table(table, n)
+    _expect_one_device(table, *lists)
+    a = PageTablesArgs()
+    a.n_seq, a.page_size, a.n_pages, a.max_pages, a.max_tokens = n, page_size, ring.numel(), table.shape[1], slots.numel()
+    for name, t in (("n_cached", n_cached), ("n_new", n_new), ("held", held), ("held_out", held_out), ("table", table),
+                    ("ring", ring), ("ring_at", ring_at), ("ring_at_out", ring_at_out), ("n_kv", n_kv), ("q_off", q_off),
+                    ("slots", slots), ("pos", pos), ("seq", seq), ("n_refused", n_refused)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    a.table_nb = table.stride(0) * 4
+    a.stream = stream
+    return a
+
+
+def paged_append_args(kv, layer, n_dims, freq_base, stream, k, v, slots, pos, q=None, q_out=None, axis=None, freq=None,
+                      q_norm=None, k_norm=None, eps=0.0):
+    """Builds PagedAppendArgs from torch tensors as norm_rope_args does; slots (n_tokens) and pos (n_axes,
+    n_tokens), or (n_tokens,) for one axis, are int32 device tensors, axis n_dims / 2 numbers on the host."""
+    n = norm_rope_args(kv, layer, 0, n_dims, freq_base, stream, k, v, q=q, q_out=q_out, freq=freq, q_norm=q_norm,
+                       k_norm=k_norm, eps=eps)
+    _expect_ints("slots", slots)
+    _expect(slots.numel() == n.n_tokens, "slots: a cache row for each token")
+    pos = pos if pos.dim() == 2 else pos.reshape(1, -1)
+    _expect(_is_int32(pos) and 1 <= pos.shape[0] <= 4 and pos.shape[1] == n.n_tokens and
+            (pos.stride(1) == 1 or pos.shape[1] <= 1), "pos: int32 rows (n_axes, n_tokens), up to four")
+    _expect_one_device(k, slots, pos)
+    _expect(axis is None or len(axis) == n_dims // 2, "axis: one for each of n_dims / 2 pairs")
+    a = PagedAppendArgs()
+    for name in ("kv", "layer", "n_tokens", "n_dims", "freq_base", "freq", "eps", "q_norm", "k_norm", "n_head", "q", "q_nb",
+                 "q_out", "q_out_nb", "k", "k_nb", "v", "v_nb", "stream"):
+        setattr(a, name, getattr(n, name))
+    a.slots, a.pos = slots.data_ptr(), pos.data_ptr()
+    a.n_axes, a.pos_nb = pos.shape[0], pos.stride(0) * 4
+    if axis is not None:
+        a.axis = (ctypes.c_int32 * len(axis))(*axis)
+    return a
+
+
+def paged_attn_args(kv, layer, q, out, q_off, n_kv, table, scale, stream, max_new=0, ws=None):
+    """Builds AttnPagedArgs from device tensors: q and out (n_tokens, n_head, head_dim), int32 q_off
+    (n_seq + 1), n_kv (n_seq) and table (n_seq, max_pages)."""
+    _expect(all(t.dim() == 3 and _kind(t) == MI_TYPE_F32 for t in (q, out)) and out.shape == q.shape,
+            "q, out: float32 (n_tokens, n_head, head_dim)")
+    rows = getattr(kv, "rows", None)
+    _expect(rows is None or q.shape[2] == rows[1], "q: the cache's head_dim")
+    _expect_ints("q_off, n_kv", q_off, n_kv)
+    _expect(q_off.numel() == n_kv.numel() + 1, "q_off: one more than n_kv")
+    _expect_table(table, n_kv.numel())
+    _expect_one_device(q, out, q_off, n_kv, table)
+    a = AttnPagedArgs()
+    a.kv, a.layer, a.n_seq, a.max_new = kv, layer, n_kv.numel(), max_new
+    a.n_tokens, a.n_head = q.shape[0], q.shape[1]
+    a.q_off, a.n_kv, a.table = q_off.data_ptr(), n_kv.data_ptr(), table.data_ptr()
+    a.table_nb, a.max_pages = table.stride(0) * 4, table.shape[1]
+    a.q, a.out = q.data_ptr(), out.data_ptr()
+    a.q_nb[:], a.out_nb[:] = nb3_of(q), nb3_of(out)
+    a.scale, a.ws, a.stream = scale, ws, stream
+    return a
+
+
+def verify_args(logits, off, token, u, n_path, path, tokens, stream, parent=None, draft=None, temperature=None, ws=None):
+    """Builds VerifyArgs from device tensors: logits and draft (n_rows, n_vocab), int32 off (n_seq + 1),
+    token and parent (n_rows), n_path (n_seq), path and tokens (n_seq, max_path), float32 u (n_rows) and
+    temperature (n_seq)."""
+    rows, vocab = logits.shape
+    n = n_path.numel()
+    _expect(all(t is None or (_kind(t) == MI_TYPE_F32 and t.shape == logits.shape and (t.stride(1) == 1 or vocab == 1))
+                for t in (logits, draft)), "logits, draft: float32 rows (n_rows, n_vocab)")
+    _expect_ints("off, token, parent, n_path", off, token, parent, n_path)
+    _expect(off.numel() == n + 1 and token.numel() == rows and (parent is None or parent.numel() == rows),
+            "off: n_seq + 1; token, parent: one for each row")
+    for t, m in ((u, rows), (temperature, n)):
+        _expect(t is None or (_kind(t) == MI_TYPE_F32 and t.is_contiguous() and t.numel() == m),
+                "u, temperature: contiguous float32, one for each row and for each sequence")
+    _expect(all(_is_int32(t) and t.dim() == 2 and t.shape[0] == n and (t.stride(1) == 1 or t.shape[1] == 1)
+                for t in (path, tokens)) and path.shape == tokens.shape, "path, tokens: int32 rows (n_seq, max_path)")
+    _expect_one_device(logits, draft, off, token, parent, u, temperature, n_path, path, tokens)
+    a = VerifyArgs()
+    a.n_rows, a.n_vocab, a.n_seq, a.max_path = rows, vocab, n, path.shape[1]
+    a.logits, a.nb = logits.data_ptr(), logits.stride(0) * 4
+    if draft is not None:
+        a.draft, a.draft_nb = draft.data_ptr(), draft.stride(0) * 4
+    for name, t in (("off", off), ("token", token), ("parent", parent), ("temperature", temperature), ("u", u),
+                    ("n_path", n_path), ("path", path), ("tokens", tokens)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    a.path_nb, a.tokens_nb = path.stride(0) * 4, tokens.stride(0) * 4
     a.ws, a.stream = ws, stream
     return a
 
