@@ -187,8 +187,13 @@ struct PagedAttn {
   int64_t q_s1, q_s2, o_s1, o_s2;
   int32_t n_seq, n_tokens, max_new, max_kv, page_shift, n_pages, n_rep;
   float scale_log2e;
+  float* rec;         // scratch: records of the parts; null: no unit in parts
+  unsigned* arrived;  // kArrivals counters, zero before and after
+  int32_t few_rows, least;  // set by the launcher
 };
-hipError_t launch_paged_attn(const PagedAttn& p, hipStream_t stream);
+// A call's key tiles are counted in 32 bits: at most kPagedMaxTiles of 32 keys.
+constexpr int64_t kPagedMaxTiles = INT32_MAX;
+hipError_t launch_paged_attn(const PagedAttn& p, int n_cu, size_t part_bytes, hipStream_t stream);
 
 // verify.hip. Drafted tokens against the target's probabilities (mi_hip_verify_draft).
 constexpr int kVerifyMaxNodes = 1024;

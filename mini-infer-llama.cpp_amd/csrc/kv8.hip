@@ -433,6 +433,7 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const P p) {
     }
     wave_lds_fence();
     const int half = p.n_dims / 2;
+    int pos = position_of(p, t, 0);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
 #pragma clang fp contract(off)
@@ -440,7 +441,7 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const P p) {
       if (exact) x[i] = (float)y[i];
       if (d >= p.n_dims) continue;
       const int j = d < half ? d : d - half;
-      const int pos = position_of(p, t, j);
+      if constexpr (std::is_same<P, PagedRope>::value) pos = position_of(p, t, j);
       double s, c;
       sincos((double)((float)pos * p.freq[j]), &s, &c);
       if (exact) {
@@ -458,7 +459,7 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const P p) {
     for (int i = 0; i < E; ++i) gstore<float>(o + (lane + 64 * i) * p.qo_nb[0], x[i]);
   } else {
     const int64_t to = cache_row(p, t);
-    if (to >= 0) store_row<E>(p.cache, kind - 1, to, h, lane, x);
+    if (std::is_same<P, NormRope>::value || to >= 0) store_row<E>(p.cache, kind - 1, to, h, lane, x);
   }
 }
 
@@ -561,7 +562,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const P p, int tokens) {
       continue;
     }
     const int64_t pos = cache_row(p, t0 + t);
-    if (pos < 0) continue;
+    if (std::is_same<P, PagedRope>::value && pos < 0) continue;
     char* const o = row_of(p.cache, kind - 1, pos, h);
     if (q8) {
       unsigned ma = 0, mb = 0;

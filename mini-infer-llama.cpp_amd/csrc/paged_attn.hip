@@ -1,101 +1,529 @@
-// paged_attn.hip -- attention of each sequence's new tokens over its pages.
+// paged_attn.hip -- attention of each sequence's new tokens over its pages: one, a
+// few or thousands per sequence, in one call, with all lengths read on the device.
 //
-// out_j = sum_t p_t v_t / sum_t p_t over the positions t up to the query's own,
-// p_t = 2^(s_t - m), s_t = scale log2(e) q_j.k_t, m the maximum so far, position t
-// in row table[t / page] page + t % page. A wave takes one query row: a lane's
-// key is its own for the scores, its dims are its own for the sums.
+// The mathematics and the products are tree.hip's: query j of a sequence sees the
+// positions up to its own, its output is sum_t p_t v_t / sum_t p_t with a running
+// reference. tree_rows.h takes sequences of few query rows per KV head, a second
+// launch of tree_wide_rows.h the others in row tiles of 128.
+//
+// Work. The host does not know the lengths, so every workgroup finds its share
+// itself: the key tiles of all units (sequence, KV head, row tile) form one line,
+// of which workgroup w takes tiles w * per .. (w + 1) * per - 1 whatever they belong
+// to: whole units, the end of one, the start of another. So workgroups have the
+// same work however ragged the lengths are. A causal unit has the tiles that its
+// rows see; to find the unit at a place of the line without adding up row tiles,
+// row tile r of n lies beside row tile n - 1 - r: together they have the same number
+// of tiles, but for a few that are empty. Each wave reads the lengths of 64
+// sequences at a time and adds up their tiles by itself (one round of loads and
+// six additions).
+//
+// Parts. A unit that lies in several workgroups' shares leaves a record from each
+// (its first part in slot 2 w + 1 of the workgroup where it begins, the others in
+// slot 2 w), and the last of them to arrive joins the records in their order, so
+// the bits do not depend on who that is. Records pass between XCDs: they are
+// written and read with agent-scope accesses, which go past the L2s.
+//
+// Pages. 16 keys lie in one page at least, so a tile of 32 has two page numbers,
+// the same for the whole wave: the rows' descriptors are in scalar registers as
+// for one run of rows. A lane holds the page number of 16 keys, a wave those of
+// 1024, the next 1024 on their way.
+#include <algorithm>
+
 #include "attn_common.h"
 #include "kernels.h"
+#include "tree_rows.h"
+#include "tree_wide_rows.h"
 
 namespace mi {
 
 namespace {
 
-// Element d of a row (K: a scale per 32 dims, V: one).
-template <typename KT, bool K>
-__device__ inline float element(const CacheView& c, int64_t row, int h, int d) {
-  const char* const at = c.t[K ? 0 : 1] + row * c.s2 + h * c.s1;
-  if constexpr (sizeof(KT) == 1) {
-    const int n = K ? c.head_dim / 32 : 1;
-    const char* const sc = c.scale[K ? 0 : 1] + ((row * c.n_head_kv + h) * n + (K ? d / 32 : 0)) * 2;
-    return (float)gload<int8_t>(at + d) * (float)gload<_Float16>(sc);
-  } else {
-    return (float)gload<KT>(at + d * (int)sizeof(KT));
+constexpr int kRun = 16;  // keys that share a page at least
+
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// x plus those of the lanes below.
+__device__ inline unsigned wave_scan(unsigned x) {
+  auto add = [&](auto ctrl, auto rows) {
+    x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+  };
+  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // row_shr:1
+  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15 to rows 1 and 3
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast:31 to rows 2 and 3
+  return x;
+}
+
+// A sequence's queries and keys, clamped to what is there.
+struct SeqLens {
+  int q0;      // its first row of q
+  int n_new;   // its queries (up to max_new)
+  int n_past;  // the first query's position (negative: the first queries see nothing)
+  int n_seen;  // positions that its last query sees
+};
+__device__ inline SeqLens seq_lens(const PagedAttn& p, int i) {
+  SeqLens s{0, 0, 0, 0};
+  if (i < p.n_seq) {
+    const int a = min(max(gload<int>(p.q_off + i), 0), p.n_tokens), b = min(gload<int>(p.q_off + i + 1), p.n_tokens);
+    const int n_kv = min(max(gload<int>(p.n_kv + i), 0), p.max_kv);
+    s.q0 = a;
+    s.n_new = min(max(b - a, 0), p.max_new);
+    s.n_past = n_kv - max(b - a, 0);
+    s.n_seen = max(s.n_past + s.n_new, 0);
   }
+  return s;
+}
+
+// Units of a sequence on the line, for row tiles of ROWS rows and key tiles of TK.
+template <int ROWS, int TK>
+struct Units {
+  int n_rt, n_past, n_new, n_seen, n_rep;
+  unsigned pair;  // tiles of a pair of row tiles, a few empty ones among them
+
+  __device__ inline Units(const SeqLens& s, int rep) : n_past(s.n_past), n_new(s.n_new), n_seen(s.n_seen), n_rep(rep) {
+    n_rt = (s.n_new * rep + ROWS - 1) / ROWS;
+    // The two row tiles see at most 2 n_past + ((n_rt + 1) ROWS - 2) / n_rep + 2 keys.
+    const unsigned keys = 2u * (unsigned)max(s.n_past, 0) + ((unsigned)(n_rt + 1) * ROWS - 2u) / (unsigned)rep + 2u;
+    pair = (keys + 2 * TK - 2) / TK;
+  }
+  // Key tiles of row tile rt, one at least (rows without a key are written too).
+  __device__ inline int tiles(int rt) const {
+    const int last = min(((rt + 1) * ROWS - 1) / n_rep, n_new - 1);
+    return (max(min(n_past + last + 1, n_seen), 1) + TK - 1) / TK;
+  }
+  __device__ inline unsigned per_head(bool whole) const {
+    if (whole) return (unsigned)n_rt;
+    return (unsigned)(n_rt / 2) * pair + (n_rt & 1 ? (unsigned)tiles(n_rt / 2) : 0u);
+  }
+};
+
+// The pages of a sequence, as a wave reads them: RUNS runs of 16 keys per tile.
+template <int RUNS>
+struct Pages {
+  const int* table;
+  int shift, n_pages, last;  // the last run that is there
+  int win, here, next;       // page numbers of runs 64 win + lane, and of the 64 behind
+  int slot[RUNS];            // cache row of each run of the tile at hand
+  unsigned none = 0u;        // runs without a page
+
+  __device__ __forceinline__ Pages(const PagedAttn& p, int seq, int n_seen)
+      : table(reinterpret_cast<const int*>(p.table + (int64_t)seq * p.table_nb)), shift(p.page_shift), n_pages(p.n_pages),
+        last(max(n_seen - 1, 0) / kRun) {}
+  __device__ __forceinline__ int read(int w) const {
+    return gload<int>(table + (min(64 * w + (int)(threadIdx.x % kWave), last) * kRun >> shift));
+  }
+  __device__ __forceinline__ void start(int run) {
+    win = run / 64;
+    here = read(win);
+    next = read(win + 1);
+  }
+  // Runs run .. run + RUNS - 1 (a multiple of RUNS; tiles are taken in order, 64
+  // runs further at most).
+  __device__ __forceinline__ void at(int run) {
+    if (run / 64 != win) {
+      win = run / 64;
+      here = next;
+      next = read(win + 1);
+    }
+    none = 0u;
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+      const int page = __builtin_amdgcn_readlane(here, (run + i) & 63);
+      const bool ok = (unsigned)page < (unsigned)n_pages;
+      none |= ok ? 0u : 1u << i;
+      slot[i] = ((ok ? page : 0) << shift) + ((run + i) * kRun & ((1 << shift) - 1));
+    }
+  }
+  // Any key's row, -1 if it has none.
+  __device__ __forceinline__ int row(int key) const {
+    const int page = gload<int>(table + (min(key / kRun, last) * kRun >> shift));
+    return (unsigned)page < (unsigned)n_pages ? (page << shift) + (key & ((1 << shift) - 1)) : -1;
+  }
+};
+
+// Records: a row's dims, then each row's reference and sum. Written by one XCD, read
+// by another.
+template <int D, int ROWS>
+struct Record {
+  static constexpr int FLOATS = ROWS * (D + 2);
+  static __device__ __forceinline__ void put2(float* at, float a, float b) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(at), __builtin_bit_cast(uint64_t, f32x2{a, b}), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+  }
+  static __device__ __forceinline__ f32x2 get2(const float* at) {
+    return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(at), __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_AGENT));
+  }
+};
+
+// One unit's rows and the part of its key tiles that this workgroup has.
+template <int D, typename KT, int ROWS>
+struct UnitRows {
+  const PagedAttn& p;
+  int g, q0, n_past, n_kv, rows, n_rep, row0;  // rows: of the sequence; row0: of the row tile
+  float scale_log2e;
+  bool part;
+  float* rec;
+
+  __device__ __forceinline__ unsigned visible(int token, int key0) const {
+    const int n = n_past + token - key0 + 1;
+    return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+  }
+  __device__ __forceinline__ const char* q_row(int token, int h) const {
+    return p.q + (int64_t)(q0 + token) * p.q_s2 + (int64_t)(g * n_rep + h) * p.q_s1;
+  }
+  __device__ __forceinline__ char* out_row(int token, int h) const {
+    return p.out + (int64_t)(q0 + token) * p.o_s2 + (int64_t)(g * n_rep + h) * p.o_s1;
+  }
+  __device__ __forceinline__ bool is_part() const { return part; }
+  __device__ __forceinline__ void put_sums(int r, float ref, float l) const {
+    Record<D, ROWS>::put2(rec + ROWS * D + 2 * r, ref, l);
+  }
+  __device__ __forceinline__ void put_part(int r, int d, f32x4 x) const {
+    Record<D, ROWS>::put2(rec + r * D + d, x[0], x[1]);
+    Record<D, ROWS>::put2(rec + r * D + d + 2, x[2], x[3]);
+  }
+};
+
+// tree_rows over pages.
+template <int D, typename KT, int ROWS>
+struct FewRows : UnitRows<D, KT, ROWS> {
+  static constexpr int ELT = (int)sizeof(KT);
+  int tile0, tile1, k_s2, v_s2;
+  const char* kbase;
+  const char* vbase;
+  Pages<2> pages;
+
+  __device__ __forceinline__ FewRows(const UnitRows<D, KT, ROWS>& u, int seq, int t0, int t1)
+      : UnitRows<D, KT, ROWS>(u), tile0(t0), tile1(t1), k_s2((int)u.p.cache.s2), v_s2((int)u.p.cache.s2),
+        kbase(u.p.cache.t[0] + u.g * u.p.cache.s1), vbase(u.p.cache.t[1] + u.g * u.p.cache.s1), pages(u.p, seq, u.n_kv) {
+    pages.start(2 * tile0);
+  }
+  __device__ __forceinline__ void at_tile(int tile) { pages.at(2 * tile); }
+  __device__ __forceinline__ unsigned none() const { return pages.none; }
+  __device__ __forceinline__ TileRows rows_at(const char* base, int key0) const {
+    TileRows t;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int n = pages.none >> i & 1u ? 0 : min(this->n_kv - key0 - kRun * i, kRun);
+      t.rows[i] = make_rsrc(base + (int64_t)pages.slot[i] * k_s2, n > 0 ? (unsigned)((n - 1) * k_s2 + D * ELT) : 0u);
+      t.at[i] = 0u;
+    }
+    return t;
+  }
+  __device__ __forceinline__ TileRows k_rows(int key0) const { return rows_at(kbase, key0); }
+  __device__ __forceinline__ TileRows v_rows(int key0) const { return rows_at(vbase, key0); }
+  // (every row of a page is there, so the lanes past the last key read what their
+  // queries do not see)
+  template <int NB>
+  __device__ __forceinline__ void scales(int, int c32, int half, unsigned& ksc, unsigned& vsc) const {
+    const CacheView& c = this->p.cache;
+    const int64_t at = (int64_t)((c32 < kRun ? pages.slot[0] : pages.slot[1]) + c32 % kRun) * c.n_head_kv + this->g;
+    if constexpr (NB == 4) ksc = gload<unsigned>(c.scale[0] + at * 8 + 4 * half);
+    else ksc = gload<unsigned short>(c.scale[0] + at * 4 + 2 * half);
+    vsc = gload<unsigned short>(c.scale[1] + at * 2);
+  }
+};
+
+// tree_wide_rows over pages.
+template <int D, typename KT>
+struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
+  typedef UnitRows<D, KT, WideCfg<D, KT>::ROWS> Base;
+  static constexpr int ELT = (int)sizeof(KT), TK = WideCfg<D, KT>::TK, NDB = D / 32, RUNS = TK / kRun;
+  int key_begin, key_end;
+  const char* kbase;
+  const char* vbase;
+  Pages<RUNS> pages;
+
+  __device__ __forceinline__ ManyRows(const Base& u, int seq, int k0, int k1)
+      : Base(u), key_begin(k0), key_end(k1), kbase(u.p.cache.t[0] + u.g * u.p.cache.s1),
+        vbase(u.p.cache.t[1] + u.g * u.p.cache.s1), pages(u.p, seq, u.n_kv) {
+    pages.start(key_begin / kRun);
+  }
+  __device__ __forceinline__ void at_tile(int key0) { pages.at(key0 / kRun); }
+  __device__ __forceinline__ unsigned none() const { return pages.none; }
+  struct Rows {
+    const ManyRows& w;
+    const char* base;
+    int s2, key0;
+    __device__ __forceinline__ Rows(const ManyRows& u, int which, int key)
+        : w(u), base(which == 0 ? u.kbase : u.vbase), s2((int)u.p.cache.s2), key0(key) {}
+    __device__ __forceinline__ rsrc_t rows(int run) const {
+      int slot = w.pages.slot[0];
+#pragma unroll
+      for (int i = 1; i < RUNS; ++i) slot = run == i ? w.pages.slot[i] : slot;
+      const int n = w.pages.none >> run & 1u ? 0 : min(w.n_kv - key0 - kRun * run, kRun);
+      return make_rsrc(base + (int64_t)slot * s2, n > 0 ? (unsigned)((n - 1) * s2 + D * ELT) : 0u);
+    }
+    __device__ __forceinline__ unsigned row_at(unsigned row, int run) const { return (row - kRun * run) * (unsigned)s2; }
+  };
+  struct Scale {
+    int n;  // scales of a row
+    const char* src;
+    __device__ __forceinline__ Scale(const ManyRows& w, bool k, int group) {
+      n = k ? NDB : 1;
+      src = ELT == 1 ? w.p.cache.scale[k ? 0 : 1] + 2 * (w.g * n + (k ? group : 0)) : nullptr;
+    }
+    // (every row of a page is there)
+    __device__ __forceinline__ const char* at(const ManyRows& w, int, int key) const {
+      int slot = w.pages.slot[0];
+#pragma unroll
+      for (int i = 1; i < RUNS; ++i) slot = key / kRun == i ? w.pages.slot[i] : slot;
+      return src + (int64_t)(slot + key % kRun) * (w.p.cache.n_head_kv * 2 * n);
+    }
+  };
+  // (of a key without a page: of row 0, whose value does not matter beside the NaN)
+  __device__ __forceinline__ const char* v_row(int key) const {
+    return vbase + (int64_t)max(pages.row(key), 0) * (int)this->p.cache.s2;
+  }
+  __device__ __forceinline__ const char* v_scale(int key) const {
+    return this->p.cache.scale[1] + ((int64_t)max(pages.row(key), 0) * this->p.cache.n_head_kv + this->g) * 2;
+  }
+};
+
+// The records of a unit's `n` parts (part 0 at rec, part k at rec + (2 k - 1) records)
+// into its rows: out = sum_k 2^(ref_k - M) O_k / sum_k 2^(ref_k - M) l_k. A thread
+// takes four dims of a row, and where there are few rows, groups of threads every
+// `groups`-th part; they meet in LDS in order.
+template <int D, int ROWS, typename U>
+__device__ __forceinline__ void join_parts(const U& u, const float* rec, int n, int n_rows, lds_t* lds) {
+  constexpr int kInFlight = 8, THREADS = kTreeWaves * kWave;
+  typedef Record<D, ROWS> R;
+  const int tid = threadIdx.x, units = n_rows * (D / 4);
+  int groups = 1;
+  while (units * groups * 2 <= THREADS) groups *= 2;
+  const int span = THREADS / groups, grp = tid / span;
+  for (int i = tid % span; i < units; i += span) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = grp; k0 < n; k0 += kInFlight * groups) {
+      f32x2 ml[kInFlight], a[kInFlight], b[kInFlight];
+#pragma unroll
+      for (int e = 0; e < kInFlight; ++e) {
+        const int k = min(k0 + e * groups, n - 1);
+        const float* const q = rec + (int64_t)max(2 * k - 1, 0) * R::FLOATS;
+        ml[e] = R::get2(q + ROWS * D + 2 * r);
+        a[e] = R::get2(q + r * D + d);
+        b[e] = R::get2(q + r * D + d + 2);
+      }
+#pragma unroll
+      for (int e = 0; e < kInFlight; ++e) {
+        if (k0 + e * groups >= n) continue;
+        const float mn = fmaxf(m, ml[e][0]), mu = mn == -INFINITY ? 0.f : mn;
+        const float x = fast_exp2(m - mu), y = fast_exp2(ml[e][0] - mu);
+        acc = acc * x + f32x4{a[e][0], a[e][1], b[e][0], b[e][1]} * y;
+        l = l * x + ml[e][1] * y;
+        m = mn;
+      }
+    }
+    if (groups > 1) {  // (one round: every thread has at most one unit)
+      lds_store<f32x4>(lds + tid * 24, acc);
+      lds_store<f32x2>(lds + tid * 24 + 16, f32x2{m, l});
+    }
+    if (groups == 1) {
+      const int token = (u.row0 + r) / u.n_rep;
+      const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
+      gstore(u.out_row(token, u.row0 + r - token * u.n_rep) + 4 * d, acc * inv);
+    }
+  }
+  if (groups == 1) return;
+  __syncthreads();
+  if (tid >= units) return;
+  float m = -INFINITY, l = 0.f;
+  for (int o = 0; o < groups; ++o) m = fmaxf(m, lds_load<float>(lds + (tid + o * span) * 24 + 16));
+  const float mu = m == -INFINITY ? 0.f : m;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int o = 0; o < groups; ++o) {
+    const f32x2 ml = lds_load<f32x2>(lds + (tid + o * span) * 24 + 16);
+    const float y = fast_exp2(ml[0] - mu);
+    acc += lds_load<f32x4>(lds + (tid + o * span) * 24) * y;
+    l += ml[1] * y;
+  }
+  const int r = tid / (D / 4), d = 4 * (tid % (D / 4)), token = (u.row0 + r) / u.n_rep;
+  const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
+  gstore(u.out_row(token, u.row0 + r - token * u.n_rep) + 4 * d, acc * inv);
 }
 
 }  // namespace
 
-template <int D, typename KT>
-__global__ __launch_bounds__(kWave) void paged_attn_kernel(const PagedAttn p) {
-  __shared__ float qs[D];
-  __shared__ float ps[kWave];
-  __shared__ int64_t rows[kWave];
-  const int lane = threadIdx.x, row = blockIdx.x, h = blockIdx.y, g = h / p.n_rep;
-  int seq = 0;  // the last sequence that begins at or before the row
-  for (int hi = p.n_seq - 1; seq < hi;) {
-    const int mid = (seq + hi + 1) / 2;
-    if (p.q_off[mid] <= row) seq = mid;
-    else hi = mid - 1;
+// WIDE: sequences of more than p.few_rows query rows per KV head, in row tiles of
+// 128; otherwise those of up to that many (at most 16 RT), in one.
+template <int D, typename KT, int RT, bool WIDE>
+struct PagedCfg {
+  static constexpr int ROWS = WIDE ? WideCfg<D, KT>::ROWS : 16 * RT, TK = WIDE ? WideCfg<D, KT>::TK : kTreeTile;
+  static constexpr int WORK = WIDE ? WideCfg<D, KT>::LDS : TreeCfg<D, KT, RT>::LDS;
+  static constexpr int LDS = WORK + 16;  // and a word for who joins
+  static constexpr int WAVES_PER_SIMD = WIDE ? WideCfg<D, KT>::WAVES_PER_SIMD : TreeCfg<D, KT, RT>::WAVES_PER_SIMD;
+};
+
+template <int D, typename KT, int RT, bool WIDE>
+__global__ __launch_bounds__(kTreeWaves* kWave, (PagedCfg<D, KT, RT, WIDE>::WAVES_PER_SIMD)) void paged_attn_kernel(const PagedAttn p) {
+  typedef PagedCfg<D, KT, RT, WIDE> C;
+  typedef Units<C::ROWS, C::TK> U;
+  constexpr int ROWS = C::ROWS, TK = C::TK;
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  lds_t* const lds = (lds_t*)lds_raw;
+  const int lane = threadIdx.x % kWave;
+  const bool whole = p.rec == nullptr;  // no records: no unit in parts
+  auto units_of = [&](const SeqLens& s) __attribute__((always_inline)) -> unsigned {
+    const int rows = s.n_new * p.n_rep;
+    if (rows == 0 || WIDE != (rows > p.few_rows)) return 0u;
+    return U(s, p.n_rep).per_head(whole) * (unsigned)p.cache.n_head_kv;
+  };
+
+  // ---- the line: lane i has sequence `first` + i ------------------------------------
+  int first = 0;
+  unsigned before = 0u;  // units of the sequences before
+  SeqLens lens = seq_lens(p, lane);
+  unsigned end = wave_scan(units_of(lens));
+  unsigned total = (unsigned)__builtin_amdgcn_readlane((int)end, 63);
+  for (int i = kWave; i < p.n_seq; i += kWave)
+    total += (unsigned)__builtin_amdgcn_readlane((int)wave_scan(units_of(seq_lens(p, i + lane))), 63);
+  // Shares: the same for every workgroup, `least` at least, whole rounds of the waves.
+  const unsigned n_wg = gridDim.x;
+  unsigned per = (total + n_wg - 1) / n_wg;
+  if (!whole) {
+    per = max(per, (unsigned)p.least);
+    if (!WIDE) per = (per + kTreeWaves - 1) / kTreeWaves * kTreeWaves;
   }
-  const int q0 = min(max(p.q_off[seq], 0), p.n_tokens), q1 = min(max(p.q_off[seq + 1], q0), p.n_tokens);
-  if (row < q0 || row >= q1 || row - q0 >= p.max_new) return;
-  const int n_kv = min(max(p.n_kv[seq], 0), p.max_kv);
-  const int lim = n_kv - (q1 - q0) + (row - q0) + 1;  // positions seen
-  const char* const q = p.q + row * p.q_s2 + h * p.q_s1;
-  for (int d = lane; d < D; d += kWave) qs[d] = gload<float>(q + 4 * d) * p.scale_log2e;
-  __syncthreads();
-  const int* const table = reinterpret_cast<const int*>(p.table + seq * p.table_nb);
-  float m = -INFINITY, l = 0.f, o[D / kWave];
-  for (float& x : o) x = 0.f;
-  for (int t0 = 0; t0 < lim; t0 += kWave) {
-    const int t = t0 + lane;
-    float s = -INFINITY;
-    rows[lane] = -1;
-    if (t < lim) {
-      const int page = table[t >> p.page_shift];
-      if ((unsigned)page < (unsigned)p.n_pages) {
-        const int64_t r = ((int64_t)page << p.page_shift) + (t & ((1 << p.page_shift) - 1));
-        rows[lane] = r;
-        s = 0.f;
-        for (int d = 0; d < D; ++d) s = fmaf(element<KT, true>(p.cache, r, g, d), qs[d], s);
-      } else {
-        s = NAN;
-      }
+  // An XCD's workgroups (every eighth) have one piece of the line.
+  const unsigned wg = blockIdx.x % 8 * (n_wg / 8) + blockIdx.x / 8;
+  unsigned x = min(wg * per, total);
+  const unsigned x_end = min(x + per, total);
+
+  while (x < x_end) {
+    for (;;) {
+      const unsigned all = (unsigned)__builtin_amdgcn_readlane((int)end, 63);
+      if (x < before + all) break;
+      before += all;
+      first += kWave;
+      lens = seq_lens(p, first + lane);
+      end = wave_scan(units_of(lens));
     }
-    float top = s;
-    bool bad = __builtin_amdgcn_ballot_w64(s != s) != 0ull;
-    top = wave_max(top);
-    const float now = fmaxf(m, top);
-    const float at = now == -INFINITY ? 0.f : now;
-    const float alpha = fast_exp2(m - at), e = fast_exp2(s - at);
-    m = now;
-    l = bad ? NAN : l * alpha + wave_sum(e);
-    ps[lane] = e;
-    __syncthreads();
-    for (float& x : o) x *= alpha;
-    for (int j = 0; j < kWave && t0 + j < lim; ++j)
-      if (rows[j] >= 0)
-        for (int i = 0; i < D / kWave; ++i) o[i] = fmaf(ps[j], element<KT, false>(p.cache, rows[j], g, lane + kWave * i), o[i]);
-    __syncthreads();
+    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(end > x - before));
+    const SeqLens s{__builtin_amdgcn_readlane(lens.q0, at), __builtin_amdgcn_readlane(lens.n_new, at),
+                    __builtin_amdgcn_readlane(lens.n_past, at), __builtin_amdgcn_readlane(lens.n_seen, at)};
+    const U u(s, p.n_rep);
+    const unsigned per_head = u.per_head(whole), seq_end = (unsigned)__builtin_amdgcn_readlane((int)end, at);
+    const unsigned y = x - before - (seq_end - per_head * (unsigned)p.cache.n_head_kv);
+    const int g = uniform((int)(y / per_head));
+    unsigned off = y - (unsigned)g * per_head;  // place in the head's units
+    int rt, tiles, tile;
+    if (whole) {
+      rt = uniform(u.n_rt - 1 - (int)off);
+      tiles = u.tiles(rt);
+      tile = 0;
+    } else {
+      const unsigned pairs = (unsigned)(u.n_rt / 2), j = min(off / u.pair, pairs);
+      off -= j * u.pair;
+      const unsigned left = u.pair - off;  // of the pair
+      rt = u.n_rt - 1 - (int)j;  // (the middle one, where it is alone, is both)
+      tiles = u.tiles(rt);
+      if (j < pairs && off >= (unsigned)tiles) {
+        off -= (unsigned)tiles;
+        rt = (int)j;
+        tiles = u.tiles(rt);
+        if (off >= (unsigned)tiles) {  // the empty ones behind the pair
+          x += left;
+          continue;
+        }
+      }
+      tile = (int)off;
+      rt = uniform(rt);
+      tiles = uniform(tiles);
+      tile = uniform(tile);
+    }
+    const int n = whole ? tiles : (int)min((unsigned)(tiles - tile), x_end - x);
+    const bool part = n < tiles;
+    // its first tile's place: who begins it, and how many share it
+    const unsigned x0 = x - (unsigned)tile, owner = part ? x0 / per : 0u;
+    const int parts = part ? (int)((x0 + (unsigned)tiles - 1) / per - owner) + 1 : 1;
+    float* const rec = part ? p.rec + (int64_t)(2 * wg + (tile == 0 ? 1 : 0)) * Record<D, ROWS>::FLOATS : nullptr;
+    const UnitRows<D, KT, ROWS> rows{p, g, s.q0, s.n_past, s.n_seen, s.n_new * p.n_rep, p.n_rep, rt * ROWS, p.scale_log2e, part, rec};
+    if constexpr (WIDE) {
+      const int lim = min(s.n_seen, max(s.n_past + min(((rt + 1) * ROWS - 1) / p.n_rep, s.n_new - 1) + 1, 0));
+      ManyRows<D, KT> w(rows, first + at, tile * TK, min((tile + n) * TK, lim));
+      tree_wide_rows<D, KT>(w, lds);
+    } else {
+      FewRows<D, KT, ROWS> w(rows, first + at, tile, min(tile + n, (s.n_seen + TK - 1) / TK));
+      tree_rows<D, KT, RT>(w, lds);
+    }
+    if (part) {
+      // Every wave's records are in memory before they are counted.
+      wait_vmem<0>();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        unsigned* const counter = p.arrived + kArrivalWords * owner;
+        const unsigned done = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if ((int)done == parts - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        lds_store<int>(lds + C::WORK, (int)done == parts - 1);
+      }
+      __syncthreads();
+      if (lds_load<int>(lds + C::WORK))
+        join_parts<D, ROWS>(rows, p.rec + (int64_t)(2 * owner + 1) * Record<D, ROWS>::FLOATS, parts,
+                            min(ROWS, rows.rows - rows.row0), lds);
+    }
+    x += whole ? 1u : (unsigned)n;
+    __syncthreads();  // the LDS is free for the next unit
   }
-  const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
-  char* const out = p.out + row * p.o_s2 + h * p.o_s1;
-  for (int i = 0; i < D / kWave; ++i) gstore<float>(out + 4 * (lane + kWave * i), o[i] * inv);
 }
 
-template <int D>
-static void launch_d(const PagedAttn& p, hipStream_t stream) {
-  const dim3 grid((unsigned)p.n_tokens, (unsigned)(p.n_rep * p.cache.n_head_kv));
-  if (p.cache.elt == 1) hipLaunchKernelGGL((paged_attn_kernel<D, int8_t>), grid, dim3(kWave), 0, stream, p);
-  else if (p.cache.elt == 2) hipLaunchKernelGGL((paged_attn_kernel<D, _Float16>), grid, dim3(kWave), 0, stream, p);
-  else hipLaunchKernelGGL((paged_attn_kernel<D, float>), grid, dim3(kWave), 0, stream, p);
-}
-
-hipError_t launch_paged_attn(const PagedAttn& p, hipStream_t stream) {
-  if (p.cache.head_dim == 64) launch_d<64>(p, stream);
-  else launch_d<128>(p, stream);
+template <int D, typename KT, int RT, bool WIDE>
+static hipError_t launch_paged_t(const PagedAttn& p, int n_wg, hipStream_t stream) {
+  typedef PagedCfg<D, KT, RT, WIDE> C;
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attn_kernel<D, KT, RT, WIDE>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+  if (attr != hipSuccess) return attr;
+  hipLaunchKernelGGL((paged_attn_kernel<D, KT, RT, WIDE>), dim3((unsigned)n_wg), dim3(kTreeWaves * kWave), C::LDS, stream, p);
   return hipGetLastError();
+}
+
+template <int D, typename KT>
+static hipError_t launch_paged(PagedAttn p, int n_cu, size_t part_bytes, hipStream_t stream) {
+  // Most query rows per KV head that a sequence can have decide what is launched:
+  // up to 16 or 32 rows the kernel that streams keys to registers, alone; above, it
+  // takes the sequences of up to 16, the wide kernel the rest.
+  const int64_t most = (int64_t)std::min(p.max_new, p.n_tokens) * p.n_rep;
+  const bool two = most > 16 && most <= 32, wide = most > 32;
+  p.few_rows = two ? 32 : 16;
+  // Workgroups: what the CUs hold at once, each with room for two records, and an
+  // arrival counter, a multiple of the XCDs.
+  auto grid = [&](int per_cu, int rows) {
+    int64_t n = (int64_t)n_cu * per_cu;
+    if (p.rec) n = std::min({n, (int64_t)kArrivals, (int64_t)(part_bytes / (2 * sizeof(float) * rows * (D + 2)))});
+    return (int)(n / 8 * 8);
+  };
+  constexpr bool F32 = sizeof(KT) == 4;
+  hipError_t e = hipSuccess;
+  int n_wg = grid(two ? (D == 64 ? 2 : 1) : (D == 64 ? 3 : 2), two ? 32 : 16);
+  p.least = 8;
+  PagedAttn q = p;
+  if (n_wg == 0) {  // no room for records
+    q.rec = nullptr;
+    n_wg = n_cu / 8 * 8;
+  }
+  e = two ? launch_paged_t<D, KT, 2, false>(q, n_wg, stream) : launch_paged_t<D, KT, 1, false>(q, n_wg, stream);
+  if (e != hipSuccess || !wide) return e;
+  n_wg = grid(F32 && D == 128 ? 1 : 2, 128);
+  p.least = D == 64 ? 2 : 4;
+  if (n_wg == 0) {
+    p.rec = nullptr;
+    n_wg = n_cu / 8 * 8;
+  }
+  return launch_paged_t<D, KT, 1, true>(p, n_wg, stream);
+}
+
+hipError_t launch_paged_attn(const PagedAttn& p, int n_cu, size_t part_bytes, hipStream_t stream) {
+  if (p.cache.head_dim == 64)
+    return p.cache.elt == 1   ? launch_paged<64, int8_t>(p, n_cu, part_bytes, stream)
+           : p.cache.elt == 2 ? launch_paged<64, _Float16>(p, n_cu, part_bytes, stream)
+                              : launch_paged<64, float>(p, n_cu, part_bytes, stream);
+  return p.cache.elt == 1   ? launch_paged<128, int8_t>(p, n_cu, part_bytes, stream)
+         : p.cache.elt == 2 ? launch_paged<128, _Float16>(p, n_cu, part_bytes, stream)
+                            : launch_paged<128, float>(p, n_cu, part_bytes, stream);
 }
 
 }  // namespace mi

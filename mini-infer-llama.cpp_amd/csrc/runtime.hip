@@ -2049,9 +2049,14 @@ int mi_hip_attn_paged(const mi_hip_attn_paged_args* a) {
     return fail(MI_HIP_E_INVALID, "n_seq, n_tokens and max_new must be >= 0 and max_pages positive");
   if (a->n_head <= 0 || a->n_head % kv->d.n_head_kv)
     return fail(MI_HIP_E_INVALID, "n_head %d must be a positive multiple of n_head_kv %d", a->n_head, kv->d.n_head_kv);
-  if ((int64_t)a->n_tokens * a->n_head > (1 << 26) || (int64_t)a->max_pages * kv->page_size > INT32_MAX - 64 ||
-      a->n_seq > (1 << 20))
-    return fail(MI_HIP_E_UNSUPPORTED, "more than 2^26 query rows, 2^20 sequences or about 2^31 positions of one");
+  if ((int64_t)a->n_tokens * a->n_head > (1 << 26) || a->n_seq > (1 << 20) ||
+      (int64_t)a->max_pages * kv->page_size > (1 << 30))
+    return fail(MI_HIP_E_UNSUPPORTED, "more than 2^26 query rows, 2^20 sequences or 2^30 positions of one");
+  // key tiles of all row tiles (of 128 rows, one at least per sequence), with the empty ones
+  const int64_t row_tiles = a->n_seq + (int64_t)a->n_tokens * (a->n_head / kv->d.n_head_kv) / 128;
+  if (row_tiles * kv->d.n_head_kv * ((int64_t)a->max_pages * kv->page_size / 32 + 4) > mi::kPagedMaxTiles)
+    return fail(MI_HIP_E_UNSUPPORTED, "n_seq, n_tokens and max_pages: more than 2^31 tiles of 32 positions");
+  if (kv->s2 > INT32_MAX / 32) return fail(MI_HIP_E_UNSUPPORTED, "cache rows of more than 2^26 bytes");
   if (!std::isfinite(a->scale)) return fail(MI_HIP_E_INVALID, "scale must be finite");
   if (!aligned(a->q_off, 4) || !aligned(a->n_kv, 4) || !aligned(a->table, 4))
     return fail(MI_HIP_E_INVALID, "device pointers must be 4-byte aligned");
@@ -2067,7 +2072,10 @@ int mi_hip_attn_paged(const mi_hip_attn_paged_args* a) {
       return fail(MI_HIP_E_UNSUPPORTED, "q/out nb[1], nb[2] must be multiples of 16 bytes");
   if (!aligned(a->q, 16) || !aligned(a->out, 16)) return fail(MI_HIP_E_UNSUPPORTED, "q/out must be 16-byte aligned");
   if ((rc = bind_device())) return rc;
+  mi_hip_workspace* const ws = a->ws ? a->ws : kv->ws;
   mi::PagedAttn p{};
+  p.rec = reinterpret_cast<float*>(ws->part);
+  p.arrived = ws->arrived;
   p.cache = kv->view(a->layer);
   p.q_off = a->q_off;
   p.n_kv = a->n_kv;
@@ -2087,7 +2095,7 @@ int mi_hip_attn_paged(const mi_hip_attn_paged_args* a) {
   p.n_pages = kv->d.n_ctx / kv->page_size;
   p.n_rep = a->n_head / kv->d.n_head_kv;
   p.scale_log2e = a->scale * kLog2e;
-  hipError_t e = mi::launch_paged_attn(p, static_cast<hipStream_t>(a->stream));
+  hipError_t e = mi::launch_paged_attn(p, g.n_cu, ws->part_bytes, static_cast<hipStream_t>(a->stream));
   return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "paged attention launch");
 }
 
