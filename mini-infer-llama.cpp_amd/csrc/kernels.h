@@ -197,10 +197,10 @@ hipError_t launch_paged_attn(const PagedAttn& p, int n_cu, size_t part_bytes, hi
 
 // verify.hip. Drafted tokens against the target's probabilities (mi_hip_verify_draft).
 constexpr int kVerifyMaxNodes = 1024;
-struct VerifyRow {
-  double sum;    // of the weights
-  float top;     // the largest logit; NaN: the row has a NaN or an infinity
-  int32_t best;  // its lowest token
+struct VerifyPart {  // a chunk of a row
+  double sum;    // of the weights relative to top (not of greedy rows)
+  float top;     // the largest logit, NaN if there is one
+  int32_t best;  // greedy rows: its lowest token
 };
 struct Verify {
   const char* logits;
@@ -217,10 +217,14 @@ struct Verify {
   int64_t path_nb;
   char* tokens;
   int64_t tokens_nb;
-  VerifyRow* rows;  // scratch
+  VerifyPart* parts;  // scratch of verify_scratch() bytes
+  unsigned* arrived;  // kArrivals counters, zero before and after
   int32_t n_vocab, n_rows, n_seq, max_path;
+  double* sums;       // these are set by the launcher
+  int32_t n_chunks, row0, seq0;
 };
-hipError_t launch_verify(const Verify& p, hipStream_t stream);
+size_t verify_scratch(int n_rows, int n_seq, int n_vocab, int n_cu);
+hipError_t launch_verify(const Verify& p, int n_cu, hipStream_t stream);
 
 // Arrival counters of a workspace, kArrivalWords apart: counters in one line are
 // counted one after the other in memory (64 rows of logits: 53 us, 27 apart).

@@ -2124,7 +2124,7 @@ int mi_hip_verify_draft(const mi_hip_verify_args* a) {
   if (rc) return rc;
   mi_hip_workspace* const ws = a->ws ? a->ws : g.default_ws;
   if (!ws) return fail(MI_HIP_E_STATE, "no workspace (the library default is gone)");
-  if ((size_t)a->n_rows * sizeof(mi::VerifyRow) > ws->part_bytes)
+  if (mi::verify_scratch(a->n_rows, a->n_seq, a->n_vocab, g.n_cu) > ws->part_bytes)
     return fail(MI_HIP_E_UNSUPPORTED, "n_rows %d: the workspace does not hold their parts (%zu bytes of parts)", a->n_rows,
                 ws->part_bytes);
   mi::Verify p{};
@@ -2142,12 +2142,13 @@ int mi_hip_verify_draft(const mi_hip_verify_args* a) {
   p.path_nb = (int64_t)a->path_nb;
   p.tokens = reinterpret_cast<char*>(a->tokens);
   p.tokens_nb = (int64_t)a->tokens_nb;
-  p.rows = reinterpret_cast<mi::VerifyRow*>(ws->part);
+  p.parts = reinterpret_cast<mi::VerifyPart*>(ws->part);
+  p.arrived = ws->arrived;
   p.n_vocab = a->n_vocab;
   p.n_rows = a->n_rows;
   p.n_seq = a->n_seq;
   p.max_path = a->max_path;
-  hipError_t e = mi::launch_verify(p, static_cast<hipStream_t>(a->stream));
+  hipError_t e = mi::launch_verify(p, g.n_cu, static_cast<hipStream_t>(a->stream));
   return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "verify launch");
 }
 
