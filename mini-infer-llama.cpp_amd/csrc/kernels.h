@@ -173,7 +173,7 @@ struct PageTables {
   int32_t* n_refused;  // or null
   int32_t n_seq, page_shift, n_pages, max_pages, max_tokens;
 };
-hipError_t launch_page_tables(const PageTables& p, hipStream_t stream);
+hipError_t launch_page_tables(const PageTables& p, int n_cu, hipStream_t stream);
 
 // paged_attn.hip. Attention over pages (mi_hip_attn_paged).
 struct PagedAttn {

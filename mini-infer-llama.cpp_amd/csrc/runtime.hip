@@ -1998,7 +1998,7 @@ int mi_hip_page_tables(const mi_hip_page_tables_args* a) {
   p.n_pages = a->n_pages;
   p.max_pages = a->max_pages;
   p.max_tokens = a->max_tokens;
-  hipError_t e = mi::launch_page_tables(p, static_cast<hipStream_t>(a->stream));
+  hipError_t e = mi::launch_page_tables(p, g.n_cu, static_cast<hipStream_t>(a->stream));
   return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "page tables launch");
 }
 
