@@ -285,48 +285,65 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
 
 // The records of a unit's `n` parts (part 0 at rec, part k at rec + (2 k - 1) records)
 // into its rows: out = sum_k 2^(ref_k - M) O_k / sum_k 2^(ref_k - M) l_k. A thread
-// takes four dims of a row, and where there are few rows, groups of threads every
-// `groups`-th part; they meet in LDS in order.
-template <int D, int ROWS, typename U>
+// takes four dims of EACH rows at once, whose records are on their way together;
+// where there are few rows, groups of threads take every `groups`-th part and meet
+// in LDS in order. What it takes is the records' latency, so as few rounds of loads
+// as the registers allow.
+template <int D, int ROWS, int EACH, typename U>
 __device__ __forceinline__ void join_parts(const U& u, const float* rec, int n, int n_rows, lds_t* lds) {
-  constexpr int kInFlight = 8, THREADS = kTreeWaves * kWave;
+  constexpr int kInFlight = EACH >= 8 ? 1 : 8 / EACH, THREADS = kTreeWaves * kWave;
   typedef Record<D, ROWS> R;
   const int tid = threadIdx.x, units = n_rows * (D / 4);
   int groups = 1;
   while (units * groups * 2 <= THREADS) groups *= 2;
   const int span = THREADS / groups, grp = tid / span;
-  for (int i = tid % span; i < units; i += span) {
-    const int r = i / (D / 4), d = 4 * (i % (D / 4));
-    float m = -INFINITY, l = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  auto finish = [&](int i, f32x4 acc, float m, float l) __attribute__((always_inline)) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4)), token = (u.row0 + r) / u.n_rep;
+    const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
+    gstore(u.out_row(token, u.row0 + r - token * u.n_rep) + 4 * d, acc * inv);
+  };
+  for (int i0 = tid % span; i0 < units; i0 += span * EACH) {
+    float m[EACH], l[EACH];
+    f32x4 acc[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      m[j] = -INFINITY;
+      l[j] = 0.f;
+      acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     for (int k0 = grp; k0 < n; k0 += kInFlight * groups) {
-      f32x2 ml[kInFlight], a[kInFlight], b[kInFlight];
+      f32x2 ml[kInFlight][EACH], a[kInFlight][EACH], b[kInFlight][EACH];
 #pragma unroll
       for (int e = 0; e < kInFlight; ++e) {
-        const int k = min(k0 + e * groups, n - 1);
-        const float* const q = rec + (int64_t)max(2 * k - 1, 0) * R::FLOATS;
-        ml[e] = R::get2(q + ROWS * D + 2 * r);
-        a[e] = R::get2(q + r * D + d);
-        b[e] = R::get2(q + r * D + d + 2);
+        const float* const q = rec + (int64_t)max(2 * min(k0 + e * groups, n - 1) - 1, 0) * R::FLOATS;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+          const int i = min(i0 + span * j, units - 1), r = i / (D / 4), d = 4 * (i % (D / 4));
+          ml[e][j] = R::get2(q + ROWS * D + 2 * r);
+          a[e][j] = R::get2(q + r * D + d);
+          b[e][j] = R::get2(q + r * D + d + 2);
+        }
       }
 #pragma unroll
       for (int e = 0; e < kInFlight; ++e) {
         if (k0 + e * groups >= n) continue;
-        const float mn = fmaxf(m, ml[e][0]), mu = mn == -INFINITY ? 0.f : mn;
-        const float x = fast_exp2(m - mu), y = fast_exp2(ml[e][0] - mu);
-        acc = acc * x + f32x4{a[e][0], a[e][1], b[e][0], b[e][1]} * y;
-        l = l * x + ml[e][1] * y;
-        m = mn;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+          const float mn = fmaxf(m[j], ml[e][j][0]), mu = mn == -INFINITY ? 0.f : mn;
+          const float x = fast_exp2(m[j] - mu), y = fast_exp2(ml[e][j][0] - mu);
+          acc[j] = acc[j] * x + f32x4{a[e][j][0], a[e][j][1], b[e][j][0], b[e][j][1]} * y;
+          l[j] = l[j] * x + ml[e][j][1] * y;
+          m[j] = mn;
+        }
       }
     }
-    if (groups > 1) {  // (one round: every thread has at most one unit)
-      lds_store<f32x4>(lds + tid * 24, acc);
-      lds_store<f32x2>(lds + tid * 24 + 16, f32x2{m, l});
-    }
-    if (groups == 1) {
-      const int token = (u.row0 + r) / u.n_rep;
-      const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
-      gstore(u.out_row(token, u.row0 + r - token * u.n_rep) + 4 * d, acc * inv);
+    if (groups > 1) {  // (every thread has at most one unit)
+      lds_store<f32x4>(lds + tid * 24, acc[0]);
+      lds_store<f32x2>(lds + tid * 24 + 16, f32x2{m[0], l[0]});
+    } else {
+#pragma unroll
+      for (int j = 0; j < EACH; ++j)
+        if (i0 + span * j < units) finish(i0 + span * j, acc[j], m[j], l[j]);
     }
   }
   if (groups == 1) return;
@@ -342,9 +359,7 @@ __device__ __forceinline__ void join_parts(const U& u, const float* rec, int n, 
     acc += lds_load<f32x4>(lds + (tid + o * span) * 24) * y;
     l += ml[1] * y;
   }
-  const int r = tid / (D / 4), d = 4 * (tid % (D / 4)), token = (u.row0 + r) / u.n_rep;
-  const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
-  gstore(u.out_row(token, u.row0 + r - token * u.n_rep) + 4 * d, acc * inv);
+  finish(tid, acc, m, l);
 }
 
 }  // namespace
@@ -463,7 +478,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (PagedCfg<D, KT, RT, WIDE>::WAVE
       }
       __syncthreads();
       if (lds_load<int>(lds + C::WORK))
-        join_parts<D, ROWS>(rows, p.rec + (int64_t)(2 * owner + 1) * Record<D, ROWS>::FLOATS, parts,
+        join_parts<D, ROWS, WIDE ? 8 : 1>(rows, p.rec + (int64_t)(2 * owner + 1) * Record<D, ROWS>::FLOATS, parts,
                             min(ROWS, rows.rows - rows.row0), lds);
     }
     x += whole ? 1u : (unsigned)n;
