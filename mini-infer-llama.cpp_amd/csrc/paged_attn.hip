@@ -143,20 +143,33 @@ struct Pages {
   }
 };
 
-// Records: a row's dims, then each row's reference and sum. Written by one XCD, read
-// by another.
+// A record: 16-byte pieces of four dims of a row, then each row's reference and sum.
+// Pieces that a wave holds lie together: few rows' row by row, many rows' those of
+// 32 rows side by side. Written by one XCD, read by another, so with the cache bit
+// that goes past the L2s (8 bytes at a time, as atomics do, and with rows apart, a
+// prompt's chunk of 1000 tokens after 1337 took 137 us, not XX).
+constexpr int kSc1 = 16;
 template <int D, int ROWS>
 struct Record {
-  static constexpr int FLOATS = ROWS * (D + 2);
-  static __device__ __forceinline__ void put2(float* at, float a, float b) {
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(at), __builtin_bit_cast(uint64_t, f32x2{a, b}), __ATOMIC_RELAXED,
-                       __HIP_MEMORY_SCOPE_AGENT);
+  static constexpr int FLOATS = ROWS * (D + 2), BYTES = FLOATS * 4;
+  static __device__ __forceinline__ unsigned piece_at(int r, int d) {
+    if constexpr (ROWS > 32) return (unsigned)((r / 32) * (128 * D) + (d / 4) * 512 + (r % 32) * 16);
+    else return (unsigned)(r * D + d) * 4;
   }
-  static __device__ __forceinline__ f32x2 get2(const float* at) {
-    return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(at), __ATOMIC_RELAXED,
-                                                       __HIP_MEMORY_SCOPE_AGENT));
-  }
+  static __device__ __forceinline__ unsigned sums_at(int r) { return (unsigned)(ROWS * D + 2 * r) * 4; }
 };
+__device__ inline void shared_store4(rsrc_t r, unsigned at, f32x4 x) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), r, at, 0, kSc1);
+}
+__device__ inline void shared_store2(rsrc_t r, unsigned at, f32x2 x) {
+  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), r, at, 0, kSc1);
+}
+__device__ inline f32x4 shared_load4(rsrc_t r, unsigned at) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, kSc1));
+}
+__device__ inline f32x2 shared_load2(rsrc_t r, unsigned at) {
+  return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, kSc1));
+}
 
 // One unit's rows and the part of its key tiles that this workgroup has.
 template <int D, typename KT, int ROWS>
@@ -178,12 +191,12 @@ struct UnitRows {
     return p.out + (int64_t)(q0 + token) * p.o_s2 + (int64_t)(g * n_rep + h) * p.o_s1;
   }
   __device__ __forceinline__ bool is_part() const { return part; }
+  __device__ __forceinline__ rsrc_t record() const { return make_rsrc(rec, Record<D, ROWS>::BYTES); }
   __device__ __forceinline__ void put_sums(int r, float ref, float l) const {
-    Record<D, ROWS>::put2(rec + ROWS * D + 2 * r, ref, l);
+    shared_store2(record(), Record<D, ROWS>::sums_at(r), f32x2{ref, l});
   }
   __device__ __forceinline__ void put_part(int r, int d, f32x4 x) const {
-    Record<D, ROWS>::put2(rec + r * D + d, x[0], x[1]);
-    Record<D, ROWS>::put2(rec + r * D + d + 2, x[2], x[3]);
+    shared_store4(record(), Record<D, ROWS>::piece_at(r, d), x);
   }
 };
 
@@ -293,12 +306,17 @@ template <int D, int ROWS, int EACH, typename U>
 __device__ __forceinline__ void join_parts(const U& u, const float* rec, int n, int n_rows, lds_t* lds) {
   constexpr int kInFlight = EACH >= 8 ? 1 : 8 / EACH, THREADS = kTreeWaves * kWave;
   typedef Record<D, ROWS> R;
-  const int tid = threadIdx.x, units = n_rows * (D / 4);
+  // unit i: four dims of a row, in the records' order
+  const int tid = threadIdx.x, units = (ROWS > 32 ? (n_rows + 31) / 32 * 32 : n_rows) * (D / 4);
+  auto row_of = [](int i) __attribute__((always_inline)) { return ROWS > 32 ? i / (8 * D) * 32 + i % 32 : i / (D / 4); };
+  auto dim_of = [](int i) __attribute__((always_inline)) { return ROWS > 32 ? 4 * (i / 32 % (D / 4)) : 4 * (i % (D / 4)); };
+  const rsrc_t recs = make_rsrc(rec, (unsigned)(2 * n - 1) * R::BYTES);
   int groups = 1;
   while (units * groups * 2 <= THREADS) groups *= 2;
   const int span = THREADS / groups, grp = tid / span;
   auto finish = [&](int i, f32x4 acc, float m, float l) __attribute__((always_inline)) {
-    const int r = i / (D / 4), d = 4 * (i % (D / 4)), token = (u.row0 + r) / u.n_rep;
+    const int r = row_of(i), d = dim_of(i), token = (u.row0 + r) / u.n_rep;
+    if (r >= n_rows) return;
     const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
     gstore(u.out_row(token, u.row0 + r - token * u.n_rep) + 4 * d, acc * inv);
   };
@@ -312,16 +330,16 @@ __device__ __forceinline__ void join_parts(const U& u, const float* rec, int n, 
       acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     for (int k0 = grp; k0 < n; k0 += kInFlight * groups) {
-      f32x2 ml[kInFlight][EACH], a[kInFlight][EACH], b[kInFlight][EACH];
+      f32x2 ml[kInFlight][EACH];
+      f32x4 o[kInFlight][EACH];
 #pragma unroll
       for (int e = 0; e < kInFlight; ++e) {
-        const float* const q = rec + (int64_t)max(2 * min(k0 + e * groups, n - 1) - 1, 0) * R::FLOATS;
+        const unsigned at = (unsigned)max(2 * min(k0 + e * groups, n - 1) - 1, 0) * R::BYTES;
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
-          const int i = min(i0 + span * j, units - 1), r = i / (D / 4), d = 4 * (i % (D / 4));
-          ml[e][j] = R::get2(q + ROWS * D + 2 * r);
-          a[e][j] = R::get2(q + r * D + d);
-          b[e][j] = R::get2(q + r * D + d + 2);
+          const int i = min(i0 + span * j, units - 1), r = row_of(i);
+          ml[e][j] = shared_load2(recs, at + R::sums_at(r));
+          o[e][j] = shared_load4(recs, at + R::piece_at(r, dim_of(i)));
         }
       }
 #pragma unroll
@@ -331,7 +349,7 @@ __device__ __forceinline__ void join_parts(const U& u, const float* rec, int n, 
         for (int j = 0; j < EACH; ++j) {
           const float mn = fmaxf(m[j], ml[e][j][0]), mu = mn == -INFINITY ? 0.f : mn;
           const float x = fast_exp2(m[j] - mu), y = fast_exp2(ml[e][j][0] - mu);
-          acc[j] = acc[j] * x + f32x4{a[e][j][0], a[e][j][1], b[e][j][0], b[e][j][1]} * y;
+          acc[j] = acc[j] * x + o[e][j] * y;
           l[j] = l[j] * x + ml[e][j][1] * y;
           m[j] = mn;
         }
