@@ -18,7 +18,7 @@
 // six additions).
 //
 // Parts. A unit that lies in several workgroups' shares leaves a record from each
-// (its first part in slot 2 w + 1 of the workgroup where it begins, the others in
+// (its first part in slot 2 w + 1 of the workgroup w where it begins, the others in
 // slot 2 w), and the last of them to arrive joins the records in their order, so
 // the bits do not depend on who that is. Records pass between XCDs: they are
 // written and read with agent-scope accesses, which go past the L2s.
@@ -174,12 +174,33 @@ __device__ inline f32x2 shared_load2(rsrc_t r, unsigned at) {
 // One unit's rows and the part of its key tiles that this workgroup has.
 template <int D, typename KT, int ROWS>
 struct UnitRows {
+  static constexpr int kRows = ROWS;
   const PagedAttn& p;
   int g, q0, n_past, n_kv, rows, n_rep, row0;  // rows: of the sequence; row0: of the row tile
   float scale_log2e;
-  bool part;
-  float* rec;
+  int parts, mine;     // how many workgroups share the rows' keys, which of them this is
+  float* rec;          // the record of this part
+  unsigned* arrived;   // how many have left theirs
+  lds_t* word;         // for the workgroup to agree on who joins
 
+  // The records of all parts: part k's at part_at(k).
+  __device__ __forceinline__ const float* first_record() const {
+    return rec - (int64_t)max(2 * mine - 1, 0) * Record<D, ROWS>::FLOATS;
+  }
+  static __device__ __forceinline__ unsigned part_at(int k) { return (unsigned)max(2 * k - 1, 0) * Record<D, ROWS>::BYTES; }
+  // Counts this part; true for the last one. Every wave's records are in memory
+  // before that.
+  __device__ __forceinline__ bool arrive() const {
+    wait_vmem<0>();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const int done = (int)__hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (done == parts - 1) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      lds_store<int>(word, done == parts - 1);
+    }
+    __syncthreads();
+    return lds_load<int>(word) != 0;
+  }
   __device__ __forceinline__ unsigned visible(int token, int key0) const {
     const int n = n_past + token - key0 + 1;
     return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
@@ -190,7 +211,7 @@ struct UnitRows {
   __device__ __forceinline__ char* out_row(int token, int h) const {
     return p.out + (int64_t)(q0 + token) * p.o_s2 + (int64_t)(g * n_rep + h) * p.o_s1;
   }
-  __device__ __forceinline__ bool is_part() const { return part; }
+  __device__ __forceinline__ bool is_part() const { return parts > 1; }
   __device__ __forceinline__ rsrc_t record() const { return make_rsrc(rec, Record<D, ROWS>::BYTES); }
   __device__ __forceinline__ void put_sums(int r, float ref, float l) const {
     shared_store2(record(), Record<D, ROWS>::sums_at(r), f32x2{ref, l});
@@ -256,6 +277,64 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
     pages.start(key_begin / kRun);
   }
   __device__ __forceinline__ void at_tile(int key0) { pages.at(key0 / kRun); }
+  // The last part to arrive adds up all of them in their order, its own from where
+  // it lies: a wave its 32 rows, lanes as the products left them.
+  static constexpr bool kJoins = true;
+  __device__ __forceinline__ void join(const floatx16 (&own)[NDB], float ref, float l, bool active, bool valid, int token, int h) const {
+    typedef Record<D, Base::kRows> R;
+    const int lane = threadIdx.x % kWave, kh = lane / 32;
+    const int r = 32 * uniform((int)threadIdx.x / kWave) + lane % 32;
+    if (active) {
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          this->put_part(r, 32 * db + 8 * q + 4 * kh, f32x4{own[db][4 * q], own[db][4 * q + 1], own[db][4 * q + 2], own[db][4 * q + 3]});
+      if (kh == 0) this->put_sums(r, ref, l);
+    }
+    if (!this->arrive() || !active) return;
+    const int n = this->parts;
+    const rsrc_t recs = make_rsrc(this->first_record(), (unsigned)(2 * n - 1) * R::BYTES);
+    float top = ref;
+    for (int k = 0; k < n; ++k)
+      if (k != this->mine) top = fmaxf(top, shared_load2(recs, Base::part_at(k) + R::sums_at(r))[0]);
+    const float mu = top == -INFINITY ? 0.f : top;
+    f32x4 acc[NDB][4];
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[db][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+    for (int k = 0; k < n; ++k) {
+      f32x4 x[NDB][4];
+      f32x2 ml = {ref, l};
+      if (k != this->mine) {
+        ml = shared_load2(recs, Base::part_at(k) + R::sums_at(r));
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x[db][q] = shared_load4(recs, Base::part_at(k) + R::piece_at(r, 32 * db + 8 * q + 4 * kh));
+      } else {
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x[db][q] = f32x4{own[db][4 * q], own[db][4 * q + 1], own[db][4 * q + 2], own[db][4 * q + 3]};
+      }
+      const float y = fast_exp2(ml[0] - mu);
+      sum += ml[1] * y;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[db][q] += x[db][q] * y;
+    }
+    if (!valid) return;
+    const float inv = top == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;
+    char* const out = this->out_row(token, h);
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) gstore(out + 4 * (32 * db + 8 * q + 4 * kh), acc[db][q] * inv);
+  }
   __device__ __forceinline__ unsigned none() const { return pages.none; }
   struct Rows {
     const ManyRows& w;
@@ -296,72 +375,53 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
   }
 };
 
-// The records of a unit's `n` parts (part 0 at rec, part k at rec + (2 k - 1) records)
-// into its rows: out = sum_k 2^(ref_k - M) O_k / sum_k 2^(ref_k - M) l_k. A thread
-// takes four dims of EACH rows at once, whose records are on their way together;
-// where there are few rows, groups of threads take every `groups`-th part and meet
-// in LDS in order. What it takes is the records' latency, so as few rounds of loads
-// as the registers allow.
-template <int D, int ROWS, int EACH, typename U>
-__device__ __forceinline__ void join_parts(const U& u, const float* rec, int n, int n_rows, lds_t* lds) {
-  constexpr int kInFlight = EACH >= 8 ? 1 : 8 / EACH, THREADS = kTreeWaves * kWave;
+// The records of a unit's parts into its rows: out = sum_k 2^(ref_k - M) O_k / sum_k 2^(ref_k - M) l_k. A thread
+// takes four dims of a row; where there are few rows, groups of threads take every
+// `groups`-th part and meet in LDS in order. What it takes is the records' latency,
+// so as few rounds of loads as the registers allow.
+template <int D, int ROWS, typename U>
+__device__ __forceinline__ void join_parts(const U& u, int n_rows, lds_t* lds) {
+  constexpr int kInFlight = 8, THREADS = kTreeWaves * kWave;
   typedef Record<D, ROWS> R;
-  // unit i: four dims of a row, in the records' order
-  const int tid = threadIdx.x, units = (ROWS > 32 ? (n_rows + 31) / 32 * 32 : n_rows) * (D / 4);
-  auto row_of = [](int i) __attribute__((always_inline)) { return ROWS > 32 ? i / (8 * D) * 32 + i % 32 : i / (D / 4); };
-  auto dim_of = [](int i) __attribute__((always_inline)) { return ROWS > 32 ? 4 * (i / 32 % (D / 4)) : 4 * (i % (D / 4)); };
-  const rsrc_t recs = make_rsrc(rec, (unsigned)(2 * n - 1) * R::BYTES);
+  const int tid = threadIdx.x, units = n_rows * (D / 4);
+  const int n = u.parts;
+  const rsrc_t recs = make_rsrc(u.first_record(), (unsigned)(2 * n - 1) * R::BYTES);
   int groups = 1;
   while (units * groups * 2 <= THREADS) groups *= 2;
   const int span = THREADS / groups, grp = tid / span;
   auto finish = [&](int i, f32x4 acc, float m, float l) __attribute__((always_inline)) {
-    const int r = row_of(i), d = dim_of(i), token = (u.row0 + r) / u.n_rep;
-    if (r >= n_rows) return;
+    const int r = i / (D / 4), d = 4 * (i % (D / 4)), token = (u.row0 + r) / u.n_rep;
     const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
     gstore(u.out_row(token, u.row0 + r - token * u.n_rep) + 4 * d, acc * inv);
   };
-  for (int i0 = tid % span; i0 < units; i0 += span * EACH) {
-    float m[EACH], l[EACH];
-    f32x4 acc[EACH];
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      m[j] = -INFINITY;
-      l[j] = 0.f;
-      acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+  for (int i = tid % span; i < units; i += span) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int k0 = grp; k0 < n; k0 += kInFlight * groups) {
-      f32x2 ml[kInFlight][EACH];
-      f32x4 o[kInFlight][EACH];
+      f32x2 ml[kInFlight];
+      f32x4 o[kInFlight];
 #pragma unroll
       for (int e = 0; e < kInFlight; ++e) {
-        const unsigned at = (unsigned)max(2 * min(k0 + e * groups, n - 1) - 1, 0) * R::BYTES;
-#pragma unroll
-        for (int j = 0; j < EACH; ++j) {
-          const int i = min(i0 + span * j, units - 1), r = row_of(i);
-          ml[e][j] = shared_load2(recs, at + R::sums_at(r));
-          o[e][j] = shared_load4(recs, at + R::piece_at(r, dim_of(i)));
-        }
+        const unsigned at = U::part_at(min(k0 + e * groups, n - 1));
+        ml[e] = shared_load2(recs, at + R::sums_at(r));
+        o[e] = shared_load4(recs, at + R::piece_at(r, d));
       }
 #pragma unroll
       for (int e = 0; e < kInFlight; ++e) {
         if (k0 + e * groups >= n) continue;
-#pragma unroll
-        for (int j = 0; j < EACH; ++j) {
-          const float mn = fmaxf(m[j], ml[e][j][0]), mu = mn == -INFINITY ? 0.f : mn;
-          const float x = fast_exp2(m[j] - mu), y = fast_exp2(ml[e][j][0] - mu);
-          acc[j] = acc[j] * x + o[e][j] * y;
-          l[j] = l[j] * x + ml[e][j][1] * y;
-          m[j] = mn;
-        }
+        const float mn = fmaxf(m, ml[e][0]), mu = mn == -INFINITY ? 0.f : mn;
+        const float x = fast_exp2(m - mu), y = fast_exp2(ml[e][0] - mu);
+        acc = acc * x + o[e] * y;
+        l = l * x + ml[e][1] * y;
+        m = mn;
       }
     }
     if (groups > 1) {  // (every thread has at most one unit)
-      lds_store<f32x4>(lds + tid * 24, acc[0]);
-      lds_store<f32x2>(lds + tid * 24 + 16, f32x2{m[0], l[0]});
+      lds_store<f32x4>(lds + tid * 24, acc);
+      lds_store<f32x2>(lds + tid * 24 + 16, f32x2{m, l});
     } else {
-#pragma unroll
-      for (int j = 0; j < EACH; ++j)
-        if (i0 + span * j < units) finish(i0 + span * j, acc[j], m[j], l[j]);
+      finish(i, acc, m, l);
     }
   }
   if (groups == 1) return;
@@ -422,8 +482,10 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (PagedCfg<D, KT, RT, WIDE>::WAVE
     per = max(per, (unsigned)p.least);
     if (!WIDE) per = (per + kTreeWaves - 1) / kTreeWaves * kTreeWaves;
   }
-  // An XCD's workgroups (every eighth) have one piece of the line.
-  const unsigned wg = blockIdx.x % 8 * (n_wg / 8) + blockIdx.x / 8;
+  // An XCD's workgroups (every eighth) have one piece of the line, all XCDs as many.
+  const unsigned busy = (total + per - 1) / per, each = (busy + 7) / 8;
+  if (blockIdx.x / 8 >= each) return;
+  const unsigned wg = blockIdx.x % 8 * each + blockIdx.x / 8;
   unsigned x = min(wg * per, total);
   const unsigned x_end = min(x + per, total);
 
@@ -474,8 +536,10 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (PagedCfg<D, KT, RT, WIDE>::WAVE
     // its first tile's place: who begins it, and how many share it
     const unsigned x0 = x - (unsigned)tile, owner = part ? x0 / per : 0u;
     const int parts = part ? (int)((x0 + (unsigned)tiles - 1) / per - owner) + 1 : 1;
-    float* const rec = part ? p.rec + (int64_t)(2 * wg + (tile == 0 ? 1 : 0)) * Record<D, ROWS>::FLOATS : nullptr;
-    const UnitRows<D, KT, ROWS> rows{p, g, s.q0, s.n_past, s.n_seen, s.n_new * p.n_rep, p.n_rep, rt * ROWS, p.scale_log2e, part, rec};
+    const int mine = part ? (int)(x / per - owner) : 0;
+    float* const rec = part ? p.rec + (int64_t)(2 * wg + (mine == 0 ? 1 : 0)) * Record<D, ROWS>::FLOATS : nullptr;
+    const UnitRows<D, KT, ROWS> rows{p, g, s.q0, s.n_past, s.n_seen, s.n_new * p.n_rep, p.n_rep, rt * ROWS, p.scale_log2e,
+                                     parts, mine, rec, p.arrived + kArrivalWords * owner, lds + C::WORK};
     if constexpr (WIDE) {
       const int lim = min(s.n_seen, max(s.n_past + min(((rt + 1) * ROWS - 1) / p.n_rep, s.n_new - 1) + 1, 0));
       ManyRows<D, KT> w(rows, first + at, tile * TK, min((tile + n) * TK, lim));
@@ -483,21 +547,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (PagedCfg<D, KT, RT, WIDE>::WAVE
     } else {
       FewRows<D, KT, ROWS> w(rows, first + at, tile, min(tile + n, (s.n_seen + TK - 1) / TK));
       tree_rows<D, KT, RT>(w, lds);
-    }
-    if (part) {
-      // Every wave's records are in memory before they are counted.
-      wait_vmem<0>();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        unsigned* const counter = p.arrived + kArrivalWords * owner;
-        const unsigned done = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if ((int)done == parts - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        lds_store<int>(lds + C::WORK, (int)done == parts - 1);
-      }
-      __syncthreads();
-      if (lds_load<int>(lds + C::WORK))
-        join_parts<D, ROWS, WIDE ? 8 : 1>(rows, p.rec + (int64_t)(2 * owner + 1) * Record<D, ROWS>::FLOATS, parts,
-                            min(ROWS, rows.rows - rows.row0), lds);
+      if (part && rows.arrive()) join_parts<D, ROWS>(rows, rows.rows, lds);
     }
     x += whole ? 1u : (unsigned)n;
     __syncthreads();  // the LDS is free for the next unit

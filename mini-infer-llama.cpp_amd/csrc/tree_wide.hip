@@ -48,6 +48,7 @@ namespace {
 template <int D, typename KT>
 struct WideWork {
   static constexpr int ELT = (int)sizeof(KT), TK = WideCfg<D, KT>::TK, NDB = D / 32, ROWS = WideCfg<D, KT>::ROWS;
+  static constexpr bool kJoins = false;
   const TreeParams& p;
   const TreeItem& it;
   int g, n_past, n_kv, row0, rows, n_rep, key_begin, key_end;

@@ -12,7 +12,8 @@
 //   Scale(w, of K, group).at(w, key0, key): 8-bit caches: a key's scale;
 //   v_row, v_scale(key); visible(token, key0): which of 32 keys a query sees;
 //   q_row, out_row(token, head of the group);
-//   is_part(): the result is one part of the rows' keys: put_sums, put_part take it.
+//   is_part(): the result is one part of the rows' keys: put_sums, put_part take it,
+//     or (kJoins) join, which every wave calls.
 #pragma once
 
 #include "tree_common.h"
@@ -495,9 +496,17 @@ __device__ __forceinline__ void tree_wide_rows(W& w, lds_t* const lds) {
   }
 
   // ---- the wave's rows ------------------------------------------------------------
-  if (!active) return;
   const float lt = sum32(l);
   constexpr float unit_o = Q8 ? kByteUnscale : 1.f;  // of the values' 2^-10
+  if constexpr (W::kJoins) {
+    if (w.is_part()) {
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) o[db] *= unit_o;
+      w.join(o, ref, lt, active, valid, token, h);
+      return;
+    }
+  }
+  if (!active) return;
   if (w.is_part()) {
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
