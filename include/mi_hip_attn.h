@@ -249,7 +249,7 @@ int mi_hip_kv_destroy(mi_hip_kv* kv);
  * position. What reads a cache as one sequence refuses it (MI_HIP_E_UNSUPPORTED):
  * the other attention entry points, mi_hip_rope_append, mi_hip_norm_rope_append,
  * mi_hip_kv_keep and mi_hip_kv_bind. No staging for host nodes; its workspace is
- * for the paged calls (parts of 34 MB at head_dim 64, 68 MB at 128). No counterpart
+ * for the paged calls (parts of 39 MB at head_dim 64, 77 MB at 128). No counterpart
  * in the reference. */
 int mi_hip_kv_create_paged(const mi_hip_kv_desc* desc, int32_t page_size, mi_hip_kv** out);
 

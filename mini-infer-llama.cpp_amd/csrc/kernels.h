@@ -175,7 +175,14 @@ struct PageTables {
 };
 hipError_t launch_page_tables(const PageTables& p, int n_cu, hipStream_t stream);
 
-// paged_attn.hip. Attention over pages (mi_hip_attn_paged).
+// paged_attn.hip. Attention over pages (mi_hip_attn_paged). A line of work, set by
+// the launcher: its records (two for each workgroup; null: no unit in parts), its
+// arrival counters, the least share of a workgroup in key tiles.
+struct PagedLine {
+  float* rec;
+  unsigned* arrived;
+  int32_t least;
+};
 struct PagedAttn {
   CacheView cache;
   const int32_t* q_off;
@@ -187,13 +194,14 @@ struct PagedAttn {
   int64_t q_s1, q_s2, o_s1, o_s2;
   int32_t n_seq, n_tokens, max_new, max_kv, page_shift, n_pages, n_rep;
   float scale_log2e;
-  float* rec;         // scratch: records of the parts; null: no unit in parts
-  unsigned* arrived;  // kArrivals counters, zero before and after
-  int32_t few_rows, least;  // set by the launcher
+  int32_t few_rows;      // set by the launcher: rows up to which a sequence is on the line `few`
+  PagedLine few, many;
 };
 // A call's key tiles are counted in 32 bits: at most kPagedMaxTiles of 32 keys.
 constexpr int64_t kPagedMaxTiles = INT32_MAX;
-hipError_t launch_paged_attn(const PagedAttn& p, int n_cu, size_t part_bytes, hipStream_t stream);
+// Scratch: parts, or null, and kArrivals counters, zero before and after.
+hipError_t launch_paged_attn(const PagedAttn& p, float* parts, size_t part_bytes, unsigned* arrived, int n_cu,
+                             hipStream_t stream);
 
 // verify.hip. Drafted tokens against the target's probabilities (mi_hip_verify_draft).
 constexpr int kVerifyMaxNodes = 1024;

@@ -3,11 +3,11 @@
 //
 // The mathematics and the products are tree.hip's: query j of a sequence sees the
 // positions up to its own, its output is sum_t p_t v_t / sum_t p_t with a running
-// reference. tree_rows.h takes sequences of few query rows per KV head, a second
-// launch of tree_wide_rows.h the others in row tiles of 128.
+// reference. Sequences of few query rows per KV head go through tree_rows.h, others
+// in row tiles of 128 through tree_wide_rows.h.
 //
 // Work. The host does not know the lengths, so every workgroup finds its share
-// itself: the key tiles of all units (sequence, KV head, row tile) form one line,
+// itself: the key tiles of all units (sequence, KV head, row tile) of a kind form one line,
 // of which workgroup w takes tiles w * per .. (w + 1) * per - 1 whatever they belong
 // to: whole units, the end of one, the start of another. So workgroups have the
 // same work however ragged the lengths are. A causal unit has the tiles that its
@@ -39,6 +39,15 @@ namespace mi {
 namespace {
 
 constexpr int kRun = 16;  // keys that share a page at least
+
+// threadIdx.x as a value of its own: what is formed from it is formed where it is
+// used, and not kept in registers across the units of a workgroup (which spill
+// for it: 1000 tokens after 1337, 28/4 heads of 128, F16 XX us, so YY).
+__device__ __forceinline__ int thread_here() {
+  int t = (int)threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
 
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
@@ -112,7 +121,7 @@ struct Pages {
       : table(reinterpret_cast<const int*>(p.table + (int64_t)seq * p.table_nb)), shift(p.page_shift), n_pages(p.n_pages),
         last(max(n_seen - 1, 0) / kRun) {}
   __device__ __forceinline__ int read(int w) const {
-    return gload<int>(table + (min(64 * w + (int)(threadIdx.x % kWave), last) * kRun >> shift));
+    return gload<int>(table + (min(64 * w + thread_here() % kWave, last) * kRun >> shift));
   }
   __device__ __forceinline__ void start(int run) {
     win = run / 64;
@@ -201,6 +210,7 @@ struct UnitRows {
     __syncthreads();
     return lds_load<int>(word) != 0;
   }
+  __device__ __forceinline__ int thread() const { return thread_here(); }
   __device__ __forceinline__ unsigned visible(int token, int key0) const {
     const int n = n_past + token - key0 + 1;
     return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
@@ -282,8 +292,8 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
   static constexpr bool kJoins = true;
   __device__ __forceinline__ void join(const floatx16 (&own)[NDB], float ref, float l, bool active, bool valid, int token, int h) const {
     typedef Record<D, Base::kRows> R;
-    const int lane = threadIdx.x % kWave, kh = lane / 32;
-    const int r = 32 * uniform((int)threadIdx.x / kWave) + lane % 32;
+    const int tid = thread_here(), lane = tid % kWave, kh = lane / 32;
+    const int r = 32 * uniform(tid / kWave) + lane % 32;
     if (active) {
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
@@ -295,16 +305,12 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
     if (!this->arrive() || !active) return;
     const int n = this->parts;
     const rsrc_t recs = make_rsrc(this->first_record(), (unsigned)(2 * n - 1) * R::BYTES);
-    float top = ref;
-    for (int k = 0; k < n; ++k)
-      if (k != this->mine) top = fmaxf(top, shared_load2(recs, Base::part_at(k) + R::sums_at(r))[0]);
-    const float mu = top == -INFINITY ? 0.f : top;
     f32x4 acc[NDB][4];
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[db][q] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
+    float top = -INFINITY, sum = 0.f;
     for (int k = 0; k < n; ++k) {
       f32x4 x[NDB][4];
       f32x2 ml = {ref, l};
@@ -320,12 +326,14 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
 #pragma unroll
           for (int q = 0; q < 4; ++q) x[db][q] = f32x4{own[db][4 * q], own[db][4 * q + 1], own[db][4 * q + 2], own[db][4 * q + 3]};
       }
-      const float y = fast_exp2(ml[0] - mu);
-      sum += ml[1] * y;
+      const float now = fmaxf(top, ml[0]), mu = now == -INFINITY ? 0.f : now;
+      const float a = fast_exp2(top - mu), b = fast_exp2(ml[0] - mu);
+      top = now;
+      sum = sum * a + ml[1] * b;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[db][q] += x[db][q] * y;
+        for (int q = 0; q < 4; ++q) acc[db][q] = acc[db][q] * a + x[db][q] * b;
     }
     if (!valid) return;
     const float inv = top == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;
@@ -383,7 +391,7 @@ template <int D, int ROWS, typename U>
 __device__ __forceinline__ void join_parts(const U& u, int n_rows, lds_t* lds) {
   constexpr int kInFlight = 8, THREADS = kTreeWaves * kWave;
   typedef Record<D, ROWS> R;
-  const int tid = threadIdx.x, units = n_rows * (D / 4);
+  const int tid = thread_here(), units = n_rows * (D / 4);
   const int n = u.parts;
   const rsrc_t recs = make_rsrc(u.first_record(), (unsigned)(2 * n - 1) * R::BYTES);
   int groups = 1;
@@ -442,25 +450,23 @@ __device__ __forceinline__ void join_parts(const U& u, int n_rows, lds_t* lds) {
 
 }  // namespace
 
-// WIDE: sequences of more than p.few_rows query rows per KV head, in row tiles of
-// 128; otherwise those of up to that many (at most 16 RT), in one.
+// A line of units: sequences of more than few_rows query rows per KV head in row
+// tiles of 128 (WIDE), or those of up to that many (at most 16 RT) in one.
 template <int D, typename KT, int RT, bool WIDE>
-struct PagedCfg {
+struct LineCfg {
   static constexpr int ROWS = WIDE ? WideCfg<D, KT>::ROWS : 16 * RT, TK = WIDE ? WideCfg<D, KT>::TK : kTreeTile;
-  static constexpr int WORK = WIDE ? WideCfg<D, KT>::LDS : TreeCfg<D, KT, RT>::LDS;
-  static constexpr int LDS = WORK + 16;  // and a word for who joins
+  static constexpr int LDS = WIDE ? WideCfg<D, KT>::LDS : TreeCfg<D, KT, RT>::LDS;
   static constexpr int WAVES_PER_SIMD = WIDE ? WideCfg<D, KT>::WAVES_PER_SIMD : TreeCfg<D, KT, RT>::WAVES_PER_SIMD;
 };
 
+// This workgroup's share of a line.
 template <int D, typename KT, int RT, bool WIDE>
-__global__ __launch_bounds__(kTreeWaves* kWave, (PagedCfg<D, KT, RT, WIDE>::WAVES_PER_SIMD)) void paged_attn_kernel(const PagedAttn p) {
-  typedef PagedCfg<D, KT, RT, WIDE> C;
+__device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& line, lds_t* const lds, lds_t* const word) {
+  typedef LineCfg<D, KT, RT, WIDE> C;
   typedef Units<C::ROWS, C::TK> U;
   constexpr int ROWS = C::ROWS, TK = C::TK;
-  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
-  lds_t* const lds = (lds_t*)lds_raw;
-  const int lane = threadIdx.x % kWave;
-  const bool whole = p.rec == nullptr;  // no records: no unit in parts
+  const int lane = thread_here() % kWave;
+  const bool whole = line.rec == nullptr;  // no records: no unit in parts
   auto units_of = [&](const SeqLens& s) __attribute__((always_inline)) -> unsigned {
     const int rows = s.n_new * p.n_rep;
     if (rows == 0 || WIDE != (rows > p.few_rows)) return 0u;
@@ -479,7 +485,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (PagedCfg<D, KT, RT, WIDE>::WAVE
   const unsigned n_wg = gridDim.x;
   unsigned per = (total + n_wg - 1) / n_wg;
   if (!whole) {
-    per = max(per, (unsigned)p.least);
+    per = max(per, (unsigned)line.least);
     if (!WIDE) per = (per + kTreeWaves - 1) / kTreeWaves * kTreeWaves;
   }
   // An XCD's workgroups (every eighth) have one piece of the line, all XCDs as many.
@@ -537,9 +543,9 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (PagedCfg<D, KT, RT, WIDE>::WAVE
     const unsigned x0 = x - (unsigned)tile, owner = part ? x0 / per : 0u;
     const int parts = part ? (int)((x0 + (unsigned)tiles - 1) / per - owner) + 1 : 1;
     const int mine = part ? (int)(x / per - owner) : 0;
-    float* const rec = part ? p.rec + (int64_t)(2 * wg + (mine == 0 ? 1 : 0)) * Record<D, ROWS>::FLOATS : nullptr;
+    float* const rec = part ? line.rec + (int64_t)(2 * wg + (mine == 0 ? 1 : 0)) * Record<D, ROWS>::FLOATS : nullptr;
     const UnitRows<D, KT, ROWS> rows{p, g, s.q0, s.n_past, s.n_seen, s.n_new * p.n_rep, p.n_rep, rt * ROWS, p.scale_log2e,
-                                     parts, mine, rec, p.arrived + kArrivalWords * owner, lds + C::WORK};
+                                     parts, mine, rec, line.arrived + kArrivalWords * owner, word};
     if constexpr (WIDE) {
       const int lim = min(s.n_seen, max(s.n_past + min(((rt + 1) * ROWS - 1) / p.n_rep, s.n_new - 1) + 1, 0));
       ManyRows<D, KT> w(rows, first + at, tile * TK, min((tile + n) * TK, lim));
@@ -554,59 +560,98 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (PagedCfg<D, KT, RT, WIDE>::WAVE
   }
 }
 
-template <int D, typename KT, int RT, bool WIDE>
-static hipError_t launch_paged_t(const PagedAttn& p, int n_wg, hipStream_t stream) {
-  typedef PagedCfg<D, KT, RT, WIDE> C;
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attn_kernel<D, KT, RT, WIDE>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
-  if (attr != hipSuccess) return attr;
-  hipLaunchKernelGGL((paged_attn_kernel<D, KT, RT, WIDE>), dim3((unsigned)n_wg), dim3(kTreeWaves * kWave), C::LDS, stream, p);
+// Few rows in every sequence.
+template <int D, typename KT, int RT>
+__global__ __launch_bounds__(kTreeWaves* kWave, (TreeCfg<D, KT, RT>::WAVES_PER_SIMD)) void paged_few_kernel(const PagedAttn p) {
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  lds_t* const lds = (lds_t*)lds_raw;
+  run_line<D, KT, RT, false>(p, p.few, lds, lds + TreeCfg<D, KT, RT>::LDS);
+}
+
+// Sequences of any number of rows: up to 16 on one line, more on another. A
+// workgroup has a share of both; the first half of the workgroups begins with the one,
+// the second with the other, so that a CU that holds one of each has keys to
+// stream, which memory bounds, beside products (1000 tokens after 1337 among 31
+// single tokens over 2667 to 4000 keys, 28/4 heads of 128, F16: XX us, in two launches
+// 144).
+template <int D, typename KT>
+struct MixedCfg {
+  typedef LineCfg<D, KT, 1, false> Few;
+  typedef LineCfg<D, KT, 1, true> Many;
+  static constexpr int LDS = Few::LDS > Many::LDS ? Few::LDS : Many::LDS;
+};
+template <int D, typename KT>
+__global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)) void paged_mixed_kernel(const PagedAttn p) {
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  lds_t* const lds = (lds_t*)lds_raw;
+  lds_t* const word = lds + MixedCfg<D, KT>::LDS;
+  const bool few_first = 2 * blockIdx.x < gridDim.x;
+#pragma unroll 1
+  for (int turn = 0; turn < 2; ++turn) {
+    if ((turn == 0) == few_first) run_line<D, KT, 1, false>(p, p.few, lds, word);
+    else run_line<D, KT, 1, true>(p, p.many, lds, word);
+  }
+}
+
+template <typename K>
+static hipError_t launch_kernel(K kernel, const PagedAttn& p, int n_wg, int lds, hipStream_t stream) {
+  hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(kTreeWaves * kWave), lds, stream, p);
   return hipGetLastError();
+}
+template <int D, typename KT, int RT>
+static hipError_t launch_few(const PagedAttn& p, int n_wg, hipStream_t stream) {
+  constexpr int lds = TreeCfg<D, KT, RT>::LDS + 16;
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_few_kernel<D, KT, RT>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  return attr != hipSuccess ? attr : launch_kernel(paged_few_kernel<D, KT, RT>, p, n_wg, lds, stream);
+}
+template <int D, typename KT>
+static hipError_t launch_mixed(const PagedAttn& p, int n_wg, hipStream_t stream) {
+  constexpr int lds = MixedCfg<D, KT>::LDS + 16;
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_mixed_kernel<D, KT>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  return attr != hipSuccess ? attr : launch_kernel(paged_mixed_kernel<D, KT>, p, n_wg, lds, stream);
+}
+
+// Workgroups: what the CUs hold at once, as far as there are arrival counters (one
+// for each and line) and records (two), a multiple of the XCDs.
+static int workgroups(int64_t n, int64_t counters, size_t part_bytes, size_t record_bytes) {
+  return (int)(std::min({n, counters, (int64_t)(part_bytes / (2 * record_bytes))}) / 8 * 8);
 }
 
 template <int D, typename KT>
-static hipError_t launch_paged(PagedAttn p, int n_cu, size_t part_bytes, hipStream_t stream) {
-  // Most query rows per KV head that a sequence can have decide what is launched:
-  // up to 16 or 32 rows the kernel that streams keys to registers, alone; above, it
-  // takes the sequences of up to 16, the wide kernel the rest.
+static hipError_t launch_paged(PagedAttn p, float* parts, size_t part_bytes, unsigned* arrived, int n_cu, hipStream_t stream) {
+  // Most query rows per KV head that a sequence can have decide what is launched.
   const int64_t most = (int64_t)std::min(p.max_new, p.n_tokens) * p.n_rep;
-  const bool two = most > 16 && most <= 32, wide = most > 32;
+  const bool mixed = most > 32, two = !mixed && most > 16;
   p.few_rows = two ? 32 : 16;
-  // Workgroups: what the CUs hold at once, each with room for two records, and an
-  // arrival counter, a multiple of the XCDs.
-  auto grid = [&](int per_cu, int rows) {
-    int64_t n = (int64_t)n_cu * per_cu;
-    if (p.rec) n = std::min({n, (int64_t)kArrivals, (int64_t)(part_bytes / (2 * sizeof(float) * rows * (D + 2)))});
-    return (int)(n / 8 * 8);
-  };
-  constexpr bool F32 = sizeof(KT) == 4;
-  hipError_t e = hipSuccess;
-  int n_wg = grid(two ? (D == 64 ? 2 : 1) : (D == 64 ? 3 : 2), two ? 32 : 16);
-  p.least = 8;
-  PagedAttn q = p;
-  if (n_wg == 0) {  // no room for records
-    q.rec = nullptr;
-    n_wg = n_cu / 8 * 8;
+  p.few.least = 8;
+  p.many.least = D == 64 ? 2 : 4;
+  p.few.arrived = arrived;
+  p.many.arrived = arrived + kArrivalWords * (kArrivals / 2);
+  p.few.rec = p.many.rec = nullptr;
+  const size_t few_bytes = (two ? 32 : 16) * (D + 2) * sizeof(float), many_bytes = 128 * (D + 2) * sizeof(float);
+  const int per_cu = mixed ? WideCfg<D, KT>::WAVES_PER_SIMD : two ? (D == 64 ? 2 : 1) : (D == 64 ? 3 : 2);
+  int n_wg = workgroups((int64_t)n_cu * per_cu, mixed ? kArrivals / 2 : kArrivals, parts ? part_bytes : 0,
+                        few_bytes + (mixed ? many_bytes : 0));
+  if (n_wg > 0) {
+    p.many.rec = parts;
+    p.few.rec = mixed ? parts + (size_t)2 * n_wg * many_bytes / sizeof(float) : parts;
+  } else {  // no room for records: no unit in parts
+    n_wg = n_cu * per_cu / 8 * 8;
   }
-  e = two ? launch_paged_t<D, KT, 2, false>(q, n_wg, stream) : launch_paged_t<D, KT, 1, false>(q, n_wg, stream);
-  if (e != hipSuccess || !wide) return e;
-  n_wg = grid(F32 && D == 128 ? 1 : 2, 128);
-  p.least = D == 64 ? 2 : 4;
-  if (n_wg == 0) {
-    p.rec = nullptr;
-    n_wg = n_cu / 8 * 8;
-  }
-  return launch_paged_t<D, KT, 1, true>(p, n_wg, stream);
+  if (mixed) return launch_mixed<D, KT>(p, n_wg, stream);
+  return two ? launch_few<D, KT, 2>(p, n_wg, stream) : launch_few<D, KT, 1>(p, n_wg, stream);
 }
 
-hipError_t launch_paged_attn(const PagedAttn& p, int n_cu, size_t part_bytes, hipStream_t stream) {
+hipError_t launch_paged_attn(const PagedAttn& p, float* parts, size_t part_bytes, unsigned* arrived, int n_cu, hipStream_t stream) {
   if (p.cache.head_dim == 64)
-    return p.cache.elt == 1   ? launch_paged<64, int8_t>(p, n_cu, part_bytes, stream)
-           : p.cache.elt == 2 ? launch_paged<64, _Float16>(p, n_cu, part_bytes, stream)
-                              : launch_paged<64, float>(p, n_cu, part_bytes, stream);
-  return p.cache.elt == 1   ? launch_paged<128, int8_t>(p, n_cu, part_bytes, stream)
-         : p.cache.elt == 2 ? launch_paged<128, _Float16>(p, n_cu, part_bytes, stream)
-                            : launch_paged<128, float>(p, n_cu, part_bytes, stream);
+    return p.cache.elt == 1   ? launch_paged<64, int8_t>(p, parts, part_bytes, arrived, n_cu, stream)
+           : p.cache.elt == 2 ? launch_paged<64, _Float16>(p, parts, part_bytes, arrived, n_cu, stream)
+                              : launch_paged<64, float>(p, parts, part_bytes, arrived, n_cu, stream);
+  return p.cache.elt == 1   ? launch_paged<128, int8_t>(p, parts, part_bytes, arrived, n_cu, stream)
+         : p.cache.elt == 2 ? launch_paged<128, _Float16>(p, parts, part_bytes, arrived, n_cu, stream)
+                            : launch_paged<128, float>(p, parts, part_bytes, arrived, n_cu, stream);
 }
 
 }  // namespace mi

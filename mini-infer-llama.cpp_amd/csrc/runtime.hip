@@ -1404,7 +1404,9 @@ static int kv_make(const mi_hip_kv_desc* d, int32_t page_size, mi_hip_kv** out) 
   int groups = 1;  // (no decode launch of mi_hip_attn_fwd uses a paged cache's)
   size_t rec_bytes = 0;
   if (!page_size) ws_capacity(d->n_head_kv, d->n_head / d->n_head_kv, d->head_dim, &groups, &rec_bytes);
-  if ((rc = ws_create(groups, rec_bytes, (page_size ? 2 : 1) * ws_part_bytes(d->head_dim), &kv->ws))) {
+  // (paged: two records of 128 rows and two of 16 for each of two workgroups per CU)
+  const size_t part_bytes = ws_part_bytes(d->head_dim);
+  if ((rc = ws_create(groups, rec_bytes, page_size ? part_bytes * 9 / 4 : part_bytes, &kv->ws))) {
     (void)hipStreamDestroy(kv->stream);
     dev_free(kv->stage, kv->stage_bytes);
     dev_free(kv->base, kv->bytes);
@@ -2074,8 +2076,6 @@ int mi_hip_attn_paged(const mi_hip_attn_paged_args* a) {
   if ((rc = bind_device())) return rc;
   mi_hip_workspace* const ws = a->ws ? a->ws : kv->ws;
   mi::PagedAttn p{};
-  p.rec = reinterpret_cast<float*>(ws->part);
-  p.arrived = ws->arrived;
   p.cache = kv->view(a->layer);
   p.q_off = a->q_off;
   p.n_kv = a->n_kv;
@@ -2095,7 +2095,8 @@ int mi_hip_attn_paged(const mi_hip_attn_paged_args* a) {
   p.n_pages = kv->d.n_ctx / kv->page_size;
   p.n_rep = a->n_head / kv->d.n_head_kv;
   p.scale_log2e = a->scale * kLog2e;
-  hipError_t e = mi::launch_paged_attn(p, g.n_cu, ws->part_bytes, static_cast<hipStream_t>(a->stream));
+  hipError_t e = mi::launch_paged_attn(p, reinterpret_cast<float*>(ws->part), ws->part_bytes, ws->arrived, g.n_cu,
+                                       static_cast<hipStream_t>(a->stream));
   return e == hipSuccess ? MI_HIP_OK : hip_fail(e, "paged attention launch");
 }
 

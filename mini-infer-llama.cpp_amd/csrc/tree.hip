@@ -80,6 +80,7 @@ struct TreeWork {
   const char* vbase;
   float* rec;
 
+  __device__ __forceinline__ int thread() const { return (int)threadIdx.x; }
   __device__ __forceinline__ void at_tile(int) {}
   __device__ __forceinline__ unsigned none() const { return 0u; }
   // The descriptors start at the tile's first row (64-bit), so a cache of any

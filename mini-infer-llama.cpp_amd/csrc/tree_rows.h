@@ -4,6 +4,7 @@
 //
 // What the rows and keys are is W's matter (TreeWork of tree.hip: a run of cache
 // rows; paged_attn.hip: pages):
+//   thread(): threadIdx.x;
 //   n_past, rows, n_rep, scale_log2e, k_s2, v_s2 (bytes between rows), tile0, tile1
 //   at_tile(tile): the tile whose rows are loaded next;
 //   k_rows(key0), v_rows(key0): descriptors of its two times 16 rows, which read
@@ -88,8 +89,8 @@ __device__ __forceinline__ void tree_rows(W& w, lds_t* const lds) {
   typedef TreeCfg<D, KT, RT> C;
   constexpr int NB = C::NB, NE = C::NE, ROWS = C::ROWS, ELT = C::ELT, KB = C::KB, KW = C::KW, VW = C::VW;
   constexpr bool Q8 = C::Q8, F32 = C::F32;
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int tid = w.thread(), lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int c = lane & 15, q4 = lane >> 4;
 
   // ---- loads of a key tile --------------------------------------------------
@@ -504,7 +505,7 @@ __device__ __forceinline__ void tree_rows(W& w, lds_t* const lds) {
   // thread: four dims of a row
 #pragma unroll
   for (int e = 0; e < ROWS * D / 4; e += kTreeWaves * kWave) {
-    const int idx = e + threadIdx.x, r = idx / (D / 4), d = 4 * (idx % (D / 4));
+    const int idx = e + tid, r = idx / (D / 4), d = 4 * (idx % (D / 4));
     if (r >= w.rows) continue;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll

@@ -57,6 +57,7 @@ struct WideWork {
   const char* vbase;
   float* rec;
 
+  __device__ __forceinline__ int thread() const { return (int)threadIdx.x; }
   __device__ __forceinline__ void at_tile(int) {}
   __device__ __forceinline__ unsigned none() const { return 0u; }
   // The descriptor starts at the tile's first row and ends after its last valid one.

@@ -3,6 +3,7 @@
 //
 // What the rows and keys are is W's matter (WideWork of tree_wide.hip: a run of
 // cache rows; paged_attn.hip: pages):
+//   thread(): threadIdx.x;
 //   n_past, n_kv, row0, rows, n_rep, scale_log2e, key_begin, key_end (whole tiles
 //     but for the last);
 //   at_tile(key0): the tile that is fetched next; none(): of the tile fetched
@@ -93,7 +94,7 @@ __device__ __forceinline__ void tree_wide_rows(W& w, lds_t* const lds) {
   constexpr int PL = C::PL, PLANE = C::PLANE;
   constexpr bool Q8 = C::Q8, F32 = C::F32;
   constexpr int THREADS = kTreeWaves * kWave;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int tid = w.thread(), lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int c = lane & 31, kh = lane >> 5;
 
