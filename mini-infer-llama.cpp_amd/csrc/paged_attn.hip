@@ -145,6 +145,10 @@ struct Pages {
       slot[i] = ((ok ? page : 0) << shift) + ((run + i) * kRun & ((1 << shift) - 1));
     }
   }
+  __device__ __forceinline__ int slot_of(int i) const {
+    const int a = slot[0], b = slot[1], c = slot[RUNS - 2], d = slot[RUNS - 1];  // (values: not a choice of addresses)
+    return i < RUNS - 2 ? (i == 0 ? a : b) : (i == RUNS - 2 ? c : d);
+  }
   // Any key's row, -1 if it has none.
   __device__ __forceinline__ int row(int key) const {
     const int page = gload<int>(table + (min(key / kRun, last) * kRun >> shift));
@@ -264,7 +268,7 @@ struct FewRows : UnitRows<D, KT, ROWS> {
   template <int NB>
   __device__ __forceinline__ void scales(int, int c32, int half, unsigned& ksc, unsigned& vsc) const {
     const CacheView& c = this->p.cache;
-    const int64_t at = (int64_t)((c32 < kRun ? pages.slot[0] : pages.slot[1]) + c32 % kRun) * c.n_head_kv + this->g;
+    const int64_t at = (int64_t)(pages.slot_of(c32 / kRun) + c32 % kRun) * c.n_head_kv + this->g;
     if constexpr (NB == 4) ksc = gload<unsigned>(c.scale[0] + at * 8 + 4 * half);
     else ksc = gload<unsigned short>(c.scale[0] + at * 4 + 2 * half);
     vsc = gload<unsigned short>(c.scale[1] + at * 2);
@@ -351,9 +355,7 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
     __device__ __forceinline__ Rows(const ManyRows& u, int which, int key)
         : w(u), base(which == 0 ? u.kbase : u.vbase), s2((int)u.p.cache.s2), key0(key) {}
     __device__ __forceinline__ rsrc_t rows(int run) const {
-      int slot = w.pages.slot[0];
-#pragma unroll
-      for (int i = 1; i < RUNS; ++i) slot = run == i ? w.pages.slot[i] : slot;
+      const int slot = w.pages.slot_of(run);
       const int n = w.pages.none >> run & 1u ? 0 : min(w.n_kv - key0 - kRun * run, kRun);
       return make_rsrc(base + (int64_t)slot * s2, n > 0 ? (unsigned)((n - 1) * s2 + D * ELT) : 0u);
     }
@@ -368,9 +370,7 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
     }
     // (every row of a page is there)
     __device__ __forceinline__ const char* at(const ManyRows& w, int, int key) const {
-      int slot = w.pages.slot[0];
-#pragma unroll
-      for (int i = 1; i < RUNS; ++i) slot = key / kRun == i ? w.pages.slot[i] : slot;
+      const int slot = w.pages.slot_of(key / kRun);
       return src + (int64_t)(slot + key % kRun) * (w.p.cache.n_head_kv * 2 * n);
     }
   };
