@@ -182,6 +182,7 @@ struct PagedLine {
   float* rec;
   unsigned* arrived;
   int32_t least;
+  float join;  // what joining a part takes, in key tiles' time
 };
 struct PagedAttn {
   CacheView cache;

@@ -102,10 +102,13 @@ struct Units {
     const int last = min(((rt + 1) * ROWS - 1) / n_rep, n_new - 1);
     return (max(min(n_past + last + 1, n_seen), 1) + TK - 1) / TK;
   }
-  __device__ inline unsigned per_head(bool whole) const {
+  // Places of a head's units on the line: whole units, or their tiles; pairs and the
+  // middle row tile in multiples of `pad`, so that no share of that size holds two.
+  __device__ inline unsigned per_head(bool whole, unsigned pad) const {
     if (whole) return (unsigned)n_rt;
-    return (unsigned)(n_rt / 2) * pair + (n_rt & 1 ? (unsigned)tiles(n_rt / 2) : 0u);
+    return (unsigned)(n_rt / 2) * padded(pair, pad) + (n_rt & 1 ? padded((unsigned)tiles(n_rt / 2), pad) : 0u);
   }
+  static __device__ inline unsigned padded(unsigned x, unsigned pad) { return pad > 1u ? (x + pad - 1u) / pad * pad : x; }
 };
 
 // The pages of a sequence, as a wave reads them: RUNS runs of 16 keys per tile.
@@ -291,8 +294,8 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
     pages.start(key_begin / kRun);
   }
   __device__ __forceinline__ void at_tile(int key0) { pages.at(key0 / kRun); }
-  // The last part to arrive adds up all of them in their order, its own from where
-  // it lies: a wave its 32 rows, lanes as the products left them.
+  // The last part to arrive adds up all of them in their order: a wave its 32 rows,
+  // lanes as the products left them, kInFlight parts on their way at once.
   static constexpr bool kJoins = true;
   __device__ __forceinline__ void join(const floatx16 (&own)[NDB], float ref, float l, bool active, bool valid, int token, int h) const {
     typedef Record<D, Base::kRows> R;
@@ -309,35 +312,37 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
     if (!this->arrive() || !active) return;
     const int n = this->parts;
     const rsrc_t recs = make_rsrc(this->first_record(), (unsigned)(2 * n - 1) * R::BYTES);
+    constexpr int kInFlight = D == 64 ? 4 : 2;
     f32x4 acc[NDB][4];
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[db][q] = f32x4{0.f, 0.f, 0.f, 0.f};
     float top = -INFINITY, sum = 0.f;
-    for (int k = 0; k < n; ++k) {
-      f32x4 x[NDB][4];
-      f32x2 ml = {ref, l};
-      if (k != this->mine) {
-        ml = shared_load2(recs, Base::part_at(k) + R::sums_at(r));
+    for (int k0 = 0; k0 < n; k0 += kInFlight) {
+      f32x4 x[kInFlight][NDB][4];
+      f32x2 ml[kInFlight];
+#pragma unroll
+      for (int e = 0; e < kInFlight; ++e) {
+        const unsigned at = Base::part_at(min(k0 + e, n - 1));
+        ml[e] = shared_load2(recs, at + R::sums_at(r));
 #pragma unroll
         for (int db = 0; db < NDB; ++db)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) x[db][q] = shared_load4(recs, Base::part_at(k) + R::piece_at(r, 32 * db + 8 * q + 4 * kh));
-      } else {
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) x[db][q] = f32x4{own[db][4 * q], own[db][4 * q + 1], own[db][4 * q + 2], own[db][4 * q + 3]};
+          for (int q = 0; q < 4; ++q) x[e][db][q] = shared_load4(recs, at + R::piece_at(r, 32 * db + 8 * q + 4 * kh));
       }
-      const float now = fmaxf(top, ml[0]), mu = now == -INFINITY ? 0.f : now;
-      const float a = fast_exp2(top - mu), b = fast_exp2(ml[0] - mu);
-      top = now;
-      sum = sum * a + ml[1] * b;
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
+      for (int e = 0; e < kInFlight; ++e) {
+        if (k0 + e >= n) continue;
+        const float now = fmaxf(top, ml[e][0]), mu = now == -INFINITY ? 0.f : now;
+        const float a = fast_exp2(top - mu), b = fast_exp2(ml[e][0] - mu);
+        top = now;
+        sum = sum * a + ml[e][1] * b;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[db][q] = acc[db][q] * a + x[db][q] * b;
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[db][q] = acc[db][q] * a + x[e][db][q] * b;
+      }
     }
     if (!valid) return;
     const float inv = top == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;
@@ -459,34 +464,69 @@ struct LineCfg {
   static constexpr int WAVES_PER_SIMD = WIDE ? WideCfg<D, KT>::WAVES_PER_SIMD : TreeCfg<D, KT, RT>::WAVES_PER_SIMD;
 };
 
+// LDS behind the kernels': each wave's sequences at hand, and a word for who joins.
+constexpr int kState = kTreeWaves * 5 * 4 * kWave + 16;
+
 // This workgroup's share of a line.
 template <int D, typename KT, int RT, bool WIDE>
-__device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& line, lds_t* const lds, lds_t* const word) {
+__device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& line, lds_t* const lds, lds_t* const state) {
   typedef LineCfg<D, KT, RT, WIDE> C;
   typedef Units<C::ROWS, C::TK> U;
   constexpr int ROWS = C::ROWS, TK = C::TK;
-  const int lane = thread_here() % kWave;
   const bool whole = line.rec == nullptr;  // no records: no unit in parts
+  unsigned pad = 1u;
   auto units_of = [&](const SeqLens& s) __attribute__((always_inline)) -> unsigned {
     const int rows = s.n_new * p.n_rep;
     if (rows == 0 || WIDE != (rows > p.few_rows)) return 0u;
-    return U(s, p.n_rep).per_head(whole) * (unsigned)p.cache.n_head_kv;
+    return U(s, p.n_rep).per_head(whole, pad) * (unsigned)p.cache.n_head_kv;
   };
 
   // ---- the line: lane i has sequence `first` + i ------------------------------------
+  // Lengths and running sums are kept in LDS, by each wave its own: while a unit is
+  // worked on, the registers are its own.
+  lds_t* const kept_at = state + uniform(thread_here() / kWave) * (5 * 4 * kWave);
   int first = 0;
   unsigned before = 0u;  // units of the sequences before
-  SeqLens lens = seq_lens(p, lane);
-  unsigned end = wave_scan(units_of(lens));
-  unsigned total = (unsigned)__builtin_amdgcn_readlane((int)end, 63);
-  for (int i = kWave; i < p.n_seq; i += kWave)
-    total += (unsigned)__builtin_amdgcn_readlane((int)wave_scan(units_of(seq_lens(p, i + lane))), 63);
-  // Shares: the same for every workgroup, `least` at least, whole rounds of the waves.
+  auto keep = [&](int lane, const SeqLens& s, unsigned end) __attribute__((always_inline)) {
+    const int x[5] = {s.q0, s.n_new, s.n_past, s.n_seen, (int)end};
+#pragma unroll
+    for (int j = 0; j < 5; ++j) lds_store<int>(kept_at + 4 * (kWave * j + lane), x[j]);
+  };
+  unsigned total = 0u;
+  int longest = 0;  // keys, about
+  auto add_up = [&]() __attribute__((always_inline)) {
+    total = 0u;
+    for (int i = (p.n_seq - 1) / kWave * kWave; i >= 0; i -= kWave) {  // (the first 64 last: they stay)
+      const int lane = thread_here() % kWave;
+      const SeqLens s = seq_lens(p, i + lane);
+      const unsigned units = units_of(s), end = wave_scan(units);
+      total += (unsigned)__builtin_amdgcn_readlane((int)end, 63);
+      longest = max(longest, units > 0u ? s.n_seen : 0);
+      if (i == 0) keep(lane, s, end);
+    }
+  };
+  add_up();
+  // Shares: the same for every workgroup, few rows in whole rounds of the waves.
   const unsigned n_wg = gridDim.x;
-  unsigned per = (total + n_wg - 1) / n_wg;
+  unsigned per = max((total + n_wg - 1) / n_wg, 1u);
   if (!whole) {
-    per = max(per, (unsigned)line.least);
-    if (!WIDE) per = (per + kTreeWaves - 1) / kTreeWaves * kTreeWaves;
+    // A unit's parts are joined some at a time, so a long one takes per + (tiles /
+    // per) `join` tiles' time, the least for per = sqrt(tiles join).
+    const float tiles = wave_max((float)longest) * (1.f / TK);
+    unsigned want = (unsigned)uniform((int)fminf(fmaxf((float)line.least, sqrtf(tiles * line.join)), ceilf(tiles)));
+    if (!WIDE) {
+      per = (per + kTreeWaves - 1) / kTreeWaves * kTreeWaves;
+      want = (want + kTreeWaves - 1) / kTreeWaves * kTreeWaves;
+    }
+    if (want > per) {
+      // Fewer workgroups than there are: as long as they are enough, none has two units.
+      per = pad = want;
+      add_up();
+      if ((total + per - 1) / per > n_wg) {
+        pad = 1u;
+        add_up();
+      }
+    }
   }
   // An XCD's workgroups (every eighth) have one piece of the line, all XCDs as many.
   const unsigned busy = (total + per - 1) / per, each = (busy + 7) / 8;
@@ -496,19 +536,24 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
   const unsigned x_end = min(x + per, total);
 
   while (x < x_end) {
+    wave_lds_fence();
+    const int lane = thread_here() % kWave;
+    unsigned end = (unsigned)lds_load<int>(kept_at + 4 * (kWave * 4 + lane));
     for (;;) {
       const unsigned all = (unsigned)__builtin_amdgcn_readlane((int)end, 63);
       if (x < before + all) break;
       before += all;
       first += kWave;
-      lens = seq_lens(p, first + lane);
-      end = wave_scan(units_of(lens));
+      const SeqLens s = seq_lens(p, first + lane);
+      end = wave_scan(units_of(s));
+      keep(lane, s, end);
+      wave_lds_fence();
     }
     const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(end > x - before));
-    const SeqLens s{__builtin_amdgcn_readlane(lens.q0, at), __builtin_amdgcn_readlane(lens.n_new, at),
-                    __builtin_amdgcn_readlane(lens.n_past, at), __builtin_amdgcn_readlane(lens.n_seen, at)};
+    auto kept = [&](int j) __attribute__((always_inline)) { return uniform(lds_load<int>(kept_at + 4 * (kWave * j + at))); };
+    const SeqLens s{kept(0), kept(1), kept(2), kept(3)};
     const U u(s, p.n_rep);
-    const unsigned per_head = u.per_head(whole), seq_end = (unsigned)__builtin_amdgcn_readlane((int)end, at);
+    const unsigned per_head = u.per_head(whole, pad), seq_end = (unsigned)__builtin_amdgcn_readlane((int)end, at);
     const unsigned y = x - before - (seq_end - per_head * (unsigned)p.cache.n_head_kv);
     const int g = uniform((int)(y / per_head));
     unsigned off = y - (unsigned)g * per_head;  // place in the head's units
@@ -518,11 +563,15 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
       tiles = u.tiles(rt);
       tile = 0;
     } else {
-      const unsigned pairs = (unsigned)(u.n_rt / 2), j = min(off / u.pair, pairs);
-      off -= j * u.pair;
-      const unsigned left = u.pair - off;  // of the pair
+      const unsigned pairs = (unsigned)(u.n_rt / 2), pair = U::padded(u.pair, pad), j = min(off / pair, pairs);
+      off -= j * pair;
+      const unsigned left = pair - off;  // of the pair
       rt = u.n_rt - 1 - (int)j;  // (the middle one, where it is alone, is both)
       tiles = u.tiles(rt);
+      if (j == pairs && off >= (unsigned)tiles) {  // the empty ones behind the middle one
+        x += U::padded((unsigned)tiles, pad) - off;
+        continue;
+      }
       if (j < pairs && off >= (unsigned)tiles) {
         off -= (unsigned)tiles;
         rt = (int)j;
@@ -545,7 +594,7 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
     const int mine = part ? (int)(x / per - owner) : 0;
     float* const rec = part ? line.rec + (int64_t)(2 * wg + (mine == 0 ? 1 : 0)) * Record<D, ROWS>::FLOATS : nullptr;
     const UnitRows<D, KT, ROWS> rows{p, g, s.q0, s.n_past, s.n_seen, s.n_new * p.n_rep, p.n_rep, rt * ROWS, p.scale_log2e,
-                                     parts, mine, rec, line.arrived + kArrivalWords * owner, word};
+                                     parts, mine, rec, line.arrived + kArrivalWords * owner, state + kState - 16};
     if constexpr (WIDE) {
       const int lim = min(s.n_seen, max(s.n_past + min(((rt + 1) * ROWS - 1) / p.n_rep, s.n_new - 1) + 1, 0));
       ManyRows<D, KT> w(rows, first + at, tile * TK, min((tile + n) * TK, lim));
@@ -584,12 +633,12 @@ template <int D, typename KT>
 __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)) void paged_mixed_kernel(const PagedAttn p) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   lds_t* const lds = (lds_t*)lds_raw;
-  lds_t* const word = lds + MixedCfg<D, KT>::LDS;
+  lds_t* const state = lds + MixedCfg<D, KT>::LDS;
   const bool few_first = 2 * blockIdx.x < gridDim.x;
 #pragma unroll 1
   for (int turn = 0; turn < 2; ++turn) {
-    if ((turn == 0) == few_first) run_line<D, KT, 1, false>(p, p.few, lds, word);
-    else run_line<D, KT, 1, true>(p, p.many, lds, word);
+    if ((turn == 0) == few_first) run_line<D, KT, 1, false>(p, p.few, lds, state);
+    else run_line<D, KT, 1, true>(p, p.many, lds, state);
   }
 }
 
@@ -600,14 +649,14 @@ static hipError_t launch_kernel(K kernel, const PagedAttn& p, int n_wg, int lds,
 }
 template <int D, typename KT, int RT>
 static hipError_t launch_few(const PagedAttn& p, int n_wg, hipStream_t stream) {
-  constexpr int lds = TreeCfg<D, KT, RT>::LDS + 16;
+  constexpr int lds = TreeCfg<D, KT, RT>::LDS + kState;
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_few_kernel<D, KT, RT>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   return attr != hipSuccess ? attr : launch_kernel(paged_few_kernel<D, KT, RT>, p, n_wg, lds, stream);
 }
 template <int D, typename KT>
 static hipError_t launch_mixed(const PagedAttn& p, int n_wg, hipStream_t stream) {
-  constexpr int lds = MixedCfg<D, KT>::LDS + 16;
+  constexpr int lds = MixedCfg<D, KT>::LDS + kState;
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_mixed_kernel<D, KT>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   return attr != hipSuccess ? attr : launch_kernel(paged_mixed_kernel<D, KT>, p, n_wg, lds, stream);
@@ -627,6 +676,8 @@ static hipError_t launch_paged(PagedAttn p, float* parts, size_t part_bytes, uns
   p.few_rows = two ? 32 : 16;
   p.few.least = 8;
   p.many.least = D == 64 ? 2 : 4;
+  p.few.join = D == 64 ? 0.25f : 0.7f;
+  p.many.join = D == 64 ? 0.4f : sizeof(KT) == 4 ? 0.7f : 1.2f;
   p.few.arrived = arrived;
   p.many.arrived = arrived + kArrivalWords * (kArrivals / 2);
   p.few.rec = p.many.rec = nullptr;
