@@ -28,6 +28,7 @@
 // for one run of rows. A lane holds the page number of 16 keys, a wave those of
 // 1024, the next 1024 on their way.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.h"
 #include "kernels.h"
@@ -85,6 +86,8 @@ __device__ inline SeqLens seq_lens(const PagedAttn& p, int i) {
   return s;
 }
 
+__device__ inline unsigned padded(unsigned x, unsigned pad) { return pad > 1u ? (x + pad - 1u) / pad * pad : x; }
+
 // Units of a sequence on the line, for row tiles of ROWS rows and key tiles of TK.
 template <int ROWS, int TK>
 struct Units {
@@ -108,7 +111,43 @@ struct Units {
     if (whole) return (unsigned)n_rt;
     return (unsigned)(n_rt / 2) * padded(pair, pad) + (n_rt & 1 ? padded((unsigned)tiles(n_rt / 2), pad) : 0u);
   }
-  static __device__ inline unsigned padded(unsigned x, unsigned pad) { return pad > 1u ? (x + pad - 1u) / pad * pad : x; }
+  // The row tile and key tile at a place; false behind the last one, then with what
+  // is left of the empty places.
+  __device__ inline bool find(unsigned off, bool whole, unsigned pad, int& rt, int& n_tiles, int& tile, unsigned& left) const {
+    tile = 0;
+    if (whole) {
+      rt = n_rt - 1 - (int)off;
+      n_tiles = tiles(rt);
+      return true;
+    }
+    const unsigned pairs = (unsigned)(n_rt / 2), span = padded(pair, pad), j = min(off / span, pairs);
+    off -= j * span;
+    rt = n_rt - 1 - (int)j;  // (the middle one, where it is alone, is both)
+    n_tiles = tiles(rt);
+    left = (j < pairs ? span : padded((unsigned)n_tiles, pad)) - off;
+    if (j < pairs && off >= (unsigned)n_tiles) {
+      off -= (unsigned)n_tiles;
+      rt = (int)j;
+      n_tiles = tiles(rt);
+    }
+    tile = (int)off;
+    return off < (unsigned)n_tiles;
+  }
+};
+
+// The same where all rows are one tile.
+template <int TK>
+struct OneUnit {
+  int n_tiles_;
+  __device__ inline OneUnit(const SeqLens& s, int) : n_tiles_((max(s.n_seen, 1) + TK - 1) / TK) {}
+  __device__ inline unsigned per_head(bool whole, unsigned pad) const { return whole ? 1u : padded((unsigned)n_tiles_, pad); }
+  __device__ inline bool find(unsigned off, bool whole, unsigned pad, int& rt, int& n_tiles, int& tile, unsigned& left) const {
+    rt = 0;
+    n_tiles = n_tiles_;
+    tile = whole ? 0 : (int)off;
+    left = per_head(whole, pad) - off;
+    return tile < n_tiles_;
+  }
 };
 
 // The pages of a sequence, as a wave reads them: RUNS runs of 16 keys per tile.
@@ -394,7 +433,7 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
 // so as few rounds of loads as the registers allow.
 template <int D, int ROWS, typename U>
 __device__ __forceinline__ void join_parts(const U& u, int n_rows, lds_t* lds) {
-  constexpr int kInFlight = 8, THREADS = kTreeWaves * kWave;
+  constexpr int kInFlight = 16, THREADS = kTreeWaves * kWave;
   typedef Record<D, ROWS> R;
   const int tid = thread_here(), units = n_rows * (D / 4);
   const int n = u.parts;
@@ -471,7 +510,7 @@ constexpr int kState = kTreeWaves * 5 * 4 * kWave + 16;
 template <int D, typename KT, int RT, bool WIDE>
 __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& line, lds_t* const lds, lds_t* const state) {
   typedef LineCfg<D, KT, RT, WIDE> C;
-  typedef Units<C::ROWS, C::TK> U;
+  typedef typename std::conditional<WIDE, Units<C::ROWS, C::TK>, OneUnit<C::TK>>::type U;
   constexpr int ROWS = C::ROWS, TK = C::TK;
   const bool whole = line.rec == nullptr;  // no records: no unit in parts
   unsigned pad = 1u;
@@ -494,25 +533,31 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
   };
   unsigned total = 0u;
   int longest = 0;  // keys, about
-  auto add_up = [&]() __attribute__((always_inline)) {
+  auto add_up = [&](bool again) __attribute__((always_inline)) {
     total = 0u;
     for (int i = (p.n_seq - 1) / kWave * kWave; i >= 0; i -= kWave) {  // (the first 64 last: they stay)
       const int lane = thread_here() % kWave;
-      const SeqLens s = seq_lens(p, i + lane);
+      SeqLens s;
+      if (again && i == 0) {
+        auto x = [&](int j) __attribute__((always_inline)) { return lds_load<int>(kept_at + 4 * (kWave * j + lane)); };
+        s = SeqLens{x(0), x(1), x(2), x(3)};
+      } else {
+        s = seq_lens(p, i + lane);
+      }
       const unsigned units = units_of(s), end = wave_scan(units);
       total += (unsigned)__builtin_amdgcn_readlane((int)end, 63);
       longest = max(longest, units > 0u ? s.n_seen : 0);
       if (i == 0) keep(lane, s, end);
     }
   };
-  add_up();
+  add_up(false);
   // Shares: the same for every workgroup, few rows in whole rounds of the waves.
   const unsigned n_wg = gridDim.x;
   unsigned per = max((total + n_wg - 1) / n_wg, 1u);
   if (!whole) {
     // A unit's parts are joined some at a time, so a long one takes per + (tiles /
     // per) `join` tiles' time, the least for per = sqrt(tiles join).
-    const float tiles = wave_max((float)longest) * (1.f / TK);
+    const float tiles = wave_max_dpp((float)longest) * (1.f / TK);
     unsigned want = (unsigned)uniform((int)fminf(fmaxf((float)line.least, sqrtf(tiles * line.join)), ceilf(tiles)));
     if (!WIDE) {
       per = (per + kTreeWaves - 1) / kTreeWaves * kTreeWaves;
@@ -521,10 +566,12 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
     if (want > per) {
       // Fewer workgroups than there are: as long as they are enough, none has two units.
       per = pad = want;
-      add_up();
+      wave_lds_fence();
+      add_up(true);
       if ((total + per - 1) / per > n_wg) {
         pad = 1u;
-        add_up();
+        wave_lds_fence();
+        add_up(true);
       }
     }
   }
@@ -556,42 +603,20 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
     const unsigned per_head = u.per_head(whole, pad), seq_end = (unsigned)__builtin_amdgcn_readlane((int)end, at);
     const unsigned y = x - before - (seq_end - per_head * (unsigned)p.cache.n_head_kv);
     const int g = uniform((int)(y / per_head));
-    unsigned off = y - (unsigned)g * per_head;  // place in the head's units
     int rt, tiles, tile;
-    if (whole) {
-      rt = uniform(u.n_rt - 1 - (int)off);
-      tiles = u.tiles(rt);
-      tile = 0;
-    } else {
-      const unsigned pairs = (unsigned)(u.n_rt / 2), pair = U::padded(u.pair, pad), j = min(off / pair, pairs);
-      off -= j * pair;
-      const unsigned left = pair - off;  // of the pair
-      rt = u.n_rt - 1 - (int)j;  // (the middle one, where it is alone, is both)
-      tiles = u.tiles(rt);
-      if (j == pairs && off >= (unsigned)tiles) {  // the empty ones behind the middle one
-        x += U::padded((unsigned)tiles, pad) - off;
-        continue;
-      }
-      if (j < pairs && off >= (unsigned)tiles) {
-        off -= (unsigned)tiles;
-        rt = (int)j;
-        tiles = u.tiles(rt);
-        if (off >= (unsigned)tiles) {  // the empty ones behind the pair
-          x += left;
-          continue;
-        }
-      }
-      tile = (int)off;
-      rt = uniform(rt);
-      tiles = uniform(tiles);
-      tile = uniform(tile);
+    unsigned left = 0u;
+    if (!u.find(y - (unsigned)g * per_head, whole, pad, rt, tiles, tile, left)) {
+      x += left;
+      continue;
     }
+    rt = uniform(rt);
+    tiles = uniform(tiles);
+    tile = uniform(tile);
     const int n = whole ? tiles : (int)min((unsigned)(tiles - tile), x_end - x);
     const bool part = n < tiles;
     // its first tile's place: who begins it, and how many share it
-    const unsigned x0 = x - (unsigned)tile, owner = part ? x0 / per : 0u;
-    const int parts = part ? (int)((x0 + (unsigned)tiles - 1) / per - owner) + 1 : 1;
-    const int mine = part ? (int)(x / per - owner) : 0;
+    const unsigned x0 = x - (unsigned)tile, owner = part && tile > 0 ? x0 / per : wg;
+    const int parts = part ? (int)((x0 + (unsigned)tiles - 1) / per - owner) + 1 : 1, mine = (int)(wg - owner);
     float* const rec = part ? line.rec + (int64_t)(2 * wg + (mine == 0 ? 1 : 0)) * Record<D, ROWS>::FLOATS : nullptr;
     const UnitRows<D, KT, ROWS> rows{p, g, s.q0, s.n_past, s.n_seen, s.n_new * p.n_rep, p.n_rep, rt * ROWS, p.scale_log2e,
                                      parts, mine, rec, line.arrived + kArrivalWords * owner, state + kState - 16};
@@ -676,7 +701,7 @@ static hipError_t launch_paged(PagedAttn p, float* parts, size_t part_bytes, uns
   p.few_rows = two ? 32 : 16;
   p.few.least = 8;
   p.many.least = D == 64 ? 2 : 4;
-  p.few.join = D == 64 ? 0.25f : 0.7f;
+  p.few.join = D == 64 ? 0.35f : 0.5f;
   p.many.join = D == 64 ? 0.4f : sizeof(KT) == 4 ? 0.7f : 1.2f;
   p.few.arrived = arrived;
   p.many.arrived = arrived + kArrivalWords * (kArrivals / 2);
