@@ -211,6 +211,11 @@ struct VerifyPart {  // a chunk of a row
   float top;     // the largest logit, NaN if there is one
   int32_t best;  // greedy rows: its lowest token
 };
+struct VerifyLeft {  // a sequence whose last token is drawn from max(p - draft, 0)
+  double scale, inv, u;  // of the logits; 1 / the sum of the weights; the number it is drawn by
+  float top;
+  int32_t row, down, at;  // rows of the logits and of the draft (-1: no such sequence), place in tokens
+};
 struct Verify {
   const char* logits;
   int64_t nb;
@@ -229,8 +234,9 @@ struct Verify {
   VerifyPart* parts;  // scratch of verify_scratch() bytes
   unsigned* arrived;  // kArrivals counters, zero before and after
   int32_t n_vocab, n_rows, n_seq, max_path;
-  double* sums;       // these are set by the launcher
-  int32_t n_chunks, row0, seq0;
+  VerifyLeft* left;   // these are set by the launcher
+  double* sums;
+  int32_t n_chunks, row0, seq0, max_nodes;
 };
 size_t verify_scratch(int n_rows, int n_seq, int n_vocab, int n_cu);
 hipError_t launch_verify(const Verify& p, int n_cu, hipStream_t stream);

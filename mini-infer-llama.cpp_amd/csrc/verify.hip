@@ -13,9 +13,8 @@
 // each drafted token's probability, walks from node to node, and draws: the
 // chunks' sums say which chunk the token is in, whose weights are then formed once
 // more. Where a draft's token was turned down, what is left is a difference of
-// probabilities that has to be summed over the row first: then the sequence has a
-// workgroup per chunk, all of which walk, each sums its chunk, and the last one to
-// get there draws.
+// probabilities that has to be summed over the row first: verify_rest_kernel does
+// that with several workgroups a sequence, the last of which draws.
 #include <algorithm>
 
 #include "attn_common.h"
@@ -40,25 +39,25 @@ __device__ inline f32x4 load_row(const char* row, int i, int n, float pad) {
   return v;
 }
 
-// 2^t for t <= 0 (down to -infinity): the power series of e^(f ln 2) for the fraction
-// f in [-1/2, 1/2], whose twelfth term is below 2^-47 and thirteenth below 2^-52.
+// 2^t for t <= 0 (down to -infinity): the whole part is the low word of t + 1.5 2^52,
+// the fraction f in [-1/2, 1/2] by 1 + f g(f), g of
+// degree 9 through (2^f - 1) / f at the ten Chebyshev points: at most 6e-16 off, and 1
+// for 0. (The power series needs two terms more.)
 __device__ inline double exp2_d(double t) {
   t = fmax(t, -2000.0);
-  const double n = __builtin_rint(t), f = (t - n) * 0x1.62e42fefa39efp-1;  // ln 2
-  double s = 1.0 / 479001600.0;
-  s = fma(s, f, 1.0 / 39916800.0);
-  s = fma(s, f, 1.0 / 3628800.0);
-  s = fma(s, f, 1.0 / 362880.0);
-  s = fma(s, f, 1.0 / 40320.0);
-  s = fma(s, f, 1.0 / 5040.0);
-  s = fma(s, f, 1.0 / 720.0);
-  s = fma(s, f, 1.0 / 120.0);
-  s = fma(s, f, 1.0 / 24.0);
-  s = fma(s, f, 1.0 / 6.0);
-  s = fma(s, f, 0.5);
+  const double m = t + 0x1.8p+52, f = t - (m - 0x1.8p+52);
+  double s = 0x1.e5e9f548e5726p-28;
+  s = fma(s, f, 0x1.b6571de2f2351p-24);
+  s = fma(s, f, 0x1.62bfe46117445p-20);
+  s = fma(s, f, 0x1.ffcb76789860fp-17);
+  s = fma(s, f, 0x1.4309130378460p-13);
+  s = fma(s, f, 0x1.5d87fe908f88ap-10);
+  s = fma(s, f, 0x1.3b2ab6fba385fp-7);
+  s = fma(s, f, 0x1.c6b08d7044119p-5);
+  s = fma(s, f, 0x1.ebfbdff82c590p-3);
+  s = fma(s, f, 0x1.62e42fefa39f7p-1);
   s = fma(s, f, 1.0);
-  s = fma(s, f, 1.0);
-  return __builtin_amdgcn_ldexp(s, (int)n);
+  return __builtin_amdgcn_ldexp(s, (int)__builtin_bit_cast(uint64_t, m));
 }
 constexpr double kLog2e = 0x1.71547652b82fep+0;
 
@@ -102,8 +101,13 @@ __global__ __launch_bounds__(kRowThreads) void verify_rows_kernel(const Verify p
   const int n = min(CHUNK, p.n_vocab - base);
   const char* const in = p.logits + row * p.nb + 4 * (int64_t)base;
   f32x4 x[PER];
+  if (n == CHUNK) {  // (all on their way at once)
 #pragma unroll
-  for (int k = 0; k < PER; ++k) x[k] = load_row(in, 4 * (tid + kRowThreads * k), n, -INFINITY);
+    for (int k = 0; k < PER; ++k) x[k] = load4(in + 16 * (tid + kRowThreads * k));
+  } else {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) x[k] = load_row(in, 4 * (tid + kRowThreads * k), n, -INFINITY);
+  }
   int seq = 0;  // the last sequence that begins at or before the row
   if (p.temperature) {
     for (int i = 0; i < p.n_seq; i += kWave)
@@ -183,21 +187,48 @@ __device__ inline RowSums join_row(const Verify& p, int row, double scale, int l
   return r;
 }
 
-// The walk's shared memory.
+// The walk's shared memory: arrays of as many nodes as a sequence can have.
 struct Walk {
-  double prob[kVerifyMaxNodes];  // of each node's token in its parent's row
-  double bar[kVerifyMaxNodes];   // u, or u draft
-  double sum[kVerifyMaxNodes];   // rows
-  float top[kVerifyMaxNodes];
-  int best[kVerifyMaxNodes];
-  int token[kVerifyMaxNodes], up[kVerifyMaxNodes], down[kVerifyMaxNodes];
-  double part[kWalkWaves];
-  int last[kWalkWaves];
-  int cur, n_down, len, chunk, joins;
-  double before, target;
+  double* prob;  // of each node's token in its parent's row
+  double* bar;   // u, or u draft
+  double* sum;   // rows
+  float* top;
+  int* best;
+  int *token, *up, *down;
+  double* part;  // of the waves
+  int* last;
+  struct Found {
+    int cur, n_down, len, chunk, joins, unused;
+    double before, target;
+  }* f;
+  static constexpr int kNodeBytes = 3 * 8 + 5 * 4, kFixed = kWalkWaves * (8 + 2 * 4) + (int)sizeof(Found);
+  __device__ inline Walk(char* lds, int nodes) {
+    f = reinterpret_cast<Found*>(lds);
+    part = reinterpret_cast<double*>(f + 1);
+    prob = part + kWalkWaves;
+    bar = prob + nodes;
+    sum = bar + nodes;
+    top = reinterpret_cast<float*>(sum + nodes);
+    best = reinterpret_cast<int*>(top + nodes);
+    token = best + nodes;
+    up = token + nodes;
+    down = up + nodes;
+    last = down + nodes;
+  }
 };
 
-// The sum over the workgroup, the same on every thread; `below`: over the threads below.
+// The sum over the workgroup, the same on every thread.
+__device__ inline double block_total(Walk& s, double x) {
+  x = wave_sum_f64(x);
+  __syncthreads();  // (s.part has been read)
+  if (threadIdx.x % kWave == 0) s.part[threadIdx.x / kWave] = x;
+  __syncthreads();
+  double all = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWalkWaves; ++w) all += s.part[w];
+  return all;
+}
+// The same, and `below`: over the threads below.
 __device__ inline double block_sum(Walk& s, double x, double& below) {
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const double incl = wave_scan(x, lane);
@@ -214,20 +245,140 @@ __device__ inline double block_sum(Walk& s, double x, double& below) {
   return all;
 }
 
+// What a sequence's last token is drawn from: p of the row, or with LESS max(p - draft,
+// 0), in chunks of CHUNK tokens, PER in a row for each thread.
+template <int CHUNK, bool LESS>
+struct Remainder {
+  static constexpr int PER = CHUNK / kWalkThreads;
+  const char *x, *q;  // the row's logits, the draft's probabilities
+  float top;
+  double scale, inv;  // inv: 1 / the sum of the weights
+  int n_vocab;
+  const int *token, *down;  // n_out tokens that are left out: token[down[e]]
+  int n_out;
+
+  struct Tokens {
+    f32x4 x[PER / 4], q[PER / 4];
+  };
+  __device__ __forceinline__ void load(int k, Tokens& v) const {
+    const int base = k * CHUNK, m = min(CHUNK, n_vocab - base), i0 = (int)threadIdx.x * PER;
+    const char* const xk = x + 4 * (int64_t)base;
+    const char* const qk = LESS ? q + 4 * (int64_t)base : nullptr;
+    if (m == CHUNK) {  // (all on their way at once)
+#pragma unroll
+      for (int j = 0; j < PER / 4; ++j) {
+        v.x[j] = load4(xk + 4 * (i0 + 4 * j));
+        if (LESS) v.q[j] = load4(qk + 4 * (i0 + 4 * j));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER / 4; ++j) {
+        v.x[j] = load_row(xk, i0 + 4 * j, m, -INFINITY);
+        if (LESS) v.q[j] = load_row(qk, i0 + 4 * j, m, 0.f);
+      }
+    }
+  }
+  // The thread's tokens of chunk k: what is left of each, and their sum.
+  __device__ __forceinline__ double rest(int k, const Tokens& v, double (&w)[PER]) const {
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      w[j] = weight(v.x[j / 4][j % 4], top, scale);
+      if (LESS) w[j] = fmax(w[j] * inv - (double)v.q[j / 4][j % 4], 0.0);
+    }
+    for (int e = 0; e < n_out; ++e) {
+      const unsigned t = (unsigned)(token[down[e]] - k * CHUNK - (int)threadIdx.x * PER);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) w[j] = t == (unsigned)j ? 0.0 : w[j];
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sum += w[j];
+    return sum;
+  }
+
+  // The token drawn by u, given each chunk's sum: the first with a weight up to which
+  // the sum is above u times the whole; -1 if nothing is left. Called by all threads,
+  // valid on thread 0.
+  template <typename ChunkSum>
+  __device__ int draw(Walk& s, double u, int n_chunks, ChunkSum chunk_sum) const {
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    if (wave == 0) {
+      double total = 0.0, first[2] = {0.0, 0.0};  // (the first 128 chunks' are kept)
+      for (int k = 0; k < n_chunks; k += kWave) {
+        const double c = k + lane < n_chunks ? chunk_sum(k + lane) : 0.0;
+        if (k < kWave) first[0] = c;
+        else if (k < 2 * kWave) first[1] = c;
+        total += wave_sum_f64(c);
+      }
+      const double target = u * total;
+      double before = 0.0, start = 0.0;
+      int chunk = -1;
+      for (int k = 0; k < n_chunks; k += kWave) {
+        const double c = k < kWave ? first[0] : k < 2 * kWave ? first[1] : k + lane < n_chunks ? chunk_sum(k + lane) : 0.0;
+        const double incl = before + wave_scan(c, lane);
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(c > 0.0 && incl > target);
+        const uint64_t any = __builtin_amdgcn_ballot_w64(c > 0.0);
+        if (hit || any) {  // (the last with a weight, if rounding passes them all)
+          const int at = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
+          chunk = k + at;
+          start = __shfl(incl - c, at, kWave);
+        }
+        if (hit) break;
+        before = __shfl(incl, kWave - 1, kWave);
+      }
+      if (lane == 0) {
+        s.f->chunk = chunk;
+        s.f->before = start;
+        s.f->target = target;
+      }
+    }
+    __syncthreads();
+    const int chunk = s.f->chunk;
+    if (chunk < 0) return -1;
+    Tokens v;
+    double w[PER], below;
+    load(chunk, v);
+    const double target = s.f->target;
+    block_sum(s, rest(chunk, v, w), below);
+    double cum = s.f->before + below;
+    int first = INT32_MAX, last = -1;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      cum += w[j];
+      const int t = chunk * CHUNK + tid * PER + j;
+      if (w[j] > 0.0) {
+        last = t;
+        if (cum > target) first = min(first, t);
+      }
+    }
+    first = wave_min(first);
+    last = wave_max_int(last);
+    if (lane == 0) {
+      s.last[wave] = last;
+      s.last[kWalkWaves + wave] = first;
+    }
+    __syncthreads();
+    for (int o = 0; o < kWalkWaves; ++o) {
+      last = max(last, s.last[o]);
+      first = min(first, s.last[kWalkWaves + o]);
+    }
+    return first != INT32_MAX ? first : last;
+  }
+};
+
 }  // namespace
 
-// CHUNK tokens a chunk, eight or four in a row per thread.
+// A workgroup per sequence.
 template <int CHUNK, bool DRAFT>
 __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const Verify p) {
-  constexpr int PER = CHUNK / kWalkThreads;
-  __shared__ Walk s;
-  const int seq = p.seq0 + blockIdx.y, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const bool writes = blockIdx.x == 0;
-  const int r0 = min(max(p.off[seq], 0), p.n_rows), n = min(min(max(p.off[seq + 1], r0), p.n_rows) - r0, kVerifyMaxNodes);
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  Walk s(lds_raw, p.max_nodes);
+  const int seq = p.seq0 + blockIdx.x, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int r0 = min(max(p.off[seq], 0), p.n_rows), n = min(min(max(p.off[seq + 1], r0), p.n_rows) - r0, p.max_nodes);
   int* const path = reinterpret_cast<int*>(p.path + seq * p.path_nb);
   int* const out = reinterpret_cast<int*>(p.tokens + seq * p.tokens_nb);
+  if (DRAFT && tid == 0) p.left[blockIdx.x].down = -1;  // (nothing for verify_rest_kernel)
   if (n <= 0) {
-    if (!writes) return;
     for (int i = tid; i < p.max_path; i += kWalkThreads) path[i] = out[i] = -1;
     if (tid == 0) p.n_path[seq] = 0;
     return;
@@ -266,18 +417,15 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const Verify 
   if (tid == 0) {
     int cur = 0, len = 1, n_down = 0;
     double left = 1.0;
-    if (writes) path[0] = 0;
+    path[0] = 0;
     for (int c = 1; c < n && len < p.max_path; ++c) {
       if (s.up[c] != cur) continue;
       bool again = false;
       for (int e = 0; e < n_down; ++e) again = again || s.token[s.down[e]] == s.token[c];
       const double pc = again ? 0.0 : s.prob[c];
       if ((DRAFT ? s.bar[c] : s.bar[c] * left) < pc) {
-        if (writes) {
-          out[len - 1] = s.token[c];
-          path[len] = c;
-        }
-        ++len;
+        out[len - 1] = s.token[c];
+        path[len++] = c;
         cur = c;
         n_down = 0;
         left = 1.0;
@@ -286,158 +434,94 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const Verify 
         s.down[n_down++] = c;
       }
     }
-    s.cur = cur;
-    s.len = len;
-    s.n_down = len < p.max_path ? n_down : 0;
-    if (writes) p.n_path[seq] = len;
+    s.f->cur = cur;
+    s.f->len = len;
+    s.f->n_down = len < p.max_path ? n_down : 0;
+    p.n_path[seq] = len;
   }
   __syncthreads();
-  const int cur = s.cur, n_down = s.n_down, len = s.len;
+  const int cur = s.f->cur, n_down = s.f->n_down, len = s.f->len;
+  for (int i = len + tid; i < p.max_path; i += kWalkThreads) path[i] = out[i] = -1;
   const bool less = DRAFT && n_down > 0;  // the draft's probabilities come off
-  if (!less && !writes) return;
-  if (writes) {
-    for (int i = len + tid; i < p.max_path; i += kWalkThreads) path[i] = out[i] = -1;
-  }
   const float top = s.top[cur];
   const char* const x = p.logits + (r0 + cur) * p.nb;
-  const char* const q = less ? p.draft + (r0 + s.down[0]) * p.draft_nb : nullptr;
   if (!(top > -INFINITY && top < INFINITY)) {  // no distribution, no token
-    if (writes && tid == 0) out[len - 1] = -1;
+    if (tid == 0) out[len - 1] = -1;
     return;
   }
   if (scale == 0.0) {
     // (the best token is never turned down, unless a draft had nothing else)
-    if (writes && tid == 0) {
+    if (tid == 0) {
       const int t = s.best[cur];
-      out[len - 1] = less && !(gload<float>(q + 4 * (int64_t)t) < 1.f) ? -1 : t;
+      const float q = less ? gload<float>(p.draft + (r0 + s.down[0]) * p.draft_nb + 4 * (int64_t)t) : 0.f;
+      out[len - 1] = q < 1.f ? t : -1;
     }
     return;
   }
-  // What is left of chunk k: the thread's PER tokens in w, their sum.
-  const double inv = 1.0 / s.sum[cur];
-  auto rest = [&](int k, double (&w)[PER]) __attribute__((always_inline)) -> double {
-    const int base = k * CHUNK, m = min(CHUNK, p.n_vocab - base), i0 = tid * PER;
-    double sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < PER; j += 4) {
-      const f32x4 v = load_row(x + 4 * (int64_t)base, i0 + j, m, -INFINITY);
-      f32x4 d = {0.f, 0.f, 0.f, 0.f};
-      if (less) d = load_row(q + 4 * (int64_t)base, i0 + j, m, 0.f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        w[j + e] = weight(v[e], top, scale);
-        if (less) w[j + e] = fmax(w[j + e] * inv - (double)d[e], 0.0);
-      }
-    }
-    if (!DRAFT) {
-      for (int e = 0; e < n_down; ++e) {
-        const unsigned t = (unsigned)(s.token[s.down[e]] - base - i0);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) w[j] = t == (unsigned)j ? 0.0 : w[j];
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < PER; ++j) sum += w[j];
-    return sum;
-  };
-  double w[PER], below;
-  double* const sums = p.sums + (int64_t)blockIdx.y * p.n_chunks;  // of the sequence's chunks, where `less`
-  if (less) {
-    for (int k = blockIdx.x; k < p.n_chunks; k += gridDim.x) {
-      const double all = block_sum(s, rest(k, w), below);
-      if (tid == 0)
-        __hip_atomic_store(reinterpret_cast<uint64_t*>(sums + k), __builtin_bit_cast(uint64_t, all), __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-    }
-    if (tid == 0) {
-      wait_vmem<0>();
-      unsigned* const counter = p.arrived + kArrivalWords * blockIdx.y;
-      const unsigned done = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (done == gridDim.x - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      s.joins = done == gridDim.x - 1;
-    }
-    __syncthreads();
-    if (!s.joins) return;
+  if (less) {  // the rest of the row is another kernel's
+    if (tid == 0) p.left[blockIdx.x] = VerifyLeft{scale, 1.0 / s.sum[cur], s.bar[0], top, r0 + cur, r0 + s.down[0], len - 1};
+    return;
   }
+  const Remainder<CHUNK, false> row{x, nullptr, top, scale, 0.0, p.n_vocab, s.token, s.down, DRAFT ? 0 : n_down};
   // Chunks that tokens turned down have left are summed anew (into s.prob, by the token).
-  const int n_out = DRAFT ? 0 : n_down;
-  for (int e = 0; e < n_out; ++e) {
+  for (int e = 0; e < row.n_out; ++e) {
     const int t = s.token[s.down[e]];
-    const double all = (unsigned)t < (unsigned)p.n_vocab ? block_sum(s, rest(t / CHUNK, w), below) : 0.0;
+    double all = 0.0;
+    if ((unsigned)t < (unsigned)p.n_vocab) {
+      typename Remainder<CHUNK, false>::Tokens v;
+      double w[Remainder<CHUNK, false>::PER];
+      row.load(t / CHUNK, v);
+      all = block_total(s, row.rest(t / CHUNK, v, w));
+    }
     if (tid == 0) s.prob[e] = all;
   }
   __syncthreads();
-  auto chunk_sum = [&](int k) __attribute__((always_inline)) -> double {
-    if (k >= p.n_chunks) return 0.0;
-    if (less)
-      return __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const uint64_t*>(sums + k), __ATOMIC_RELAXED,
-                                                          __HIP_MEMORY_SCOPE_AGENT));
+  const int t = row.draw(s, s.bar[0], p.n_chunks, [&](int k) __attribute__((always_inline)) -> double {
     const VerifyPart c = p.parts[(int64_t)(r0 + cur) * p.n_chunks + k];
     double sum = c.top > -INFINITY ? c.sum * weight(c.top, top, scale) : 0.0;
-    for (int e = 0; e < n_out; ++e) sum = s.token[s.down[e]] / CHUNK == k ? s.prob[e] : sum;
+    for (int e = 0; e < row.n_out; ++e) sum = s.token[s.down[e]] / CHUNK == k ? s.prob[e] : sum;
     return sum;
-  };
-  // The chunk that holds the token.
-  if (wave == 0) {
-    double total = 0.0;
-    for (int k = 0; k < p.n_chunks; k += kWave) total += wave_sum_f64(chunk_sum(k + lane));
-    const double target = s.bar[0] * total;
-    double before = 0.0, start = 0.0;
-    int chunk = -1;
-    for (int k = 0; k < p.n_chunks; k += kWave) {
-      const double c = chunk_sum(k + lane);
-      const double incl = before + wave_scan(c, lane);
-      const uint64_t hit = __builtin_amdgcn_ballot_w64(c > 0.0 && incl > target);
-      const uint64_t any = __builtin_amdgcn_ballot_w64(c > 0.0);
-      if (hit || any) {  // (the last with a weight, if rounding passes them all)
-        const int at = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
-        chunk = k + at;
-        start = __shfl(incl - c, at, kWave);
-      }
-      if (hit) break;
-      before = __shfl(incl, kWave - 1, kWave);
-    }
-    if (lane == 0) {
-      s.chunk = chunk;
-      s.before = start;
-      s.target = target;
-    }
+  });
+  if (tid == 0) out[len - 1] = t;
+}
+
+// Sequences whose draft's token was turned down: the workgroups of grid row y sum what
+// is left of the row of sequence seq0 + y, the last to arrive draws.
+template <int CHUNK>
+__global__ __launch_bounds__(kWalkThreads) void verify_rest_kernel(const Verify p) {
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  typedef Remainder<CHUNK, true> R;
+  Walk s(lds_raw, 0);
+  const VerifyLeft left = p.left[blockIdx.y];
+  if (left.down < 0) return;
+  const R row{p.logits + left.row * p.nb, p.draft + left.down * p.draft_nb, left.top, left.scale, left.inv, p.n_vocab,
+              nullptr, nullptr, 0};
+  double* const sums = p.sums + (int64_t)blockIdx.y * p.n_chunks;
+  const int tid = threadIdx.x;
+  typename R::Tokens v;
+  double w[R::PER];
+  row.load(blockIdx.x, v);
+  for (int k = blockIdx.x; k < p.n_chunks; k += gridDim.x) {
+    if (k != (int)blockIdx.x) row.load(k, v);
+    const double all = block_total(s, row.rest(k, v, w));
+    if (tid == 0)
+      __hip_atomic_store(reinterpret_cast<uint64_t*>(sums + k), __builtin_bit_cast(uint64_t, all), __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
   }
-  __syncthreads();
-  const int chunk = s.chunk;
-  if (chunk < 0) {  // nothing is left
-    if (tid == 0) out[len - 1] = -1;
-    return;
-  }
-  // The token: the first with a weight whose sum is above the target, or the last.
-  const double mine_sum = rest(chunk, w), target = s.target;
-  block_sum(s, mine_sum, below);
-  double cum = s.before + below;
-  int first = INT32_MAX, last = -1;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    cum += w[j];
-    const int t = chunk * CHUNK + tid * PER + j;
-    if (w[j] > 0.0) {
-      last = t;
-      if (cum > target) first = min(first, t);
-    }
-  }
-  first = wave_min(first);
-  last = wave_max_int(last);
-  __syncthreads();
-  if (lane == 0) {
-    s.last[wave] = last;
-    s.down[wave] = first;
-  }
-  __syncthreads();
   if (tid == 0) {
-    for (int o = 1; o < kWalkWaves; ++o) {
-      first = min(first, s.down[o]);
-      last = max(last, s.last[o]);
-    }
-    out[len - 1] = first != INT32_MAX ? first : last;
+    wait_vmem<0>();
+    unsigned* const counter = p.arrived + kArrivalWords * blockIdx.y;
+    const unsigned done = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (done == gridDim.x - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s.f->joins = done == gridDim.x - 1;
   }
+  __syncthreads();
+  if (!s.f->joins) return;
+  const int t = row.draw(s, left.u, p.n_chunks, [&](int k) __attribute__((always_inline)) -> double {
+    return __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const uint64_t*>(sums + k), __ATOMIC_RELAXED,
+                                                        __HIP_MEMORY_SCOPE_AGENT));
+  });
+  if (tid == 0) reinterpret_cast<int*>(p.tokens + (p.seq0 + (int)blockIdx.y) * p.tokens_nb)[left.at] = t;
 }
 
 // Chunks of 2048 tokens while a launch has few workgroups.
@@ -448,14 +532,17 @@ static int chunk_of(int64_t n_rows, int n_vocab, int n_cu) {
 size_t verify_scratch(int n_rows, int n_seq, int n_vocab, int n_cu) {
   const int chunk = chunk_of(n_rows, n_vocab, n_cu);
   const size_t chunks = ((size_t)n_vocab + chunk - 1) / chunk;
-  return chunks * ((size_t)n_rows * sizeof(VerifyPart) + (size_t)std::min(n_seq, kArrivals) * sizeof(double));
+  return chunks * (size_t)n_rows * sizeof(VerifyPart) + (size_t)std::min(n_seq, kArrivals) * (sizeof(VerifyLeft) + chunks * sizeof(double));
 }
 
 template <int CHUNK>
 static hipError_t launch_verify_t(Verify p, int n_cu, hipStream_t stream) {
   constexpr int kRows = 65535;  // of a grid
   p.n_chunks = (p.n_vocab + CHUNK - 1) / CHUNK;
-  p.sums = reinterpret_cast<double*>(p.parts + (int64_t)p.n_rows * p.n_chunks);
+  p.left = reinterpret_cast<VerifyLeft*>(p.parts + (int64_t)p.n_rows * p.n_chunks);
+  p.sums = reinterpret_cast<double*>(p.left + std::min(p.n_seq, kArrivals));
+  p.max_nodes = std::min(p.n_rows, kVerifyMaxNodes);
+  const int lds = Walk::kFixed + Walk::kNodeBytes * p.max_nodes;
   hipError_t e = hipSuccess;
   for (p.row0 = 0; p.row0 < p.n_rows && e == hipSuccess; p.row0 += kRows) {
     hipLaunchKernelGGL(verify_rows_kernel<CHUNK>, dim3((unsigned)p.n_chunks, (unsigned)std::min(kRows, p.n_rows - p.row0)),
@@ -465,9 +552,16 @@ static hipError_t launch_verify_t(Verify p, int n_cu, hipStream_t stream) {
   // As many sequences a launch as there are arrival counters.
   for (p.seq0 = 0; p.seq0 < p.n_seq && e == hipSuccess; p.seq0 += kArrivals) {
     const int n = std::min(kArrivals, p.n_seq - p.seq0);
-    const unsigned wgs = p.draft ? (unsigned)std::min(p.n_chunks, std::max(1, 2 * n_cu / n)) : 1u;
-    if (p.draft) hipLaunchKernelGGL((verify_walk_kernel<CHUNK, true>), dim3(wgs, (unsigned)n), dim3(kWalkThreads), 0, stream, p);
-    else hipLaunchKernelGGL((verify_walk_kernel<CHUNK, false>), dim3(wgs, (unsigned)n), dim3(kWalkThreads), 0, stream, p);
+    if (!p.draft) {
+      hipLaunchKernelGGL((verify_walk_kernel<CHUNK, false>), dim3((unsigned)n), dim3(kWalkThreads), lds, stream, p);
+    } else {
+      hipLaunchKernelGGL((verify_walk_kernel<CHUNK, true>), dim3((unsigned)n), dim3(kWalkThreads), lds, stream, p);
+      e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      // (up to 16 workgroups per CU: 4 of them, with the next chunk on its way, 64 rows 7 us slower)
+      const unsigned wgs = (unsigned)std::min(p.n_chunks, std::max(1, 16 * n_cu / n));
+      hipLaunchKernelGGL(verify_rest_kernel<CHUNK>, dim3(wgs, (unsigned)n), dim3(kWalkThreads), Walk::kFixed, stream, p);
+    }
     e = hipGetLastError();
   }
   return e;
