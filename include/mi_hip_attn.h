@@ -104,11 +104,13 @@ typedef struct mi_hip_workspace_desc {
 
 /* One device allocation covering any decode launch of up to 32 items of this
  * head shape (mi_hip_attn_decode_batch's limit per launch) and, with 17 MB (head_dim
- * 64) or 34 MB of parts, any call of mi_hip_attn_tree and mi_hip_logits_adjust. Where
- * the allocation limit or the device has no room for the parts, a workspace (a cache's
- * own and the default one too) is made without them: mi_hip_attn_tree then keeps each
- * item's keys in one piece, which is slow over long caches, and
- * mi_hip_logits_adjust refuses to give ids with it (MI_HIP_E_UNSUPPORTED). */
+ * 64) or 34 MB of parts, any call of mi_hip_attn_tree, mi_hip_attn_paged,
+ * mi_hip_verify_draft and mi_hip_logits_adjust. Where the allocation limit or the
+ * device has no room for the parts, a workspace (a cache's own and the default one
+ * too) is made without them: mi_hip_attn_tree and mi_hip_attn_paged then keep each
+ * sequence's keys in one piece, which is slow over long caches, and
+ * mi_hip_logits_adjust's ids and mi_hip_verify_draft are refused with it
+ * (MI_HIP_E_UNSUPPORTED). */
 int mi_hip_workspace_create(const mi_hip_workspace_desc* desc, mi_hip_workspace** out);
 int mi_hip_workspace_destroy(mi_hip_workspace* ws);
 
@@ -436,7 +438,8 @@ int mi_hip_attn_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* mask
  *     max_tokens (a batch that is padded). pos and seq may be NULL;
  *   n_refused: how many sequences are refused, or NULL.
  * Negative lengths count as 0. No other memory of the call may overlap what it
- * writes. Calls on one pool must be ordered. May be captured into a graph. No
+ * writes (with held or ring_at in place one workgroup does the whole call, else
+ * large batches have several). Calls on one pool must be ordered. May be captured into a graph. No
  * counterpart in the reference. */
 typedef struct mi_hip_page_tables_args {
   int32_t n_seq;
@@ -511,7 +514,9 @@ int mi_hip_paged_append(const mi_hip_paged_append_args* args);
  * with more than max_new queries the rest are left as they were. Products, sums and
  * values that are not finite as in mi_hip_attn_tree, with the choice of kernel per
  * sequence (n_rep times its queries up to 32, or more). The same bits on every
- * run with the same lengths. Scratch for joining the parts of long sequences: ws,
+ * run with the same lengths. At most 2^20 sequences, 2^26 query rows (tokens times
+ * heads), 2^30 positions of a sequence, and 2^31 tiles of 32 positions in all
+ * (MI_HIP_E_UNSUPPORTED). Scratch for joining the parts of long sequences: ws,
  * else the cache's own; calls that share one must be ordered. May be captured into
  * a graph. No counterpart in the reference. */
 typedef struct mi_hip_attn_paged_args {
@@ -558,9 +563,11 @@ int mi_hip_attn_paged(const mi_hip_attn_paged_args* args);
  *   path: their numbers in the sequence, as mi_hip_kv_keep takes them, then -1;
  *   tokens: the accepted drafted tokens and the token drawn, n_path in all, then -1.
  * The token drawn is -1 if its row has a NaN or a +infinity, or nothing but -infinity
- * (then no child is accepted either); child tokens outside [0, n_vocab) are turned
- * down. u is clamped to [0, 1). Scratch: ws, else the library default; calls that
- * share one must be ordered. May be captured into a graph. No counterpart in the
+ * (then no child is accepted either), and where every w is 0; child tokens outside
+ * [0, n_vocab) are turned down. u is clamped to [0, 1), a NaN to 0; a temperature of
+ * +infinity has all finite logits alike, a negative one or NaN counts as 0. Scratch:
+ * the parts of ws, else of the library default (MI_HIP_E_UNSUPPORTED where they do
+ * not hold 16 bytes for each 2048 logits); calls that share one must be ordered. May be captured into a graph. No counterpart in the
  * reference. */
 typedef struct mi_hip_verify_args {
   const float* logits;      /* device, n_rows rows of n_vocab */

@@ -86,7 +86,7 @@ __global__ __launch_bounds__(kSeqs) void page_tables_kernel(const PageTables p) 
       head = (unsigned)(h < 0 ? h + p.n_pages : h);
       n_free = (unsigned)max((int64_t)0, min((int64_t)tail0 - head0, (int64_t)p.n_pages));
     }
-    const unsigned need = ((unsigned)cached + (unsigned)fresh + (1u << p.page_shift) - 1u) >> p.page_shift;
+    const unsigned need = (unsigned)(((uint64_t)cached + (uint64_t)fresh + (1u << p.page_shift) - 1u) >> p.page_shift);
     bool fits = need <= (unsigned)p.max_pages;
     unsigned take = fits && need > (unsigned)held ? need - held : 0u, give = need < (unsigned)held ? held - need : 0u;
     unsigned end[3];

@@ -64,7 +64,7 @@ constexpr double kLog2e = 0x1.71547652b82fep+0;
 // What a row's logits are multiplied by, 0 for the greedy choice.
 __device__ inline double row_scale(const Verify& p, int seq) {
   const float t = p.temperature ? p.temperature[seq] : 1.f;
-  return t > 0.f ? kLog2e / (double)t : 0.0;
+  return t > 0.f ? fmax(kLog2e / (double)t, 1e-300) : 0.0;  // (infinity: all weights 1)
 }
 __device__ inline double weight(float x, float top, double scale) { return exp2_d(((double)x - (double)top) * scale); }
 
