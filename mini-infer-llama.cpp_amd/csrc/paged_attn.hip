@@ -336,8 +336,7 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
   // The last part to arrive adds up all of them in their order: a wave its 32 rows,
   // lanes as the products left them, kInFlight parts on their way at once.
   static constexpr bool kJoins = true;
-  __device__ __forceinline__ void join(const floatx16 (&own)[NDB], float ref, float l, bool active, bool valid, int token, int h) const {
-    typedef Record<D, Base::kRows> R;
+  __device__ __forceinline__ void join(const floatx16 (&own)[NDB], float ref, float l, bool active) const {
     const int tid = thread_here(), lane = tid % kWave, kh = lane / 32;
     const int r = 32 * uniform(tid / kWave) + lane % 32;
     if (active) {
@@ -348,27 +347,36 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
           this->put_part(r, 32 * db + 8 * q + 4 * kh, f32x4{own[db][4 * q], own[db][4 * q + 1], own[db][4 * q + 2], own[db][4 * q + 3]});
       if (kh == 0) this->put_sums(r, ref, l);
     }
-    if (!this->arrive() || !active) return;
-    const int n = this->parts;
+    if (!this->arrive()) return;
+    // (up to 64 rows: two waves for each 32, a half of the dims each)
+    const int wave = uniform(tid / kWave), blocks = uniform((min(this->rows - this->row0, Base::kRows) + 31) / 32);
+    if (blocks <= 2) add_up<NDB / 2, D == 64 ? 8 : 4>(wave & 1, wave / 2 * (NDB / 2), lane);
+    else add_up<NDB, D == 64 ? 4 : 2>(wave, 0, lane);
+  }
+  // Rows 32 `block` .., dims 32 db0 .. 32 (db0 + DBS) - 1.
+  template <int DBS, int kInFlight>
+  __device__ __forceinline__ void add_up(int block, int db0, int lane) const {
+    typedef Record<D, Base::kRows> R;
+    const int r = 32 * block + lane % 32, kh = lane / 32, row = this->row0 + r, n = this->parts;
+    if (this->row0 + 32 * block >= this->rows) return;
     const rsrc_t recs = make_rsrc(this->first_record(), (unsigned)(2 * n - 1) * R::BYTES);
-    constexpr int kInFlight = D == 64 ? 4 : 2;
-    f32x4 acc[NDB][4];
+    f32x4 acc[DBS][4];
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
+    for (int db = 0; db < DBS; ++db)
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[db][q] = f32x4{0.f, 0.f, 0.f, 0.f};
     float top = -INFINITY, sum = 0.f;
     for (int k0 = 0; k0 < n; k0 += kInFlight) {
-      f32x4 x[kInFlight][NDB][4];
+      f32x4 x[kInFlight][DBS][4];
       f32x2 ml[kInFlight];
 #pragma unroll
       for (int e = 0; e < kInFlight; ++e) {
         const unsigned at = Base::part_at(min(k0 + e, n - 1));
         ml[e] = shared_load2(recs, at + R::sums_at(r));
 #pragma unroll
-        for (int db = 0; db < NDB; ++db)
+        for (int db = 0; db < DBS; ++db)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) x[e][db][q] = shared_load4(recs, at + R::piece_at(r, 32 * db + 8 * q + 4 * kh));
+          for (int q = 0; q < 4; ++q) x[e][db][q] = shared_load4(recs, at + R::piece_at(r, 32 * (db0 + db) + 8 * q + 4 * kh));
       }
 #pragma unroll
       for (int e = 0; e < kInFlight; ++e) {
@@ -378,18 +386,19 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
         top = now;
         sum = sum * a + ml[e][1] * b;
 #pragma unroll
-        for (int db = 0; db < NDB; ++db)
+        for (int db = 0; db < DBS; ++db)
 #pragma unroll
           for (int q = 0; q < 4; ++q) acc[db][q] = acc[db][q] * a + x[e][db][q] * b;
       }
     }
-    if (!valid) return;
+    if (row >= this->rows) return;
+    const int token = row / this->n_rep;
     const float inv = top == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;
-    char* const out = this->out_row(token, h);
+    char* const out = this->out_row(token, row - token * this->n_rep);
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
+    for (int db = 0; db < DBS; ++db)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) gstore(out + 4 * (32 * db + 8 * q + 4 * kh), acc[db][q] * inv);
+      for (int q = 0; q < 4; ++q) gstore(out + 4 * (32 * (db0 + db) + 8 * q + 4 * kh), acc[db][q] * inv);
   }
   __device__ __forceinline__ unsigned none() const { return pages.none; }
   struct Rows {

@@ -503,7 +503,7 @@ __device__ __forceinline__ void tree_wide_rows(W& w, lds_t* const lds) {
     if (w.is_part()) {
 #pragma unroll
       for (int db = 0; db < NDB; ++db) o[db] *= unit_o;
-      w.join(o, ref, lt, active, valid, token, h);
+      w.join(o, ref, lt, active);
       return;
     }
   }
