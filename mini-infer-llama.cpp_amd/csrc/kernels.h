@@ -182,6 +182,7 @@ struct PagedLine {
   float* rec;
   unsigned* arrived;
   int32_t least;
+  int32_t spare;  // tiles more than its share that a workgroup takes so that none has two units
   float join;  // what joining a part takes, in key tiles' time
 };
 struct PagedAttn {

@@ -105,6 +105,8 @@ struct Units {
     const int last = min(((rt + 1) * ROWS - 1) / n_rep, n_new - 1);
     return (max(min(n_past + last + 1, n_seen), 1) + TK - 1) / TK;
   }
+  // What does not share a workgroup where places are padded, of a head (pairs do).
+  __device__ inline unsigned apart() const { return n_rt == 1 ? 1u : 1u << 10; }
   // Places of a head's units on the line: whole units, or their tiles; pairs and the
   // middle row tile in multiples of `pad`, so that no share of that size holds two.
   __device__ inline unsigned per_head(bool whole, unsigned pad) const {
@@ -140,6 +142,7 @@ template <int TK>
 struct OneUnit {
   int n_tiles_;
   __device__ inline OneUnit(const SeqLens& s, int) : n_tiles_((max(s.n_seen, 1) + TK - 1) / TK) {}
+  __device__ inline unsigned apart() const { return 1u; }
   __device__ inline unsigned per_head(bool whole, unsigned pad) const { return whole ? 1u : padded((unsigned)n_tiles_, pad); }
   __device__ inline bool find(unsigned off, bool whole, unsigned pad, int& rt, int& n_tiles, int& tile, unsigned& left) const {
     rt = 0;
@@ -523,10 +526,13 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
   constexpr int ROWS = C::ROWS, TK = C::TK;
   const bool whole = line.rec == nullptr;  // no records: no unit in parts
   unsigned pad = 1u;
+  unsigned apart = 0u;  // of the lane's sequences
   auto units_of = [&](const SeqLens& s) __attribute__((always_inline)) -> unsigned {
     const int rows = s.n_new * p.n_rep;
     if (rows == 0 || WIDE != (rows > p.few_rows)) return 0u;
-    return U(s, p.n_rep).per_head(whole, pad) * (unsigned)p.cache.n_head_kv;
+    const U u(s, p.n_rep);
+    apart += u.apart();
+    return u.per_head(whole, pad) * (unsigned)p.cache.n_head_kv;
   };
 
   // ---- the line: lane i has sequence `first` + i ------------------------------------
@@ -559,31 +565,50 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
       if (i == 0) keep(lane, s, end);
     }
   };
-  add_up(false);
   // Shares: the same for every workgroup, few rows in whole rounds of the waves.
   const unsigned n_wg = gridDim.x;
-  unsigned per = max((total + n_wg - 1) / n_wg, 1u);
-  if (!whole) {
-    // A unit's parts are joined some at a time, so a long one takes per + (tiles /
-    // per) `join` tiles' time, the least for per = sqrt(tiles join).
-    const float tiles = wave_max_dpp((float)longest) * (1.f / TK);
-    unsigned want = (unsigned)uniform((int)fminf(fmaxf((float)line.least, sqrtf(tiles * line.join)), ceilf(tiles)));
-    if (!WIDE) {
-      per = (per + kTreeWaves - 1) / kTreeWaves * kTreeWaves;
-      want = (want + kTreeWaves - 1) / kTreeWaves * kTreeWaves;
-    }
-    if (want > per) {
-      // Fewer workgroups than there are: as long as they are enough, none has two units.
-      per = pad = want;
-      wave_lds_fence();
-      add_up(true);
-      if ((total + per - 1) / per > n_wg) {
-        pad = 1u;
-        wave_lds_fence();
-        add_up(true);
+  unsigned per = 1u;
+  auto rounds = [&](unsigned x) __attribute__((always_inline)) -> unsigned {
+    return WIDE ? x : (x + kTreeWaves - 1) / kTreeWaves * kTreeWaves;
+  };
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {  // (one copy of the code, which a short call waits for)
+    wave_lds_fence();
+    add_up(pass > 0);
+    if (pass == 0) {
+      per = max((total + n_wg - 1) / n_wg, 1u);
+      if (whole) break;
+      per = rounds(per);
+      // A unit's parts are joined some at a time, so a long one takes per + (tiles /
+      // per) `join` tiles' time, the least for per = sqrt(tiles join).
+      const float tiles = wave_max_dpp((float)longest) * (1.f / TK);
+      const unsigned want = rounds((unsigned)uniform((int)fminf(fmaxf((float)line.least, sqrtf(tiles * line.join)), ceilf(tiles))));
+      // Where these are fewer workgroups than there are, or a few tiles more a share
+      // are enough, none has two units.
+      if (want > per) {
+        per = pad = want;
+      } else {
+        const unsigned units = (unsigned)__builtin_amdgcn_readlane((int)wave_scan(apart), 63) * (unsigned)p.cache.n_head_kv;
+        if (units > n_wg / 2 || total == 0u) break;
+        pad = max(rounds((total - 1) / (n_wg - units / 2) + 1), per);
+        if (pad - per > (unsigned)line.spare) {
+          pad = 1u;
+          break;
+        }
       }
+    } else if (pass == 1) {
+      if ((total + pad - 1) / pad <= n_wg) {
+        per = pad;
+        break;
+      }
+      pad = 1u;
     }
   }
+  // (all of these are the wave's, which the compiler has to know: descriptors that it
+  // takes for a lane's own are loaded through in loops)
+  per = (unsigned)uniform((int)per);
+  pad = (unsigned)uniform((int)pad);
+  total = (unsigned)uniform((int)total);
   // An XCD's workgroups (every eighth) have one piece of the line, all XCDs as many.
   const unsigned busy = (total + per - 1) / per, each = (busy + 7) / 8;
   if (blockIdx.x / 8 >= each) return;
@@ -710,6 +735,8 @@ static hipError_t launch_paged(PagedAttn p, float* parts, size_t part_bytes, uns
   p.few_rows = two ? 32 : 16;
   p.few.least = 8;
   p.many.least = D == 64 ? 2 : 4;
+  p.few.spare = mixed ? 0 : 4;
+  p.many.spare = 1;
   p.few.join = D == 64 ? 0.35f : 0.5f;
   p.many.join = D == 64 ? 0.4f : sizeof(KT) == 4 ? 0.7f : 1.2f;
   p.few.arrived = arrived;
