@@ -18,7 +18,8 @@
 // at a time by itself, into LDS, and takes its share of their pages and tokens, a
 // thread for each, whose sequence it finds there. (Lengths that are also written
 // cannot be read by several workgroups: held or ring_at in place, one does it all.)
-// Bound: the chain of two loads (lengths, then pages) and the launch.
+// Bound: the chain of two loads (lengths, then pages) and the launch (8 requests 6.4 us,
+// 1024 requests with 37000 tokens 8.6, an empty launch 3.6).
 #include <algorithm>
 
 #include "attn_common.h"

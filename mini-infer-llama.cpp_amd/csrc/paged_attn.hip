@@ -27,6 +27,15 @@
 // the same for the whole wave: the rows' descriptors are in scalar registers as
 // for one run of rows. A lane holds the page number of 16 keys, a wave those of
 // 1024, the next 1024 on their way.
+//
+// Bound: single tokens by the cache's bytes (64 over 8192 keys, 28/4 heads of 128, 8-bit:
+// 467 MB in 107 us, 6.9 TB/s for a read of nothing else takes 68, and widening the
+// bytes the rest), long chunks by the matrix pipe (2048 tokens after 6000, F16: 424 us,
+// two products at a large matrix product's rate 363). Between them what a share costs
+// besides its tiles is what counts: about 6 us from the launch to the first tile
+// (lengths, pages, rows: three loads one after the other), and 8 to 10 for records to
+// go through memory and be joined, which short chunks pay twice (1000 tokens from
+// nothing: 45 us, 13 of them products).
 #include <algorithm>
 #include <type_traits>
 
@@ -43,7 +52,8 @@ constexpr int kRun = 16;  // keys that share a page at least
 
 // threadIdx.x as a value of its own: what is formed from it is formed where it is
 // used, and not kept in registers across the units of a workgroup (which spill
-// for it: 1000 tokens after 1337, 28/4 heads of 128, F16 XX us, so YY).
+// for it: 1000 tokens after 1337 among 31 single tokens over 2667 to 4000 keys, 28/4
+// heads of 128, F16 189 us, so 122).
 __device__ __forceinline__ int thread_here() {
   int t = (int)threadIdx.x;
   asm volatile("" : "+v"(t));
@@ -205,7 +215,7 @@ struct Pages {
 // Pieces that a wave holds lie together: few rows' row by row, many rows' those of
 // 32 rows side by side. Written by one XCD, read by another, so with the cache bit
 // that goes past the L2s (8 bytes at a time, as atomics do, and with rows apart, a
-// prompt's chunk of 1000 tokens after 1337 took 137 us, not XX).
+// prompt's chunk of 1000 tokens after 1337 took 137 us, not 101).
 constexpr int kSc1 = 16;
 template <int D, int ROWS>
 struct Record {
@@ -680,8 +690,8 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (TreeCfg<D, KT, RT>::WAVES_PER_S
 // workgroup has a share of both; the first half of the workgroups begins with the one,
 // the second with the other, so that a CU that holds one of each has keys to
 // stream, which memory bounds, beside products (1000 tokens after 1337 among 31
-// single tokens over 2667 to 4000 keys, 28/4 heads of 128, F16: XX us, in two launches
-// 144).
+// single tokens over 2667 to 4000 keys, 28/4 heads of 128, F16: 122 to 125 us, in two
+// launches 144).
 template <int D, typename KT>
 struct MixedCfg {
   typedef LineCfg<D, KT, 1, false> Few;

@@ -15,6 +15,10 @@
 // more. Where a draft's token was turned down, what is left is a difference of
 // probabilities that has to be summed over the row first: verify_rest_kernel does
 // that with several workgroups a sequence, the last of which draws.
+//
+// Bound: for many rows the vector unit, 27 instructions a logit, 20 of them double
+// (384 rows of 151936: 54 us, 33 to read them; five fma fewer take 8 us less), for few
+// the three launches' chains of loads (six rows 13 us).
 #include <algorithm>
 
 #include "attn_common.h"
