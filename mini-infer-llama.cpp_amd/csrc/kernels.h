@@ -183,7 +183,7 @@ struct PagedLine {
   unsigned* arrived;
   int32_t least;
   int32_t spare;  // tiles more than its share that a workgroup takes so that none has two units
-  float join;  // what joining a part takes, in key tiles' time
+  float join, fixed;  // what joining takes for each part, and at all, in key tiles' time
 };
 struct PagedAttn {
   CacheView cache;

@@ -115,8 +115,7 @@ struct Units {
     const int last = min(((rt + 1) * ROWS - 1) / n_rep, n_new - 1);
     return (max(min(n_past + last + 1, n_seen), 1) + TK - 1) / TK;
   }
-  // What does not share a workgroup where places are padded, of a head (pairs do).
-  __device__ inline unsigned apart() const { return n_rt == 1 ? 1u : 1u << 10; }
+  __device__ inline int count() const { return n_rt; }  // of a head
   // Places of a head's units on the line: whole units, or their tiles; pairs and the
   // middle row tile in multiples of `pad`, so that no share of that size holds two.
   __device__ inline unsigned per_head(bool whole, unsigned pad) const {
@@ -152,7 +151,7 @@ template <int TK>
 struct OneUnit {
   int n_tiles_;
   __device__ inline OneUnit(const SeqLens& s, int) : n_tiles_((max(s.n_seen, 1) + TK - 1) / TK) {}
-  __device__ inline unsigned apart() const { return 1u; }
+  __device__ inline int count() const { return 1; }
   __device__ inline unsigned per_head(bool whole, unsigned pad) const { return whole ? 1u : padded((unsigned)n_tiles_, pad); }
   __device__ inline bool find(unsigned off, bool whole, unsigned pad, int& rt, int& n_tiles, int& tile, unsigned& left) const {
     rt = 0;
@@ -534,14 +533,16 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
   typedef LineCfg<D, KT, RT, WIDE> C;
   typedef typename std::conditional<WIDE, Units<C::ROWS, C::TK>, OneUnit<C::TK>>::type U;
   constexpr int ROWS = C::ROWS, TK = C::TK;
-  const bool whole = line.rec == nullptr;  // no records: no unit in parts
+  bool whole = line.rec == nullptr;  // no unit in parts, as there are no records
   unsigned pad = 1u;
-  unsigned apart = 0u;  // of the lane's sequences
+  unsigned n_units = 0u;  // of the lane's sequences and a head
+  bool pairs = false;     // of row tiles
   auto units_of = [&](const SeqLens& s) __attribute__((always_inline)) -> unsigned {
     const int rows = s.n_new * p.n_rep;
     if (rows == 0 || WIDE != (rows > p.few_rows)) return 0u;
     const U u(s, p.n_rep);
-    apart += u.apart();
+    n_units += (unsigned)u.count();
+    pairs = pairs || u.count() > 1;
     return u.per_head(whole, pad) * (unsigned)p.cache.n_head_kv;
   };
 
@@ -593,13 +594,20 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
       // per) `join` tiles' time, the least for per = sqrt(tiles join).
       const float tiles = wave_max_dpp((float)longest) * (1.f / TK);
       const unsigned want = rounds((unsigned)uniform((int)fminf(fmaxf((float)line.least, sqrtf(tiles * line.join)), ceilf(tiles))));
-      // Where these are fewer workgroups than there are, or a few tiles more a share
-      // are enough, none has two units.
+      const unsigned units = (unsigned)__builtin_amdgcn_readlane((int)wave_scan(n_units), 63) * (unsigned)p.cache.n_head_kv;
+      // Parts cost `fixed` tiles' time too: units up to that long stay whole while each
+      // has a workgroup of its own.
+      if (units <= n_wg && tiles <= 2.f * sqrtf(tiles * line.join) + line.fixed) {
+        whole = true;
+        per = 1u;
+        continue;
+      }
+      // Where shares of `want` are fewer than the workgroups, or a few tiles more a share
+      // make them so, none has two units.
       if (want > per) {
         per = pad = want;
       } else {
-        const unsigned units = (unsigned)__builtin_amdgcn_readlane((int)wave_scan(apart), 63) * (unsigned)p.cache.n_head_kv;
-        if (units > n_wg / 2 || total == 0u) break;
+        if (units > n_wg / 2 || total == 0u || __builtin_amdgcn_ballot_w64(pairs) != 0ull) break;
         pad = max(rounds((total - 1) / (n_wg - units / 2) + 1), per);
         if (pad - per > (unsigned)line.spare) {
           pad = 1u;
@@ -607,6 +615,7 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
         }
       }
     } else if (pass == 1) {
+      if (whole) break;
       if ((total + pad - 1) / pad <= n_wg) {
         per = pad;
         break;
@@ -749,6 +758,11 @@ static hipError_t launch_paged(PagedAttn p, float* parts, size_t part_bytes, uns
   p.few_rows = two ? 32 : 16;
   p.few.least = 8;
   p.many.least = D == 64 ? 2 : 4;
+  // In tiles (one of 32 keys in few rows is a wave's, F32's take longer): 500 keys of one
+  // token, 14/2 heads of 64, F16 whole 8.2 us, in parts 9.6; 100 tokens from nothing,
+  // 28/4 heads of 128, F16 21 and 31, timed alone.
+  p.few.fixed = (D == 64 ? 12.f : 8.f) - (sizeof(KT) == 4 ? 4.f : 0.f);
+  p.many.fixed = D == 64 && sizeof(KT) == 4 ? 1.f : 2.f;
   p.few.spare = mixed ? 0 : 4;
   p.many.spare = 1;
   p.few.join = D == 64 ? 0.35f : 0.5f;
