@@ -588,7 +588,7 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
     add_up(pass > 0);
     if (pass == 0) {
       per = max((total + n_wg - 1) / n_wg, 1u);
-      if (whole) break;
+      if (whole || total == 0u) break;
       per = rounds(per);
       // A unit's parts are joined some at a time, so a long one takes per + (tiles /
       // per) `join` tiles' time, the least for per = sqrt(tiles join).
@@ -607,7 +607,7 @@ __device__ __forceinline__ void run_line(const PagedAttn& p, const PagedLine& li
       if (want > per) {
         per = pad = want;
       } else {
-        if (units > n_wg / 2 || total == 0u || __builtin_amdgcn_ballot_w64(pairs) != 0ull) break;
+        if (units > n_wg / 2 || __builtin_amdgcn_ballot_w64(pairs) != 0ull) break;
         pad = max(rounds((total - 1) / (n_wg - units / 2) + 1), per);
         if (pad - per > (unsigned)line.spare) {
           pad = 1u;

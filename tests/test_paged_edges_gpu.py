@@ -101,6 +101,26 @@ def test_pages_shared_by_sequences(hip, stream, cache):
     b.close()
 
 
+@pytest.mark.parametrize("cache", list(KINDS))
+@pytest.mark.parametrize("d,hkv,rep,seqs", [
+    (64, 2, 7, [(1500 - 7 * i, 1) for i in range(64)]),               # shares a little larger, no workgroup with two units
+    (64, 2, 7, [(1500 - 11 * i, 6) for i in range(32)]),              # the same, more than 16 rows
+    (128, 4, 7, [(100, 100)]),                                        # row tiles of few keys, each whole
+    (128, 4, 7, [(250, 250)]),                                        # and of a few more, in parts
+    (128, 2, 7, [(1000 + i, 1) for i in range(8)] + [(300, 300)]),    # two short lines
+    (64, 2, 7, [(700, 1), (40, 1), (3, 1), (520, 30), (64, 64)]),
+    (64, 1, 7, [(40 + i % 90, 1) for i in range(300)] + [(20 + i % 50, 20) for i in range(300)]),  # more units than workgroups
+])
+def test_shares(hip, stream, cache, d, hkv, rep, seqs):
+    """Lengths on both sides of the rules by which units are cut into shares."""
+    b = Batch(hip, np.random.default_rng([d, len(seqs)]), cache, d, hkv, rep, 16, seqs, lead=1, tail=2)
+    got = b.run(stream)
+    b.check(got)
+    assert np.array_equal(got, b.run(stream))
+    b.check(b.run(stream, max_new=max(n for _, n in seqs)), "max_new")
+    b.close()
+
+
 def softmax_rows(rng, rows, vocab):
     x = rng.standard_normal((rows, vocab))
     e = np.exp(x - x.max(1, keepdims=True))
