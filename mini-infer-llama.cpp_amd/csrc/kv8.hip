@@ -21,6 +21,7 @@
 // F16 cache 23.4, 8-bit 23.8 (143 MB, of which the launch before has left a part in
 // the memory-side cache; among other passes 32.1, 4.4 TB/s); a few rows 2 to 4, a
 // launch's own time.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -370,8 +371,7 @@ hipError_t launch_kv_keep(const KvKeep& p, hipStream_t stream) {
 // P: NormRope (rows n_past + token of a cache, one position per token) or
 // PagedRope (rows by slots, positions by axes; a token without a row has its Q
 // written only). Positions of three axes cost no more than one's (1225 tokens, 28/4
-// heads of 128, 8-bit: 13.4 us, as with one axis; 8192 tokens, F16: 63 us, the rate of a
-// large copy). A workgroup's first rows on their way beside the angles were not faster
+// heads of 128, 8-bit: 11.0 us, as with one axis; 8192 tokens, F16: 58 us, 4.9 TB/s). A workgroup's first rows on their way beside the angles were not faster
 // with few tokens, and 10 us slower with 8192.
 __device__ inline int position_of(const NormRope& p, int t, int) { return p.pos ? gload<int>(p.pos + t) : p.n_past + t; }
 __device__ inline int position_of(const PagedRope& p, int t, int pair) {
@@ -612,16 +612,21 @@ static hipError_t launch_rope_rows(const P& p, hipStream_t stream) {
   if (p.n_dims == p.cache.head_dim && (!p.q || (rows_aligned(p.q, p.q_nb, 4) && rows_aligned(p.q_out, p.qo_nb, 4))) &&
       rows_aligned(p.k, p.k_nb, 4) && rows_aligned(p.v, p.v_nb, 4) && at16(p.q_norm) && at16(p.k_norm)) {
     if (p.n_tokens == 0) return hipSuccess;
-    // Up to two workgroups of kRopeTokens tokens per CU: a workgroup per 256 lanes'
-    // worth of one token's rows instead, more angles for more workgroups. 28/4 heads
-    // of 128, F16 cache (us): 64 tokens 3.5 (by fours 8.9), 1024 8.8 (11.7), 2048
-    // 15.6 (15.2), 4096 26.7 (23.8).
+    // A workgroup with rows for its lanes twice over, as far as kRopeTokens: one token of
+    // 28/4 heads of 128, four of 14/2 of 64, these in two workgroups, which have the same
+    // angles. Few tokens: one each, its rows in two workgroups, in more where that leaves
+    // CUs without. F16, three axes, timed alone (us), one token in 3 / 2 / 1 workgroups and
+    // four in one / two: 28/4 heads of 128, 600 tokens 11.6 / 10.8 / 11.6, 15.9 / 12.9, 1225
+    // 16.0 / 15.1 / 14.6, 18.5 / 15.4, 6000 54.1 / 50.2 / 48.6, 58.2 / 51.9; 14/2 heads of
+    // 64, 1225 tokens 9.9 in one, 11.1 / 10.2, 3000 14.3 and 13.0 / 13.0.
     const int per_tok = p.n_head + 2 * p.cache.n_head_kv, rows = 256 / (p.cache.head_dim / 8);
-    const bool few = p.n_tokens < 2 * 256 * kRopeTokens;
-    const dim3 grid((unsigned)(few ? p.n_tokens : (p.n_tokens + kRopeTokens - 1) / kRopeTokens),
-                    (unsigned)(few ? (per_tok + rows - 1) / rows : 1));
-    if (p.cache.head_dim == 64) hipLaunchKernelGGL((norm_rope_kernel<64, P>), grid, dim3(256), 0, stream, p, few ? 1 : kRopeTokens);
-    else hipLaunchKernelGGL((norm_rope_kernel<128, P>), grid, dim3(256), 0, stream, p, few ? 1 : kRopeTokens);
+    const int most = std::min(std::max((2 * rows + per_tok - 1) / per_tok, 1), kRopeTokens);
+    const bool few = p.n_tokens < (most == 1 ? 768 : 384 * most);
+    const int tokens = few ? 1 : most, pieces = (tokens * per_tok + rows - 1) / rows;
+    const int wgs = few && p.n_tokens * pieces <= 256 ? pieces : std::min(few || most > 1 ? 2 : 1, pieces);
+    const dim3 grid((unsigned)((p.n_tokens + tokens - 1) / tokens), (unsigned)wgs);
+    if (p.cache.head_dim == 64) hipLaunchKernelGGL((norm_rope_kernel<64, P>), grid, dim3(256), 0, stream, p, tokens);
+    else hipLaunchKernelGGL((norm_rope_kernel<128, P>), grid, dim3(256), 0, stream, p, tokens);
     return hipGetLastError();
   }
   const int64_t rows = (int64_t)p.n_tokens * (p.n_head + 2 * p.cache.n_head_kv);
