@@ -700,11 +700,11 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (TreeCfg<D, KT, RT>::WAVES_PER_S
 }
 
 // Sequences of any number of rows: up to 16 on one line, more on another. A
-// workgroup has a share of both; the first half of the workgroups begins with the one,
-// the second with the other, so that a CU that holds one of each has keys to
+// workgroup has a share of both; the second half of the workgroups begins with the one,
+// the first with the other, so that a CU that holds one of each has keys to
 // stream, which memory bounds, beside products (1000 tokens after 1337 among 31
-// single tokens over 2667 to 4000 keys, 28/4 heads of 128, F16: 122 to 125 us, in two
-// launches 144).
+// single tokens over 2667 to 4000 keys, 28/4 heads of 128, F16: 117 us, the halves the
+// other way round 124 to 127, in two launches 144).
 template <int D, typename KT>
 struct MixedCfg {
   typedef LineCfg<D, KT, 1, false> Few;
@@ -716,7 +716,7 @@ __global__ __launch_bounds__(kTreeWaves* kWave, (WideCfg<D, KT>::WAVES_PER_SIMD)
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   lds_t* const lds = (lds_t*)lds_raw;
   lds_t* const state = lds + MixedCfg<D, KT>::LDS;
-  const bool few_first = 2 * blockIdx.x < gridDim.x;
+  const bool few_first = 2 * blockIdx.x >= gridDim.x;
 #pragma unroll 1
   for (int turn = 0; turn < 2; ++turn) {
     if ((turn == 0) == few_first) run_line<D, KT, 1, false>(p, p.few, lds, state);
