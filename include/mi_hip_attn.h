@@ -513,7 +513,8 @@ int mi_hip_paged_append(const mi_hip_paged_append_args* args);
  * clamped: q_off to [0, n_tokens], n_kv to [0, max_pages * page_size]; of a sequence
  * with more than max_new queries the rest are left as they were. Products, sums and
  * values that are not finite as in mi_hip_attn_tree, with the choice of kernel per
- * sequence (n_rep times its queries up to 32, or more). The same bits on every
+ * sequence: few query rows (n_rep times its queries) are up to 16, or up to 32 where
+ * max_new allows no sequence more, others the rows beyond. The same bits on every
  * run with the same lengths. At most 2^20 sequences, 2^26 query rows (tokens times
  * heads), 2^30 positions of a sequence, and 2^31 tiles of 32 positions in all
  * (MI_HIP_E_UNSUPPORTED). Scratch for joining the parts of long sequences: ws,

@@ -1,5 +1,5 @@
 """Distances of the vector instructions that the paged attention kernels issue as inline asm (CPU only;
-hipcc cross-compiles). tests/test_asm_hazards.py pins the checker."""
+hipcc cross-compiles). The scan itself is pinned by tests/test_asm_hazards.py."""
 import os
 import shutil
 import subprocess
