@@ -351,7 +351,7 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
   __device__ __forceinline__ void join(const floatx16 (&own)[NDB], float ref, float l, bool active) const {
     const int tid = thread_here(), lane = tid % kWave, kh = lane / 32;
     const int r = 32 * uniform(tid / kWave) + lane % 32;
-    if (active) {
+    if (active && this->row0 + r < this->rows) {
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -370,7 +370,7 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
   __device__ __forceinline__ void add_up(int block, int db0, int lane) const {
     typedef Record<D, Base::kRows> R;
     const int r = 32 * block + lane % 32, kh = lane / 32, row = this->row0 + r, n = this->parts;
-    if (this->row0 + 32 * block >= this->rows) return;
+    if (row >= this->rows) return;
     const rsrc_t recs = make_rsrc(this->first_record(), (unsigned)(2 * n - 1) * R::BYTES);
     f32x4 acc[DBS][4];
 #pragma unroll
@@ -403,7 +403,6 @@ struct ManyRows : UnitRows<D, KT, WideCfg<D, KT>::ROWS> {
           for (int q = 0; q < 4; ++q) acc[db][q] = acc[db][q] * a + x[e][db][q] * b;
       }
     }
-    if (row >= this->rows) return;
     const int token = row / this->n_rep;
     const float inv = top == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;
     char* const out = this->out_row(token, row - token * this->n_rep);
