@@ -71,7 +71,9 @@ __global__ __launch_bounds__(kSeqs) void page_tables_kernel(const PageTables p) 
   __shared__ Shared s;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const unsigned n_pages = (unsigned)p.n_pages;
-  const unsigned at = blockIdx.x * kSeqs + tid, step = gridDim.x * kSeqs;  // of the pages and the tokens
+  // Of the pages and the tokens, in 64 bits: the running sums may be any 32 bits, and a
+  // start that wrapped would fall on what belongs to the sequences before.
+  const uint64_t at = blockIdx.x * kSeqs + tid, step = gridDim.x * kSeqs;
   const bool writes = blockIdx.x == 0;
   const int head0 = p.ring_at[0], tail0 = p.ring_at[1];
   unsigned tokens = 0, taken = 0, given = 0, granted = 0;  // before the sequences at hand
@@ -140,21 +142,24 @@ __global__ __launch_bounds__(kSeqs) void page_tables_kernel(const PageTables p) 
     __syncthreads();
     granted = s.granted;
     // Pages taken by these sequences: page k of the ring's.
-    for (unsigned k = taken + at; k < granted; k += step) {
+    for (uint64_t k64 = taken + at; k64 < granted; k64 += step) {
+      const unsigned k = (unsigned)k64;
       const int q = find(s.take_end, n, k);
       int* const row = reinterpret_cast<int*>(p.table + (int64_t)(first + q) * p.table_nb);
       row[s.need[q] - (int)(s.take_end[q] - k)] = p.ring[(head + k) % n_pages];
     }
     // Pages given back.
     const unsigned given_end = s.give_end[kSeqs - 1];
-    for (unsigned k = given + at; k < given_end; k += step) {
+    for (uint64_t k64 = given + at; k64 < given_end; k64 += step) {
+      const unsigned k = (unsigned)k64;
       const int q = find(s.give_end, n, k);
       const int* const row = reinterpret_cast<const int*>(p.table + (int64_t)(first + q) * p.table_nb);
       p.ring[(head + n_free + k) % n_pages] = row[s.held[q] - (int)(s.give_end[q] - k)];
     }
     // Tokens.
     const unsigned q_end = min(s.q_end[kSeqs - 1], most);
-    for (unsigned t = tokens + at; t < q_end; t += step) {
+    for (uint64_t t64 = tokens + at; t64 < q_end; t64 += step) {
+      const unsigned t = (unsigned)t64;
       const int q = find(s.q_end, n, t);
       const int pos = (int)((unsigned)s.cached[q] + (t - (s.q_end[q] - (unsigned)s.fresh[q])));
       int slot = -1;
@@ -179,7 +184,7 @@ __global__ __launch_bounds__(kSeqs) void page_tables_kernel(const PageTables p) 
     n_free = (unsigned)max((int64_t)0, min((int64_t)tail0 - head0, (int64_t)p.n_pages));
   }
   // The batch's padding.
-  for (unsigned t = min(tokens, (unsigned)p.max_tokens) + at; t < (unsigned)p.max_tokens; t += step) {
+  for (uint64_t t = min(tokens, (unsigned)p.max_tokens) + at; t < (unsigned)p.max_tokens; t += step) {
     p.slots[t] = -1;
     if (p.pos) p.pos[t] = 0;
     if (p.seq) p.seq[t] = -1;

@@ -145,3 +145,24 @@ def test_steps_of_a_server_in_a_graph(hip, stream):
         s["cached"], s["new"] = np.where(kept < 500, kept, 0), rng.integers(0, 30, n)
         c.inputs["cached"].copy_(dev(s["cached"].astype(np.int32)))
         c.inputs["new"].copy_(dev(s["new"].astype(np.int32)))
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("spare", [3, 6000])
+def test_long_requests_before_more_sequences(hip, stream, in_place, spare):
+    """Requests whose tokens together pass 32 bits stand among the first 1024 sequences of 2100: they, and
+    those behind them, do not fit the batch, and the ones before keep their rows. (6000 tokens: the
+    tables have several workgroups.)"""
+    rng = np.random.default_rng(21)
+    n, big = 2100, 2 ** 31 - 1
+    cached, new, held = requests(rng, n, 16, 60, 9)
+    new[0] = 5
+    new[[500, 600, 700, 1023]] = big
+    rows = int(new[:500].sum())
+    s = state(rng, n, 16, cached, np.where(new == big, 0, new), held, 6000, width=10)
+    s.update(new=new, max_tokens=rows + spare)
+    c = Call(s, stream, in_place)
+    hip.check(hip.mi_hip_page_tables(ctypes.byref(c.args)))
+    want, got = ref.page_tables(**s), c.got()
+    assert want["n_kv"][:500].any() and (want["slots"][:rows] >= 0).any()
+    same(got, want)
