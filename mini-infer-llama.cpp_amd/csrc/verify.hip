@@ -258,7 +258,7 @@ struct Remainder {
   float top;
   double scale, inv;  // inv: 1 / the sum of the weights
   int n_vocab;
-  const int *token, *down;  // n_out tokens that are left out: token[down[e]]
+  const int *token, *down;  // n_out tokens of the vocabulary that are left out: token[down[e]]
   int n_out;
 
   struct Tokens {
@@ -435,7 +435,8 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const Verify 
         left = 1.0;
       } else {
         left -= pc;
-        s.down[n_down++] = c;
+        // (a token outside the vocabulary takes nothing off the row, and has no chunk of it)
+        if (DRAFT || (unsigned)s.token[c] < (unsigned)p.n_vocab) s.down[n_down++] = c;
       }
     }
     s.f->cur = cur;
@@ -469,14 +470,11 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const Verify 
   const Remainder<CHUNK, false> row{x, nullptr, top, scale, 0.0, p.n_vocab, s.token, s.down, DRAFT ? 0 : n_down};
   // Chunks that tokens turned down have left are summed anew (into s.prob, by the token).
   for (int e = 0; e < row.n_out; ++e) {
-    const int t = s.token[s.down[e]];
-    double all = 0.0;
-    if ((unsigned)t < (unsigned)p.n_vocab) {
-      typename Remainder<CHUNK, false>::Tokens v;
-      double w[Remainder<CHUNK, false>::PER];
-      row.load(t / CHUNK, v);
-      all = block_total(s, row.rest(t / CHUNK, v, w));
-    }
+    const int chunk = s.token[s.down[e]] / CHUNK;
+    typename Remainder<CHUNK, false>::Tokens v;
+    double w[Remainder<CHUNK, false>::PER];
+    row.load(chunk, v);
+    const double all = block_total(s, row.rest(chunk, v, w));
     if (tid == 0) s.prob[e] = all;
   }
   __syncthreads();

@@ -365,3 +365,28 @@ def test_rows_beyond_the_workspace(hip, stream):
     a = c.call(hip, stream)
     a.n_rows = 2 ** 31 - 1
     assert hip.mi_hip_verify_draft(ctypes.byref(a)) == 5 and "workspace" in hip.last_error()
+
+
+@pytest.mark.parametrize("vocab", [500, 9000, 60000])
+@pytest.mark.parametrize("kind", ["chain", "tree", "draft"])
+def test_tokens_outside_the_vocabulary_leave_it_whole(hip, stream, vocab, kind):
+    """Drafted tokens that are no tokens are turned down, and nothing is missing from what the next one is drawn
+    from: neither the vocabulary's first tokens nor its last ones."""
+    rng = np.random.default_rng([vocab, len(kind)])
+    none = np.array([-1, -2, -2047, -4097, -2 ** 31, vocab, vocab + 1, 2 ** 31 - 1])
+    n, nodes = 64, 4 if kind == "tree" else 2
+    off = np.arange(n + 1) * nodes
+    logits = rng.standard_normal((n * nodes, vocab)).astype(np.float32)
+    token = rng.choice(none, n * nodes)
+    parent = draft = None
+    if kind == "tree":
+        parent = np.zeros(n * nodes, np.int32)
+        token[3::4] = logits[0::4].argmax(1)  # one that is, among those that are not
+    if kind == "draft":
+        draft, _ = draft_rows(rng, logits, off, 1.0)
+    u = rng.random(n * nodes).astype(np.float32)
+    u[0::nodes] = (np.arange(n) + 0.5) / n  # draws from all of the vocabulary
+    c = Case(logits, off, token, u, parent, draft)
+    got = c.run(hip, stream)
+    assert c.check(got) <= 1
+    assert (got[2][:, 0] >= 0).all() and got[2][:, 0].min() < vocab // 8 and got[2][:, 0].max() >= vocab - vocab // 8
