@@ -86,11 +86,12 @@ struct SeqLens {
 __device__ inline SeqLens seq_lens(const PagedAttn& p, int i) {
   SeqLens s{0, 0, 0, 0};
   if (i < p.n_seq) {
-    const int a = min(max(gload<int>(p.q_off + i), 0), p.n_tokens), b = min(gload<int>(p.q_off + i + 1), p.n_tokens);
+    // (the end at the start at least: the difference of any two numbers may leave 32 bits)
+    const int a = min(max(gload<int>(p.q_off + i), 0), p.n_tokens), b = min(max(gload<int>(p.q_off + i + 1), a), p.n_tokens);
     const int n_kv = min(max(gload<int>(p.n_kv + i), 0), p.max_kv);
     s.q0 = a;
-    s.n_new = min(max(b - a, 0), p.max_new);
-    s.n_past = n_kv - max(b - a, 0);
+    s.n_new = min(b - a, p.max_new);
+    s.n_past = n_kv - (b - a);
     s.n_seen = max(s.n_past + s.n_new, 0);
   }
   return s;

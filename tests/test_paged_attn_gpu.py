@@ -316,3 +316,27 @@ def test_refusals(hip, stream):
     assert (b.out == 7.5).all()
     hip.check(hip.mi_hip_kv_destroy(plain))
     b.close()
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_offsets_at_the_end_of_their_type(hip, stream, new):
+    """An offset of -2^31 counts as 0: the sequence that ends there has no queries, the next one begins at row 0.
+    max_new reaches beyond the rows that there are, which guards hold."""
+    import torch
+    b = Batch(hip, np.random.default_rng(14), "f16", 64, 2, 3, 16, [(100, 4), (50, 2), (90, new)])
+    rows = b.t - 2
+    guarded = torch.full((rows + 80,) + tuple(b.out.shape[1:]), 7.5, device="cuda")
+    q = torch.zeros_like(guarded)
+    q[:rows] = b.dq[:rows]
+    outs = []
+    for low in (0, -1, -2 ** 31, -2 ** 31 + 3):
+        b.dq_off.copy_(dev(np.array([6, low, 4, rows], np.int32)))
+        guarded.fill_(7.5)
+        a = mh.paged_attn_args(b.kv, 1, q[:rows], guarded[:rows], b.dq_off, b.dn_kv, b.dtable, b.scale, stream,
+                               max_new=0 if new == 1 else 64)
+        hip.check(hip.mi_hip_attn_paged(ctypes.byref(a)))
+        torch.cuda.synchronize()
+        outs.append(guarded.cpu().numpy())
+        assert (outs[-1][rows:] == 7.5).all()
+        assert all(np.array_equal(x, outs[0]) for x in outs)
+    b.close()
