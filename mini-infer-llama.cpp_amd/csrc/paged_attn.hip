@@ -459,6 +459,11 @@ __device__ __forceinline__ void join_parts(const U& u, int n_rows, lds_t* lds) {
   const int tid = thread_here(), units = n_rows * (D / 4);
   const int n = u.parts;
   const rsrc_t recs = make_rsrc(u.first_record(), (unsigned)(2 * n - 1) * R::BYTES);
+  // A thread's part in LDS: four dims, and behind those of all threads its reference and sum.
+  constexpr int kDims = 16, kPair = 8, kSums = THREADS * kDims;
+  static_assert(kDims % alignof(f32x4) == 0 && kPair % alignof(f32x2) == 0 && kSums % alignof(f32x2) == 0,
+                "every thread's part has its type's alignment");
+  static_assert(kSums + THREADS * kPair <= TreeCfg<D, float, 1>::LDS, "they fit the kernel's LDS");
   int groups = 1;
   while (units * groups * 2 <= THREADS) groups *= 2;
   const int span = THREADS / groups, grp = tid / span;
@@ -491,8 +496,8 @@ __device__ __forceinline__ void join_parts(const U& u, int n_rows, lds_t* lds) {
       }
     }
     if (groups > 1) {  // (every thread has at most one unit)
-      lds_store<f32x4>(lds + tid * 24, acc);
-      lds_store<f32x2>(lds + tid * 24 + 16, f32x2{m, l});
+      lds_store<f32x4>(lds + tid * kDims, acc);
+      lds_store<f32x2>(lds + kSums + tid * kPair, f32x2{m, l});
     } else {
       finish(i, acc, m, l);
     }
@@ -501,13 +506,13 @@ __device__ __forceinline__ void join_parts(const U& u, int n_rows, lds_t* lds) {
   __syncthreads();
   if (tid >= units) return;
   float m = -INFINITY, l = 0.f;
-  for (int o = 0; o < groups; ++o) m = fmaxf(m, lds_load<float>(lds + (tid + o * span) * 24 + 16));
+  for (int o = 0; o < groups; ++o) m = fmaxf(m, lds_load<float>(lds + kSums + (tid + o * span) * kPair));
   const float mu = m == -INFINITY ? 0.f : m;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int o = 0; o < groups; ++o) {
-    const f32x2 ml = lds_load<f32x2>(lds + (tid + o * span) * 24 + 16);
+    const f32x2 ml = lds_load<f32x2>(lds + kSums + (tid + o * span) * kPair);
     const float y = fast_exp2(ml[0] - mu);
-    acc += lds_load<f32x4>(lds + (tid + o * span) * 24) * y;
+    acc += lds_load<f32x4>(lds + (tid + o * span) * kDims) * y;
     l += ml[1] * y;
   }
   finish(tid, acc, m, l);
