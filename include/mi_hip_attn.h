@@ -437,6 +437,8 @@ int mi_hip_attn_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* mask
  *     its page is none), position and sequence; -1, 0 and -1 from q_off[n_seq] to
  *     max_tokens (a batch that is padded). pos and seq may be NULL;
  *   n_refused: how many sequences are refused, or NULL.
+ * A refused sequence's tokens keep their places in the batch, without rows: what
+ * mi_hip_verify_draft says of them does not count, its cached length stays as it is.
  * Negative lengths count as 0. No other memory of the call may overlap what it
  * writes (with held or ring_at in place one workgroup does the whole call, else
  * large batches have several). Calls on one pool must be ordered. May be captured into a graph. No
