@@ -439,6 +439,9 @@ int mi_hip_attn_tree(const mi_hip_attn_args* items, const mi_hip_tree_mask* mask
  *   n_refused: how many sequences are refused, or NULL.
  * A refused sequence's tokens keep their places in the batch, without rows: what
  * mi_hip_verify_draft says of them does not count, its cached length stays as it is.
+ * Each page is free or held by one sequence, and once: the call does not count a
+ * page's users, and one that is held twice would be given back twice. Pages that
+ * sequences share stay out of it (table may begin behind them).
  * Negative lengths count as 0. No other memory of the call may overlap what it
  * writes (with held or ring_at in place one workgroup does the whole call, else
  * large batches have several). Calls on one pool must be ordered. May be captured into a graph. No

@@ -1,5 +1,5 @@
 """Steps of a server over a paged cache as the integration guide describes them: sequences that are refused
-for want of pages, and prompts among chains of drafted tokens."""
+for want of pages, prompts among chains of drafted tokens, and pages that sequences share."""
 import ctypes
 
 import numpy as np
@@ -114,4 +114,56 @@ def test_refused_sequences_and_prompts_among_chains(hip, stream, kind, captured,
         free = s.ring.cpu().numpy()[np.arange(*at) % n_pages]
         assert np.array_equal(np.sort(np.concatenate([table[i, :held[i]] for i in range(n)] + [free])), np.arange(n_pages))
     assert waited > 0  # some were refused, and granted later
+    s.close()
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_pages_of_a_common_prompt(hip, stream, kind):
+    """Two pages of a prompt stand in front of every table row and outside of what the tables' call manages: its
+    rows begin behind them, and positions and lengths get theirs added. They are never given back or dealt."""
+    import torch
+    n, n_pages, lead, d, hkv, rep = 4, 30, 2, 64, 2, 7
+    s = Server(hip, kind, n, n_pages, 60, 10, d, hkv, rep, 1, 6, 100, 4)
+    ring = s.ring.cpu().numpy()
+    shared, front = ring[:lead].copy(), lead * PAGE
+    s.ring_at.copy_(dev(np.array([lead, n_pages], np.int32)))  # two pages are with the prompt
+    s.table[:, :lead] = dev(shared)
+    rng = np.random.default_rng(8)
+    pk, pv = (rng.standard_normal((front, hkv, d)).astype(np.float32) for _ in range(2))
+    slots = (shared[np.arange(front) // PAGE] * PAGE + np.arange(front) % PAGE).astype(np.int32)
+    a = mh.paged_append_args(s.kv, 0, d, 1e6, stream, dev(pk), dev(pv), dev(slots), dev(np.arange(front, dtype=np.int32)), freq=s.freq,
+                             k_norm=s.wk, eps=1e-6)
+    hip.check(hip.mi_hip_paged_append(ctypes.byref(a)))
+    torch.cuda.synchronize()
+    prompt = [s.rows(0, w, 0, front, stream) for w in (0, 1)]
+    cached = np.zeros(n, int)  # without the prompt
+    for turn in range(8):
+        new = rng.integers(1, 16, n)
+        if turn in (3, 5):  # requests end
+            cached[turn % n], new[turn % n] = 0, 0
+        s.cached.copy_(dev(cached.astype(np.int32)))
+        s.new.copy_(dev(new.astype(np.int32)))
+        gen = torch.Generator(device="cuda").manual_seed(turn)
+        for x in (s.q, s.k, s.v):
+            x.copy_(torch.randn(x.shape, device="cuda", generator=gen))
+        a = mh.page_tables_args(PAGE, s.cached, s.new, s.held, s.held, s.table[:, lead:], s.ring, s.ring_at, s.ring_at, s.n_kv,
+                                s.q_off, s.slots, stream, pos=s.pos, n_refused=s.refused)
+        hip.check(hip.mi_hip_page_tables(ctypes.byref(a)))
+        s.pos.add_(front)
+        s.n_kv.copy_(torch.where(s.n_kv > 0, s.n_kv + front, torch.zeros_like(s.n_kv)))
+        s.attend(stream, max_new=15)
+        torch.cuda.synchronize()
+        assert s.refused.item() == 0
+        off, n_kv = s.q_off.cpu().numpy(), s.n_kv.cpu().numpy()
+        assert np.array_equal(n_kv, np.where(new > 0, front + cached + new, 0))
+        for i in np.nonzero(new)[0]:
+            rows = slice(int(off[i]), int(off[i + 1]))
+            assert np.array_equal(s.pos.cpu().numpy()[rows], front + cached[i] + np.arange(new[i]))
+            check_attention(s, 0, i, int(n_kv[i]), rows, stream, (turn, i))
+            assert all(np.array_equal(s.rows(0, w, i, front, stream), prompt[w]) for w in (0, 1))
+        cached += new
+        held, table, at = s.held.cpu().numpy(), s.table.cpu().numpy(), s.ring_at.cpu().numpy()
+        free = s.ring.cpu().numpy()[np.arange(*at) % n_pages]
+        owned = np.concatenate([table[i, lead:lead + held[i]] for i in range(n)] + [free, shared])
+        assert np.array_equal(np.sort(owned), np.arange(n_pages)) and (table[:, :lead] == shared).all()
     s.close()
