@@ -104,13 +104,13 @@ typedef struct mi_hip_workspace_desc {
 
 /* One device allocation covering any decode launch of up to 32 items of this
  * head shape (mi_hip_attn_decode_batch's limit per launch) and, with 17 MB (head_dim
- * 64) or 34 MB of parts, any call of mi_hip_attn_tree, mi_hip_attn_paged,
- * mi_hip_verify_draft and mi_hip_logits_adjust. Where the allocation limit or the
- * device has no room for the parts, a workspace (a cache's own and the default one
- * too) is made without them: mi_hip_attn_tree and mi_hip_attn_paged then keep each
- * sequence's keys in one piece, which is slow over long caches, and
- * mi_hip_logits_adjust's ids and mi_hip_verify_draft are refused with it
- * (MI_HIP_E_UNSUPPORTED). */
+ * 64) or 34 MB of parts, any call of mi_hip_attn_tree, mi_hip_attn_paged and
+ * mi_hip_logits_adjust, and those of mi_hip_verify_draft whose scratch (the size is
+ * given there) the parts hold. Where the allocation limit or the device has no room
+ * for the parts, a workspace (a cache's own and the default one too) is made without
+ * them: mi_hip_attn_tree and mi_hip_attn_paged then keep each sequence's keys in one
+ * piece, which is slow over long caches, and mi_hip_logits_adjust's ids and
+ * mi_hip_verify_draft are refused with it (MI_HIP_E_UNSUPPORTED). */
 int mi_hip_workspace_create(const mi_hip_workspace_desc* desc, mi_hip_workspace** out);
 int mi_hip_workspace_destroy(mi_hip_workspace* ws);
 
@@ -572,9 +572,11 @@ int mi_hip_attn_paged(const mi_hip_attn_paged_args* args);
  * (then no child is accepted either), and where every w is 0; child tokens outside
  * [0, n_vocab) are turned down. u is clamped to [0, 1), a NaN to 0; a temperature of
  * +infinity has all finite logits alike, a negative one or NaN counts as 0. Scratch:
- * the parts of ws, else of the library default (MI_HIP_E_UNSUPPORTED where they do
- * not hold 16 bytes for each 2048 logits); calls that share one must be ordered. May be captured into a graph. No counterpart in the
- * reference. */
+ * the parts of ws, else of the library default (34 MB); of them a call takes, with
+ * c = n_vocab / 2048 rounded up, at most 16 c n_rows + (8 c + 40) min(n_seq, 1024)
+ * bytes, and is refused where they hold less than it takes (MI_HIP_E_UNSUPPORTED).
+ * Calls that share one must be ordered. May be captured into a graph. No counterpart
+ * in the reference. */
 typedef struct mi_hip_verify_args {
   const float* logits;      /* device, n_rows rows of n_vocab */
   size_t nb;                /* bytes between rows */

@@ -390,3 +390,29 @@ def test_tokens_outside_the_vocabulary_leave_it_whole(hip, stream, vocab, kind):
     got = c.run(hip, stream)
     assert c.check(got) <= 1
     assert (got[2][:, 0] >= 0).all() and got[2][:, 0].min() < vocab // 8 and got[2][:, 0].max() >= vocab - vocab // 8
+
+
+@pytest.mark.parametrize("vocab,rows", [(1, 1000000), (4097, 250000)])
+def test_scratch_that_the_header_gives(hip, stream, vocab, rows):
+    """A call of the header's size is taken by the 17 MB of parts of a workspace for heads of 64, of which it
+    asks for most; one of four times the rows is refused."""
+    import torch
+    n, c = 1000, -(-vocab // 2048)
+    assert 12e6 < 16 * c * rows + (8 * c + 40) * n < 17e6
+    ws = hip.workspace_create(2, 14, 64)
+    i32 = lambda *s: torch.full(s, -9, dtype=torch.int32, device="cuda")
+    # every u is 0, so every node is accepted as far as the paths go
+    logits, u = torch.zeros(rows, vocab, device="cuda"), torch.zeros(rows, device="cuda")
+    token, off = torch.zeros(rows, dtype=torch.int32, device="cuda"), dev((np.arange(n + 1) * (rows // n)).astype(np.int32))
+    n_path, path, tokens = i32(n), i32(n, 3), i32(n, 3)
+    a = mh.verify_args(logits, off, token, u, n_path, path, tokens, stream, ws=ws)
+    a.n_rows = 4 * rows
+    assert hip.mi_hip_verify_draft(ctypes.byref(a)) == 5 and "parts" in hip.last_error()
+    torch.cuda.synchronize()
+    assert bool((n_path == -9).all())
+    a.n_rows = rows
+    hip.check(hip.mi_hip_verify_draft(ctypes.byref(a)))
+    torch.cuda.synchronize()
+    assert bool((n_path == 3).all()) and bool((tokens == 0).all())
+    assert bool((path == torch.arange(3, device="cuda")).all())
+    hip.check(hip.mi_hip_workspace_destroy(ws))
