@@ -475,6 +475,7 @@ __global__ __launch_bounds__(256) void norm_rope_row_kernel(const P p) {
 // quantised, since a value next to a border between two steps should not cross
 // it by a rounding.
 constexpr int kRopeTokens = 4;
+constexpr int kRopeWgs = 5 * 256;  // up to which more workgroups help
 
 template <int D, typename P>
 __global__ __launch_bounds__(256) void norm_rope_kernel(const P p, int tokens) {
@@ -613,18 +614,25 @@ static hipError_t launch_rope_rows(const P& p, hipStream_t stream) {
       rows_aligned(p.k, p.k_nb, 4) && rows_aligned(p.v, p.v_nb, 4) && at16(p.q_norm) && at16(p.k_norm)) {
     if (p.n_tokens == 0) return hipSuccess;
     // A workgroup with rows for its lanes twice over, as far as kRopeTokens: one token of
-    // 28/4 heads of 128, four of 14/2 of 64, these in two workgroups, which have the same
-    // angles. Few tokens: one each, its rows in two workgroups, in more where that leaves
-    // CUs without. F16, three axes, timed alone (us), one token in 3 / 2 / 1 workgroups and
-    // four in one / two: 28/4 heads of 128, 600 tokens 11.6 / 10.8 / 11.6, 15.9 / 12.9, 1225
-    // 16.0 / 15.1 / 14.6, 18.5 / 15.4, 6000 54.1 / 50.2 / 48.6, 58.2 / 51.9; 14/2 heads of
-    // 64, 1225 tokens 9.9 in one, 11.1 / 10.2, 3000 14.3 and 13.0 / 13.0.
+    // 28/4 heads of 128, four of 14/2 of 64. Few tokens: one each, its rows in as many
+    // workgroups as take one round, while there are kRopeWgs at most, else in two. The
+    // others' rows in two workgroups, which have the same angles, while there are kRopeWgs
+    // at most or each has a round and a half. F16, three axes, timed alone (us), one token
+    // in 3 / 2 / 1 workgroups and four in one / two: 28/4 heads of 128, 600 tokens 11.6 /
+    // 10.8 / 11.6, 15.9 / 12.9, 1225 16.0 / 15.1 / 14.6, 18.5 / 15.4, 6000 54.1 / 50.2 /
+    // 48.6, 58.2 / 51.9. One axis, F16 and 8-bit cache, many in a row: 256 tokens of 32/8
+    // heads of 128 in 3 / 2 workgroups 4.5 / 4.9 and 5.4 / 5.8, 512 7.7 / 7.1 and 9.0 / 8.1;
+    // four tokens of 14/2 heads of 64 in one / two, 2048 7.8 / 6.5 and 10.3 / 7.8, 4096 9.9 /
+    // 9.9 and 12.8 / 12.5; of 8/1 heads of 64, 2048 5.1 / 4.7 and 6.7 / 6.7, 4096 7.5 / 8.3
+    // and 9.6 / 11.3.
     const int per_tok = p.n_head + 2 * p.cache.n_head_kv, rows = 256 / (p.cache.head_dim / 8);
     const int most = std::min(std::max((2 * rows + per_tok - 1) / per_tok, 1), kRopeTokens);
     const bool few = p.n_tokens < (most == 1 ? 768 : 384 * most);
     const int tokens = few ? 1 : most, pieces = (tokens * per_tok + rows - 1) / rows;
-    const int wgs = few && p.n_tokens * pieces <= 256 ? pieces : std::min(few || most > 1 ? 2 : 1, pieces);
-    const dim3 grid((unsigned)((p.n_tokens + tokens - 1) / tokens), (unsigned)wgs);
+    const int groups = (p.n_tokens + tokens - 1) / tokens;
+    const bool two = few || 2 * groups <= kRopeWgs || tokens * per_tok >= 3 * rows;
+    const int wgs = few && p.n_tokens * pieces <= kRopeWgs ? pieces : std::min(two ? 2 : 1, pieces);
+    const dim3 grid((unsigned)groups, (unsigned)wgs);
     if (p.cache.head_dim == 64) hipLaunchKernelGGL((norm_rope_kernel<64, P>), grid, dim3(256), 0, stream, p, tokens);
     else hipLaunchKernelGGL((norm_rope_kernel<128, P>), grid, dim3(256), 0, stream, p, tokens);
     return hipGetLastError();

@@ -206,3 +206,29 @@ def test_refusals(hip, stream):
     assert rc(n_tokens=0) == 0
     torch.cuda.synchronize()
     hip.check(hip.mi_hip_kv_destroy(kv))
+
+
+@pytest.mark.parametrize("cache", list(KINDS))
+@pytest.mark.parametrize("d,hkv,h,t", [
+    (64, 2, 14, 1535), (64, 2, 14, 2559), (64, 1, 8, 2561), (64, 2, 14, 3003), (64, 16, 16, 767), (64, 16, 16, 3001),
+    (128, 4, 28, 426), (128, 4, 28, 427), (128, 4, 28, 769), (128, 8, 32, 200), (128, 1, 1, 2562)])
+def test_workgroups_of_any_split_give_the_same_bits(hip, stream, cache, d, hkv, h, t):
+    """Token counts on both sides of the rules that give workgroups their tokens and rows, against calls of 61
+    tokens each, whose workgroups have one."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(t)
+    q, k, v = (torch.randn((t, n, d), device="cuda", generator=g) for n in (h, hkv, hkv))
+    w, n_past = dev(np.linspace(0.5, 1.5, d).astype(np.float32)), 9
+    kv = hip.kv_create(2, n_past + t, hkv, d, h, KINDS[cache])
+    outs = [torch.full_like(q, 7.5) for _ in range(2)]
+    for layer, step in ((0, t), (1, 61)):
+        for i in range(0, t, step):
+            a = mh.norm_rope_args(kv, layer, n_past + i, d, 1e6, stream, k[i:i + step], v[i:i + step], q=q[i:i + step],
+                                  q_out=outs[layer][i:i + step], q_norm=w, k_norm=w, eps=EPS)
+            hip.check(hip.mi_hip_norm_rope_append(ctypes.byref(a)))
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[1])
+    for which in (0, 1):
+        one, many = (read(hip, kv, layer, which, 0, n_past + t, hkv, d, stream) for layer in (0, 1))
+        assert np.array_equal(one, many) and one[n_past:].any() and not one[:n_past].any()
+    hip.check(hip.mi_hip_kv_destroy(kv))
