@@ -108,8 +108,10 @@ struct Units {
   __device__ inline Units(const SeqLens& s, int rep) : n_past(s.n_past), n_new(s.n_new), n_seen(s.n_seen), n_rep(rep) {
     n_rt = (s.n_new * rep + ROWS - 1) / ROWS;
     // The two row tiles see at most 2 n_past + ((n_rt + 1) ROWS - 2) / n_rep + 2 keys.
+    // (and twice what the last one sees: where queries are more than positions, those that
+    // see nothing would fill the line, beyond what it is counted in)
     const unsigned keys = 2u * (unsigned)max(s.n_past, 0) + ((unsigned)(n_rt + 1) * ROWS - 2u) / (unsigned)rep + 2u;
-    pair = (keys + 2 * TK - 2) / TK;
+    pair = min((keys + 2 * TK - 2) / TK, 2u * (((unsigned)max(s.n_seen, 1) + TK - 1) / TK));
   }
   // Key tiles of row tile rt, one at least (rows without a key are written too).
   __device__ inline int tiles(int rt) const {

@@ -340,3 +340,20 @@ def test_offsets_at_the_end_of_their_type(hip, stream, new):
         assert (outs[-1][rows:] == 7.5).all()
         assert all(np.array_equal(x, outs[0]) for x in outs)
     b.close()
+
+
+@pytest.mark.parametrize("n_kv,new", [(16, 9000000), (40, 5000), (300, 2000)])
+def test_far_more_queries_than_positions(hip, stream, n_kv, new):
+    """The queries that see no position give zeros, however many they are; the last ones see theirs."""
+    import torch
+    b = Batch(hip, np.random.default_rng(15), "f16", 64, 1, 1, 16, [(n_kv, n_kv)])
+    last = dev(b.q)
+    q = last[-1:].expand(new, 1, 64)  # (every query the same row, which takes no memory)
+    out = torch.full((new, 1, 64), 7.5, device="cuda")
+    a = mh.paged_attn_args(b.kv, 1, q, out, dev(np.array([0, new], np.int32)), b.dn_kv, b.dtable[:, :-(-n_kv // 16)], b.scale, stream)
+    hip.check(hip.mi_hip_attn_paged(ctypes.byref(a)))
+    torch.cuda.synchronize()
+    assert bool((out[:new - n_kv] == 0).all())
+    b.q = np.repeat(b.q[-1:], n_kv, 0)
+    b.check(out[new - n_kv:].cpu().numpy().astype(np.float64))
+    b.close()
