@@ -1963,6 +1963,7 @@ int mi_hip_page_tables(const mi_hip_page_tables_args* a) {
   if (!a) return fail(MI_HIP_E_INVALID, "args is NULL");
   if (a->n_seq < 0 || a->max_tokens < 0) return fail(MI_HIP_E_INVALID, "n_seq and max_tokens must be >= 0");
   if (a->n_pages < 1 || a->max_pages < 1) return fail(MI_HIP_E_INVALID, "n_pages and max_pages must be positive");
+  if (a->n_seq > 1 << 30) return fail(MI_HIP_E_UNSUPPORTED, "n_seq %d: more than 2^30 sequences", a->n_seq);
   if (int rc = check_page_size(a->page_size)) return rc;
   if ((int64_t)a->n_pages * a->page_size > INT32_MAX || (int64_t)a->max_pages * a->page_size > INT32_MAX - 64)
     return fail(MI_HIP_E_UNSUPPORTED, "2^31 rows of the pool or of a sequence, or more");
