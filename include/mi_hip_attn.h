@@ -572,12 +572,12 @@ int mi_hip_attn_paged(const mi_hip_attn_paged_args* args);
  * The token drawn is -1 if its row has a NaN or a +infinity, or nothing but -infinity
  * (then no child is accepted either), and where every w is 0; child tokens outside
  * [0, n_vocab) are turned down. u is clamped to [0, 1), a NaN to 0; a temperature of
- * +infinity has all finite logits alike, a negative one or NaN counts as 0. Scratch:
- * the parts of ws, else of the library default (34 MB); of them a call takes, with
- * c = n_vocab / 2048 rounded up, at most 16 c n_rows + (8 c + 40) min(n_seq, 1024)
- * bytes, and is refused where they hold less than it takes (MI_HIP_E_UNSUPPORTED).
- * Calls that share one must be ordered. May be captured into a graph. No counterpart
- * in the reference. */
+ * +infinity has all finite logits alike, a negative one or NaN counts as 0. At most
+ * 2^30 sequences (MI_HIP_E_UNSUPPORTED). Scratch: the parts of ws, else of the
+ * library default (34 MB); of them a call takes, with c = n_vocab / 2048 rounded up,
+ * at most 16 c n_rows + (8 c + 40) min(n_seq, 1024) bytes, and is refused where they
+ * hold less than it takes (MI_HIP_E_UNSUPPORTED). Calls that share one must be
+ * ordered. May be captured into a graph. No counterpart in the reference. */
 typedef struct mi_hip_verify_args {
   const float* logits;      /* device, n_rows rows of n_vocab */
   size_t nb;                /* bytes between rows */

@@ -2106,6 +2106,7 @@ int mi_hip_verify_draft(const mi_hip_verify_args* a) {
   if (a->n_vocab <= 0 || a->n_rows < 0 || a->n_seq < 0 || a->max_path < 1)
     return fail(MI_HIP_E_INVALID, "n_vocab and max_path must be positive, n_rows and n_seq >= 0");
   if (a->n_vocab > INT32_MAX - (1 << 16)) return fail(MI_HIP_E_UNSUPPORTED, "n_vocab %d", a->n_vocab);
+  if (a->n_seq > 1 << 30) return fail(MI_HIP_E_UNSUPPORTED, "n_seq %d: more than 2^30 sequences", a->n_seq);
   if ((a->n_seq > 0 && (!a->off || !a->n_path || !a->path || !a->tokens)) ||
       (a->n_seq > 0 && a->n_rows > 0 && (!a->logits || !a->token || !a->u)))
     return fail(MI_HIP_E_INVALID, "only parent, draft, temperature and ws may be NULL");

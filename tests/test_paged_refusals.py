@@ -131,3 +131,9 @@ def test_builders(lib):
 def test_page_tables_of_too_many_sequences(lib, n, code):
     # (as many as may be go on to the next check, of the table's rows)
     assert rc_of(lib, "mi_hip_page_tables", tables(), n_seq=n, table_nb=36) == code, lib.last_error()
+
+
+@pytest.mark.parametrize("n,code", [(1 << 30, 1), ((1 << 30) + 1, 5), (2 ** 31 - 1, 5)])
+def test_verification_of_too_many_sequences(lib, n, code):
+    # (as many as may be go on to the next check, of the pointers)
+    assert rc_of(lib, "mi_hip_verify_draft", verify(), n_seq=n, off=None) == code, lib.last_error()
