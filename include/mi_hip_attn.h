@@ -517,15 +517,19 @@ int mi_hip_paged_append(const mi_hip_paged_append_args* args);
  * position never shows in its output, infinities and NaN included. A position whose
  * table entry is not in [0, n_ctx / page_size) has a row of NaN. Lengths count as
  * clamped: q_off to [0, n_tokens], n_kv to [0, max_pages * page_size]; of a sequence
- * with more than max_new queries the rest are left as they were. Products, sums and
- * values that are not finite as in mi_hip_attn_tree, with the choice of kernel per
- * sequence: few query rows (n_rep times its queries) are up to 16, or up to 32 where
- * max_new allows no sequence more, others the rows beyond. The same bits on every
- * run with the same lengths. At most 2^20 sequences, 2^26 query rows (tokens times
- * heads), 2^30 positions of a sequence, and 2^31 tiles of 32 positions in all
- * (MI_HIP_E_UNSUPPORTED). Scratch for joining the parts of long sequences: ws,
- * else the cache's own; calls that share one must be ordered. May be captured into
- * a graph. No counterpart in the reference. */
+ * with more than max_new queries the rest are left as they were. q_off ascends: the
+ * sequences' rows do not overlap, and the limit on tiles below counts them once. A
+ * max_new that is known chooses the kernel: without it single tokens take the one
+ * that has room for chunks (32 over 2000 keys, 14/2 heads of 64, F16: 19 us, with
+ * max_new 1 15). Products, sums and values that are not finite as in
+ * mi_hip_attn_tree, with the choice of kernel per sequence: few query rows (n_rep
+ * times its queries) are up to 16, or up to 32 where max_new allows no sequence
+ * more, others the rows beyond. The same bits on every run with the same lengths. At
+ * most 2^20 sequences, 2^26 query rows (tokens times heads), 2^30 positions of a
+ * sequence, and 2^31 tiles of 32 positions in all (MI_HIP_E_UNSUPPORTED). Scratch
+ * for joining the parts of long sequences: ws, else the cache's own; calls that
+ * share one must be ordered. May be captured into a graph. No counterpart in the
+ * reference. */
 typedef struct mi_hip_attn_paged_args {
   mi_hip_kv* kv;          /* of mi_hip_kv_create_paged */
   int32_t layer;

@@ -371,8 +371,9 @@ hipError_t launch_kv_keep(const KvKeep& p, hipStream_t stream) {
 // P: NormRope (rows n_past + token of a cache, one position per token) or
 // PagedRope (rows by slots, positions by axes; a token without a row has its Q
 // written only). Positions of three axes cost no more than one's (1225 tokens, 28/4
-// heads of 128, 8-bit: 11.0 us, as with one axis; 8192 tokens, F16: 58 us, 4.9 TB/s). A workgroup's first rows on their way beside the angles were not faster
-// with few tokens, and 10 us slower with 8192.
+// heads of 128, 8-bit: 11.0 us, as with one axis; 8192 tokens, F16: 58 us, 4.9 TB/s). A
+// workgroup's first rows on their way beside the angles were not faster with few
+// tokens, and 10 us slower with 8192.
 __device__ inline int position_of(const NormRope& p, int t, int) { return p.pos ? gload<int>(p.pos + t) : p.n_past + t; }
 __device__ inline int position_of(const PagedRope& p, int t, int pair) {
   const unsigned axis = p.axis[pair / 16] >> (2 * (pair % 16)) & 3u;
@@ -387,7 +388,7 @@ __device__ inline int64_t cache_row(const PagedRope& p, int t) {
 
 // A wave per row, any strides and n_dims, each lane with angles of its own in double
 // precision (4096 tokens of 28/4 heads of 128 with 96 dims rotated: 72.4 us, 8-bit
-// cache 80.9, where the form below, whose angles are once per token, takes 23 to 25
+// cache 80.9, where the form below, whose angles are once per token, takes 24 to 26
 // for all dims): the row passes through LDS so that a
 // lane finds its dims' partners. K on its way to an 8-bit cache stays in double
 // precision until it is quantised, as in the form for aligned rows below.

@@ -17,7 +17,8 @@
 // So workgroups need nothing of each other: each forms the sums of 1024 sequences
 // at a time by itself, into LDS, and takes its share of their pages and tokens, a
 // thread for each, whose sequence it finds there. (Lengths that are also written
-// cannot be read by several workgroups: held or ring_at in place, one does it all.)
+// cannot be read by several workgroups: held or ring_at in place, one does it all, 1024
+// requests with 38000 tokens in 40 us instead of 7.)
 // Bound: the chain of two loads (lengths, then pages) and the launch (8 requests 6.4 us,
 // 1024 requests with 37000 tokens 8.6, an empty launch 3.6).
 #include <algorithm>

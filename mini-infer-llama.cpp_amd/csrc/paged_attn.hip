@@ -14,8 +14,9 @@
 // rows see; to find the unit at a place of the line without adding up row tiles,
 // row tile r of n lies beside row tile n - 1 - r: together they have the same number
 // of tiles, but for a few that are empty. Each wave reads the lengths of 64
-// sequences at a time and adds up their tiles by itself (one round of loads and
-// six additions).
+// sequences at a time and adds up their tiles by itself, a round of loads and six
+// additions for each 64, in up to three passes (the later ones have the first 64
+// sequences' lengths in LDS), then goes on from the first ones to its share.
 //
 // Parts. A unit that lies in several workgroups' shares leaves a record from each
 // (its first part in slot 2 w + 1 of the workgroup w where it begins, the others in
@@ -35,7 +36,7 @@
 // besides its tiles is what counts: about 6 us from the launch to the first tile
 // (lengths, pages, rows: three loads one after the other), and 8 to 10 for records to
 // go through memory and be joined, which short chunks pay twice (1000 tokens from
-// nothing: 45 us, 13 of them products).
+// nothing, 28/4 heads of 128, F16: 52 us in a row of calls, 13 of them products).
 #include <algorithm>
 #include <type_traits>
 
@@ -53,7 +54,8 @@ constexpr int kRun = 16;  // keys that share a page at least
 // threadIdx.x as a value of its own: what is formed from it is formed where it is
 // used, and not kept in registers across the units of a workgroup (which spill
 // for it: 1000 tokens after 1337 among 31 single tokens over 2667 to 4000 keys, 28/4
-// heads of 128, F16 189 us, so 122).
+// heads of 128, F16 189 us, so 122). Of the 18 kernels one still spills a register,
+// the mixed one of 8-bit caches and heads of 128.
 __device__ __forceinline__ int thread_here() {
   int t = (int)threadIdx.x;
   asm volatile("" : "+v"(t));

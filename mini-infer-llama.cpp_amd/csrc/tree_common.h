@@ -1,4 +1,5 @@
-// tree_common.h -- what the tree-attention kernels (tree.hip, tree_wide.hip) share.
+// tree_common.h -- what the tree-attention kernels (tree.hip, tree_wide.hip) and those over
+// pages (paged_attn.hip) share.
 #pragma once
 
 #include "attn_common.h"

@@ -17,8 +17,8 @@
 // that with several workgroups a sequence, the last of which draws.
 //
 // Bound: for many rows the vector unit, 27 instructions a logit, 20 of them double
-// (384 rows of 151936: 54 us, 33 to read them; five fma fewer take 8 us less), for few
-// the launches' chains of loads (up to six rows 13 us).
+// (384 rows of 151936: 54 us, 33 to read them), for few the launches' chains of loads
+// (up to six rows 13 us).
 #include <algorithm>
 
 #include "attn_common.h"
