@@ -631,7 +631,7 @@ static hipError_t launch_rope_rows(const P& p, hipStream_t stream) {
     const bool few = p.n_tokens < (most == 1 ? 768 : 384 * most);
     const int tokens = few ? 1 : most, pieces = (tokens * per_tok + rows - 1) / rows;
     const int groups = (p.n_tokens + tokens - 1) / tokens;
-    const bool two = few || 2 * groups <= kRopeWgs || tokens * per_tok >= 3 * rows;
+    const bool two = few || groups <= kRopeWgs / 2 || tokens * per_tok >= 3 * rows;
     const int wgs = few && p.n_tokens * pieces <= kRopeWgs ? pieces : std::min(two ? 2 : 1, pieces);
     const dim3 grid((unsigned)groups, (unsigned)wgs);
     if (p.cache.head_dim == 64) hipLaunchKernelGGL((norm_rope_kernel<64, P>), grid, dim3(256), 0, stream, p, tokens);
